@@ -1,0 +1,88 @@
+// Layout and number format of the 8-bit paged cache (include/tgis_kv8.h); shared by cache8.cu and attention8*.cu.
+//
+// A (page, kv head) is one run of 8448 bytes, fetched by one bulk copy: K codes | V codes | K scales | V scales.
+//   K  [32 tok][8 chunks of 16 dims, chunk c at place c ^ (tok & 7)][16]: the 128-byte swizzled K-major operand of the tensor cores;
+//      ldmatrix of 8 tokens of one chunk touches all banks once.
+//   V  [2 halves of 16 tok][128 dims][16 places]: V transposed, the unswizzled K-major operand (8 dims x 16 places are a core matrix).
+//      Token t of a half lies at place v8_place(t), so that the scores that a thread holds after S = Q K^T by mma.sync (columns
+//      2i, 2i + 1 of neighbouring 8-token tiles) are the four consecutive k places that it needs for P V: nothing is exchanged.
+#pragma once
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace tgis {
+
+constexpr int KV8_CODES = KV_BLOCK * HEAD_DIM;                 // bytes of a page's K (or V) codes per head
+constexpr int KV8_PAGE = 2 * KV8_CODES + 2 * KV_BLOCK * 4;     // 8448
+constexpr int KV8_K_SCALES = 2 * KV8_CODES, KV8_V_SCALES = KV8_K_SCALES + KV_BLOCK * 4;
+constexpr float KV8_TOP = 448.f;                               // largest e4m3 number
+constexpr float KV8_TINY = 1.17549435e-38f;                    // 2^-126: quotients by it stay within e4m3's range
+
+// byte of dim d of token t (of 32) in the K codes
+__host__ __device__ __forceinline__ constexpr int k8_at(int t, int d) { return t * HEAD_DIM + (((d >> 4) ^ (t & 7)) << 4) + (d & 15); }
+// token bits (j, i, i, v) of a half -> place bits (i, i, j, v)
+__host__ __device__ __forceinline__ constexpr int v8_place(int t) { return (t >> 1 & 3) << 2 | (t >> 3 & 1) << 1 | (t & 1); }
+__host__ __device__ __forceinline__ constexpr int v8_at(int t, int d) { return (t >> 4) * (KV8_CODES / 2) + d * 16 + v8_place(t & 15); }
+
+// low byte from lo, high byte from hi
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// the two numbers of e4m3x2, as a pair of fp16 (exact)
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)c));
+  return r;
+}
+__device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
+  float2 f;
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b;}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+  return f;
+}
+
+// cudaFuncSetAttribute once a device
+struct OncePerDevice {
+  static constexpr int MAX = 64;
+  bool done[MAX] = {};
+  template <class F>
+  cudaError_t operator()(F&& f) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < MAX && done[dev]) return cudaSuccess;
+    e = f();
+    if (e == cudaSuccess && dev < MAX) done[dev] = true;   // (two threads at once: set twice, to the same value)
+    return e;
+  }
+};
+
+// ---- launchers (cache8.cu, attention8.cu); arguments as in include/tgis_kv8.h
+cudaError_t kv8_write_launch(uint8_t* pages, int n_pages, int n_kv, const __nv_bfloat16* qkv, int64_t ld, int T, int n_q, const int32_t* positions,
+                             const int32_t* slots, const __nv_bfloat16* cos_sin, int n_positions, __nv_bfloat16* q_out, int64_t ldq,
+                             int32_t* status, cudaStream_t stream);
+cudaError_t kv8_read_launch(const uint8_t* pages, int n_pages, int n_kv, const int32_t* slots, int T, __nv_bfloat16* k_out, int64_t ldk,
+                            __nv_bfloat16* v_out, int64_t ldv, int32_t* status, cudaStream_t stream);
+struct Attn8Args {
+  const uint8_t* pages;
+  int n_pages, n_kv;
+  const __nv_bfloat16* q;
+  int64_t ldq;
+  int T, n_q;
+  const AttnSeq* seqs;
+  int n_seqs;
+  const int32_t* block_table;
+  int bt_rows, bt_stride;
+  const uint64_t* tree;
+  float scale;
+  int max_q, max_kv;
+  __nv_bfloat16* out;
+  int64_t ldo;
+  int32_t* status;
+};
+size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv);
+cudaError_t attn8_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream, int* launches = nullptr);
+
+}  // namespace tgis

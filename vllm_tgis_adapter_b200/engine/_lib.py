@@ -155,6 +155,9 @@ KERNEL_SYMBOLS = [
     "tgis_k_sampler", "tgis_k_sampler_ex", "tgis_k_sampler_masked", "tgis_k_lora", "tgis_k_lora_bench", "tgis_k_lora_swiglu", "tgis_k_silu_mul_interleaved", "tgis_k_gemm_any", "tgis_k_gemm_any_room", "tgis_k_rmsnorm_f32", "tgis_k_resid_tail", "tgis_k_latent_prep", "tgis_k_latent_q_rope", "tgis_k_latent_attn", "tgis_k_moe_route", "tgis_k_moe_align", "tgis_k_moe_route_grouped", "tgis_k_dyt_tail", "tgis_k_lightning_scan", "tgis_k_retention_scan", "tgis_k_gla_scan", "tgis_k_moe_table_align", "tgis_k_resid_tail_plain", "tgis_k_capattn_prep", "tgis_k_capattn", "tgis_k_sigattn_prep", "tgis_k_sigattn", "tgis_k_poolattn_prep", "tgis_k_poolattn", "tgis_k_delta_scan", "tgis_k_ssd_scan", "tgis_k_token_shift", "tgis_k_short_conv", "tgis_k_selective_scan", "tgis_k_outer_scan", "tgis_k_head_norm_gate", "tgis_k_resid_tail_pair", "tgis_k_resid_tail_two", "tgis_k_sizeof_sample_row", "tgis_k_sizeof_sample_out", "tgis_k_kv_block",
 ]
 
+# ... and include/tgis_kv8.h
+KV8_SYMBOLS = ["tgis_kv8_write", "tgis_kv8_read", "tgis_kv8_attention_workspace", "tgis_kv8_attention", "tgis_kv8_last_error"]
+
 _LIB: C.CDLL | None = None
 
 
@@ -261,6 +264,12 @@ def load_library() -> C.CDLL:
     lib.tgis_k_resid_tail_plain.argtypes = [vp, vp, vp, f32, i32, vp, vp, vp, vp, vp, i32, vp, vp, f32, i32, i32]
     lib.tgis_k_head_norm_gate.argtypes = [vp, i32, i32, i32, vp, vp, i32, i32, f32, vp, i32, i32]
     lib.tgis_k_resid_tail_pair.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, f32, i32, i32]
+    lib.tgis_kv8_last_error.restype = C.c_char_p
+    lib.tgis_kv8_write.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, vp, vp, i32, vp, i64, vp, vp]
+    lib.tgis_kv8_read.argtypes = [vp, i32, i32, vp, i32, vp, i64, vp, i64, vp, vp]
+    lib.tgis_kv8_attention_workspace.restype = i64
+    lib.tgis_kv8_attention_workspace.argtypes = [i32] * 6
+    lib.tgis_kv8_attention.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, i32, vp, i32, i32, vp, f32, i32, i32, vp, i64, vp, i64, vp, vp]
     _LIB = lib
     return lib
 
