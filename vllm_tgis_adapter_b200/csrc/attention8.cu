@@ -21,13 +21,13 @@
 #include "cache8.cuh"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "tc_attention.cuh"
 
 namespace tgis {
 namespace {
 
 constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 3, R8_MINB = 2;
 constexpr int R8_SPLIT = 128;                 // tokens of a split
-constexpr float R8_LO = 16.f;                 // lo parts are held times this
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
@@ -42,35 +42,6 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// four numbers as hi parts and as lo parts
-__device__ __forceinline__ void split4(float x0, float x1, float x2, float x3, uint32_t& hi, uint32_t& lo) {
-  const uint32_t h0 = e4m3x2(x0, x1), h1 = e4m3x2(x2, x3);
-  const float2 f0 = f16x2_to_f32x2(e4m3x2_to_f16x2(h0)), f1 = f16x2_to_f32x2(e4m3x2_to_f16x2(h1));
-  hi = h0 | h1 << 16;
-  lo = e4m3x2((x0 - f0.x) * R8_LO, (x1 - f0.y) * R8_LO) | e4m3x2((x2 - f1.x) * R8_LO, (x3 - f1.y) * R8_LO) << 16;
-}
-// 2^e that brings a magnitude (the bits of a number >= 0) to [128, 256); no more than 2^126
-__device__ __forceinline__ float power_up(uint32_t bits) {
-  const int ex = min(max((int)(bits >> 23), 8), 254);
-  return __uint_as_float((uint32_t)(261 - ex) << 23);   // 2^(134 - ex)
-}
-__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > 4000000000ll) return false;   // about two seconds: no copy takes that long
-  return true;
-}
-
-__device__ __forceinline__ bool seq_fits(const Attn8Args& a, const AttnSeq& s) {
-  return s.q_len >= 0 && s.q_len <= a.max_q && s.kv_len >= s.q_len && s.kv_len <= a.max_kv && s.q_start >= 0 && s.q_start <= a.T - s.q_len &&
-         s.block_row >= 0 && s.block_row < a.bt_rows && (s.kv_len + KV_BLOCK - 1) / KV_BLOCK <= a.bt_stride && (a.tree == nullptr || s.q_len <= TGIS_KV8_MAX_TREE);
-}
-__device__ __forceinline__ AttnSeq load_seq(const Attn8Args& a, int s) {
-  const int4 v = reinterpret_cast<const int4*>(a.seqs)[s];
-  return AttnSeq{v.x, v.y, v.z, v.w};
-}
-
 struct RowsItem {
   AttnSeq sq;
   int kvh, chunk, split, tok0, n_tok;         // keys tok0 .. tok0 + n_tok - 1 of the sequence (of the split, and seen by a row of the chunk)
@@ -245,7 +216,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
     const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * 8 * MT / G + 1 : 0);
     const int n_blk = it.n_blk();
     for (int jb = 0; jb < n_blk; ++jb) {
-      if (!wait_bounded(&full[c_st], c_ph)) {
+      if (!bounded_wait(&full[c_st], c_ph)) {
         alive = false;
         break;
       }
@@ -284,8 +255,8 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 ks = *reinterpret_cast<const float2*>(k_scale + 8 * j + 2 * t4);
-            x[j][0] = (s[mt][j][0] + s[mt][j][2] * (1.f / R8_LO)) * (ks.x * q_mul[mt]);
-            x[j][1] = (s[mt][j][1] + s[mt][j][3] * (1.f / R8_LO)) * (ks.y * q_mul[mt]);
+            x[j][0] = (s[mt][j][0] + s[mt][j][2] * (1.f / KV8_LO)) * (ks.x * q_mul[mt]);
+            x[j][1] = (s[mt][j][1] + s[mt][j][3] * (1.f / KV8_LO)) * (ks.y * q_mul[mt]);
           }
           if (open) {
 #pragma unroll
@@ -339,8 +310,8 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
             for (int h = 0; h < 2; ++h) {
               float c[4] = {0.f, 0.f, 0.f, 0.f};
               mma_e4m3(c, pa[mt], vb[2 * h], vb[2 * h + 1]);
-              o[mt][n + h][0] = fmaf(fmaf(c[2], 1.f / R8_LO, c[0]), add[mt], o[mt][n + h][0] * keep[mt]);
-              o[mt][n + h][1] = fmaf(fmaf(c[3], 1.f / R8_LO, c[1]), add[mt], o[mt][n + h][1] * keep[mt]);
+              o[mt][n + h][0] = fmaf(fmaf(c[2], 1.f / KV8_LO, c[0]), add[mt], o[mt][n + h][0] * keep[mt]);
+              o[mt][n + h][1] = fmaf(fmaf(c[3], 1.f / KV8_LO, c[1]), add[mt], o[mt][n + h][1] * keep[mt]);
             }
         }
       }
@@ -416,10 +387,12 @@ __global__ void __launch_bounds__(256) attn8_merge_kernel(const __grid_constant_
 
 struct RowsPlan {
   int mt, split, max_splits;
+  bool prompt;                                // attention8_prompt.cu
 };
-RowsPlan rows_plan(int n_q, int n_kv, int max_q, int max_kv) {
+RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   RowsPlan p{};
-  const int rows = max_q * (n_q / n_kv);
+  const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
+  p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   p.mt = rows > 8 ? 2 : 1;
   p.split = rows <= 256 ? R8_SPLIT : (std::max(max_kv, 1) + KV_BLOCK - 1) / KV_BLOCK * KV_BLOCK;
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
@@ -443,13 +416,17 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
 }  // namespace
 
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
-  const RowsPlan p = rows_plan(n_q, n_kv, max_q, max_kv);
+  const RowsPlan p = rows_plan(T, n_seqs, n_q, n_kv, max_q, max_kv);
+  if (p.prompt) return attn8_prompt_workspace(ATTN8_MAX_SMS);
   return p.max_splits > 1 ? (size_t)T * n_q * p.max_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
 }
 
 cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches) {
   if (args.n_seqs <= 0 || args.T <= 0) return cudaSuccess;
-  const RowsPlan p = rows_plan(args.n_q, args.n_kv, args.max_q, args.max_kv);
+  num_sms = std::min(num_sms, ATTN8_MAX_SMS);
+  const RowsPlan p = rows_plan(args.T, args.n_seqs, args.n_q, args.n_kv, args.max_q, args.max_kv);
+  if (launches != nullptr) *launches = 2;
+  if (p.prompt) return attn8_prompt_launch(args, workspace, num_sms, stream);
   RowsArgs a;
   static_cast<Attn8Args&>(a) = args;
   a.split = p.split;
@@ -457,7 +434,7 @@ cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cu
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_ml = a.part_o + (size_t)a.T * a.n_q * a.max_splits * HEAD_DIM;
   cudaError_t e = p.mt == 1 ? rows_launch<1>(a, num_sms, stream) : rows_launch<2>(a, num_sms, stream);
-  if (launches != nullptr) *launches = p.max_splits > 1 ? 2 : 1;
+  if (launches != nullptr && p.max_splits == 1) *launches = 1;
   if (e != cudaSuccess || p.max_splits == 1) return e;
   const int y = std::min((args.max_q * args.n_q + 7) / 8, 64);
   return launch_k(attn8_merge_kernel, dim3(a.n_seqs, y), dim3(256), 0, stream, a);

@@ -1,0 +1,703 @@
+// Attention over the 8-bit paged cache (include/tgis_kv8.h; layout and number format: cache8.cuh) of prompts, their portions and wide
+// drafted trees, on tcgen05.
+//
+// A unit is up to 2 TM query tokens of one sequence and one kv head, half of them in each of two accumulators (row = token * G + head of the
+// group, TM = 128 / G); a step is one tile of 128 keys of a unit.  All steps of the call lie in one row, sequence after sequence,
+// and every CTA takes an equal stretch of them: a stretch that begins or ends inside a unit leaves that unit's sums (o, m, l) in
+// the workspace, and attn8_join_kernel joins them in order.  So a long prompt, many short ones and a few drafts over long contexts
+// all keep every SM busy to the end, and the workspace is two units a CTA whatever the lengths are.  Lengths and pages are read on
+// the device.
+//
+//   S = Q K^T  e4m3 x e4m3 -> fp32 (kind::f8f6f4): K as the cache holds it (a block is 32 rows of the 128-byte swizzled form), a query row as
+//              hi + lo, two e4m3 numbers that are exact but for the smallest entries (cache8.cuh split4; lo is not scaled here: both
+//              products go to one accumulator, and numbers below 2^-18 of the row's largest are cut);
+//   P V        f16 x f16 -> fp32 (kind::f16): two warps widen V to f16 (exact) into the unswizzled K-major form; a probability times
+//              its row's scale is one f16 number of 11 bits.  It is held times 2^7 / r, r the power of two at or above the scales so far, and the
+//              reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
+//              most) and nothing above 2^-31 of the largest is lost.
+// Scores and probabilities of a row are one thread's; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are written in that
+// order.  A row with a NaN for its scale gets zeros here and a bit; who sees it gets NaN for its sum.
+//
+// No wait is unbounded: after about two seconds a role gives up, the call's status says so; copies and MMAs in flight land first and TMEM is
+// freed on every path.
+#include <algorithm>
+
+#include "cache8.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "tc_attention.cuh"
+
+namespace tgis {
+namespace {
+
+constexpr int P8_THREADS = 384;                             // warps 0..3, 4..7: softmax of an accumulator; copies, MMAs, two that widen V
+constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 10;
+constexpr int P8_REGS_SOFTMAX = 208, P8_REGS_OTHER = 88;    // 256 x 208 + 128 x 88 = 384 x 168, what the launch gives every thread
+constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
+constexpr int P8_STAGES = 2;
+constexpr int P8_TILE8 = P8_KV * HEAD_DIM;                  // bytes of a tile's codes; of one accumulator's hi (or lo) parts of Q
+constexpr int P8_SCALES = P8_BLOCKS * 2 * KV_BLOCK * 4;     // as they lie in the cache, block by block: K scales | V scales
+constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
+constexpr float P8_HELD = 128.f;                            // probabilities are held times this
+
+struct TileScales {
+  float k[P8_KV];              // over k_unit; 0 where there is none
+  float v[P8_KV];              // times P8_HELD / r
+  uint32_t poison[P8_BLOCKS];  // tokens whose key or value row is not a number
+  uint32_t absent;             // blocks whose page does not exist (bits)
+  float unit;                  // r / P8_HELD
+  float k_unit;                // power of two at or above the tile's key scales: products of codes times scales stay in range
+  uint32_t pad;
+};
+struct P8Smem {
+  uint8_t q[2][2][P8_TILE8];   // accumulator, hi | lo
+  uint8_t k[P8_STAGES][P8_TILE8];
+  uint8_t v16[P8_STAGES][2 * P8_TILE8];
+  uint8_t v8[P8_STAGES][P8_TILE8];
+  uint8_t raw[P8_STAGES][P8_SCALES];
+  TileScales sc[P8_STAGES];
+  uint64_t q_full[2], k_full[P8_STAGES], k_empty[P8_STAGES], v8_full[P8_STAGES], v8_empty[P8_STAGES], v_full[P8_STAGES], v_empty[P8_STAGES], s_full[2],
+      p_full[2], o_full[2];
+  uint32_t absent[P8_STAGES];  // by the copying warp, with v8
+  uint32_t tmem_base;
+  int gave_up;
+  uint32_t wsum[P8_THREADS / 32];
+  uint32_t total;
+  uint32_t prefix[1];          // steps ahead of each sequence
+};
+static_assert(sizeof(TileScales) % 16 == 0 && offsetof(P8Smem, sc) % 16 == 0 && offsetof(P8Smem, q_full) % 8 == 0, "");
+
+struct PromptArgs : Attn8Args {
+  int G, TM;
+  float *frag_o, *frag_ml;     // [CTA][0: of a unit begun before it, 1: of one that ends behind it][256 rows]([128])
+};
+
+// ---- the row of steps
+struct SeqUnits {
+  AttnSeq sq;
+  int n_units, tokens;         // of a unit (the last one may have fewer)
+};
+__device__ __forceinline__ SeqUnits units_of(const PromptArgs& a, int s) {
+  SeqUnits u;
+  u.sq = load_seq(a, s);
+  if (!seq_fits(a, u.sq)) u.sq.q_len = 0;
+  u.n_units = (u.sq.q_len + 2 * a.TM - 1) / (2 * a.TM);
+  u.tokens = u.n_units > 0 ? (u.sq.q_len + u.n_units - 1) / u.n_units : 0;
+  return u;
+}
+// keys that some row of unit i sees
+__device__ __forceinline__ int keys_of(const PromptArgs& a, const SeqUnits& u, int i) {
+  return a.tree != nullptr ? u.sq.kv_len : u.sq.kv_len - u.sq.q_len + min((i + 1) * u.tokens, u.sq.q_len);
+}
+__device__ __forceinline__ int steps_of(const PromptArgs& a, const SeqUnits& u, int i) { return (keys_of(a, u, i) + P8_KV - 1) / P8_KV; }
+
+// steps of all sequences ahead of each; by every thread of a CTA of THREADS
+template <int THREADS>
+__device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefix, uint32_t* wsum) {
+  const int warp = threadIdx.x >> 5, lane = (int)lane_id();
+  uint32_t carry = 0;
+  for (int base = 0; base < a.n_seqs; base += THREADS) {
+    const int s = base + threadIdx.x;
+    uint32_t n = 0;
+    if (s < a.n_seqs) {
+      const SeqUnits u = units_of(a, s);
+      for (int i = 0; i < u.n_units; ++i) n += (uint32_t)steps_of(a, u, i);
+      n *= (uint32_t)a.n_kv;
+    }
+    uint32_t sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) wsum[warp] = sum;
+    __syncthreads();
+    uint32_t before = carry;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += wsum[w];
+      carry += wsum[w];
+    }
+    if (s < a.n_seqs) prefix[s] = before + sum - n;
+    __syncthreads();
+  }
+  return carry;
+}
+__device__ __forceinline__ uint32_t stretch_begin(uint32_t total, uint32_t cta, uint32_t n) { return (uint32_t)((uint64_t)total * cta / n); }
+
+// One unit's steps [tile0, tile1) of a CTA's stretch after the other
+struct Walk {
+  const PromptArgs& a;
+  const uint32_t* prefix;
+  uint32_t at, end;
+  int s = -1, i = 0, kvh = 0, steps = 0, tile0 = 0, tile1 = 0;
+  SeqUnits u;
+  __device__ Walk(const PromptArgs& a_, const uint32_t* p, uint32_t begin, uint32_t end_) : a(a_), prefix(p), at(begin), end(end_) {}
+  __device__ void find() {     // the unit that step `at` belongs to
+    int lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= at) lo = mid;
+      else hi = mid;
+    }
+    s = lo;
+    u = units_of(a, s);
+    uint32_t left = at - prefix[s];
+    for (i = 0;; ++i) {
+      steps = steps_of(a, u, i);
+      if (left < (uint32_t)(steps * a.n_kv) || i >= u.n_units - 1) break;
+      left -= (uint32_t)(steps * a.n_kv);
+    }
+    kvh = (int)(left / (uint32_t)steps);
+    tile0 = (int)(left - (uint32_t)(kvh * steps));
+  }
+  __device__ bool next() {
+    if (at >= end) return false;
+    if (s < 0) {
+      find();
+    } else {                   // the stretch goes on: the unit before ended
+      tile0 = 0;
+      if (++kvh == a.n_kv) {
+        kvh = 0;
+        if (++i == u.n_units) {
+          do u = units_of(a, ++s);
+          while (u.n_units == 0);
+          i = 0;
+        }
+        steps = steps_of(a, u, i);
+      }
+    }
+    tile1 = min(steps, tile0 + (int)(end - at));
+    at += (uint32_t)(tile1 - tile0);
+    return true;
+  }
+  __device__ int keys() const { return keys_of(a, u, i); }
+  __device__ int tokens() const { return min(u.tokens, u.sq.q_len - i * u.tokens); }
+  __device__ int half() const { return (tokens() + 1) / 2; }   // tokens of the first accumulator; the second has the others
+  __device__ bool two() const { return tokens() > 1; }
+  __device__ bool whole() const { return tile0 == 0 && tile1 == steps; }
+  __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys() + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
+};
+
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// C fp32, A and B e4m3 (kind::f8f6f4) or f16 (kind::f16): both formats are number 0; K-major operands
+__device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __grid_constant__ PromptArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  P8Smem& sm = *reinterpret_cast<P8Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = (int)lane_id();
+  if (warp == P8_WARP_MMA) {
+    if (elect_one()) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.q_full[i], 4);
+        mbar_init(&sm.s_full[i], 1);
+        mbar_init(&sm.p_full[i], 4);
+        mbar_init(&sm.o_full[i], 1);
+      }
+      for (int i = 0; i < P8_STAGES; ++i) {
+        mbar_init(&sm.k_full[i], 1);
+        mbar_init(&sm.k_empty[i], 1);
+        mbar_init(&sm.v8_full[i], 1);
+        mbar_init(&sm.v8_empty[i], 2);
+        mbar_init(&sm.v_full[i], 2);
+        mbar_init(&sm.v_empty[i], 1);
+      }
+      sm.gave_up = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc<512>(&sm.tmem_base);
+  }
+  griddep_launch();
+  griddep_wait();
+  if (blockIdx.x == 0 && a.status != nullptr)
+    for (int s = threadIdx.x; s < a.n_seqs; s += P8_THREADS)
+      if (!seq_fits(a, load_seq(a, s))) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
+  const uint32_t total = lay_out<P8_THREADS>(a, sm.prefix, sm.wsum);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = sm.tmem_base;   // [S0 | S1 | O0 | O1], 128 columns each
+  Walk w(a, sm.prefix, stretch_begin(total, blockIdx.x, gridDim.x), stretch_begin(total, blockIdx.x + 1, gridDim.x));
+  bool ok = true;
+  if (warp >= P8_WARP_COPY) {
+    set_regs<P8_REGS_OTHER, false>();
+    if (warp == P8_WARP_COPY) {
+      // ===================== copies =====================
+      int st = 0;
+      uint32_t ph = 1;         // the first pass over the rings finds them empty
+      while (ok && w.next()) {
+        const int n_blk = (w.keys() + KV_BLOCK - 1) / KV_BLOCK;
+        auto page_of = [&](int j) {   // lane: block lane & 3 of tile j
+          const int b = j * P8_BLOCKS + (lane & 3);
+          return b < n_blk ? a.block_table[(size_t)w.u.sq.block_row * a.bt_stride + b] : 0;
+        };
+        int page = page_of(w.tile0);
+        for (int j = w.tile0; j < w.tile1; ++j) {
+          const int nb = w.blocks(j);
+          const bool there = page >= 0 && page < a.n_pages;
+          const uint32_t absent = __ballot_sync(0xffffffffu, !there && lane < nb);
+          if (absent != 0 && lane == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_BAD_PAGE);
+          // (an absent page's keys are not seen; some page's codes stand in for it, for they are numbers)
+          const uint8_t* src = a.pages + ((size_t)(there ? page : 0) * a.n_kv + w.kvh) * KV8_PAGE;
+          const int b = lane & 3, kind = lane >> 2;   // lanes 0..3 K codes, 4..7 V codes, 8..11 scales
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty[st], ph));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[st], nb * KV8_CODES);
+          __syncwarp();
+          if (kind == 0 && b < nb) bulk_load_1d(sm.k[st] + b * KV8_CODES, src, KV8_CODES, &sm.k_full[st]);
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v8_empty[st], ph));
+          if (!ok) break;
+          if (lane == 0) {
+            sm.absent[st] = absent;
+            mbar_arrive_expect_tx(&sm.v8_full[st], nb * (KV8_CODES + 2 * KV_BLOCK * 4));
+          }
+          __syncwarp();
+          if (kind == 1 && b < nb) bulk_load_1d(sm.v8[st] + b * KV8_CODES, src + KV8_CODES, KV8_CODES, &sm.v8_full[st]);
+          if (kind == 2 && b < nb) bulk_load_1d(sm.raw[st] + b * (2 * KV_BLOCK * 4), src + KV8_K_SCALES, 2 * KV_BLOCK * 4, &sm.v8_full[st]);
+          if (++st == P8_STAGES) st = 0, ph ^= 1;
+          if (j + 1 < w.tile1) page = page_of(j + 1);
+        }
+      }
+    } else if (warp == P8_WARP_MMA) {
+      // ===================== MMAs =====================
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
+      auto scores = [&](int g, int nb) {
+        const uint32_t idesc = idesc_of(128, nb * KV_BLOCK), k = smem_u32(sm.k[kst]);
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int ks = 0; ks < HEAD_DIM / 32; ++ks)
+            mma_f8(tmem_base + g * 128, make_smem_desc_sw128(smem_u32(sm.q[g][part]) + ks * 32), make_smem_desc_sw128(k + ks * 32), idesc, part + ks > 0);
+        tc_commit(&sm.s_full[g]);
+      };
+      auto values = [&](int g, int nb, bool first) {
+        const uint32_t idesc = idesc_of(128, HEAD_DIM), v = smem_u32(sm.v16[vst]);
+        for (int ks = 0; ks < 2 * nb; ++ks)   // 16 tokens: two core matrices along k
+          mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + ks * 8, smem_desc(v + ks * 2 * (HEAD_DIM * 16), HEAD_DIM * 16, 128, 0), idesc, !(first && ks == 0));
+      };
+      while (ok && w.next()) {
+        const int groups = w.two() ? 2 : 1;
+        for (int g = 0; g < groups && ok; ++g) {
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.q_full[g], qph[g]));
+          qph[g] ^= 1;
+        }
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(&sm.k_full[kst], kph));
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          for (int g = 0; g < groups; ++g) scores(g, w.blocks(w.tile0));
+          tc_commit(&sm.k_empty[kst]);
+        }
+        __syncwarp();
+        if (++kst == P8_STAGES) kst = 0, kph ^= 1;
+        for (int j = w.tile0; j < w.tile1 && ok; ++j) {
+          const bool more = j + 1 < w.tile1;
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full[vst], vph));
+          for (int g = 0; g < groups && ok; ++g) {
+            ok = __all_sync(0xffffffffu, bounded_wait(&sm.p_full[g], pph[g]) && (g > 0 || !more || bounded_wait(&sm.k_full[kst], kph)));
+            if (!ok) break;
+            pph[g] ^= 1;
+            tc_fence_after();
+            if (elect_one()) {
+              values(g, w.blocks(j), j == w.tile0);
+              if (more) scores(g, w.blocks(j + 1));
+              if (g == groups - 1) {
+                tc_commit(&sm.v_empty[vst]);
+                if (more) tc_commit(&sm.k_empty[kst]);
+              }
+              if (!more) tc_commit(&sm.o_full[g]);
+            }
+            __syncwarp();
+          }
+          if (++vst == P8_STAGES) vst = 0, vph ^= 1;
+          if (more && ++kst == P8_STAGES) kst = 0, kph ^= 1;
+        }
+      }
+    } else {
+      // ===================== V to f16, scales =====================
+      const int half = warp - P8_WARP_WIDEN;
+      int st = 0;
+      uint32_t full = 0, empty = 1;
+      while (ok && w.next()) {
+        float r = 0.f;
+        for (int j = w.tile0; j < w.tile1; ++j) {
+          const int nb = w.blocks(j);
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v8_full[st], full) && bounded_wait(&sm.v_empty[st], empty));
+          if (!ok) break;
+          // sixteen codes (one dim, half a block) -> two rows of eight f16 numbers
+          for (int c = half * 32 + lane; c < nb * 2 * HEAD_DIM; c += 64) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sm.v8[st] + c * 16);
+            const int dim = c & (HEAD_DIM - 1), k = c / HEAD_DIM;
+            uint8_t* to = sm.v16[st] + k * 2 * (HEAD_DIM * 16) + dim * 16;
+            *reinterpret_cast<uint4*>(to) = make_uint4(e4m3x2_to_f16x2(x.x & 0xffffu), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y & 0xffffu), e4m3x2_to_f16x2(x.y >> 16));
+            *reinterpret_cast<uint4*>(to + HEAD_DIM * 16) = make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
+          }
+          if (half == 0) {
+            const uint32_t absent = sm.absent[st];
+            TileScales& t = sm.sc[st];
+            float ks[P8_BLOCKS], vs[P8_BLOCKS], top = 0.f, top_k = 0.f;
+            uint32_t odd = 0;
+#pragma unroll
+            for (int b = 0; b < P8_BLOCKS; ++b) {
+              const float* raw = reinterpret_cast<const float*>(sm.raw[st]) + b * 2 * KV_BLOCK;
+              const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < w.u.sq.kv_len;
+              ks[b] = there ? raw[lane] : 0.f;
+              vs[b] = there ? raw[KV_BLOCK + lane] : 0.f;
+              const bool fine = ks[b] < INFINITY && vs[b] < INFINITY;
+              if (!fine) ks[b] = vs[b] = 0.f;
+              odd = __ballot_sync(0xffffffffu, !fine);
+              if (lane == 0) t.poison[b] = odd;
+              top = fmaxf(top, vs[b]);
+              top_k = fmaxf(top_k, ks[b]);
+            }
+            const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top)), most_k = __reduce_max_sync(0xffffffffu, __float_as_uint(top_k));
+            r = fmaxf(r, fmaxf(__uint_as_float((most + 0x7fffffu) & 0x7f800000u), 0x1p-118f));
+            const float k_unit = fmaxf(__uint_as_float((most_k + 0x7fffffu) & 0x7f800000u), 0x1p-126f);
+#pragma unroll
+            for (int b = 0; b < P8_BLOCKS; ++b) {
+              t.k[b * KV_BLOCK + lane] = ks[b] * (1.f / k_unit);
+              t.v[b * KV_BLOCK + lane] = vs[b] * (P8_HELD / r);
+            }
+            if (lane == 0) {
+              t.absent = absent;
+              t.unit = r / P8_HELD;
+              t.k_unit = k_unit;
+            }
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sm.v_full[st]);
+            mbar_arrive(&sm.v8_empty[st]);
+          }
+          if (++st == P8_STAGES) st = 0, full ^= 1, empty ^= 1;
+        }
+      }
+    }
+  } else {
+    // ===================== softmax: thread = row =====================
+    set_regs<P8_REGS_SOFTMAX, true>();
+    const int g = warp >> 2;
+    const int r = (warp & 3) * 32 + lane, tok = r / a.G, head = r - tok * a.G;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem_base + g * 128 + lanes, o_t = tmem_base + 256 + g * 128 + lanes;
+    uint32_t sph = 0, oph = 0, vph = 0;
+    int vst = 0;
+    while (ok && w.next()) {
+      if (g == 1 && !w.two()) {   // (its stages pass)
+        for (int j = w.tile0; j < w.tile1; ++j)
+          if (++vst == P8_STAGES) vst = 0, vph ^= 1;
+        continue;
+      }
+      const int in_unit = g * w.half() + tok;
+      const bool mine = tok < w.half() && in_unit < w.tokens();
+      const int row = w.u.sq.q_start + w.i * w.u.tokens + in_unit, qhead = w.kvh * a.G + head;
+      const int before = w.u.sq.kv_len - w.u.sq.q_len;      // keys that were there before the step
+      int lim = before + w.i * w.u.tokens + in_unit;        // causal: last key seen
+      unsigned long long word = 0;
+      if (!mine) lim = 0x7fffffff;
+      else if (a.tree != nullptr) lim = before - 1, word = a.tree[row] & ~0ull >> (TGIS_KV8_MAX_TREE - w.u.sq.q_len);
+      // ---- the row of Q, twice
+      float qm;
+      {
+        uint4 x[HEAD_DIM / 8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < HEAD_DIM / 8; ++c) {
+          x[c] = mine ? reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)qhead * HEAD_DIM)[c] : make_uint4(0, 0, 0, 0);
+          const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
+        }
+        float up = power_up(top);
+        qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / up;   // (hidden scores are -inf before they are scaled)
+        if (a.scale < 0.f) up = -up;
+#pragma unroll
+        for (int c = 0; c < HEAD_DIM / 16; ++c) {
+          const uint32_t v[8] = {x[2 * c].x, x[2 * c].y, x[2 * c].z, x[2 * c].w, x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            split4(__uint_as_float(v[2 * i] << 16) * up, __uint_as_float(v[2 * i] & 0xffff0000u) * up, __uint_as_float(v[2 * i + 1] << 16) * up,
+                   __uint_as_float(v[2 * i + 1] & 0xffff0000u) * up, hi[i], lo[i], 1.f);
+          const int at = r * HEAD_DIM + ((c ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(sm.q[g][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(sm.q[g][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full[g]);
+      float m = 0.f, l = 0.f, unit = 0.f;
+      for (int j = w.tile0; j < w.tile1; ++j) {
+        const int nb = w.blocks(j);
+        ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full[vst], vph) && bounded_wait(&sm.s_full[g], sph));
+        if (!ok) break;
+        sph ^= 1;
+        tc_fence_after();
+        const TileScales& sc = sm.sc[vst];
+        const int seen = lim - j * P8_KV;                   // last column seen (of the keys before a draft)
+        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || sc.absent != 0);
+        uint32_t vis[P8_BLOCKS];                            // columns that the row sees, where some are hidden
+#pragma unroll
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          vis[c] = seen >= c * 32 + 31 ? 0xffffffffu : seen < c * 32 ? 0u : (2u << (seen - c * 32)) - 1u;
+          if (a.tree != nullptr && mine) {
+            const int d = c * 32 - (seen + 1);              // node of the block's first column
+            if (d > -32 && d < 64) vis[c] |= d >= 0 ? (uint32_t)(word >> d) : (uint32_t)word << -d;
+          }
+          if (sc.absent >> c & 1) vis[c] = 0;
+        }
+        uint32_t s[P8_KV];
+#pragma unroll
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          if (c >= nb) break;
+          tmem_ld_x32(s_t + c * 32, s + c * 32);
+        }
+        tmem_ld_wait();
+        float mx[P8_BLOCKS] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          if (c >= nb) break;
+          const uint64_t* ks = reinterpret_cast<const uint64_t*>(sc.k + c * 32);
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x, y;
+            unpack2(mul2(pack2(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])), ks[i / 2]), x, y);
+            s[c * 32 + i] = __float_as_uint(x);
+            s[c * 32 + i + 1] = __float_as_uint(y);
+          }
+        }
+        if (mask) {
+#pragma unroll
+          for (int c = 0; c < P8_BLOCKS; ++c) {
+            if (c >= nb) break;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(vis[c] >> i & 1)) s[c * 32 + i] = __float_as_uint(-INFINITY);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          if (c >= nb) break;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])));
+          if ((sc.poison[c] & vis[c]) != 0) l = __uint_as_float(0x7fc00000u);
+        }
+        const float qk = qm * sc.k_unit;
+        uint64_t qm2 = pack2(qk, qk);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qk;
+        const float unit_now = sc.unit;
+        if (j == w.tile0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, top > m + P8_SLACK) || unit_now != unit) {
+          // the products that wrote O retired before these scores did
+          float f = top > m + P8_SLACK ? ex2(m - top) : 1.f;
+          if (top > m + P8_SLACK) m = top;
+          l *= f;
+          f *= unit / unit_now;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_t + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_x16(o_t + c * 16, o);
+          }
+        }
+        unit = unit_now;
+        const float ref = m == -INFINITY ? 0.f : m;   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
+        const uint64_t neg_m = pack2(-ref, -ref);
+        if (fabsf(ref) > 0x1p20f) {
+          // an exact product less a rounded one is no longer below a step of the exponent: round the scores first, as their maximum was
+#pragma unroll
+          for (int i = 0; i < P8_KV; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
+          qm2 = pack2(1.f, 1.f);
+        }
+        uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+        for (int c = 0; c < 2 * P8_BLOCKS; ++c) {
+          if (c >= 2 * nb) break;
+          const uint64_t* vs = reinterpret_cast<const uint64_t*>(sc.v + c * 16);
+          uint32_t p[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int pair = 4 * (i & 1) + (i >> 1);  // places 2 i, 2 i + 1 of the half (cache8.cuh v8_place)
+            const int col = c * 16 + 2 * pair;
+            float x, y;
+            unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
+            const uint64_t e = pack2(ex2(x), ex2(y));
+            if (i & 1) sum1 = add2(sum1, e);
+            else sum0 = add2(sum0, e);
+            unpack2(mul2(e, vs[pair]), x, y);
+            p[i] = f16x2(x, y);
+          }
+          tmem_st_x8(s_t + c * 8, p);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[g]);
+        if (++vst == P8_STAGES) vst = 0, vph ^= 1;
+        float x, y;
+        unpack2(add2(sum0, sum1), x, y);
+        l += x + y;
+      }
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, bounded_wait(&sm.o_full[g], oph));
+      if (!ok) break;
+      oph ^= 1;
+      tc_fence_after();
+      if (w.whole()) {
+        const float inv = l == 0.f ? 0.f : unit / l;
+        __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)qhead * HEAD_DIM;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld_x32(o_t + c * 32, o);
+          tmem_ld_wait();
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = cvt2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
+              *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      } else {
+        const size_t slot = ((size_t)blockIdx.x * 2 + (w.tile0 == 0)) * 256 + g * 128 + r;
+        float* dst = a.frag_o + slot * HEAD_DIM;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          tmem_ld_x32(o_t + c * 32, o);
+          tmem_ld_wait();
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(dst + c * 32 + i * 4) = make_float4(__uint_as_float(o[i * 4]) * unit, __uint_as_float(o[i * 4 + 1]) * unit,
+                                                                            __uint_as_float(o[i * 4 + 2]) * unit, __uint_as_float(o[i * 4 + 3]) * unit);
+          }
+        }
+        if (mine) *reinterpret_cast<float2*>(a.frag_ml + slot * 2) = make_float2(m, l);
+      }
+      tc_fence_before();
+    }
+  }
+  if (!ok && lane == 0) sm.gave_up = 1;
+  tc_fence_before();
+  __syncthreads();
+  // after a wait that ran out copies and MMAs of the other roles may be in flight; they are done long before this millisecond is over
+  if (*reinterpret_cast<volatile int*>(&sm.gave_up)) {
+    if (threadIdx.x == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_STALLED);
+    for (const long long t0 = clock64(); clock64() - t0 < 2000000ll;) {}
+  }
+  __syncthreads();
+  if (warp == P8_WARP_MMA) {
+    tc_fence_after();
+    tmem_dealloc<512>(tmem_base);
+  }
+}
+
+// A unit that is cut behind CTA b's stretch and begins in it: its parts joined in the order of the keys, a warp a row
+constexpr int J8_WARPS = 8;
+__global__ void __launch_bounds__(J8_WARPS * 32) attn8_join_kernel(const __grid_constant__ PromptArgs a, int n_ctas) {
+  extern __shared__ uint32_t prefix_s[];
+  __shared__ uint32_t wsum[J8_WARPS];
+  griddep_launch();
+  griddep_wait();
+  const uint32_t total = lay_out<J8_WARPS * 32>(a, prefix_s, wsum);
+  const uint32_t begin = stretch_begin(total, blockIdx.x, n_ctas), end = stretch_begin(total, blockIdx.x + 1, n_ctas);
+  if (end <= begin || end >= total) return;
+  Walk w(a, prefix_s, end - 1, total);
+  w.find();
+  const int left = w.steps - 1 - w.tile0;                   // steps of the unit behind the stretch
+  if (left == 0 || (uint32_t)w.tile0 > end - 1 - begin) return;
+  int last = blockIdx.x;                                    // CTA with the unit's last step
+  while (stretch_begin(total, last + 1, n_ctas) < end + left) ++last;
+  const int lane = (int)lane_id(), n = last - (int)blockIdx.x + 1, half = w.half();
+  for (int r = blockIdx.y * J8_WARPS + (threadIdx.x >> 5); r < 256; r += gridDim.y * J8_WARPS) {
+    const int tok = (r & 127) / a.G, head = (r & 127) - tok * a.G, in_unit = (r >> 7) * half + tok;
+    if (tok >= half || in_unit >= w.tokens()) continue;
+    // part k: of CTA blockIdx.x + k; its first is that of a unit begun there
+    auto slot = [&](int k) { return ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * 256 + r; };
+    float m = -INFINITY;
+    auto there = [&](int k) {                               // (CTAs without steps leave nothing)
+      return stretch_begin(total, blockIdx.x + k + 1, n_ctas) > stretch_begin(total, blockIdx.x + k, n_ctas);
+    };
+    for (int k = lane; k < n; k += 32)
+      if (there(k)) m = fmaxf(m, a.frag_ml[slot(k) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+      if (!there(k)) continue;
+      const float2 ml = *reinterpret_cast<const float2*>(a.frag_ml + slot(k) * 2);
+      const float4 v = reinterpret_cast<const float4*>(a.frag_o + slot(k) * HEAD_DIM)[lane];
+      const float f = ex2(ml.x - ref);
+      l += ml.y * f;
+      x[0] += v.x * f; x[1] += v.y * f; x[2] += v.z * f; x[3] += v.w * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int row = w.u.sq.q_start + w.i * w.u.tokens + in_unit;
+    *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)(w.kvh * a.G + head) * HEAD_DIM + lane * 4) =
+        make_uint2(cvt2(x[0] * inv, x[1] * inv), cvt2(x[2] * inv, x[3] * inv));
+  }
+}
+
+}  // namespace
+
+bool attn8_prompt_takes(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
+  const int G = n_q / n_kv, TM = 128 / std::max(G, 1);
+  if (TM < 1) return false;
+  const double steps = ((double)T / TM + n_seqs) * ((double)max_kv / P8_KV + 1) * n_kv;
+  return steps < 2e9;
+}
+
+size_t attn8_prompt_workspace(int num_sms) { return (size_t)num_sms * 2 * 256 * (HEAD_DIM + 2) * sizeof(float); }
+
+cudaError_t attn8_prompt_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream) {
+  PromptArgs a;
+  static_cast<Attn8Args&>(a) = args;
+  a.G = a.n_q / a.n_kv;
+  a.TM = 128 / a.G;
+  const size_t smem = sizeof(P8Smem) + 1024 + (size_t)a.n_seqs * 4;
+  static OncePerDevice once;
+  cudaError_t e = once([] {
+    return cudaFuncSetAttribute(attn8_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(P8Smem) + 1024 + TGIS_KV8_MAX_SEQS * 4));
+  });
+  if (e != cudaSuccess) return e;
+  const long long units = (long long)a.n_seqs * ((a.max_q + 2 * a.TM - 1) / (2 * a.TM)) * a.n_kv;
+  const int grid = (int)std::max<long long>(1, std::min<long long>(num_sms, units * ((a.max_kv + P8_KV - 1) / P8_KV)));
+  a.frag_o = reinterpret_cast<float*>(workspace);
+  a.frag_ml = a.frag_o + (size_t)num_sms * 2 * 256 * HEAD_DIM;
+  e = launch_k(attn8_prompt_kernel, dim3(grid), dim3(P8_THREADS), smem, stream, a);
+  if (e != cudaSuccess || grid == 1 || a.max_kv <= P8_KV) return e;   // (units of one step are never cut)
+  return launch_k(attn8_join_kernel, dim3(grid, 4), dim3(J8_WARPS * 32), a.n_seqs * 4, stream, a, grid);
+}
+
+}  // namespace tgis

@@ -16,8 +16,8 @@ PKG = CSRC.parent
 LIB_DIR = PKG / "lib"
 OBJ_DIR = CSRC / "build"
 LIB_PATH = LIB_DIR / "libtgis_engine.so"
-SOURCES = ["gemm_tcgen05.cu", "gemm_pair.cu", "gemm_skinny.cu", "gemm_ref.cu", "gemm_any.cu", "elementwise.cu", "attention.cu", "attention_prefill.cu", "attention_latent.cu", "attention_capped.cu", "attention_sigmoid.cu", "attention_pooled.cu", "cache8.cu", "attention8.cu", "recurrent.cu", "lightning.cu", "moe.cu", "sampler.cu", "lora.cu", "opt.cu", "engine.cu", "test_api.cu"]
-HEADERS = ["ptx.cuh", "launch.cuh", "kernels.h", "cache8.cuh", "../../include/tgis_engine.h", "../../include/tgis_kernels.h", "../../include/tgis_kv8.h"]
+SOURCES = ["gemm_tcgen05.cu", "gemm_pair.cu", "gemm_skinny.cu", "gemm_ref.cu", "gemm_any.cu", "elementwise.cu", "attention.cu", "attention_prefill.cu", "attention_latent.cu", "attention_capped.cu", "attention_sigmoid.cu", "attention_pooled.cu", "cache8.cu", "attention8.cu", "attention8_prompt.cu", "recurrent.cu", "lightning.cu", "moe.cu", "sampler.cu", "lora.cu", "opt.cu", "engine.cu", "test_api.cu"]
+HEADERS = ["ptx.cuh", "launch.cuh", "kernels.h", "cache8.cuh", "tc_attention.cuh", "../../include/tgis_engine.h", "../../include/tgis_kernels.h", "../../include/tgis_kv8.h"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -9,6 +9,7 @@
 #pragma once
 #include <stdint.h>
 
+#include "../../include/tgis_kv8.h"
 #include "kernels.h"
 
 namespace tgis {
@@ -43,6 +44,19 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return f;
 }
 
+constexpr float KV8_LO = 16.f;                                 // lo parts are held times this
+// four numbers as hi parts and as lo parts
+__device__ __forceinline__ void split4(float x0, float x1, float x2, float x3, uint32_t& hi, uint32_t& lo, float lo_mul = KV8_LO) {
+  const uint32_t h0 = e4m3x2(x0, x1), h1 = e4m3x2(x2, x3);
+  const float2 f0 = f16x2_to_f32x2(e4m3x2_to_f16x2(h0)), f1 = f16x2_to_f32x2(e4m3x2_to_f16x2(h1));
+  hi = h0 | h1 << 16;
+  lo = e4m3x2((x0 - f0.x) * lo_mul, (x1 - f0.y) * lo_mul) | e4m3x2((x2 - f1.x) * lo_mul, (x3 - f1.y) * lo_mul) << 16;
+}
+// 2^e that brings a magnitude (the bits of a number >= 0) to [128, 256); no more than 2^126
+__device__ __forceinline__ float power_up(uint32_t bits) {
+  const int ex = min(max((int)(bits >> 23), 8), 254);
+  return __uint_as_float((uint32_t)(261 - ex) << 23);   // 2^(134 - ex)
+}
 // cudaFuncSetAttribute once a device
 struct OncePerDevice {
   static constexpr int MAX = 64;
@@ -82,7 +96,22 @@ struct Attn8Args {
   int64_t ldo;
   int32_t* status;
 };
+// whether a record agrees with what the call said
+__device__ __forceinline__ bool seq_fits(const Attn8Args& a, const AttnSeq& s) {
+  return s.q_len >= 0 && s.q_len <= a.max_q && s.kv_len >= s.q_len && s.kv_len <= a.max_kv && s.q_start >= 0 && s.q_start <= a.T - s.q_len &&
+         s.block_row >= 0 && s.block_row < a.bt_rows && (s.kv_len + KV_BLOCK - 1) / KV_BLOCK <= a.bt_stride && (a.tree == nullptr || s.q_len <= TGIS_KV8_MAX_TREE);
+}
+__device__ __forceinline__ AttnSeq load_seq(const Attn8Args& a, int s) {
+  const int4 v = reinterpret_cast<const int4*>(a.seqs)[s];
+  return AttnSeq{v.x, v.y, v.z, v.w};
+}
+
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv);
+// attention8_prompt.cu: more rows than the warps' own tensor cores take in one pass
+bool attn8_prompt_takes(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv);   // (sizes that its counters hold)
+constexpr int ATTN8_MAX_SMS = 160;             // what workspaces are sized for, so that their size asks no device
+size_t attn8_prompt_workspace(int num_sms);
+cudaError_t attn8_prompt_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream);
 cudaError_t attn8_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream, int* launches = nullptr);
 
 }  // namespace tgis
