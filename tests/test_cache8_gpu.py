@@ -7,6 +7,8 @@ operands (codes times scales); a probability keeps 8 bits (2^-8 at most, as hi +
 A probability times its row's scale s also loses up to half of e4m3's smallest step, 2^-10, of its lo part, 2^-14 where the largest of its 32 tokens
 is brought to 128 at least: 2^-21 of that one, which is at most max s (p <= 1, and the sum of p that all is divided by is 1 at least).  A number c s
 of the sum is off by 2^-21 |c| max s: 2^-21 max s * sum |c| in all, where a row with large weight holds zeros for codes.
+Calls with more than 16 rows a sequence and kv head (max_q * group) hold keys, codes times scales, in f16: each number is off by 2^-12 of itself, a
+score by d = 2^-12 |scale| sum |q k| at most, a weight by a factor between exp(-2 d) and exp(2 d) for the largest d of the row.
 """
 import math
 import random
@@ -69,12 +71,12 @@ def filled(n_pages, n_kv, seed, spread=0.5):
 
 
 def reference(cache, q, seqs, bt, scale, tree=None):
-    """(out, sum p |v|) in 64 bits; rows that see nothing are zeros, rows without a sequence NaN."""
+    """(out, sum p |v|, largest |scale| sum |q k|) in 64 bits; rows that see nothing are zeros, rows without a sequence NaN."""
     k, v = pages_natural(cache)
     T, n_q = q.shape[0], q.shape[1] // D
     G = n_q // cache.n_kv
     out = torch.full((T, n_q, D), math.nan, dtype=torch.float64, device="cuda")
-    size = out.clone()
+    size, most = out.clone(), torch.zeros(T, n_q, 1, dtype=torch.float64, device="cuda")
     for start, new, all_, row in seqs:
         for i in range(new):
             old = all_ - new
@@ -89,7 +91,8 @@ def reference(cache, q, seqs, bt, scale, tree=None):
             p = torch.softmax(torch.einsum("hgd,khd->hgk", qq, kk) * scale, dim=-1)
             out[start + i] = torch.einsum("hgk,khd->hgd", p, vv).reshape(n_q, D)
             size[start + i] = torch.einsum("hgk,khd->hgd", p, vv.abs()).reshape(n_q, D)
-    return out.view(T, -1), size.view(T, -1)
+            most[start + i] = (torch.einsum("hgd,khd->hgk", qq.abs(), kk.abs()).amax(-1) * abs(scale)).reshape(n_q, 1)
+    return out.view(T, -1), size.view(T, -1), most.expand(T, n_q, D).reshape(T, -1)
 
 
 def floor_of(cache, seqs, bt, T, n_q):
@@ -132,12 +135,13 @@ def attend_case(lengths, n_q, n_kv, seed, tree=None, scale=D ** -0.5, q_size=1.0
     max_q, max_kv = max(s[1] for s in seqs) + (0 if tree else max_more), max(s[2] for s in seqs) + max_more
     got = cache.attend(q, ints(seqs), ints(bt), scale, max_q, max_kv, out=out, tree=t)
     cache.check()
-    want, size = reference(cache, q, seqs, bt, scale, words)
+    want, size, most = reference(cache, q, seqs, bt, scale, words)
+    keys = torch.expm1(2 * 2.0 ** -12 * most) if max_q * (n_q // n_kv) > 16 else torch.zeros_like(most)
     named = ~want.isnan().all(dim=1)
     assert bool((got[~named] == 7.0).all()), "rows that no sequence names were touched"
     off = (got[named].double() - want[named]).abs()
     # (2^-133: half a step of the smallest bf16 numbers)
-    may = TOL * size[named] + floor_of(cache, seqs, bt, T, n_q)[named] + 2.0 ** -133
+    may = (TOL + keys[named]) * size[named] + floor_of(cache, seqs, bt, T, n_q)[named] + 2.0 ** -133
     assert bool((off <= may).all()), f"off by {(off / may).max().item():.4g} of what it may"
     return cache, q, seqs, bt, got
 
@@ -508,8 +512,8 @@ def test_a_conversation_over_the_cache():
     whole.check(), steps.check()
     assert torch.equal(whole.pages.view(6, n_kv, -1)[[3, 1, 4, 0]], steps.pages.view(6, n_kv, -1)[[3, 1, 4, 0]])
     # other splits and orders of the same sums: each within TOL of exact
-    _, size = reference(whole, q_all(whole, qkv, cs, total), [[0, total, total, 0]], bt.tolist(), scale)
-    assert bool(((got.double() - want.double()).abs() <= 2 * TOL * size + 1e-6).all())
+    _, size, most = reference(whole, q_all(whole, qkv, cs, total), [[0, total, total, 0]], bt.tolist(), scale)
+    assert bool(((got.double() - want.double()).abs() <= 2 * (TOL + torch.expm1(2 * 2.0 ** -12 * most)) * size + 1e-6).all())
 
 
 def q_all(cache, qkv, cs, total):

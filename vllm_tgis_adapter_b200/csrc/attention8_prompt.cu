@@ -8,13 +8,14 @@
 // all keep every SM busy to the end, and the workspace is two units a CTA whatever the lengths are.  Lengths and pages are read on
 // the device.
 //
-//   S = Q K^T  e4m3 x e4m3 -> fp32 (kind::f8f6f4): K as the cache holds it (a block is 32 rows of the 128-byte swizzled form), a query row as
-//              hi + lo, two e4m3 numbers that are exact but for the smallest entries (cache8.cuh split4; lo is not scaled here: both
-//              products go to one accumulator, and numbers below 2^-18 of the row's largest are cut);
-//   P V        f16 x f16 -> fp32 (kind::f16): two warps widen V to f16 (exact) into the unswizzled K-major form; a probability times
-//              its row's scale is one f16 number of 11 bits.  It is held times 2^7 / r, r the power of two at or above the scales so far, and the
-//              reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
-//              most) and nothing above 2^-31 of the largest is lost.
+// Both products are f16 x f16 -> fp32 (kind::f16).  Four warps widen K and V as they multiply them by their rows' scales (a code has 4 bits,
+// so a product rounded to f16's 11 is off by 2^-12; a key's scale is applied as two f16 numbers, for an error of the whole row's
+// would be one of its score); both are held relative to a power of two at or above the scales, the tile's for K, that of the keys so far
+// for V.  A query row is exact in f16 but for numbers 2^-22 of its largest and below.  A probability is one f16 number of 11 bits,
+// held times 2^7; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
+// most) and nothing above 2^-31 of the largest is lost.  (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the
+// products cost the same and every score takes a multiplication by its key's scale, every probability one by its value's:
+// 361 against XXX us for 1859 tokens behind 6144, 32 / 8 heads.)
 // Scores and probabilities of a row are one thread's; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are written in that
 // order.  A row with a NaN for its scale gets zeros here and a bit; who sees it gets NaN for its sum.
 //
@@ -30,42 +31,39 @@
 namespace tgis {
 namespace {
 
-constexpr int P8_THREADS = 384;                             // warps 0..3, 4..7: softmax of an accumulator; copies, MMAs, two that widen V
-constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 10;
-constexpr int P8_REGS_SOFTMAX = 208, P8_REGS_OTHER = 88;    // 256 x 208 + 128 x 88 = 384 x 168, what the launch gives every thread
+constexpr int P8_THREADS = 512;                             // warps 0..3, 4..7: softmax of an accumulator; 8 copies, 9 MMAs, 12..15 widen K and V
+constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 12, P8_WIDEN_WARPS = 4;
+constexpr int P8_REGS_SOFTMAX = 168, P8_REGS_OTHER = 88;    // 256 x 168 + 256 x 88 = 512 x 128, what the launch gives every thread
 constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
-constexpr int P8_STAGES = 2;
-constexpr int P8_TILE8 = P8_KV * HEAD_DIM;                  // bytes of a tile's codes; of one accumulator's hi (or lo) parts of Q
-constexpr int P8_SCALES = P8_BLOCKS * 2 * KV_BLOCK * 4;     // as they lie in the cache, block by block: K scales | V scales
+constexpr int P8_STAGES = 2;                                // tiles as they come from the cache
+constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile of K or V, of one accumulator's Q, in f16
 constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
-constexpr float P8_HELD = 128.f;                            // probabilities are held times this
+constexpr float P8_HELD = 7.f;                              // exp2 domain: probabilities and their sums are held times 2^7
+constexpr float P8_V_TOP = 64.f, P8_K_TOP = 16.f;           // largest scale that a code (448 at most) is multiplied by
+constexpr uint32_t P8_COST = 2;                             // what the beginning and the end of a unit take, in steps
 
-struct TileScales {
-  float k[P8_KV];              // over k_unit; 0 where there is none
-  float v[P8_KV];              // times P8_HELD / r
+// What the softmax has to know of a tile, beside its scores
+struct TileNotes {
   uint32_t poison[P8_BLOCKS];  // tokens whose key or value row is not a number
   uint32_t absent;             // blocks whose page does not exist (bits)
-  float unit;                  // r / P8_HELD
-  float k_unit;                // power of two at or above the tile's key scales: products of codes times scales stay in range
+  float k_unit, v_unit;        // what a number of K, of V is in units of
   uint32_t pad;
 };
 struct P8Smem {
-  uint8_t q[2][2][P8_TILE8];   // accumulator, hi | lo
-  uint8_t k[P8_STAGES][P8_TILE8];
-  uint8_t v16[P8_STAGES][2 * P8_TILE8];
-  uint8_t v8[P8_STAGES][P8_TILE8];
-  uint8_t raw[P8_STAGES][P8_SCALES];
-  TileScales sc[P8_STAGES];
-  uint64_t q_full[2], k_full[P8_STAGES], k_empty[P8_STAGES], v8_full[P8_STAGES], v8_empty[P8_STAGES], v_full[P8_STAGES], v_empty[P8_STAGES], s_full[2],
+  // unswizzled K-major operands: [8 numbers along k][128 rows][8]
+  uint8_t q[2][P8_TILE], k[P8_TILE], v[P8_TILE];
+  uint8_t raw[P8_STAGES][P8_BLOCKS * KV8_PAGE];
+  uint16_t v_mul[P8_WIDEN_WARPS][P8_KV];   // scales of the value rows at their places, a copy for every warp that multiplies by them
+  TileNotes notes[2];          // of even and odd tiles
+  uint64_t raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], k_full, k_empty, v_full, v_empty, s_full[2],
       p_full[2], o_full[2];
-  uint32_t absent[P8_STAGES];  // by the copying warp, with v8
+  uint32_t absent[P8_STAGES];  // by the copying warp
   uint32_t tmem_base;
   int gave_up;
   uint32_t wsum[P8_THREADS / 32];
-  uint32_t total;
   uint32_t prefix[1];          // steps ahead of each sequence
 };
-static_assert(sizeof(TileScales) % 16 == 0 && offsetof(P8Smem, sc) % 16 == 0 && offsetof(P8Smem, q_full) % 8 == 0, "");
+static_assert(offsetof(P8Smem, raw) % 128 == 0 && KV8_PAGE % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, raw_full) % 8 == 0, "");
 
 struct PromptArgs : Attn8Args {
   int G, TM;
@@ -101,7 +99,7 @@ __device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefi
     uint32_t n = 0;
     if (s < a.n_seqs) {
       const SeqUnits u = units_of(a, s);
-      for (int i = 0; i < u.n_units; ++i) n += (uint32_t)steps_of(a, u, i);
+      for (int i = 0; i < u.n_units; ++i) n += P8_COST + (uint32_t)steps_of(a, u, i);
       n *= (uint32_t)a.n_kv;
     }
     uint32_t sum = n;
@@ -124,7 +122,10 @@ __device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefi
 }
 __device__ __forceinline__ uint32_t stretch_begin(uint32_t total, uint32_t cta, uint32_t n) { return (uint32_t)((uint64_t)total * cta / n); }
 
-// One unit's steps [tile0, tile1) of a CTA's stretch after the other
+__device__ __forceinline__ uint32_t cta_of(uint32_t total, uint32_t at, uint32_t n) { return (uint32_t)((((uint64_t)at + 1) * n - 1) / total); }
+
+// One unit's steps [tile0, tile1) of a CTA's stretch after the other.  A unit's first P8_COST places in the row of steps stand for what its
+// beginning and end take: nothing is done there.
 struct Walk {
   const PromptArgs& a;
   const uint32_t* prefix;
@@ -132,7 +133,7 @@ struct Walk {
   int s = -1, i = 0, kvh = 0, steps = 0, tile0 = 0, tile1 = 0;
   SeqUnits u;
   __device__ Walk(const PromptArgs& a_, const uint32_t* p, uint32_t begin, uint32_t end_) : a(a_), prefix(p), at(begin), end(end_) {}
-  __device__ void find() {     // the unit that step `at` belongs to
+  __device__ uint32_t find() {     // the unit that place `at` belongs to; `at` less its first place
     int lo = 0, hi = a.n_seqs;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -144,19 +145,20 @@ struct Walk {
     uint32_t left = at - prefix[s];
     for (i = 0;; ++i) {
       steps = steps_of(a, u, i);
-      if (left < (uint32_t)(steps * a.n_kv) || i >= u.n_units - 1) break;
-      left -= (uint32_t)(steps * a.n_kv);
+      const uint32_t all = (steps + P8_COST) * a.n_kv;
+      if (left < all || i >= u.n_units - 1) break;
+      left -= all;
     }
-    kvh = (int)(left / (uint32_t)steps);
-    tile0 = (int)(left - (uint32_t)(kvh * steps));
+    kvh = (int)(left / (steps + P8_COST));
+    return left - kvh * (steps + P8_COST);
   }
   __device__ bool next() {
-    if (at >= end) return false;
-    if (s < 0) {
-      find();
-    } else {                   // the stretch goes on: the unit before ended
-      tile0 = 0;
-      if (++kvh == a.n_kv) {
+    do {
+      if (at >= end) return false;
+      uint32_t place = 0;
+      if (s < 0) {
+        place = find();
+      } else if (++kvh == a.n_kv) {   // the stretch goes on: the unit before ended
         kvh = 0;
         if (++i == u.n_units) {
           do u = units_of(a, ++s);
@@ -165,9 +167,11 @@ struct Walk {
         }
         steps = steps_of(a, u, i);
       }
-    }
-    tile1 = min(steps, tile0 + (int)(end - at));
-    at += (uint32_t)(tile1 - tile0);
+      const uint32_t stop = min(steps + P8_COST, place + (end - at));
+      at += stop - place;
+      tile0 = place > P8_COST ? (int)(place - P8_COST) : 0;
+      tile1 = stop > P8_COST ? (int)(stop - P8_COST) : 0;
+    } while (tile1 <= tile0);
     return true;
   }
   __device__ int keys() const { return keys_of(a, u, i); }
@@ -178,26 +182,25 @@ struct Walk {
   __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys() + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
 };
 
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// C fp32, A and B e4m3 (kind::f8f6f4) or f16 (kind::f16): both formats are number 0; K-major operands
+// C fp32, A and B f16, K-major
 __device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
-__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-  return d;
-}
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t hmul2(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t x, uint32_t y, uint32_t z) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
+  return r;
+}
+// power of two at or above a number > 0 (its bits)
+__device__ __forceinline__ float power_above(uint32_t bits) { return __uint_as_float((bits + 0x7fffffu) & 0x7f800000u); }
 
 __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __grid_constant__ PromptArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -207,18 +210,19 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sm.q_full[i], 4);
+        mbar_init(&sm.note_full[i], P8_WIDEN_WARPS);
         mbar_init(&sm.s_full[i], 1);
         mbar_init(&sm.p_full[i], 4);
         mbar_init(&sm.o_full[i], 1);
       }
       for (int i = 0; i < P8_STAGES; ++i) {
-        mbar_init(&sm.k_full[i], 1);
-        mbar_init(&sm.k_empty[i], 1);
-        mbar_init(&sm.v8_full[i], 1);
-        mbar_init(&sm.v8_empty[i], 2);
-        mbar_init(&sm.v_full[i], 2);
-        mbar_init(&sm.v_empty[i], 1);
+        mbar_init(&sm.raw_full[i], 1);
+        mbar_init(&sm.raw_empty[i], P8_WIDEN_WARPS);
       }
+      mbar_init(&sm.k_full, P8_WIDEN_WARPS);
+      mbar_init(&sm.k_empty, 1);
+      mbar_init(&sm.v_full, P8_WIDEN_WARPS);
+      mbar_init(&sm.v_empty, 1);
       sm.gave_up = 0;
       fence_barrier_init();
     }
@@ -257,42 +261,31 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           if (absent != 0 && lane == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_BAD_PAGE);
           // (an absent page's keys are not seen; some page's codes stand in for it, for they are numbers)
           const uint8_t* src = a.pages + ((size_t)(there ? page : 0) * a.n_kv + w.kvh) * KV8_PAGE;
-          const int b = lane & 3, kind = lane >> 2;   // lanes 0..3 K codes, 4..7 V codes, 8..11 scales
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty[st], ph));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sm.k_full[st], nb * KV8_CODES);
-          __syncwarp();
-          if (kind == 0 && b < nb) bulk_load_1d(sm.k[st] + b * KV8_CODES, src, KV8_CODES, &sm.k_full[st]);
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v8_empty[st], ph));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_empty[st], ph));
           if (!ok) break;
           if (lane == 0) {
             sm.absent[st] = absent;
-            mbar_arrive_expect_tx(&sm.v8_full[st], nb * (KV8_CODES + 2 * KV_BLOCK * 4));
+            mbar_arrive_expect_tx(&sm.raw_full[st], nb * KV8_PAGE);
           }
           __syncwarp();
-          if (kind == 1 && b < nb) bulk_load_1d(sm.v8[st] + b * KV8_CODES, src + KV8_CODES, KV8_CODES, &sm.v8_full[st]);
-          if (kind == 2 && b < nb) bulk_load_1d(sm.raw[st] + b * (2 * KV_BLOCK * 4), src + KV8_K_SCALES, 2 * KV_BLOCK * 4, &sm.v8_full[st]);
+          if (lane < nb) bulk_load_1d(sm.raw[st] + lane * KV8_PAGE, src, KV8_PAGE, &sm.raw_full[st]);
           if (++st == P8_STAGES) st = 0, ph ^= 1;
           if (j + 1 < w.tile1) page = page_of(j + 1);
         }
       }
     } else if (warp == P8_WARP_MMA) {
       // ===================== MMAs =====================
-      int kst = 0, vst = 0;
       uint32_t kph = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
+      auto operand = [](const uint8_t* p, int ks) { return smem_desc(smem_u32(p) + ks * 2 * (128 * 16), 128 * 16, 128, 0); };   // 16 numbers along k
       auto scores = [&](int g, int nb) {
-        const uint32_t idesc = idesc_of(128, nb * KV_BLOCK), k = smem_u32(sm.k[kst]);
+        const uint32_t idesc = idesc_of(128, nb * KV_BLOCK);
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int ks = 0; ks < HEAD_DIM / 32; ++ks)
-            mma_f8(tmem_base + g * 128, make_smem_desc_sw128(smem_u32(sm.q[g][part]) + ks * 32), make_smem_desc_sw128(k + ks * 32), idesc, part + ks > 0);
+        for (int ks = 0; ks < HEAD_DIM / 16; ++ks) tc_mma_f16(tmem_base + g * 128, operand(sm.q[g], ks), operand(sm.k, ks), idesc, ks > 0);
         tc_commit(&sm.s_full[g]);
       };
       auto values = [&](int g, int nb, bool first) {
-        const uint32_t idesc = idesc_of(128, HEAD_DIM), v = smem_u32(sm.v16[vst]);
-        for (int ks = 0; ks < 2 * nb; ++ks)   // 16 tokens: two core matrices along k
-          mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + ks * 8, smem_desc(v + ks * 2 * (HEAD_DIM * 16), HEAD_DIM * 16, 128, 0), idesc, !(first && ks == 0));
+        const uint32_t idesc = idesc_of(128, HEAD_DIM);
+        for (int ks = 0; ks < 2 * nb; ++ks) mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + ks * 8, operand(sm.v, ks), idesc, !(first && ks == 0));
       };
       while (ok && w.next()) {
         const int groups = w.two() ? 2 : 1;
@@ -300,96 +293,138 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.q_full[g], qph[g]));
           qph[g] ^= 1;
         }
-        ok = ok && __all_sync(0xffffffffu, bounded_wait(&sm.k_full[kst], kph));
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(&sm.k_full, kph));
         if (!ok) break;
+        kph ^= 1;
         tc_fence_after();
         if (elect_one()) {
           for (int g = 0; g < groups; ++g) scores(g, w.blocks(w.tile0));
-          tc_commit(&sm.k_empty[kst]);
+          tc_commit(&sm.k_empty);
         }
         __syncwarp();
-        if (++kst == P8_STAGES) kst = 0, kph ^= 1;
         for (int j = w.tile0; j < w.tile1 && ok; ++j) {
           const bool more = j + 1 < w.tile1;
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full[vst], vph));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full, vph));
+          vph ^= 1;
           for (int g = 0; g < groups && ok; ++g) {
-            ok = __all_sync(0xffffffffu, bounded_wait(&sm.p_full[g], pph[g]) && (g > 0 || !more || bounded_wait(&sm.k_full[kst], kph)));
+            ok = __all_sync(0xffffffffu, bounded_wait(&sm.p_full[g], pph[g]));
             if (!ok) break;
             pph[g] ^= 1;
             tc_fence_after();
             if (elect_one()) {
               values(g, w.blocks(j), j == w.tile0);
-              if (more) scores(g, w.blocks(j + 1));
-              if (g == groups - 1) {
-                tc_commit(&sm.v_empty[vst]);
-                if (more) tc_commit(&sm.k_empty[kst]);
-              }
+              if (g == groups - 1) tc_commit(&sm.v_empty);
               if (!more) tc_commit(&sm.o_full[g]);
             }
             __syncwarp();
+            if (!more) continue;
+            if (g == 0) {
+              ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_full, kph));
+              kph ^= 1;
+              if (!ok) break;
+              tc_fence_after();
+            }
+            if (elect_one()) {
+              scores(g, w.blocks(j + 1));
+              if (g == groups - 1) tc_commit(&sm.k_empty);
+            }
+            __syncwarp();
           }
-          if (++vst == P8_STAGES) vst = 0, vph ^= 1;
-          if (more && ++kst == P8_STAGES) kst = 0, kph ^= 1;
         }
       }
-    } else {
-      // ===================== V to f16, scales =====================
-      const int half = warp - P8_WARP_WIDEN;
-      int st = 0;
+    } else if (warp >= P8_WARP_WIDEN) {
+      // ===================== K and V to f16 =====================
+      const int mine = warp - P8_WARP_WIDEN, part = mine * 32 + lane;   // block; token of the tile, dim
+      int st = 0, odd_tile = 0;
       uint32_t full = 0, empty = 1;
       while (ok && w.next()) {
         float r = 0.f;
         for (int j = w.tile0; j < w.tile1; ++j) {
           const int nb = w.blocks(j);
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v8_full[st], full) && bounded_wait(&sm.v_empty[st], empty));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_full[st], full));
           if (!ok) break;
-          // sixteen codes (one dim, half a block) -> two rows of eight f16 numbers
-          for (int c = half * 32 + lane; c < nb * 2 * HEAD_DIM; c += 64) {
-            const uint4 x = *reinterpret_cast<const uint4*>(sm.v8[st] + c * 16);
-            const int dim = c & (HEAD_DIM - 1), k = c / HEAD_DIM;
-            uint8_t* to = sm.v16[st] + k * 2 * (HEAD_DIM * 16) + dim * 16;
-            *reinterpret_cast<uint4*>(to) = make_uint4(e4m3x2_to_f16x2(x.x & 0xffffu), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y & 0xffffu), e4m3x2_to_f16x2(x.y >> 16));
-            *reinterpret_cast<uint4*>(to + HEAD_DIM * 16) = make_uint4(e4m3x2_to_f16x2(x.z & 0xffffu), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w & 0xffffu), e4m3x2_to_f16x2(x.w >> 16));
+          const uint8_t* raw = sm.raw[st];
+          // ---- scales: every warp looks at all of them
+          const uint32_t absent = sm.absent[st];
+          float top_k = 0.f, top_v = 0.f, my_k = 0.f, vs[P8_BLOCKS];
+          uint32_t my_odd = 0;
+#pragma unroll
+          for (int b = 0; b < P8_BLOCKS; ++b) {
+            const float* sc = reinterpret_cast<const float*>(raw + b * KV8_PAGE + KV8_K_SCALES);
+            const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < w.u.sq.kv_len;
+            float k = there ? sc[lane] : 0.f;
+            vs[b] = there ? sc[KV_BLOCK + lane] : 0.f;
+            const bool fine = k < INFINITY && vs[b] < INFINITY;
+            if (!fine) k = vs[b] = 0.f;
+            const uint32_t odd = __ballot_sync(0xffffffffu, !fine);
+            top_k = fmaxf(top_k, k);
+            top_v = fmaxf(top_v, vs[b]);
+            if (b == mine) my_k = k, my_odd = odd;
           }
-          if (half == 0) {
-            const uint32_t absent = sm.absent[st];
-            TileScales& t = sm.sc[st];
-            float ks[P8_BLOCKS], vs[P8_BLOCKS], top = 0.f, top_k = 0.f;
-            uint32_t odd = 0;
+          const float k_top = fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))), 0x1p-118f);
+          r = fmaxf(r, fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))), 0x1p-118f));
+          uint16_t* v_mul = sm.v_mul[mine];
 #pragma unroll
-            for (int b = 0; b < P8_BLOCKS; ++b) {
-              const float* raw = reinterpret_cast<const float*>(sm.raw[st]) + b * 2 * KV_BLOCK;
-              const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < w.u.sq.kv_len;
-              ks[b] = there ? raw[lane] : 0.f;
-              vs[b] = there ? raw[KV_BLOCK + lane] : 0.f;
-              const bool fine = ks[b] < INFINITY && vs[b] < INFINITY;
-              if (!fine) ks[b] = vs[b] = 0.f;
-              odd = __ballot_sync(0xffffffffu, !fine);
-              if (lane == 0) t.poison[b] = odd;
-              top = fmaxf(top, vs[b]);
-              top_k = fmaxf(top_k, ks[b]);
-            }
-            const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top)), most_k = __reduce_max_sync(0xffffffffu, __float_as_uint(top_k));
-            r = fmaxf(r, fmaxf(__uint_as_float((most + 0x7fffffu) & 0x7f800000u), 0x1p-118f));
-            const float k_unit = fmaxf(__uint_as_float((most_k + 0x7fffffu) & 0x7f800000u), 0x1p-126f);
-#pragma unroll
-            for (int b = 0; b < P8_BLOCKS; ++b) {
-              t.k[b * KV_BLOCK + lane] = ks[b] * (1.f / k_unit);
-              t.v[b * KV_BLOCK + lane] = vs[b] * (P8_HELD / r);
-            }
-            if (lane == 0) {
+          for (int b = 0; b < P8_BLOCKS; ++b) v_mul[b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * (P8_V_TOP / r), 0.f);
+          // ---- K: this thread's token, sixteen dims at a time -> two rows of eight numbers
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty, empty));
+          if (!ok) break;
+          // (the scores of the tile before are done, so who reads the notes of the one before that has finished)
+          TileNotes& t = sm.notes[odd_tile];
+          if (lane == 0) {
+            t.poison[mine] = my_odd;
+            if (mine == 0) {
               t.absent = absent;
-              t.unit = r / P8_HELD;
-              t.k_unit = k_unit;
+              t.k_unit = k_top / P8_K_TOP;
+              t.v_unit = r / P8_V_TOP;
+            }
+          }
+          if (mine < nb) {
+            const float k = my_k * (P8_K_TOP / k_top);
+            const uint32_t h1 = f16x2(k, k), lo = f16x2(k - f16x2_to_f32x2(h1).x, k - f16x2_to_f32x2(h1).x);
+            const uint8_t* from = raw + mine * KV8_PAGE + lane * HEAD_DIM;
+#pragma unroll
+            for (int c = 0; c < HEAD_DIM / 16; ++c) {
+              const uint4 x = *reinterpret_cast<const uint4*>(from + ((c ^ (lane & 7)) << 4));
+              const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+              uint32_t o[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t h = e4m3x2_to_f16x2(i & 1 ? in[i >> 1] >> 16 : in[i >> 1] & 0xffffu);
+                o[i] = hfma2(h, h1, hmul2(h, lo));
+              }
+              *reinterpret_cast<uint4*>(sm.k + 2 * c * 2048 + part * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(sm.k + (2 * c + 1) * 2048 + part * 16) = make_uint4(o[4], o[5], o[6], o[7]);
             }
           }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&sm.v_full[st]);
-            mbar_arrive(&sm.v8_empty[st]);
+            mbar_arrive(&sm.k_full);
+            mbar_arrive(&sm.note_full[odd_tile]);
           }
-          if (++st == P8_STAGES) st = 0, full ^= 1, empty ^= 1;
+          // ---- V: this thread's dim, sixteen tokens at a time
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_empty, empty));
+          if (!ok) break;
+#pragma unroll 2
+          for (int h = 0; h < 2 * nb; ++h) {
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + (h >> 1) * KV8_PAGE + KV8_CODES + (h & 1) * (KV8_CODES / 2) + part * 16);
+            const uint4 m0 = *reinterpret_cast<const uint4*>(v_mul + h * 16), m1 = *reinterpret_cast<const uint4*>(v_mul + h * 16 + 8);
+            uint8_t* to = sm.v + h * 2 * 2048 + part * 16;
+            *reinterpret_cast<uint4*>(to) = make_uint4(hmul2(e4m3x2_to_f16x2(x.x & 0xffffu), m0.x), hmul2(e4m3x2_to_f16x2(x.x >> 16), m0.y),
+                                                       hmul2(e4m3x2_to_f16x2(x.y & 0xffffu), m0.z), hmul2(e4m3x2_to_f16x2(x.y >> 16), m0.w));
+            *reinterpret_cast<uint4*>(to + 2048) = make_uint4(hmul2(e4m3x2_to_f16x2(x.z & 0xffffu), m1.x), hmul2(e4m3x2_to_f16x2(x.z >> 16), m1.y),
+                                                              hmul2(e4m3x2_to_f16x2(x.w & 0xffffu), m1.z), hmul2(e4m3x2_to_f16x2(x.w >> 16), m1.w));
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&sm.v_full);
+            mbar_arrive(&sm.raw_empty[st]);
+          }
+          if (++st == P8_STAGES) st = 0, full ^= 1;
+          empty ^= 1;
+          odd_tile ^= 1;
         }
       }
     }
@@ -400,12 +435,10 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     const int r = (warp & 3) * 32 + lane, tok = r / a.G, head = r - tok * a.G;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem_base + g * 128 + lanes, o_t = tmem_base + 256 + g * 128 + lanes;
-    uint32_t sph = 0, oph = 0, vph = 0;
-    int vst = 0;
+    uint32_t sph = 0, oph = 0, tile = 0;   // tile: of the CTA
     while (ok && w.next()) {
-      if (g == 1 && !w.two()) {   // (its stages pass)
-        for (int j = w.tile0; j < w.tile1; ++j)
-          if (++vst == P8_STAGES) vst = 0, vph ^= 1;
+      if (g == 1 && !w.two()) {
+        tile += (uint32_t)(w.tile1 - w.tile0);
         continue;
       }
       const int in_unit = g * w.half() + tok;
@@ -416,7 +449,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       unsigned long long word = 0;
       if (!mine) lim = 0x7fffffff;
       else if (a.tree != nullptr) lim = before - 1, word = a.tree[row] & ~0ull >> (TGIS_KV8_MAX_TREE - w.u.sq.q_len);
-      // ---- the row of Q, twice
+      // ---- the row of Q, its largest number at 128 to 256
       float qm;
       {
         uint4 x[HEAD_DIM / 8];
@@ -432,16 +465,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / up;   // (hidden scores are -inf before they are scaled)
         if (a.scale < 0.f) up = -up;
 #pragma unroll
-        for (int c = 0; c < HEAD_DIM / 16; ++c) {
-          const uint32_t v[8] = {x[2 * c].x, x[2 * c].y, x[2 * c].z, x[2 * c].w, x[2 * c + 1].x, x[2 * c + 1].y, x[2 * c + 1].z, x[2 * c + 1].w};
-          uint32_t hi[4], lo[4];
+        for (int c = 0; c < HEAD_DIM / 8; ++c) {
+          const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+          uint32_t h[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            split4(__uint_as_float(v[2 * i] << 16) * up, __uint_as_float(v[2 * i] & 0xffff0000u) * up, __uint_as_float(v[2 * i + 1] << 16) * up,
-                   __uint_as_float(v[2 * i + 1] & 0xffff0000u) * up, hi[i], lo[i], 1.f);
-          const int at = r * HEAD_DIM + ((c ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(sm.q[g][0] + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(sm.q[g][1] + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          for (int i = 0; i < 4; ++i) h[i] = f16x2(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+          *reinterpret_cast<uint4*>(sm.q[g] + c * 2048 + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
       fence_proxy_async();
@@ -450,11 +479,13 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       float m = 0.f, l = 0.f, unit = 0.f;
       for (int j = w.tile0; j < w.tile1; ++j) {
         const int nb = w.blocks(j);
-        ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full[vst], vph) && bounded_wait(&sm.s_full[g], sph));
+        // (in this order: with its scores there, a tile's notes are, and the next tile's in their place are not)
+        ok = __all_sync(0xffffffffu, bounded_wait(&sm.s_full[g], sph) && bounded_wait(&sm.note_full[tile & 1], tile >> 1 & 1));
         if (!ok) break;
         sph ^= 1;
         tc_fence_after();
-        const TileScales& sc = sm.sc[vst];
+        const TileNotes& sc = sm.notes[tile & 1];
+        ++tile;
         const int seen = lim - j * P8_KV;                   // last column seen (of the keys before a draft)
         const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || sc.absent != 0);
         uint32_t vis[P8_BLOCKS];                            // columns that the row sees, where some are hidden
@@ -467,46 +498,33 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           }
           if (sc.absent >> c & 1) vis[c] = 0;
         }
-        uint32_t s[P8_KV];
+        // the scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill)
+        uint32_t s[2][KV_BLOCK];
+        float mx[2] = {-INFINITY, -INFINITY};
+        tmem_ld_x32(s_t, s[0]);
 #pragma unroll
         for (int c = 0; c < P8_BLOCKS; ++c) {
           if (c >= nb) break;
-          tmem_ld_x32(s_t + c * 32, s + c * 32);
-        }
-        tmem_ld_wait();
-        float mx[P8_BLOCKS] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
-          if (c >= nb) break;
-          const uint64_t* ks = reinterpret_cast<const uint64_t*>(sc.k + c * 32);
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float x, y;
-            unpack2(mul2(pack2(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])), ks[i / 2]), x, y);
-            s[c * 32 + i] = __float_as_uint(x);
-            s[c * 32 + i + 1] = __float_as_uint(y);
-          }
-        }
-        if (mask) {
-#pragma unroll
-          for (int c = 0; c < P8_BLOCKS; ++c) {
-            if (c >= nb) break;
+          tmem_ld_wait();
+          if (c + 1 < P8_BLOCKS && c + 1 < nb) tmem_ld_x32(s_t + (c + 1) * 32, s[(c + 1) & 1]);
+          uint32_t (&x)[KV_BLOCK] = s[c & 1];
+          if (mask) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(vis[c] >> i & 1)) s[c * 32 + i] = __float_as_uint(-INFINITY);
+              if (!(vis[c] >> i & 1)) x[i] = __float_as_uint(-INFINITY);
           }
-        }
 #pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
-          if (c >= nb) break;
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[c] = fmaxf(mx[c], fmaxf(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])));
+          for (int i = 0; i < 32; i += 4) {
+            mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+            mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+          }
           if ((sc.poison[c] & vis[c]) != 0) l = __uint_as_float(0x7fc00000u);
         }
+        tmem_ld_x32(s_t, s[0]);
         const float qk = qm * sc.k_unit;
         uint64_t qm2 = pack2(qk, qk);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qk;
-        const float unit_now = sc.unit;
+        const float top = fmaxf(mx[0], mx[1]) * qk;
+        const float unit_now = sc.v_unit;
         if (j == w.tile0) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + P8_SLACK) || unit_now != unit) {
@@ -527,38 +545,45 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         }
         unit = unit_now;
         const float ref = m == -INFINITY ? 0.f : m;   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
-        const uint64_t neg_m = pack2(-ref, -ref);
-        if (fabsf(ref) > 0x1p20f) {
-          // an exact product less a rounded one is no longer below a step of the exponent: round the scores first, as their maximum was
-#pragma unroll
-          for (int i = 0; i < P8_KV; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
-          qm2 = pack2(1.f, 1.f);
-        }
+        const uint64_t neg_m = pack2(P8_HELD - ref, P8_HELD - ref);
+        // an exact product less a rounded one may be far from zero where both are large: such scores are rounded first, as their maximum was
+        const bool large = fabsf(ref) > 0x1p20f;
+        if (large) qm2 = pack2(1.f, 1.f);
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-        for (int c = 0; c < 2 * P8_BLOCKS; ++c) {
-          if (c >= 2 * nb) break;
-          const uint64_t* vs = reinterpret_cast<const uint64_t*>(sc.v + c * 16);
-          uint32_t p[8];
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          if (c >= nb) break;
+          tmem_ld_wait();
+          if (c + 1 < P8_BLOCKS && c + 1 < nb) tmem_ld_x32(s_t + (c + 1) * 32, s[(c + 1) & 1]);
+          uint32_t (&v)[KV_BLOCK] = s[c & 1];
+          if (mask) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int pair = 4 * (i & 1) + (i >> 1);  // places 2 i, 2 i + 1 of the half (cache8.cuh v8_place)
-            const int col = c * 16 + 2 * pair;
+            for (int i = 0; i < 32; ++i)
+              if (!(vis[c] >> i & 1)) v[i] = __float_as_uint(-INFINITY);
+          }
+          if (large) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * qk);
+          }
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            // places 2 i, 2 i + 1 of the block (cache8.cuh v8_place)
+            const int col = (i >> 3) * 16 + 2 * (4 * (i & 1) + (i >> 1 & 3));
             float x, y;
-            unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
-            const uint64_t e = pack2(ex2(x), ex2(y));
-            if (i & 1) sum1 = add2(sum1, e);
-            else sum0 = add2(sum0, e);
-            unpack2(mul2(e, vs[pair]), x, y);
+            unpack2(fma2(pack2(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), qm2, neg_m), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            if (i & 1) sum1 = add2(sum1, pack2(x, y));
+            else sum0 = add2(sum0, pack2(x, y));
             p[i] = f16x2(x, y);
           }
-          tmem_st_x8(s_t + c * 8, p);
+          tmem_st_x16(s_t + c * 16, p);   // (over scores that have been read)
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[g]);
-        if (++vst == P8_STAGES) vst = 0, vph ^= 1;
         float x, y;
         unpack2(add2(sum0, sum1), x, y);
         l += x + y;
@@ -632,15 +657,15 @@ __global__ void __launch_bounds__(J8_WARPS * 32) attn8_join_kernel(const __grid_
   const uint32_t begin = stretch_begin(total, blockIdx.x, n_ctas), end = stretch_begin(total, blockIdx.x + 1, n_ctas);
   if (end <= begin || end >= total) return;
   Walk w(a, prefix_s, end - 1, total);
-  w.find();
-  const int left = w.steps - 1 - w.tile0;                   // steps of the unit behind the stretch
-  if (left == 0 || (uint32_t)w.tile0 > end - 1 - begin) return;
-  int last = blockIdx.x;                                    // CTA with the unit's last step
-  while (stretch_begin(total, last + 1, n_ctas) < end + left) ++last;
+  const uint32_t place = w.find(), left = w.steps + P8_COST - 1 - place;   // places of the unit behind the stretch
+  if (left == 0 || place < P8_COST) return;                 // not cut, or no step of it taken
+  if (place > end - 1 - begin + P8_COST) return;            // begun before the stretch (its first step, not what goes ahead of it)
+  const int last = (int)cta_of(total, end - 1 + left, n_ctas);   // CTA with the unit's last step
   const int lane = (int)lane_id(), n = last - (int)blockIdx.x + 1, half = w.half();
-  for (int r = blockIdx.y * J8_WARPS + (threadIdx.x >> 5); r < 256; r += gridDim.y * J8_WARPS) {
+  {
+    const int r = blockIdx.y * J8_WARPS + (threadIdx.x >> 5);
     const int tok = (r & 127) / a.G, head = (r & 127) - tok * a.G, in_unit = (r >> 7) * half + tok;
-    if (tok >= half || in_unit >= w.tokens()) continue;
+    if (tok >= half || in_unit >= w.tokens()) return;
     // part k: of CTA blockIdx.x + k; its first is that of a unit begun there
     auto slot = [&](int k) { return ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * 256 + r; };
     float m = -INFINITY;
@@ -697,7 +722,7 @@ cudaError_t attn8_prompt_launch(const Attn8Args& args, void* workspace, int num_
   a.frag_ml = a.frag_o + (size_t)num_sms * 2 * 256 * HEAD_DIM;
   e = launch_k(attn8_prompt_kernel, dim3(grid), dim3(P8_THREADS), smem, stream, a);
   if (e != cudaSuccess || grid == 1 || a.max_kv <= P8_KV) return e;   // (units of one step are never cut)
-  return launch_k(attn8_join_kernel, dim3(grid, 4), dim3(J8_WARPS * 32), a.n_seqs * 4, stream, a, grid);
+  return launch_k(attn8_join_kernel, dim3(grid, 256 / J8_WARPS), dim3(J8_WARPS * 32), a.n_seqs * 4, stream, a, grid);
 }
 
 }  // namespace tgis
