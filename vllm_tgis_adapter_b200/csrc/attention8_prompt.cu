@@ -31,9 +31,10 @@
 namespace tgis {
 namespace {
 
-constexpr int P8_THREADS = 512;                             // warps 0..3, 4..7: softmax of an accumulator; 8 copies, 9 MMAs, 12..15 widen K and V
-constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 12, P8_WIDEN_WARPS = 4;
-constexpr int P8_REGS_SOFTMAX = 168, P8_REGS_OTHER = 88;    // 256 x 168 + 256 x 88 = 512 x 128, what the launch gives every thread
+constexpr int P8_THREADS = 512;                             // warps 0..3, 4..7: softmax of an accumulator; 8 walk and copies, 9 MMAs,
+                                                            // 12..15 widen K and V
+constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 12, P8_WIDEN = 4;
+constexpr int P8_REGS_SOFTMAX = 192, P8_REGS_OTHER = 64;    // 256 x 192 + 256 x 64 = 512 x 128, what the launch gives every thread
 constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
 constexpr int P8_STAGES = 2;                                // tiles as they come from the cache
 constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile of K or V, of one accumulator's Q, in f16
@@ -45,17 +46,31 @@ constexpr uint32_t P8_COST = 2;                             // what the beginnin
 // What the softmax has to know of a tile, beside its scores
 struct TileNotes {
   uint32_t poison[P8_BLOCKS];  // tokens whose key or value row is not a number
-  uint32_t absent;             // blocks whose page does not exist (bits)
+  uint32_t special;            // bits 0..3: blocks whose page does not exist; bit 4: there are poisoned tokens
   float k_unit, v_unit;        // what a number of K, of V is in units of
   uint32_t pad;
 };
+// Steps [tile0, tile1) of a unit: the copying warp walks the row of steps, the others take from its list
+struct Task {
+  int tile0, tile1;            // tile1 0: no more
+  int keys, kv_len, before;    // that some row of the unit sees; of the sequence; ahead of its queries
+  int first, tokens, half;     // of the unit: first token (of the sequence's queries), tokens, those of the first accumulator
+  int row0, kvh, cut;          // row of the first token; bits: 1 begins behind the unit's first step, 2 ends ahead of its last
+  uint32_t word_mask_lo, word_mask_hi;   // nodes of the draft
+  uint32_t pad[3];
+  __device__ bool two() const { return tokens > 1; }
+  __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
+};
+constexpr int P8_TASKS = 4;
 struct P8Smem {
-  // unswizzled K-major operands: [8 numbers along k][128 rows][8]
+  // K-major operands under the 128-byte swizzle, p8_at
   uint8_t q[2][P8_TILE], k[P8_TILE], v[P8_TILE];
   uint8_t raw[P8_STAGES][P8_BLOCKS * KV8_PAGE];
-  uint16_t v_mul[P8_WIDEN_WARPS][P8_KV];   // scales of the value rows at their places, a copy for every warp that multiplies by them
+  // scales of value rows as f16 multipliers at their places, of even and odd tiles, a copy for every warp that uses them
+  __align__(16) uint16_t v_mul[P8_WIDEN][2][P8_KV];
   TileNotes notes[2];          // of even and odd tiles
-  uint64_t raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], k_full, k_empty, v_full, v_empty, s_full[2],
+  Task task[P8_TASKS];
+  uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], k_full, k_empty, v_full, v_empty, s_full[2],
       p_full[2], o_full[2];
   uint32_t absent[P8_STAGES];  // by the copying warp
   uint32_t tmem_base;
@@ -63,7 +78,10 @@ struct P8Smem {
   uint32_t wsum[P8_THREADS / 32];
   uint32_t prefix[1];          // steps ahead of each sequence
 };
-static_assert(offsetof(P8Smem, raw) % 128 == 0 && KV8_PAGE % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, raw_full) % 8 == 0, "");
+static_assert((2 * P8_TILE + 2 * P8_TILE) % 1024 == 0 && sizeof(((P8Smem*)0)->raw[0]) % 128 == 0 && offsetof(P8Smem, raw) % 128 == 0 && KV8_PAGE % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, raw_full) % 8 == 0, "");
+
+// eight numbers (16 bytes) of a row: [2 halves of 64 numbers][128 rows][8 groups, group g at place g ^ (row & 7)]
+__device__ __forceinline__ int p8_at(int row, int group) { return (group >> 3) * (P8_TILE / 2) + row * 128 + (((group & 7) ^ (row & 7)) << 4); }
 
 struct PromptArgs : Attn8Args {
   int G, TM;
@@ -177,8 +195,6 @@ struct Walk {
   __device__ int keys() const { return keys_of(a, u, i); }
   __device__ int tokens() const { return min(u.tokens, u.sq.q_len - i * u.tokens); }
   __device__ int half() const { return (tokens() + 1) / 2; }   // tokens of the first accumulator; the second has the others
-  __device__ bool two() const { return tokens() > 1; }
-  __device__ bool whole() const { return tile0 == 0 && tile1 == steps; }
   __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys() + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
 };
 
@@ -199,6 +215,16 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t x, uint32_t y, uint32_t z) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(z));
   return r;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// of a power of two from 2^-126 to 2^126
+__device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 // power of two at or above a number > 0 (its bits)
 __device__ __forceinline__ float power_above(uint32_t bits) { return __uint_as_float((bits + 0x7fffffu) & 0x7f800000u); }
 
@@ -210,18 +236,22 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sm.q_full[i], 4);
-        mbar_init(&sm.note_full[i], P8_WIDEN_WARPS);
+        mbar_init(&sm.note_full[i], P8_WIDEN);
         mbar_init(&sm.s_full[i], 1);
         mbar_init(&sm.p_full[i], 4);
         mbar_init(&sm.o_full[i], 1);
       }
       for (int i = 0; i < P8_STAGES; ++i) {
         mbar_init(&sm.raw_full[i], 1);
-        mbar_init(&sm.raw_empty[i], P8_WIDEN_WARPS);
+        mbar_init(&sm.raw_empty[i], P8_WIDEN);
       }
-      mbar_init(&sm.k_full, P8_WIDEN_WARPS);
+      for (int i = 0; i < P8_TASKS; ++i) {
+        mbar_init(&sm.task_full[i], 1);
+        mbar_init(&sm.task_empty[i], 8 + 1 + P8_WIDEN);
+      }
+      mbar_init(&sm.k_full, P8_WIDEN);
       mbar_init(&sm.k_empty, 1);
-      mbar_init(&sm.v_full, P8_WIDEN_WARPS);
+      mbar_init(&sm.v_full, P8_WIDEN);
       mbar_init(&sm.v_empty, 1);
       sm.gave_up = 0;
       fence_barrier_init();
@@ -239,15 +269,54 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = sm.tmem_base;   // [S0 | S1 | O0 | O1], 128 columns each
-  Walk w(a, sm.prefix, stretch_begin(total, blockIdx.x, gridDim.x), stretch_begin(total, blockIdx.x + 1, gridDim.x));
   bool ok = true;
+  int ti = 0;                                // list of tasks
+  uint32_t tph = 0;
+  // the next task, NULL: there is none (or a wait ran out)
+  auto take = [&]() -> const Task* {
+    ok = __all_sync(0xffffffffu, bounded_wait(&sm.task_full[ti], tph));
+    return ok && sm.task[ti].tile1 != 0 ? &sm.task[ti] : nullptr;
+  };
+  auto done_with = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.task_empty[ti]);
+    if (++ti == P8_TASKS) ti = 0, tph ^= 1;
+  };
   if (warp >= P8_WARP_COPY) {
     set_regs<P8_REGS_OTHER, false>();
     if (warp == P8_WARP_COPY) {
-      // ===================== copies =====================
+      // ===================== walk, copies =====================
+      Walk w(a, sm.prefix, stretch_begin(total, blockIdx.x, gridDim.x), stretch_begin(total, blockIdx.x + 1, gridDim.x));
       int st = 0;
       uint32_t ph = 1;         // the first pass over the rings finds them empty
-      while (ok && w.next()) {
+      tph = 1;
+      for (;;) {
+        const bool more = w.next();
+        ok = __all_sync(0xffffffffu, bounded_wait(&sm.task_empty[ti], tph));
+        if (!ok) break;
+        if (lane == 0) {
+          Task& t = sm.task[ti];
+          t.tile0 = w.tile0;
+          t.tile1 = more ? w.tile1 : 0;
+          if (more) {
+            t.keys = w.keys();
+            t.kv_len = w.u.sq.kv_len;
+            t.before = w.u.sq.kv_len - w.u.sq.q_len;
+            t.first = w.i * w.u.tokens;
+            t.tokens = w.tokens();
+            t.half = w.half();
+            t.row0 = w.u.sq.q_start + t.first;
+            t.kvh = w.kvh;
+            t.cut = (w.tile0 > 0 ? 1 : 0) | (w.tile1 < w.steps ? 2 : 0);
+            const unsigned long long nodes = ~0ull >> (TGIS_KV8_MAX_TREE - min(w.u.sq.q_len, TGIS_KV8_MAX_TREE));
+            t.word_mask_lo = (uint32_t)nodes;
+            t.word_mask_hi = (uint32_t)(nodes >> 32);
+          }
+          mbar_arrive(&sm.task_full[ti]);
+        }
+        __syncwarp();
+        if (++ti == P8_TASKS) ti = 0, tph ^= 1;
+        if (!more) break;
         const int n_blk = (w.keys() + KV_BLOCK - 1) / KV_BLOCK;
         auto page_of = [&](int j) {   // lane: block lane & 3 of tile j
           const int b = j * P8_BLOCKS + (lane & 3);
@@ -272,11 +341,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           if (++st == P8_STAGES) st = 0, ph ^= 1;
           if (j + 1 < w.tile1) page = page_of(j + 1);
         }
+        if (!ok) break;
       }
     } else if (warp == P8_WARP_MMA) {
       // ===================== MMAs =====================
       uint32_t kph = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
-      auto operand = [](const uint8_t* p, int ks) { return smem_desc(smem_u32(p) + ks * 2 * (128 * 16), 128 * 16, 128, 0); };   // 16 numbers along k
+      auto operand = [](const uint8_t* p, int ks) { return make_smem_desc_sw128(smem_u32(p) + (ks >> 2) * (P8_TILE / 2) + (ks & 3) * 32); };   // 16 numbers along k
       auto scores = [&](int g, int nb) {
         const uint32_t idesc = idesc_of(128, nb * KV_BLOCK);
 #pragma unroll
@@ -287,8 +357,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         const uint32_t idesc = idesc_of(128, HEAD_DIM);
         for (int ks = 0; ks < 2 * nb; ++ks) mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + ks * 8, operand(sm.v, ks), idesc, !(first && ks == 0));
       };
-      while (ok && w.next()) {
-        const int groups = w.two() ? 2 : 1;
+      while (const Task* tp = take()) {
+        const int groups = tp->two() ? 2 : 1, tile0 = tp->tile0, tile1 = tp->tile1;
+        const Task task = *tp;   // (its sizes)
         for (int g = 0; g < groups && ok; ++g) {
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.q_full[g], qph[g]));
           qph[g] ^= 1;
@@ -298,12 +369,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         kph ^= 1;
         tc_fence_after();
         if (elect_one()) {
-          for (int g = 0; g < groups; ++g) scores(g, w.blocks(w.tile0));
+          for (int g = 0; g < groups; ++g) scores(g, task.blocks(tile0));
           tc_commit(&sm.k_empty);
         }
         __syncwarp();
-        for (int j = w.tile0; j < w.tile1 && ok; ++j) {
-          const bool more = j + 1 < w.tile1;
+        for (int j = tile0; j < tile1 && ok; ++j) {
+          const bool more = j + 1 < tile1;
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full, vph));
           vph ^= 1;
           for (int g = 0; g < groups && ok; ++g) {
@@ -312,7 +383,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
             pph[g] ^= 1;
             tc_fence_after();
             if (elect_one()) {
-              values(g, w.blocks(j), j == w.tile0);
+              values(g, task.blocks(j), j == tile0);
               if (g == groups - 1) tc_commit(&sm.v_empty);
               if (!more) tc_commit(&sm.o_full[g]);
             }
@@ -325,107 +396,143 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
               tc_fence_after();
             }
             if (elect_one()) {
-              scores(g, w.blocks(j + 1));
+              scores(g, task.blocks(j + 1));
               if (g == groups - 1) tc_commit(&sm.k_empty);
             }
             __syncwarp();
           }
         }
+        if (!ok) break;
+        done_with();
       }
     } else if (warp >= P8_WARP_WIDEN) {
-      // ===================== K and V to f16 =====================
-      const int mine = warp - P8_WARP_WIDEN, part = mine * 32 + lane;   // block; token of the tile, dim
-      int st = 0, odd_tile = 0;
-      uint32_t full = 0, empty = 1;
-      while (ok && w.next()) {
+      // ===================== K, V to f16: thread = token, then dim =====================
+      const int mine = warp - P8_WARP_WIDEN, part = mine * 32 + lane;
+      const uint32_t swizzle = (uint32_t)(lane & 7) << 4, out_row = (uint32_t)part * 128 + swizzle;
+      const uint32_t k_out = smem_u32(sm.k) + out_row, v_out = smem_u32(sm.v) + out_row, v_mul = smem_u32(sm.v_mul[mine]);
+      int st = 0, odd_tile = 0;               // of the tile whose K is next
+      uint32_t full = 0, k_empty = 1, v_empty = 1;
+      while (const Task* tp = take()) {
+        const int tile0 = tp->tile0, tile1 = tp->tile1, kv_len = tp->kv_len;
         float r = 0.f;
-        for (int j = w.tile0; j < w.tile1; ++j) {
-          const int nb = w.blocks(j);
+        uint32_t hi = 0, lo = 0;              // this thread's key scale as two f16 numbers, each twice
+        TileNotes mem;                        // (poison[0]: of this warp's block)
+        // Scales of tile j, which every warp looks at all of (lane = token of a block).  Done ahead of the waits for buffers, which
+        // come once a step and all at once
+        auto scales = [&](int j) {
+          const int nb = tp->blocks(j);
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_full[st], full));
-          if (!ok) break;
-          const uint8_t* raw = sm.raw[st];
-          // ---- scales: every warp looks at all of them
+          if (!ok) return;
           const uint32_t absent = sm.absent[st];
-          float top_k = 0.f, top_v = 0.f, my_k = 0.f, vs[P8_BLOCKS];
-          uint32_t my_odd = 0;
+          float my_k = 0.f, vs[P8_BLOCKS], top_k = 0.f, top_v = 0.f;
+          uint32_t any_odd = 0;
 #pragma unroll
           for (int b = 0; b < P8_BLOCKS; ++b) {
-            const float* sc = reinterpret_cast<const float*>(raw + b * KV8_PAGE + KV8_K_SCALES);
-            const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < w.u.sq.kv_len;
+            const float* sc = reinterpret_cast<const float*>(sm.raw[st] + b * KV8_PAGE + KV8_K_SCALES);
+            const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < kv_len;
             float k = there ? sc[lane] : 0.f;
             vs[b] = there ? sc[KV_BLOCK + lane] : 0.f;
             const bool fine = k < INFINITY && vs[b] < INFINITY;
             if (!fine) k = vs[b] = 0.f;
             const uint32_t odd = __ballot_sync(0xffffffffu, !fine);
+            any_odd |= odd;
             top_k = fmaxf(top_k, k);
             top_v = fmaxf(top_v, vs[b]);
-            if (b == mine) my_k = k, my_odd = odd;
+            if (b == mine) my_k = k, mem.poison[0] = odd;
           }
           const float k_top = fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))), 0x1p-118f);
           r = fmaxf(r, fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))), 0x1p-118f));
-          uint16_t* v_mul = sm.v_mul[mine];
+          const float v_to = P8_V_TOP * one_over(r), k = my_k * (P8_K_TOP * one_over(k_top));
+          hi = f16x2(k, k);
+          lo = f16x2(k - f16x2_to_f32x2(hi).x, k - f16x2_to_f32x2(hi).x);
 #pragma unroll
-          for (int b = 0; b < P8_BLOCKS; ++b) v_mul[b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * (P8_V_TOP / r), 0.f);
-          // ---- K: this thread's token, sixteen dims at a time -> two rows of eight numbers
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty, empty));
-          if (!ok) break;
+          for (int b = 0; b < P8_BLOCKS; ++b) sm.v_mul[mine][odd_tile][b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * v_to, 0.f);
+          mem.special = absent | (any_odd != 0 ? 1u << P8_BLOCKS : 0u);
+          mem.k_unit = k_top * (1.f / P8_K_TOP);
+          mem.v_unit = r * (1.f / P8_V_TOP);
+        };
+        // K: sixteen dims at a time -> two groups of eight numbers.  (A block that a last tile does not have is not read.)
+        auto widen_k = [&](int j) {
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty, k_empty));
+          if (!ok) return;
+          k_empty ^= 1;
           // (the scores of the tile before are done, so who reads the notes of the one before that has finished)
           TileNotes& t = sm.notes[odd_tile];
           if (lane == 0) {
-            t.poison[mine] = my_odd;
-            if (mine == 0) {
-              t.absent = absent;
-              t.k_unit = k_top / P8_K_TOP;
-              t.v_unit = r / P8_V_TOP;
-            }
+            t.poison[mine] = mem.poison[0];
+            if (mine == 0) t.special = mem.special, t.k_unit = mem.k_unit, t.v_unit = mem.v_unit;
           }
-          if (mine < nb) {
-            const float k = my_k * (P8_K_TOP / k_top);
-            const uint32_t h1 = f16x2(k, k), lo = f16x2(k - f16x2_to_f32x2(h1).x, k - f16x2_to_f32x2(h1).x);
-            const uint8_t* from = raw + mine * KV8_PAGE + lane * HEAD_DIM;
+          auto wide = [&](uint32_t two) {
+            const uint32_t h = e4m3x2_to_f16x2(two);
+            return hfma2(h, hi, hmul2(h, lo));
+          };
+          if (mine < tp->blocks(j)) {
+            const uint32_t from = smem_u32(sm.raw[st]) + (uint32_t)mine * KV8_PAGE + (uint32_t)lane * HEAD_DIM + swizzle;
 #pragma unroll
-            for (int c = 0; c < HEAD_DIM / 16; ++c) {
-              const uint4 x = *reinterpret_cast<const uint4*>(from + ((c ^ (lane & 7)) << 4));
-              const uint32_t in[4] = {x.x, x.y, x.z, x.w};
-              uint32_t o[8];
+            for (int d0 = 0; d0 < HEAD_DIM / 16; d0 += 4) {
+              uint4 x[4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t h = e4m3x2_to_f16x2(i & 1 ? in[i >> 1] >> 16 : in[i >> 1] & 0xffffu);
-                o[i] = hfma2(h, h1, hmul2(h, lo));
+              for (int d = 0; d < 4; ++d) x[d] = lds128(from ^ ((d0 + d) << 4));
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const uint32_t to = (k_out ^ (2 * d << 4)) + (d0 >> 2) * (P8_TILE / 2);
+                sts128(to, wide(x[d].x), wide(x[d].x >> 16), wide(x[d].y), wide(x[d].y >> 16));
+                sts128(to ^ 16, wide(x[d].z), wide(x[d].z >> 16), wide(x[d].w), wide(x[d].w >> 16));
               }
-              *reinterpret_cast<uint4*>(sm.k + 2 * c * 2048 + part * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(sm.k + (2 * c + 1) * 2048 + part * 16) = make_uint4(o[4], o[5], o[6], o[7]);
             }
           }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&sm.k_full);
             mbar_arrive(&sm.note_full[odd_tile]);
+            mbar_arrive(&sm.k_full);
           }
-          // ---- V: this thread's dim, sixteen tokens at a time
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_empty, empty));
-          if (!ok) break;
-#pragma unroll 2
-          for (int h = 0; h < 2 * nb; ++h) {
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + (h >> 1) * KV8_PAGE + KV8_CODES + (h & 1) * (KV8_CODES / 2) + part * 16);
-            const uint4 m0 = *reinterpret_cast<const uint4*>(v_mul + h * 16), m1 = *reinterpret_cast<const uint4*>(v_mul + h * 16 + 8);
-            uint8_t* to = sm.v + h * 2 * 2048 + part * 16;
-            *reinterpret_cast<uint4*>(to) = make_uint4(hmul2(e4m3x2_to_f16x2(x.x & 0xffffu), m0.x), hmul2(e4m3x2_to_f16x2(x.x >> 16), m0.y),
-                                                       hmul2(e4m3x2_to_f16x2(x.y & 0xffffu), m0.z), hmul2(e4m3x2_to_f16x2(x.y >> 16), m0.w));
-            *reinterpret_cast<uint4*>(to + 2048) = make_uint4(hmul2(e4m3x2_to_f16x2(x.z & 0xffffu), m1.x), hmul2(e4m3x2_to_f16x2(x.z >> 16), m1.y),
-                                                              hmul2(e4m3x2_to_f16x2(x.w & 0xffffu), m1.z), hmul2(e4m3x2_to_f16x2(x.w >> 16), m1.w));
+        };
+        // V: sixteen tokens at a time
+        auto widen_v = [&](int j, int stage, int odd) {
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_empty, v_empty));
+          if (!ok) return;
+          v_empty ^= 1;
+          const int nh = 2 * tp->blocks(j);
+          const uint32_t from = smem_u32(sm.raw[stage]) + KV8_CODES + (uint32_t)part * 16, mul = v_mul + odd * (P8_KV * 2);
+#pragma unroll
+          for (int h0 = 0; h0 < 2 * P8_BLOCKS; h0 += 2) {
+            if (h0 >= nh) break;
+            uint4 x[2], m[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              x[h] = lds128(from + (h0 >> 1) * KV8_PAGE + h * (KV8_CODES / 2));
+              m[2 * h] = lds128(mul + (h0 + h) * 32);
+              m[2 * h + 1] = lds128(mul + (h0 + h) * 32 + 16);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t to = (v_out ^ ((2 * (h0 + h) & 7) << 4)) + (h0 >> 2) * (P8_TILE / 2);
+              sts128(to, hmul2(e4m3x2_to_f16x2(x[h].x), m[2 * h].x), hmul2(e4m3x2_to_f16x2(x[h].x >> 16), m[2 * h].y), hmul2(e4m3x2_to_f16x2(x[h].y), m[2 * h].z),
+                     hmul2(e4m3x2_to_f16x2(x[h].y >> 16), m[2 * h].w));
+              sts128(to ^ 16, hmul2(e4m3x2_to_f16x2(x[h].z), m[2 * h + 1].x), hmul2(e4m3x2_to_f16x2(x[h].z >> 16), m[2 * h + 1].y),
+                     hmul2(e4m3x2_to_f16x2(x[h].w), m[2 * h + 1].z), hmul2(e4m3x2_to_f16x2(x[h].w >> 16), m[2 * h + 1].w));
+            }
           }
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&sm.v_full);
-            mbar_arrive(&sm.raw_empty[st]);
+            mbar_arrive(&sm.raw_empty[stage]);
           }
+        };
+        scales(tile0);
+        if (ok) widen_k(tile0);
+        for (int j = tile0; j < tile1 && ok; ++j) {
+          const int stage = st, odd = odd_tile;
           if (++st == P8_STAGES) st = 0, full ^= 1;
-          empty ^= 1;
           odd_tile ^= 1;
+          if (j + 1 < tile1) scales(j + 1);
+          if (ok) widen_v(j, stage, odd);
+          if (ok && j + 1 < tile1) widen_k(j + 1);
         }
+        if (!ok) break;
+        done_with();
       }
     }
   } else {
@@ -436,19 +543,19 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem_base + g * 128 + lanes, o_t = tmem_base + 256 + g * 128 + lanes;
     uint32_t sph = 0, oph = 0, tile = 0;   // tile: of the CTA
-    while (ok && w.next()) {
-      if (g == 1 && !w.two()) {
-        tile += (uint32_t)(w.tile1 - w.tile0);
+    while (const Task* tp = take()) {
+      const Task& t = *tp;
+      if (g == 1 && !t.two()) {
+        tile += (uint32_t)(t.tile1 - t.tile0);
+        done_with();
         continue;
       }
-      const int in_unit = g * w.half() + tok;
-      const bool mine = tok < w.half() && in_unit < w.tokens();
-      const int row = w.u.sq.q_start + w.i * w.u.tokens + in_unit, qhead = w.kvh * a.G + head;
-      const int before = w.u.sq.kv_len - w.u.sq.q_len;      // keys that were there before the step
-      int lim = before + w.i * w.u.tokens + in_unit;        // causal: last key seen
+      const int in_unit = g * t.half + tok;
+      const bool mine = tok < t.half && in_unit < t.tokens;
+      int lim = t.before + t.first + in_unit;               // causal: last key seen
       unsigned long long word = 0;
       if (!mine) lim = 0x7fffffff;
-      else if (a.tree != nullptr) lim = before - 1, word = a.tree[row] & ~0ull >> (TGIS_KV8_MAX_TREE - w.u.sq.q_len);
+      else if (a.tree != nullptr) lim = t.before - 1, word = a.tree[t.row0 + in_unit] & ((unsigned long long)t.word_mask_hi << 32 | t.word_mask_lo);
       // ---- the row of Q, its largest number at 128 to 256
       float qm;
       {
@@ -456,7 +563,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < HEAD_DIM / 8; ++c) {
-          x[c] = mine ? reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)qhead * HEAD_DIM)[c] : make_uint4(0, 0, 0, 0);
+          x[c] = mine ? reinterpret_cast<const uint4*>(a.q + (size_t)(t.row0 + in_unit) * a.ldq + (size_t)(t.kvh * a.G + head) * HEAD_DIM)[c] : make_uint4(0, 0, 0, 0);
           const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = max(top, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
@@ -470,15 +577,16 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           uint32_t h[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) h[i] = f16x2(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
-          *reinterpret_cast<uint4*>(sm.q[g] + c * 2048 + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[g]);
       float m = 0.f, l = 0.f, unit = 0.f;
-      for (int j = w.tile0; j < w.tile1; ++j) {
-        const int nb = w.blocks(j);
+      const int tile0 = t.tile0, tile1 = t.tile1;
+      for (int j = tile0; j < tile1; ++j) {
+        const int nb = t.blocks(j);
         // (in this order: with its scores there, a tile's notes are, and the next tile's in their place are not)
         ok = __all_sync(0xffffffffu, bounded_wait(&sm.s_full[g], sph) && bounded_wait(&sm.note_full[tile & 1], tile >> 1 & 1));
         if (!ok) break;
@@ -487,45 +595,42 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         const TileNotes& sc = sm.notes[tile & 1];
         ++tile;
         const int seen = lim - j * P8_KV;                   // last column seen (of the keys before a draft)
-        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || sc.absent != 0);
-        uint32_t vis[P8_BLOCKS];                            // columns that the row sees, where some are hidden
-#pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
-          vis[c] = seen >= c * 32 + 31 ? 0xffffffffu : seen < c * 32 ? 0u : (2u << (seen - c * 32)) - 1u;
-          if (a.tree != nullptr && mine) {
-            const int d = c * 32 - (seen + 1);              // node of the block's first column
-            if (d > -32 && d < 64) vis[c] |= d >= 0 ? (uint32_t)(word >> d) : (uint32_t)word << -d;
-          }
-          if (sc.absent >> c & 1) vis[c] = 0;
-        }
-        // the scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill)
-        uint32_t s[2][KV_BLOCK];
-        float mx[2] = {-INFINITY, -INFINITY};
-        tmem_ld_x32(s_t, s[0]);
+        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || sc.special != 0);
+        uint32_t s[P8_KV];
 #pragma unroll
         for (int c = 0; c < P8_BLOCKS; ++c) {
           if (c >= nb) break;
-          tmem_ld_wait();
-          if (c + 1 < P8_BLOCKS && c + 1 < nb) tmem_ld_x32(s_t + (c + 1) * 32, s[(c + 1) & 1]);
-          uint32_t (&x)[KV_BLOCK] = s[c & 1];
-          if (mask) {
+          tmem_ld_x32(s_t + c * 32, s + c * 32);
+        }
+        tmem_ld_wait();
+        if (mask) {
+#pragma unroll
+          for (int c = 0; c < P8_BLOCKS; ++c) {
+            if (c >= nb) break;
+            uint32_t vis = seen >= c * 32 + 31 ? 0xffffffffu : seen < c * 32 ? 0u : (2u << (seen - c * 32)) - 1u;   // columns that the row sees
+            if (a.tree != nullptr && mine) {
+              const int d = c * 32 - (seen + 1);            // node of the block's first column
+              if (d > -32 && d < 64) vis |= d >= 0 ? (uint32_t)(word >> d) : (uint32_t)word << -d;
+            }
+            if (sc.special >> c & 1) vis = 0;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!(vis[c] >> i & 1)) x[i] = __float_as_uint(-INFINITY);
+              if (!(vis >> i & 1)) s[c * 32 + i] = __float_as_uint(-INFINITY);
+            if ((sc.poison[c] & vis) != 0) l = __uint_as_float(0x7fc00000u);
           }
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            mx[0] = fmaxf(mx[0], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-            mx[1] = fmaxf(mx[1], fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
-          }
-          if ((sc.poison[c] & vis[c]) != 0) l = __uint_as_float(0x7fc00000u);
         }
-        tmem_ld_x32(s_t, s[0]);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < P8_BLOCKS; ++c) {
+          if (c >= nb) break;
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = fmaxf(mx[i >> 1 & 3], fmaxf(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])));
+        }
         const float qk = qm * sc.k_unit;
         uint64_t qm2 = pack2(qk, qk);
-        const float top = fmaxf(mx[0], mx[1]) * qk;
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qk;
         const float unit_now = sc.v_unit;
-        if (j == w.tile0) {
+        if (j == tile0) {
           m = top;
         } else if (__any_sync(0xffffffffu, top > m + P8_SLACK) || unit_now != unit) {
           // the products that wrote O retired before these scores did
@@ -547,38 +652,28 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         const float ref = m == -INFINITY ? 0.f : m;   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
         const uint64_t neg_m = pack2(P8_HELD - ref, P8_HELD - ref);
         // an exact product less a rounded one may be far from zero where both are large: such scores are rounded first, as their maximum was
-        const bool large = fabsf(ref) > 0x1p20f;
-        if (large) qm2 = pack2(1.f, 1.f);
+        if (fabsf(ref) > 0x1p20f) {
+#pragma unroll
+          for (int i = 0; i < P8_KV; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
+          qm2 = pack2(1.f, 1.f);
+        }
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
-          if (c >= nb) break;
-          tmem_ld_wait();
-          if (c + 1 < P8_BLOCKS && c + 1 < nb) tmem_ld_x32(s_t + (c + 1) * 32, s[(c + 1) & 1]);
-          uint32_t (&v)[KV_BLOCK] = s[c & 1];
-          if (mask) {
+        for (int c = 0; c < 2 * P8_BLOCKS; ++c) {
+          if (c >= 2 * nb) break;
+          uint32_t p[8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(vis[c] >> i & 1)) v[i] = __float_as_uint(-INFINITY);
-          }
-          if (large) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * qk);
-          }
-          uint32_t p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            // places 2 i, 2 i + 1 of the block (cache8.cuh v8_place)
-            const int col = (i >> 3) * 16 + 2 * (4 * (i & 1) + (i >> 1 & 3));
+          for (int i = 0; i < 8; ++i) {
+            const int col = c * 16 + 2 * (4 * (i & 1) + (i >> 1));   // places 2 i, 2 i + 1 of the half (cache8.cuh v8_place)
             float x, y;
-            unpack2(fma2(pack2(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), qm2, neg_m), x, y);
+            unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
             x = ex2(x);
             y = ex2(y);
             if (i & 1) sum1 = add2(sum1, pack2(x, y));
             else sum0 = add2(sum0, pack2(x, y));
             p[i] = f16x2(x, y);
           }
-          tmem_st_x16(s_t + c * 16, p);   // (over scores that have been read)
+          tmem_st_x8(s_t + c * 8, p);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -593,7 +688,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       if (!ok) break;
       oph ^= 1;
       tc_fence_after();
-      if (w.whole()) {
+      const int row = t.row0 + in_unit, qhead = t.kvh * a.G + head;
+      if (t.cut == 0) {
         const float inv = l == 0.f ? 0.f : unit / l;
         __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)qhead * HEAD_DIM;
 #pragma unroll
@@ -612,7 +708,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           }
         }
       } else {
-        const size_t slot = ((size_t)blockIdx.x * 2 + (w.tile0 == 0)) * 256 + g * 128 + r;
+        const size_t slot = ((size_t)blockIdx.x * 2 + ((t.cut & 1) == 0)) * 256 + g * 128 + r;
         float* dst = a.frag_o + slot * HEAD_DIM;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -629,6 +725,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         if (mine) *reinterpret_cast<float2*>(a.frag_ml + slot * 2) = make_float2(m, l);
       }
       tc_fence_before();
+      done_with();
     }
   }
   if (!ok && lane == 0) sm.gave_up = 1;
