@@ -31,10 +31,9 @@
 namespace tgis {
 namespace {
 
-constexpr int P8_THREADS = 512;                             // warps 0..3, 4..7: softmax of an accumulator; 8 walk and copies, 9 MMAs,
-                                                            // 12..15 widen K and V
-constexpr int P8_WARP_COPY = 8, P8_WARP_MMA = 9, P8_WARP_WIDEN = 12, P8_WIDEN = 4;
-constexpr int P8_REGS_SOFTMAX = 192, P8_REGS_OTHER = 64;    // 256 x 192 + 256 x 64 = 512 x 128, what the launch gives every thread
+constexpr int P8_THREADS = 768;                             // warps 0..7, 8..15: softmax of an accumulator; 16 walks and copies, 17 MMAs, 20..23 widen K and V
+constexpr int P8_WARP_COPY = 16, P8_WARP_MMA = 17, P8_WARP_WIDEN = 20, P8_WIDEN = 4;
+constexpr int P8_REGS_SOFTMAX = 88, P8_REGS_OTHER = 64;     // 512 x 88 + 256 x 64 = 768 x 80, what the launch gives every thread
 constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
 constexpr int P8_STAGES = 2;                                // tiles as they come from the cache
 constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile of K or V, of one accumulator's Q, in f16
@@ -70,7 +69,8 @@ struct P8Smem {
   __align__(16) uint16_t v_mul[P8_WIDEN][2][P8_KV];
   TileNotes notes[2];          // of even and odd tiles
   Task task[P8_TASKS];
-  uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], k_full, k_empty, v_full, v_empty, s_full[2],
+  float pair[2][2][2][128];    // what the two threads of a row tell one another: of even and odd times, accumulator, half, row
+  uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], pair_full[2][4], k_full, k_empty, v_full, v_empty, s_full[2],
       p_full[2], o_full[2];
   uint32_t absent[P8_STAGES];  // by the copying warp
   uint32_t tmem_base;
@@ -83,9 +83,15 @@ static_assert((2 * P8_TILE + 2 * P8_TILE) % 1024 == 0 && sizeof(((P8Smem*)0)->ra
 // eight numbers (16 bytes) of a row: [2 halves of 64 numbers][128 rows][8 groups, group g at place g ^ (row & 7)]
 __device__ __forceinline__ int p8_at(int row, int group) { return (group >> 3) * (P8_TILE / 2) + row * 128 + (((group & 7) ^ (row & 7)) << 4); }
 
+// What a CTA leaves of a unit that begins in its stretch and ends behind it
+struct CutUnit {
+  int row0, kvh, tokens, half, parts;   // parts 0: there is none; else its CTAs, this one the first
+  int pad[3];
+};
 struct PromptArgs : Attn8Args {
   int G, TM;
   float *frag_o, *frag_ml;     // [CTA][0: of a unit begun before it, 1: of one that ends behind it][256 rows]([128])
+  CutUnit* cut;                // [CTA]
 };
 
 // ---- the row of steps
@@ -225,6 +231,11 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
 }
 // of a power of two from 2^-126 to 2^126
 __device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 // power of two at or above a number > 0 (its bits)
 __device__ __forceinline__ float power_above(uint32_t bits) { return __uint_as_float((bits + 0x7fffffu) & 0x7f800000u); }
 
@@ -235,10 +246,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
   if (warp == P8_WARP_MMA) {
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.q_full[i], 4);
+        mbar_init(&sm.q_full[i], 8);
         mbar_init(&sm.note_full[i], P8_WIDEN);
         mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], 4);
+        mbar_init(&sm.p_full[i], 8);
+        for (int k = 0; k < 4; ++k) mbar_init(&sm.pair_full[i][k], 2);
         mbar_init(&sm.o_full[i], 1);
       }
       for (int i = 0; i < P8_STAGES; ++i) {
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       }
       for (int i = 0; i < P8_TASKS; ++i) {
         mbar_init(&sm.task_full[i], 1);
-        mbar_init(&sm.task_empty[i], 8 + 1 + P8_WIDEN);
+        mbar_init(&sm.task_empty[i], 16 + 1 + P8_WIDEN);
       }
       mbar_init(&sm.k_full, P8_WIDEN);
       mbar_init(&sm.k_empty, 1);
@@ -286,10 +298,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     set_regs<P8_REGS_OTHER, false>();
     if (warp == P8_WARP_COPY) {
       // ===================== walk, copies =====================
-      Walk w(a, sm.prefix, stretch_begin(total, blockIdx.x, gridDim.x), stretch_begin(total, blockIdx.x + 1, gridDim.x));
+      const uint32_t n = min(gridDim.x, total), b = min(blockIdx.x, n);   // (no stretch of the first n is empty)
+      Walk w(a, sm.prefix, n > 0 ? stretch_begin(total, b, n) : 0u, n > 0 ? stretch_begin(total, min(b + 1, n), n) : 0u);
       int st = 0;
       uint32_t ph = 1;         // the first pass over the rings finds them empty
       tph = 1;
+      CutUnit cut{};
       for (;;) {
         const bool more = w.next();
         ok = __all_sync(0xffffffffu, bounded_wait(&sm.task_empty[ti], tph));
@@ -317,6 +331,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         __syncwarp();
         if (++ti == P8_TASKS) ti = 0, tph ^= 1;
         if (!more) break;
+        if (w.tile0 == 0 && w.tile1 < w.steps)   // (the stretch ends here)
+          cut = CutUnit{w.u.sq.q_start + w.i * w.u.tokens, w.kvh, w.tokens(), w.half(), (int)(cta_of(total, w.at + (w.steps - w.tile1) - 1, n) - b) + 1, {}};
         const int n_blk = (w.keys() + KV_BLOCK - 1) / KV_BLOCK;
         auto page_of = [&](int j) {   // lane: block lane & 3 of tile j
           const int b = j * P8_BLOCKS + (lane & 3);
@@ -343,6 +359,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         }
         if (!ok) break;
       }
+      if (lane == 0) a.cut[blockIdx.x] = cut;
     } else if (warp == P8_WARP_MMA) {
       // ===================== MMAs =====================
       uint32_t kph = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
@@ -355,7 +372,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       };
       auto values = [&](int g, int nb, bool first) {
         const uint32_t idesc = idesc_of(128, HEAD_DIM);
-        for (int ks = 0; ks < 2 * nb; ++ks) mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + ks * 8, operand(sm.v, ks), idesc, !(first && ks == 0));
+        for (int ks = 0; ks < 2 * nb; ++ks) mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + (ks >> 2) * 64 + (ks & 3) * 8, operand(sm.v, ks), idesc, !(first && ks == 0));
       };
       while (const Task* tp = take()) {
         const int groups = tp->two() ? 2 : 1, tile0 = tp->tile0, tile1 = tp->tile1;
@@ -469,13 +486,13 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           if (mine < tp->blocks(j)) {
             const uint32_t from = smem_u32(sm.raw[st]) + (uint32_t)mine * KV8_PAGE + (uint32_t)lane * HEAD_DIM + swizzle;
 #pragma unroll
-            for (int d0 = 0; d0 < HEAD_DIM / 16; d0 += 4) {
-              uint4 x[4];
+            for (int d0 = 0; d0 < HEAD_DIM / 16; d0 += 2) {
+              uint4 x[2];
 #pragma unroll
-              for (int d = 0; d < 4; ++d) x[d] = lds128(from ^ ((d0 + d) << 4));
+              for (int d = 0; d < 2; ++d) x[d] = lds128(from ^ ((d0 + d) << 4));
 #pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                const uint32_t to = (k_out ^ (2 * d << 4)) + (d0 >> 2) * (P8_TILE / 2);
+              for (int d = 0; d < 2; ++d) {
+                const uint32_t to = (k_out ^ ((2 * (d0 + d) & 7) << 4)) + (d0 >> 2) * (P8_TILE / 2);
                 sts128(to, wide(x[d].x), wide(x[d].x >> 16), wide(x[d].y), wide(x[d].y >> 16));
                 sts128(to ^ 16, wide(x[d].z), wide(x[d].z >> 16), wide(x[d].w), wide(x[d].w >> 16));
               }
@@ -536,13 +553,22 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       }
     }
   } else {
-    // ===================== softmax: thread = row =====================
+    // ===================== softmax: two threads a row, 64 columns (and dims) each =====================
     set_regs<P8_REGS_SOFTMAX, true>();
-    const int g = warp >> 2;
-    const int r = (warp & 3) * 32 + lane, tok = r / a.G, head = r - tok * a.G;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_t = tmem_base + g * 128 + lanes, o_t = tmem_base + 256 + g * 128 + lanes;
-    uint32_t sph = 0, oph = 0, tile = 0;   // tile: of the CTA
+    const int g = warp >> 3, h = warp >> 2 & 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane, tok = r / a.G, head = r - tok * a.G;
+    const uint32_t s_t = tmem_base + g * 128 + ((uint32_t)(quarter * 32) << 16) + h * 64, o_t = s_t + 256;
+    uint32_t sph = 0, oph = 0, tile = 0, met = 0;   // tile: of the CTA; met: times that the row's threads have told one another something
+    // this thread's number said, the other one's heard
+    auto pair_up = [&](float mine) {
+      float(*to)[128] = sm.pair[met & 1][g];
+      to[h][r] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.pair_full[g][quarter]);
+      ok = __all_sync(0xffffffffu, bounded_wait(&sm.pair_full[g][quarter], met & 1));
+      ++met;
+      return to[h ^ 1][r];
+    };
     while (const Task* tp = take()) {
       const Task& t = *tp;
       if (g == 1 && !t.two()) {
@@ -559,25 +585,28 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       // ---- the row of Q, its largest number at 128 to 256
       float qm;
       {
-        uint4 x[HEAD_DIM / 8];
+        uint4 x[HEAD_DIM / 16];
         uint32_t top = 0;
+        const uint4* from = reinterpret_cast<const uint4*>(a.q + (size_t)(t.row0 + in_unit) * a.ldq + (size_t)(t.kvh * a.G + head) * HEAD_DIM + h * 64);
 #pragma unroll
-        for (int c = 0; c < HEAD_DIM / 8; ++c) {
-          x[c] = mine ? reinterpret_cast<const uint4*>(a.q + (size_t)(t.row0 + in_unit) * a.ldq + (size_t)(t.kvh * a.G + head) * HEAD_DIM)[c] : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < HEAD_DIM / 16; ++c) {
+          x[c] = mine ? from[c] : make_uint4(0, 0, 0, 0);
           const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) top = max(top, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
         }
+        top = max(top, __float_as_uint(pair_up(__uint_as_float(top))));
+        if (!ok) break;
         float up = power_up(top);
         qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / up;   // (hidden scores are -inf before they are scaled)
         if (a.scale < 0.f) up = -up;
 #pragma unroll
-        for (int c = 0; c < HEAD_DIM / 8; ++c) {
+        for (int c = 0; c < HEAD_DIM / 16; ++c) {
           const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-          uint32_t h[4];
+          uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[i] = f16x2(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
-          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          for (int i = 0; i < 4; ++i) w[i] = f16x2(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
+          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
       fence_proxy_async();
@@ -586,7 +615,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       float m = 0.f, l = 0.f, unit = 0.f;
       const int tile0 = t.tile0, tile1 = t.tile1;
       for (int j = tile0; j < tile1; ++j) {
-        const int nb = t.blocks(j);
+        const int nb = t.blocks(j) - 2 * h;                 // of this thread's half
         // (in this order: with its scores there, a tile's notes are, and the next tile's in their place are not)
         ok = __all_sync(0xffffffffu, bounded_wait(&sm.s_full[g], sph) && bounded_wait(&sm.note_full[tile & 1], tile >> 1 & 1));
         if (!ok) break;
@@ -594,41 +623,44 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         tc_fence_after();
         const TileNotes& sc = sm.notes[tile & 1];
         ++tile;
-        const int seen = lim - j * P8_KV;                   // last column seen (of the keys before a draft)
-        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || sc.special != 0);
-        uint32_t s[P8_KV];
-#pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
-          if (c >= nb) break;
-          tmem_ld_x32(s_t + c * 32, s + c * 32);
-        }
-        tmem_ld_wait();
+        const int seen = lim - j * P8_KV - h * 64;          // last column seen (of the keys before a draft)
+        const uint32_t special = sc.special;
+        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || special != 0);
+        uint32_t vis[2] = {0xffffffffu, 0xffffffffu};       // columns that the row sees
         if (mask) {
 #pragma unroll
-          for (int c = 0; c < P8_BLOCKS; ++c) {
-            if (c >= nb) break;
-            uint32_t vis = seen >= c * 32 + 31 ? 0xffffffffu : seen < c * 32 ? 0u : (2u << (seen - c * 32)) - 1u;   // columns that the row sees
+          for (int c = 0; c < 2; ++c) {
+            vis[c] = seen >= c * 32 + 31 ? 0xffffffffu : seen < c * 32 ? 0u : (2u << (seen - c * 32)) - 1u;
             if (a.tree != nullptr && mine) {
               const int d = c * 32 - (seen + 1);            // node of the block's first column
-              if (d > -32 && d < 64) vis |= d >= 0 ? (uint32_t)(word >> d) : (uint32_t)word << -d;
+              if (d > -32 && d < 64) vis[c] |= d >= 0 ? (uint32_t)(word >> d) : (uint32_t)word << -d;
             }
-            if (sc.special >> c & 1) vis = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(vis >> i & 1)) s[c * 32 + i] = __float_as_uint(-INFINITY);
-            if ((sc.poison[c] & vis) != 0) l = __uint_as_float(0x7fc00000u);
+            if (special >> (2 * h + c) & 1) vis[c] = 0;
+            if (c < nb && (sc.poison[2 * h + c] & vis[c]) != 0) l = __uint_as_float(0x7fc00000u);
           }
         }
+        auto hide = [&](uint32_t (&s)[32], uint32_t seen_of_it) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(seen_of_it >> i & 1)) s[i] = __float_as_uint(-INFINITY);
+        };
+        // the scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill)
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < P8_BLOCKS; ++c) {
+        for (int c = 0; c < 2; ++c) {
           if (c >= nb) break;
+          uint32_t s[32];
+          tmem_ld_x32(s_t + c * 32, s);
+          tmem_ld_wait();
+          if (mask) hide(s, vis[c]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = fmaxf(mx[i >> 1 & 3], fmaxf(__uint_as_float(s[c * 32 + i]), __uint_as_float(s[c * 32 + i + 1])));
+          for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
         const float qk = qm * sc.k_unit;
         uint64_t qm2 = pack2(qk, qk);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * qk;
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        top = fmaxf(top, pair_up(top)) * qk;
+        if (!ok) break;
         const float unit_now = sc.v_unit;
         if (j == tile0) {
           m = top;
@@ -638,8 +670,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           if (top > m + P8_SLACK) m = top;
           l *= f;
           f *= unit / unit_now;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
             uint32_t o[16];
             tmem_ld_32x32b_x16(o_t + c * 16, o);
             tmem_ld_wait();
@@ -652,28 +684,36 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         const float ref = m == -INFINITY ? 0.f : m;   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
         const uint64_t neg_m = pack2(P8_HELD - ref, P8_HELD - ref);
         // an exact product less a rounded one may be far from zero where both are large: such scores are rounded first, as their maximum was
-        if (fabsf(ref) > 0x1p20f) {
-#pragma unroll
-          for (int i = 0; i < P8_KV; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
-          qm2 = pack2(1.f, 1.f);
-        }
+        const bool large = fabsf(ref) > 0x1p20f;
+        if (large) qm2 = pack2(1.f, 1.f);
         uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
-        for (int c = 0; c < 2 * P8_BLOCKS; ++c) {
-          if (c >= 2 * nb) break;
-          uint32_t p[8];
+        for (int c = 0; c < 2; ++c) {
+          if (c >= nb) break;
+          uint32_t s[32];
+          tmem_ld_x32(s_t + c * 32, s);
+          tmem_ld_wait();
+          if (mask) hide(s, vis[c]);
+          if (large) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int col = c * 16 + 2 * (4 * (i & 1) + (i >> 1));   // places 2 i, 2 i + 1 of the half (cache8.cuh v8_place)
-            float x, y;
-            unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            if (i & 1) sum1 = add2(sum1, pack2(x, y));
-            else sum0 = add2(sum0, pack2(x, y));
-            p[i] = f16x2(x, y);
+            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
           }
-          tmem_st_x8(s_t + c * 8, p);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int col = k * 16 + 2 * (4 * (i & 1) + (i >> 1));   // places 2 i, 2 i + 1 of half a block (cache8.cuh v8_place)
+              float x, y;
+              unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
+              x = ex2(x);
+              y = ex2(y);
+              if (i & 1) sum1 = add2(sum1, pack2(x, y));
+              else sum0 = add2(sum0, pack2(x, y));
+              p[i] = f16x2(x, y);
+            }
+            tmem_st_x8(s_t + c * 16 + k * 8, p);   // (over scores that have been read)
+          }
         }
         tmem_st_wait();
         tc_fence_before();
@@ -688,12 +728,14 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       if (!ok) break;
       oph ^= 1;
       tc_fence_after();
+      l += pair_up(l);
+      if (!ok) break;
       const int row = t.row0 + in_unit, qhead = t.kvh * a.G + head;
       if (t.cut == 0) {
         const float inv = l == 0.f ? 0.f : unit / l;
-        __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)qhead * HEAD_DIM;
+        __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)qhead * HEAD_DIM + h * 64;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t o[32];
           tmem_ld_x32(o_t + c * 32, o);
           tmem_ld_wait();
@@ -709,9 +751,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         }
       } else {
         const size_t slot = ((size_t)blockIdx.x * 2 + ((t.cut & 1) == 0)) * 256 + g * 128 + r;
-        float* dst = a.frag_o + slot * HEAD_DIM;
+        float* dst = a.frag_o + slot * HEAD_DIM + h * 64;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t o[32];
           tmem_ld_x32(o_t + c * 32, o);
           tmem_ld_wait();
@@ -722,7 +764,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
                                                                             __uint_as_float(o[i * 4 + 2]) * unit, __uint_as_float(o[i * 4 + 3]) * unit);
           }
         }
-        if (mine) *reinterpret_cast<float2*>(a.frag_ml + slot * 2) = make_float2(m, l);
+        if (mine && h == 0) *reinterpret_cast<float2*>(a.frag_ml + slot * 2) = make_float2(m, l);
       }
       tc_fence_before();
       done_with();
@@ -743,52 +785,34 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
   }
 }
 
-// A unit that is cut behind CTA b's stretch and begins in it: its parts joined in the order of the keys, a warp a row
+// A unit that begins in CTA blockIdx.x's stretch and ends behind it: its parts joined in the order of the keys, a warp a row
 constexpr int J8_WARPS = 8;
-__global__ void __launch_bounds__(J8_WARPS * 32) attn8_join_kernel(const __grid_constant__ PromptArgs a, int n_ctas) {
-  extern __shared__ uint32_t prefix_s[];
-  __shared__ uint32_t wsum[J8_WARPS];
+__global__ void __launch_bounds__(J8_WARPS * 32) attn8_join_kernel(const __grid_constant__ PromptArgs a) {
   griddep_launch();
   griddep_wait();
-  const uint32_t total = lay_out<J8_WARPS * 32>(a, prefix_s, wsum);
-  const uint32_t begin = stretch_begin(total, blockIdx.x, n_ctas), end = stretch_begin(total, blockIdx.x + 1, n_ctas);
-  if (end <= begin || end >= total) return;
-  Walk w(a, prefix_s, end - 1, total);
-  const uint32_t place = w.find(), left = w.steps + P8_COST - 1 - place;   // places of the unit behind the stretch
-  if (left == 0 || place < P8_COST) return;                 // not cut, or no step of it taken
-  if (place > end - 1 - begin + P8_COST) return;            // begun before the stretch (its first step, not what goes ahead of it)
-  const int last = (int)cta_of(total, end - 1 + left, n_ctas);   // CTA with the unit's last step
-  const int lane = (int)lane_id(), n = last - (int)blockIdx.x + 1, half = w.half();
-  {
-    const int r = blockIdx.y * J8_WARPS + (threadIdx.x >> 5);
-    const int tok = (r & 127) / a.G, head = (r & 127) - tok * a.G, in_unit = (r >> 7) * half + tok;
-    if (tok >= half || in_unit >= w.tokens()) return;
-    // part k: of CTA blockIdx.x + k; its first is that of a unit begun there
-    auto slot = [&](int k) { return ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * 256 + r; };
-    float m = -INFINITY;
-    auto there = [&](int k) {                               // (CTAs without steps leave nothing)
-      return stretch_begin(total, blockIdx.x + k + 1, n_ctas) > stretch_begin(total, blockIdx.x + k, n_ctas);
-    };
-    for (int k = lane; k < n; k += 32)
-      if (there(k)) m = fmaxf(m, a.frag_ml[slot(k) * 2]);
+  const CutUnit u = a.cut[blockIdx.x];
+  const int lane = (int)lane_id(), r = blockIdx.y * J8_WARPS + (threadIdx.x >> 5);
+  const int tok = (r & 127) / a.G, head = (r & 127) - tok * a.G, in_unit = (r >> 7) * u.half + tok;
+  if (u.parts == 0 || tok >= u.half || in_unit >= u.tokens) return;
+  // part k: of CTA blockIdx.x + k; its first is that of a unit begun there
+  auto slot = [&](int k) { return ((size_t)(blockIdx.x + k) * 2 + (k == 0)) * 256 + r; };
+  float m = -INFINITY;
+  for (int k = lane; k < u.parts; k += 32) m = fmaxf(m, a.frag_ml[slot(k) * 2]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-      if (!there(k)) continue;
-      const float2 ml = *reinterpret_cast<const float2*>(a.frag_ml + slot(k) * 2);
-      const float4 v = reinterpret_cast<const float4*>(a.frag_o + slot(k) * HEAD_DIM)[lane];
-      const float f = ex2(ml.x - ref);
-      l += ml.y * f;
-      x[0] += v.x * f; x[1] += v.y * f; x[2] += v.z * f; x[3] += v.w * f;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int row = w.u.sq.q_start + w.i * w.u.tokens + in_unit;
-    *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)(w.kvh * a.G + head) * HEAD_DIM + lane * 4) =
-        make_uint2(cvt2(x[0] * inv, x[1] * inv), cvt2(x[2] * inv, x[3] * inv));
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < u.parts; ++k) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.frag_ml + slot(k) * 2);
+    const float4 v = reinterpret_cast<const float4*>(a.frag_o + slot(k) * HEAD_DIM)[lane];
+    const float f = ex2(ml.x - ref);
+    l += ml.y * f;
+    x[0] += v.x * f; x[1] += v.y * f; x[2] += v.z * f; x[3] += v.w * f;
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(a.out + (size_t)(u.row0 + in_unit) * a.ldo + (size_t)(u.kvh * a.G + head) * HEAD_DIM + lane * 4) =
+      make_uint2(cvt2(x[0] * inv, x[1] * inv), cvt2(x[2] * inv, x[3] * inv));
 }
 
 }  // namespace
@@ -800,7 +824,7 @@ bool attn8_prompt_takes(int T, int n_seqs, int n_q, int n_kv, int max_q, int max
   return steps < 2e9;
 }
 
-size_t attn8_prompt_workspace(int num_sms) { return (size_t)num_sms * 2 * 256 * (HEAD_DIM + 2) * sizeof(float); }
+size_t attn8_prompt_workspace(int num_sms) { return (size_t)num_sms * (2 * 256 * (HEAD_DIM + 2) * sizeof(float) + sizeof(CutUnit)); }
 
 cudaError_t attn8_prompt_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream) {
   PromptArgs a;
@@ -817,9 +841,10 @@ cudaError_t attn8_prompt_launch(const Attn8Args& args, void* workspace, int num_
   const int grid = (int)std::max<long long>(1, std::min<long long>(num_sms, units * ((a.max_kv + P8_KV - 1) / P8_KV)));
   a.frag_o = reinterpret_cast<float*>(workspace);
   a.frag_ml = a.frag_o + (size_t)num_sms * 2 * 256 * HEAD_DIM;
+  a.cut = reinterpret_cast<CutUnit*>(a.frag_ml + (size_t)num_sms * 2 * 256 * 2);
   e = launch_k(attn8_prompt_kernel, dim3(grid), dim3(P8_THREADS), smem, stream, a);
   if (e != cudaSuccess || grid == 1 || a.max_kv <= P8_KV) return e;   // (units of one step are never cut)
-  return launch_k(attn8_join_kernel, dim3(grid, 256 / J8_WARPS), dim3(J8_WARPS * 32), a.n_seqs * 4, stream, a, grid);
+  return launch_k(attn8_join_kernel, dim3(grid, 256 / J8_WARPS), dim3(J8_WARPS * 32), 0, stream, a);
 }
 
 }  // namespace tgis
