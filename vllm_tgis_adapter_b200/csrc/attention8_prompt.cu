@@ -75,7 +75,6 @@ struct P8Smem {
   uint32_t absent[P8_STAGES];  // by the copying warp
   uint32_t tmem_base;
   int gave_up;
-  uint32_t wsum[P8_THREADS / 32];
   uint32_t prefix[1];          // steps ahead of each sequence
 };
 static_assert((2 * P8_TILE + 2 * P8_TILE) % 1024 == 0 && sizeof(((P8Smem*)0)->raw[0]) % 128 == 0 && offsetof(P8Smem, raw) % 128 == 0 && KV8_PAGE % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, raw_full) % 8 == 0, "");
@@ -90,6 +89,7 @@ struct CutUnit {
 };
 struct PromptArgs : Attn8Args {
   int G, TM;
+  uint32_t per_g;              // row / G = row * per_g >> 16 for rows below 128
   float *frag_o, *frag_ml;     // [CTA][0: of a unit begun before it, 1: of one that ends behind it][256 rows]([128])
   CutUnit* cut;                // [CTA]
 };
@@ -113,18 +113,18 @@ __device__ __forceinline__ int keys_of(const PromptArgs& a, const SeqUnits& u, i
 }
 __device__ __forceinline__ int steps_of(const PromptArgs& a, const SeqUnits& u, int i) { return (keys_of(a, u, i) + P8_KV - 1) / P8_KV; }
 
-// steps of all sequences ahead of each; by every thread of a CTA of THREADS
-template <int THREADS>
-__device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefix, uint32_t* wsum) {
-  const int warp = threadIdx.x >> 5, lane = (int)lane_id();
+// steps of all sequences ahead of each, by one warp; their sum
+__device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefix) {
+  const int lane = (int)lane_id();
   uint32_t carry = 0;
-  for (int base = 0; base < a.n_seqs; base += THREADS) {
-    const int s = base + threadIdx.x;
+  for (int base = 0; base < a.n_seqs; base += 32) {
+    const int s = base + lane;
     uint32_t n = 0;
     if (s < a.n_seqs) {
       const SeqUnits u = units_of(a, s);
       for (int i = 0; i < u.n_units; ++i) n += P8_COST + (uint32_t)steps_of(a, u, i);
       n *= (uint32_t)a.n_kv;
+      if (u.n_units == 0 && blockIdx.x == 0 && a.status != nullptr && !seq_fits(a, load_seq(a, s))) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
     }
     uint32_t sum = n;
 #pragma unroll
@@ -132,16 +132,10 @@ __device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefi
       const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    if (lane == 31) wsum[warp] = sum;
-    __syncthreads();
-    uint32_t before = carry;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) before += wsum[w];
-      carry += wsum[w];
-    }
-    if (s < a.n_seqs) prefix[s] = before + sum - n;
-    __syncthreads();
+    if (s < a.n_seqs) prefix[s] = carry + sum - n;
+    carry += __shfl_sync(0xffffffffu, sum, 31);
   }
+  __syncwarp();
   return carry;
 }
 __device__ __forceinline__ uint32_t stretch_begin(uint32_t total, uint32_t cta, uint32_t n) { return (uint32_t)((uint64_t)total * cta / n); }
@@ -272,15 +266,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     tmem_alloc<512>(&sm.tmem_base);
   }
   griddep_launch();
-  griddep_wait();
-  if (blockIdx.x == 0 && a.status != nullptr)
-    for (int s = threadIdx.x; s < a.n_seqs; s += P8_THREADS)
-      if (!seq_fits(a, load_seq(a, s))) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
-  const uint32_t total = lay_out<P8_THREADS>(a, sm.prefix, sm.wsum);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = sm.tmem_base;   // [S0 | S1 | O0 | O1], 128 columns each
+  griddep_wait();
   bool ok = true;
   int ti = 0;                                // list of tasks
   uint32_t tph = 0;
@@ -298,6 +288,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     set_regs<P8_REGS_OTHER, false>();
     if (warp == P8_WARP_COPY) {
       // ===================== walk, copies =====================
+      const uint32_t total = lay_out(a, sm.prefix);
       const uint32_t n = min(gridDim.x, total), b = min(blockIdx.x, n);   // (no stretch of the first n is empty)
       Walk w(a, sm.prefix, n > 0 ? stretch_begin(total, b, n) : 0u, n > 0 ? stretch_begin(total, min(b + 1, n), n) : 0u);
       int st = 0;
@@ -366,7 +357,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       auto operand = [](const uint8_t* p, int ks) { return make_smem_desc_sw128(smem_u32(p) + (ks >> 2) * (P8_TILE / 2) + (ks & 3) * 32); };   // 16 numbers along k
       auto scores = [&](int g, int nb) {
         const uint32_t idesc = idesc_of(128, nb * KV_BLOCK);
-#pragma unroll
+#pragma unroll 2
         for (int ks = 0; ks < HEAD_DIM / 16; ++ks) tc_mma_f16(tmem_base + g * 128, operand(sm.q[g], ks), operand(sm.k, ks), idesc, ks > 0);
         tc_commit(&sm.s_full[g]);
       };
@@ -485,7 +476,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           };
           if (mine < tp->blocks(j)) {
             const uint32_t from = smem_u32(sm.raw[st]) + (uint32_t)mine * KV8_PAGE + (uint32_t)lane * HEAD_DIM + swizzle;
-#pragma unroll
+#pragma unroll 1
             for (int d0 = 0; d0 < HEAD_DIM / 16; d0 += 2) {
               uint4 x[2];
 #pragma unroll
@@ -512,9 +503,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           v_empty ^= 1;
           const int nh = 2 * tp->blocks(j);
           const uint32_t from = smem_u32(sm.raw[stage]) + KV8_CODES + (uint32_t)part * 16, mul = v_mul + odd * (P8_KV * 2);
-#pragma unroll
-          for (int h0 = 0; h0 < 2 * P8_BLOCKS; h0 += 2) {
-            if (h0 >= nh) break;
+#pragma unroll 1
+          for (int h0 = 0; h0 < nh; h0 += 2) {
             uint4 x[2], m[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -556,17 +546,20 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     // ===================== softmax: two threads a row, 64 columns (and dims) each =====================
     set_regs<P8_REGS_SOFTMAX, true>();
     const int g = warp >> 3, h = warp >> 2 & 1, quarter = warp & 3;
-    const int r = quarter * 32 + lane, tok = r / a.G, head = r - tok * a.G;
+    const int r = quarter * 32 + lane, tok = (int)(r * a.per_g >> 16);
     const uint32_t s_t = tmem_base + g * 128 + ((uint32_t)(quarter * 32) << 16) + h * 64, o_t = s_t + 256;
     uint32_t sph = 0, oph = 0, tile = 0, met = 0;   // tile: of the CTA; met: times that the row's threads have told one another something
     // this thread's number said, the other one's heard
-    auto pair_up = [&](float mine) {
-      float(*to)[128] = sm.pair[met & 1][g];
-      to[h][r] = mine;
+    auto meet = [&]() {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.pair_full[g][quarter]);
       ok = __all_sync(0xffffffffu, bounded_wait(&sm.pair_full[g][quarter], met & 1));
       ++met;
+    };
+    auto pair_up = [&](float mine) {
+      float(*to)[128] = sm.pair[met & 1][g];
+      to[h][r] = mine;
+      meet();
       return to[h ^ 1][r];
     };
     while (const Task* tp = take()) {
@@ -582,31 +575,47 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       unsigned long long word = 0;
       if (!mine) lim = 0x7fffffff;
       else if (a.tree != nullptr) lim = t.before - 1, word = a.tree[t.row0 + in_unit] & ((unsigned long long)t.word_mask_hi << 32 | t.word_mask_lo);
-      // ---- the row of Q, its largest number at 128 to 256
+      // ---- Q, every row's largest number at 128 to 256.  Eight lanes read a half row of 128 bytes, four rows at a time
+      const int sub = lane >> 3, at = lane & 7;
+      auto row_of = [&](int i, int& global_row, int& qhead) {   // the i-th of this lane's eight rows; whether it is one
+        const int rr = quarter * 32 + i * 4 + sub, tk = (int)(rr * a.per_g >> 16), iu = g * t.half + tk;
+        global_row = t.row0 + iu;
+        qhead = t.kvh * a.G + rr - tk * a.G;
+        return tk < t.half && iu < t.tokens;
+      };
       float qm;
       {
-        uint4 x[HEAD_DIM / 16];
-        uint32_t top = 0;
-        const uint4* from = reinterpret_cast<const uint4*>(a.q + (size_t)(t.row0 + in_unit) * a.ldq + (size_t)(t.kvh * a.G + head) * HEAD_DIM + h * 64);
+        uint4 x[8];
 #pragma unroll
-        for (int c = 0; c < HEAD_DIM / 16; ++c) {
-          x[c] = mine ? from[c] : make_uint4(0, 0, 0, 0);
-          const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(v[i] << 16 & 0x7fff0000u, v[i] & 0x7fff0000u));
+        for (int i = 0; i < 8; ++i) {
+          int grow, qhead;
+          x[i] = row_of(i, grow, qhead) ? *reinterpret_cast<const uint4*>(a.q + (size_t)grow * a.ldq + (size_t)qhead * HEAD_DIM + h * 64 + at * 8) : make_uint4(0, 0, 0, 0);
         }
-        top = max(top, __float_as_uint(pair_up(__uint_as_float(top))));
-        if (!ok) break;
-        float up = power_up(top);
-        qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / up;   // (hidden scores are -inf before they are scaled)
-        if (a.scale < 0.f) up = -up;
+        float(*say)[128] = sm.pair[met & 1][g];
 #pragma unroll
-        for (int c = 0; c < HEAD_DIM / 16; ++c) {
-          const uint32_t v[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(v[k] << 16 & 0x7fff0000u, v[k] & 0x7fff0000u));
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (at == 0) say[h][quarter * 32 + i * 4 + sub] = __uint_as_float(top);
+        }
+        meet();
+        if (!ok) break;
+        auto top_of = [&](int row) { return max(__float_as_uint(say[0][row]), __float_as_uint(say[1][row])); };
+        const uint32_t top = top_of(r);
+        qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / power_up(top);   // (hidden scores are -inf before they are scaled)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int rr = quarter * 32 + i * 4 + sub;
+          const float up = a.scale < 0.f ? -power_up(top_of(rr)) : power_up(top_of(rr));
+          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
           uint32_t w[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = f16x2(__uint_as_float(v[i] << 16) * up, __uint_as_float(v[i] & 0xffff0000u) * up);
-          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < 4; ++k) w[k] = f16x2(__uint_as_float(v[k] << 16) * up, __uint_as_float(v[k] & 0xffff0000u) * up);
+          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(rr, h * 8 + at)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
       fence_proxy_async();
@@ -644,15 +653,15 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           for (int i = 0; i < 32; ++i)
             if (!(seen_of_it >> i & 1)) s[i] = __float_as_uint(-INFINITY);
         };
-        // the scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill)
+        // The scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill).  The loops are not
+        // unrolled: the instruction cache does not hold the roles' code if they are
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (c >= nb) break;
+#pragma unroll 1
+        for (int c = 0; c < min(nb, 2); ++c) {
           uint32_t s[32];
           tmem_ld_x32(s_t + c * 32, s);
           tmem_ld_wait();
-          if (mask) hide(s, vis[c]);
+          if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
@@ -687,13 +696,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         const bool large = fabsf(ref) > 0x1p20f;
         if (large) qm2 = pack2(1.f, 1.f);
         uint64_t sum0 = 0, sum1 = 0;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (c >= nb) break;
+#pragma unroll 1
+        for (int c = 0; c < min(nb, 2); ++c) {
           uint32_t s[32];
           tmem_ld_x32(s_t + c * 32, s);
           tmem_ld_wait();
-          if (mask) hide(s, vis[c]);
+          if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
           if (large) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
@@ -730,42 +738,42 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       tc_fence_after();
       l += pair_up(l);
       if (!ok) break;
-      const int row = t.row0 + in_unit, qhead = t.kvh * a.G + head;
-      if (t.cut == 0) {
-        const float inv = l == 0.f ? 0.f : unit / l;
-        __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)qhead * HEAD_DIM + h * 64;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t o[32];
-          tmem_ld_x32(o_t + c * 32, o);
-          tmem_ld_wait();
-          if (mine) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t v[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] = cvt2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = make_uint4(v[0], v[1], v[2], v[3]);
-            }
-          }
+      // the rows leave through shared memory, where this warp's part of Q was (the last scores are done): eight lanes then write 128 bytes of one
+      auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c)) = make_uint4(x, y, z, w); };
+      auto send = [&](auto&& to) {
+        __syncwarp();
+#pragma unroll 2
+        for (int i = 0; i < 8; ++i) {
+          int grow, qhead;
+          if (row_of(i, grow, qhead)) *to(quarter * 32 + i * 4 + sub, grow, qhead) = *reinterpret_cast<const uint4*>(sm.q[g] + p8_at(quarter * 32 + i * 4 + sub, h * 8 + at));
         }
-      } else {
-        const size_t slot = ((size_t)blockIdx.x * 2 + ((t.cut & 1) == 0)) * 256 + g * 128 + r;
-        float* dst = a.frag_o + slot * HEAD_DIM + h * 64;
+        __syncwarp();
+      };
+      const float by = t.cut != 0 ? unit : l == 0.f ? 0.f : unit / l;
+      const size_t slot = ((size_t)blockIdx.x * 2 + ((t.cut & 1) == 0)) * 256 + g * 128;
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t o[32];
+        tmem_ld_x32(o_t + c * 32, o);
+        tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t o[32];
-          tmem_ld_x32(o_t + c * 32, o);
-          tmem_ld_wait();
-          if (mine) {
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+        if (t.cut == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4*>(dst + c * 32 + i * 4) = make_float4(__uint_as_float(o[i * 4]) * unit, __uint_as_float(o[i * 4 + 1]) * unit,
-                                                                            __uint_as_float(o[i * 4 + 2]) * unit, __uint_as_float(o[i * 4 + 3]) * unit);
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = cvt2(__uint_as_float(o[i * 8 + 2 * k]), __uint_as_float(o[i * 8 + 2 * k + 1]));
+            put(c * 4 + i, v[0], v[1], v[2], v[3]);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) put(i, o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+          send([&](int rr, int, int) { return reinterpret_cast<uint4*>(a.frag_o + (slot + rr) * HEAD_DIM + h * 64 + c * 32) + at; });
         }
-        if (mine && h == 0) *reinterpret_cast<float2*>(a.frag_ml + slot * 2) = make_float2(m, l);
       }
+      if (t.cut == 0) send([&](int, int grow, int qhead) { return reinterpret_cast<uint4*>(a.out + (size_t)grow * a.ldo + (size_t)qhead * HEAD_DIM + h * 64) + at; });
+      else if (mine && h == 0) *reinterpret_cast<float2*>(a.frag_ml + (slot + r) * 2) = make_float2(m, l);
       tc_fence_before();
       done_with();
     }
@@ -831,6 +839,7 @@ cudaError_t attn8_prompt_launch(const Attn8Args& args, void* workspace, int num_
   static_cast<Attn8Args&>(a) = args;
   a.G = a.n_q / a.n_kv;
   a.TM = 128 / a.G;
+  a.per_g = (65536 + a.G - 1) / a.G;
   const size_t smem = sizeof(P8Smem) + 1024 + (size_t)a.n_seqs * 4;
   static OncePerDevice once;
   cudaError_t e = once([] {
