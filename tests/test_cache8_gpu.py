@@ -2,8 +2,9 @@
 
 Tolerances.  Stored rows: x / s is rounded to 3 bits behind the first: half a step, 2^-4 relative, or 2^-10 s below the normal range (2^-6 s);
 the code of an fp32 rotation may be that of the neighbouring step where the 64-bit one lies on the border.  Attention reads exact
-operands (codes times scales); a probability keeps 8 bits (2^-8 at most, as hi + lo / 16 with 4 bits each) and the result is rounded to bf16
-(2^-9 of the value is half a step): |out - exact| <= (2^-8 + 2^-9 + 2^-12) * sum p |v| elementwise, 2^-12 covering fp32 sums, exponentials and scores.
+operands (codes times scales); a probability is taken to f16 (2^-12) and keeps 8 bits (2^-8 at most, as hi + lo / 16 with 4 bits each) and the result
+is rounded to bf16 (2^-9 of the value is half a step): |out - exact| <= (2^-8 + 2^-9 + 2^-11) * sum p |v| elementwise, 2^-12 of which cover fp32 sums,
+exponentials and scores.
 A probability times its row's scale s also loses up to half of e4m3's smallest step, 2^-10, of its lo part, 2^-14 where the largest of its 32 tokens
 is brought to 128 at least: 2^-21 of that one, which is at most max s (p <= 1, and the sum of p that all is divided by is 1 at least).  A number c s
 of the sum is off by 2^-21 |c| max s: 2^-21 max s * sum |c| in all, where a row with large weight holds zeros for codes.
@@ -20,7 +21,7 @@ from vllm_tgis_adapter_b200.engine.cache8 import PAGE_BYTES, Cache8
 
 pytestmark = pytest.mark.gpu
 D, PAGE, TINY = 128, 32, 2.0 ** -126
-TOL = 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -12
+TOL = 2.0 ** -8 + 2.0 ** -9 + 2.0 ** -11
 
 
 def to_e4m3(y: torch.Tensor) -> torch.Tensor:

@@ -26,8 +26,8 @@
 namespace tgis {
 namespace {
 
-constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 3, R8_MINB = 2;
-constexpr int R8_SPLIT = 128;                 // tokens of a split
+constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
+constexpr int R8_CTAS(int mt) { return mt == 1 ? 3 : 2; }   // per SM
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
@@ -39,6 +39,12 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// C = A B
+__device__ __forceinline__ void mma_e4m3_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -49,7 +55,7 @@ struct RowsItem {
 };
 
 template <int MT>
-__global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_s[R8_WARPS * R8_RING];
   __shared__ int32_t ok_s[R8_WARPS * R8_RING], wsum[R8_WARPS];
@@ -95,12 +101,11 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
     carry += total;
     __syncthreads();
   }
-  const long long n_flat = (long long)carry * a.n_kv;
-  const long long n_slots = (long long)gridDim.x * R8_WARPS;
-  auto item_at = [&](long long f) {
+  const uint32_t n_flat = (uint32_t)carry * a.n_kv, n_slots = gridDim.x * R8_WARPS;   // (host: no more than 2^31)
+  auto item_at = [&](uint32_t f) {
     RowsItem it;
-    const int e = (int)(f / a.n_kv);
-    it.kvh = (int)(f - (long long)e * a.n_kv);
+    const int e = (int)(f / (uint32_t)a.n_kv);
+    it.kvh = (int)(f - (uint32_t)(e * a.n_kv));
     int lo = 0, hi = a.n_seqs;                // last sequence whose items begin at or before e (those without items share a start)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -121,10 +126,10 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
     const int b = jb + lane;
     return b < it.n_blk() ? a.block_table[(size_t)it.sq.block_row * a.bt_stride + it.tok0 / KV_BLOCK + b] : 0;
   };
-  long long f = (long long)warp * gridDim.x + blockIdx.x;   // consecutive items land on different SMs
+  uint32_t f = warp * gridDim.x + blockIdx.x;   // consecutive items land on different SMs
   if (f >= n_flat) return;
   // ---- issue cursor: RING blocks ahead of the consumer; the item after its own is decoded when it enters its own
-  long long i_f = f;
+  uint32_t i_f = f;
   RowsItem i_it = item_at(f), i_nxt = i_it;
   int i_pages = page_of(i_it, 0), i_pages_nxt = 0, i_jb = 0, i_st = 0;
   auto ahead = [&]() {
@@ -171,7 +176,8 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
     const int n_rows = it.sq.q_len * G, prefix_len = it.sq.kv_len - it.sq.q_len;
     // ---- this thread's rows: fragments, scale into the exp2 domain, what they see
     uint32_t qa[MT][4][4];
-    float q_mul[MT], m_r[MT], l_r[MT], o[MT][16][2];
+    float q_mul[MT], m_r[MT], l_r[MT];
+    uint64_t o[MT][16];                       // two dims each
     int row_q[MT], head[MT], lim[MT];         // lim: causal, last token seen
     unsigned long long word[MT];
 #pragma unroll
@@ -210,7 +216,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
       m_r[mt] = -INFINITY;
       l_r[mt] = 0.f;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) o[mt][n][0] = o[mt][n][1] = 0.f;
+      for (int n = 0; n < 16; ++n) o[mt][n] = 0;
     }
     // every row of the chunk sees the tokens below this one
     const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * 8 * MT / G + 1 : 0);
@@ -230,10 +236,6 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
         // ---- S = Q K^T: 4 tiles of 8 tokens x 4 steps of 32 dims
         float s[MT][4][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
-#pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int kp = 0; kp < 2; ++kp) {
@@ -241,13 +243,14 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
             ldsm_x4(kb, k_base + (8 * j + ri) * HEAD_DIM + (((4 * kp + mi) ^ ri) << 4));
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma_e4m3(s[mt][j], qa[mt][2 * kp], kb[0], kb[1]);
+              if (kp == 0) mma_e4m3_first(s[mt][j], qa[mt][0], kb[0], kb[1]);
+              else mma_e4m3(s[mt][j], qa[mt][2 * kp], kb[0], kb[1]);
               mma_e4m3(s[mt][j], qa[mt][2 * kp + 1], kb[2], kb[3]);
             }
           }
         // ---- softmax: this thread has tokens 8 j + 2 t4 + e of its rows
         uint32_t pa[MT][4];
-        float keep[MT], add[MT];              // what the row's sums are multiplied by, and this block's products
+        uint64_t keep2[MT], add_hi[MT], add_lo[MT];   // what the row's sums are multiplied by, and this block's products
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           float x[4][2], top = -INFINITY;
@@ -277,25 +280,36 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const float m_new = fmaxf(m_r[mt], top);
           const float here = top == -INFINITY ? 0.f : top;   // (no score above -inf: every probability is 0, not the NaN of inf - inf)
-          const float part = top == -INFINITY ? 0.f : exp2f(top - m_new);
-          keep[mt] = m_r[mt] == -INFINITY ? 0.f : exp2f(m_r[mt] - m_new);
+          const float part = top == -INFINITY ? 0.f : ex2(top - m_new);
+          const float keep = m_r[mt] == -INFINITY ? 0.f : ex2(m_r[mt] - m_new);
+          keep2[mt] = pack2(keep, keep);
           m_r[mt] = m_new;
           float sum = 0.f, most = 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 vs = *reinterpret_cast<const float2*>(v_scale + 8 * j + 2 * t4);
-            x[j][0] = exp2f(x[j][0] - here);
-            x[j][1] = exp2f(x[j][1] - here);
+            x[j][0] = ex2(x[j][0] - here);
+            x[j][1] = ex2(x[j][1] - here);
             sum += x[j][0] + x[j][1];
-            x[j][0] = hid >> (2 * j) & 1 ? 0.f : x[j][0] * vs.x;
-            x[j][1] = hid >> (2 * j + 1) & 1 ? 0.f : x[j][1] * vs.y;
-            most = fmaxf(most, fmaxf(x[j][0], x[j][1]));
+            x[j][0] *= vs.x;
+            x[j][1] *= vs.y;
           }
-          l_r[mt] = l_r[mt] * keep[mt] + sum * (sum == 0.f ? 0.f : part);
+          if (open) {                         // (a hidden row's scale may be NaN)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (hid >> (2 * j + e) & 1) x[j][e] = 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(x[j][0], x[j][1]));
+          l_r[mt] = l_r[mt] * keep + sum * (sum == 0.f ? 0.f : part);
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
           const float up = power_up(__float_as_uint(most));
-          add[mt] = part / up;
+          const float add = part * one_over(up);
+          add_hi[mt] = pack2(add, add);
+          add_lo[mt] = pack2(add * (1.f / KV8_LO), add * (1.f / KV8_LO));
           split4(x[0][0] * up, x[0][1] * up, x[1][0] * up, x[1][1] * up, pa[mt][0], pa[mt][1]);
           split4(x[2][0] * up, x[2][1] * up, x[3][0] * up, x[3][1] * up, pa[mt][2], pa[mt][3]);
         }
@@ -308,10 +322,9 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float c[4] = {0.f, 0.f, 0.f, 0.f};
-              mma_e4m3(c, pa[mt], vb[2 * h], vb[2 * h + 1]);
-              o[mt][n + h][0] = fmaf(fmaf(c[2], 1.f / KV8_LO, c[0]), add[mt], o[mt][n + h][0] * keep[mt]);
-              o[mt][n + h][1] = fmaf(fmaf(c[3], 1.f / KV8_LO, c[1]), add[mt], o[mt][n + h][1] * keep[mt]);
+              float c[4];
+              mma_e4m3_first(c, pa[mt], vb[2 * h], vb[2 * h + 1]);
+              o[mt][n + h] = fma2(pack2(c[2], c[3]), add_lo[mt], fma2(pack2(c[0], c[1]), add_hi[mt], mul2(o[mt][n + h], keep2[mt])));
             }
         }
       }
@@ -333,15 +346,16 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
         uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)row_q[mt] * a.ldo + (size_t)head[mt] * HEAD_DIM) + t4;
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
-          const __nv_bfloat162 v = __floats2bfloat162_rn(o[mt][n][0] * inv, o[mt][n][1] * inv);
-          dst[n * 4] = *reinterpret_cast<const uint32_t*>(&v);
+          float x, y;
+          unpack2(o[mt][n], x, y);
+          dst[n * 4] = cvt2(x * inv, y * inv);
         }
       } else {
         const size_t at = ((size_t)row_q[mt] * a.n_q + head[mt]) * a.max_splits + it.split;
         float2* dst = reinterpret_cast<float2*>(a.part_o + at * HEAD_DIM) + t4;
 #pragma unroll
         for (int n = 0; n < 16; ++n)
-          dst[n * 4] = make_float2(o[mt][n][0], o[mt][n][1]);
+          reinterpret_cast<uint64_t*>(dst)[n * 4] = o[mt][n];
         if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_r[mt], l);
       }
     }
@@ -353,40 +367,70 @@ __global__ void __launch_bounds__(R8_THREADS, R8_MINB) attn8_rows_kernel(const _
   }
 }
 
-// Splits of a row joined in their order, one warp a (query, head)
-__global__ void __launch_bounds__(256) attn8_merge_kernel(const __grid_constant__ RowsArgs a) {
+// Splits of a row joined, PARTS warps a (query, head): each joins a stretch of them in their order, then the first joins the stretches
+constexpr int M8_WARPS = 8;
+template <int PARTS>
+__global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid_constant__ RowsArgs a) {
+  __shared__ float4 part_x[PARTS > 1 ? M8_WARPS : 1][32];
+  __shared__ float2 part_ml[PARTS > 1 ? M8_WARPS : 1];
   griddep_launch();
   griddep_wait();
   const AttnSeq sq = load_seq(a, blockIdx.x);
   if (!seq_fits(a, sq)) return;
-  const int lane = (int)lane_id(), n_splits = (sq.kv_len + a.split - 1) / a.split;
+  const int lane = (int)lane_id(), warp = threadIdx.x >> 5, n_splits = (sq.kv_len + a.split - 1) / a.split;
   if (n_splits <= 1) return;
-  for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < sq.q_len * a.n_q; i += gridDim.y * 8) {
+  const int n_rows = sq.q_len * a.n_q, step = gridDim.y * (M8_WARPS / PARTS);
+  for (int base = blockIdx.y * (M8_WARPS / PARTS); base < n_rows; base += step) {
+    const int i = base + warp / PARTS, part = warp % PARTS, per = (n_splits + PARTS - 1) / PARTS, s0 = part * per, s1 = min(s0 + per, n_splits);
     const int t = sq.q_start + i / a.n_q, head = i % a.n_q;
-    const size_t at = ((size_t)t * a.n_q + head) * a.max_splits;
-    float m = -INFINITY;
-    for (int s = lane; s < n_splits; s += 32) m = fmaxf(m, a.part_ml[(at + s) * 2]);
+    float m = -INFINITY, l = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < n_rows && s0 < s1) {
+      const size_t at = ((size_t)t * a.n_q + head) * a.max_splits;
+      for (int s = s0 + lane; s < s1; s += 32) m = fmaxf(m, a.part_ml[(at + s) * 2]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float m_use = m == -INFINITY ? 0.f : m;
-    float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < n_splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at + s) * 2);
-      const float4 v = reinterpret_cast<const float4*>(a.part_o + (at + s) * HEAD_DIM)[lane];
-      const float w = exp2f(ml.x - m_use);
-      l += ml.y * w;
-      x[0] += v.x * w; x[1] += v.y * w; x[2] += v.z * w; x[3] += v.w * w;
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+      for (int s = s0; s < s1; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at + s) * 2);
+        const float4 v = reinterpret_cast<const float4*>(a.part_o + (at + s) * HEAD_DIM)[lane];
+        const float f = ex2(ml.x - ref);
+        l += ml.y * f;
+        x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+      }
     }
+    if constexpr (PARTS > 1) {
+      part_x[warp][lane] = x;
+      if (lane == 0) part_ml[warp] = make_float2(m, l);
+      __syncthreads();
+      if (part == 0) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) top = fmaxf(top, part_ml[warp + k].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        l = 0.f;
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+          const float2 ml = part_ml[warp + k];
+          const float4 v = part_x[warp + k][lane];
+          const float f = ex2(ml.x - ref);
+          l += ml.y * f;
+          x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+        }
+      }
+      __syncthreads();
+      if (part != 0) continue;
+    }
+    if (i >= n_rows) continue;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0] * inv, x[1] * inv), hi = __floats2bfloat162_rn(x[2] * inv, x[3] * inv);
-    *reinterpret_cast<uint2*>(a.out + (size_t)t * a.ldo + (size_t)head * HEAD_DIM + lane * 4) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    *reinterpret_cast<uint2*>(a.out + (size_t)t * a.ldo + (size_t)head * HEAD_DIM + lane * 4) = make_uint2(cvt2(x.x * inv, x.y * inv), cvt2(x.z * inv, x.w * inv));
   }
 }
 
 struct RowsPlan {
-  int mt, split, max_splits;
+  int mt, split, max_splits, most_splits;     // most_splits: no call with the same rows and fewer keys has more
   bool prompt;                                // attention8_prompt.cu
 };
 RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
@@ -394,8 +438,17 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
   p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   p.mt = rows > 8 ? 2 : 1;
-  p.split = rows <= 256 ? R8_SPLIT : (std::max(max_kv, 1) + KV_BLOCK - 1) / KV_BLOCK * KV_BLOCK;
+  // Splits: the shortest with which all items run at once; where they do not, the longest that leaves three rounds of them
+  const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + 8 * p.mt - 1) / (8 * p.mt)), slots = 148. * R8_CTAS(p.mt) * R8_WARPS;
+  auto rounds = [&](int split) { return items * ((max_kv + split - 1) / split) / slots; };
+  p.split = 64;
+  while (p.split < 512 && rounds(p.split) > 1.) p.split *= 2;
+  if (rounds(p.split) > 1.)
+    while (p.split > 128 && rounds(p.split) < 3.) p.split /= 2;
+  if (rows > 16) p.split = 512;               // (many rows and few columns that attention8_prompt.cu does not take)
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
+  // (splits of 64 and more for one round; 128 and more where twice as long ones leave less than three)
+  p.most_splits = std::max(p.max_splits, (int)std::min((max_kv + 63) / 64 + 0., 6. * slots / items + 2.));
   return p;
 }
 
@@ -409,7 +462,8 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.max_q * (a.n_q / a.n_kv);
   const long long most = (long long)a.n_seqs * a.n_kv * a.max_splits * ((rows + 8 * MT - 1) / (8 * MT));
-  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_MINB * num_sms, (most + R8_WARPS - 1) / R8_WARPS));
+  if (most >= 1ll << 31) return cudaErrorInvalidValue;
+  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_CTAS(MT) * num_sms, (most + R8_WARPS - 1) / R8_WARPS));
   return launch_k(attn8_rows_kernel<MT>, dim3(grid), dim3(R8_THREADS), smem, stream, a);
 }
 
@@ -418,7 +472,7 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   const RowsPlan p = rows_plan(T, n_seqs, n_q, n_kv, max_q, max_kv);
   if (p.prompt) return attn8_prompt_workspace(ATTN8_MAX_SMS);
-  return p.max_splits > 1 ? (size_t)T * n_q * p.max_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
+  return p.most_splits > 1 ? (size_t)T * n_q * p.most_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
 }
 
 cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches) {
@@ -436,8 +490,9 @@ cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cu
   cudaError_t e = p.mt == 1 ? rows_launch<1>(a, num_sms, stream) : rows_launch<2>(a, num_sms, stream);
   if (launches != nullptr && p.max_splits == 1) *launches = 1;
   if (e != cudaSuccess || p.max_splits == 1) return e;
-  const int y = std::min((args.max_q * args.n_q + 7) / 8, 64);
-  return launch_k(attn8_merge_kernel, dim3(a.n_seqs, y), dim3(256), 0, stream, a);
+  const int per_cta = p.max_splits > 16 ? 1 : M8_WARPS, y = (int)std::min<long long>(((long long)args.max_q * args.n_q + per_cta - 1) / per_cta, 1024);
+  return p.max_splits > 16 ? launch_k(attn8_merge_kernel<M8_WARPS>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a)
+                           : launch_k(attn8_merge_kernel<1>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a);
 }
 
 }  // namespace tgis

@@ -223,8 +223,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// of a power of two from 2^-126 to 2^126
-__device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
