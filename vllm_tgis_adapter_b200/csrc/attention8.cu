@@ -1,16 +1,15 @@
 // Attention over the 8-bit paged cache (include/tgis_kv8.h; layout and number format: cache8.cuh): single tokens, drafted trees and
 // short portions on the warps' own tensor cores.
 //
-// Both products run on e4m3 operands as the cache holds them; what is not in 8 bits is written as two e4m3 numbers, x = hi + lo / 16
-// with hi = e4m3(x), lo = e4m3(16 (x - hi)).  A query row (bf16: 8 significant bits) times a power of two that brings its largest
-// number to [128, 256) is held exactly that way but for numbers 2^-14 of the largest and below, which lose less than 2^-22 of it.
-// Probabilities times the scales of their value rows (w = p s) are brought to the same range block by block and row by row, so that
-// they keep 8 bits (as bf16 would) and lose no more than 2^-22 of the largest w of their 32 tokens, whatever weight a token elsewhere
-// has; a block's products start at zero and join the row's sums in fp32.  The 16 rows of mma.m16n8k32 are thus 8 rows of queries
-// twice: hi in rows 0..7, lo in rows 8..15, and a thread that holds (row, row + 8) of an accumulator adds the two parts itself.
-// Measured on a B200: mma.m16n8k32 e4m3 3860 multiply-adds a clock and SM (bf16 1020), sums exact to 23 bits.
+// Both products are mma.sync f16 x f16 -> fp32, K and V widened in registers (exact) as their fragments leave shared memory; mma.sync on
+// e4m3 itself, with queries and probabilities as two e4m3 numbers each, costs the same tensor work and fifteen instructions each
+// (64 tokens behind 8000: 211 against XXX us).  A query row (bf16) times the power of two that brings its largest number to
+// [128, 256) is exact in f16 but for numbers 2^-22 of the largest and below.  Scores are multiplied by their key's scale in fp32; a
+// probability times its value row's scale is one f16 number of 11 bits, held times 2^7 / r, r the power of two at or above the
+// scales so far; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
+// most) and nothing above 2^-31 of the largest is lost.
 //
-// Work item = (sequence, 8 MT rows, kv head, split of the keys); row = token * G + head of the group.  Every warp walks its own items
+// Work item = (sequence, 8 or 16 rows, kv head, split of the keys); row = token * G + head of the group.  Every warp walks its own items
 // alone, its blocks of 32 tokens (one bulk copy each) requested RING blocks ahead across items; sequence lengths and pages are read
 // on the device, so the list of items is made by every CTA for itself: a prefix sum over the sequences.
 #include <algorithm>
@@ -27,23 +26,24 @@ namespace tgis {
 namespace {
 
 constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
-constexpr int R8_CTAS(int mt) { return mt == 1 ? 3 : 2; }   // per SM
+constexpr int R8_CTAS = 3;                    // per SM
+constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a score may exceed its row's reference; what probabilities are held times
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
   int max_splits, split;                      // split: tokens (a multiple of KV_BLOCK)
 };
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // C = A B
-__device__ __forceinline__ void mma_e4m3_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -54,8 +54,15 @@ struct RowsItem {
   __device__ int n_blk() const { return (n_tok + KV_BLOCK - 1) / KV_BLOCK; }
 };
 
-template <int MT>
-__global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {   // 8 x 8 f16 across the warp
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  return d;
+}
+
+template <int ROWS>
+__global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
+  constexpr int NT = ROWS / 8;                // column tiles of the products
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_s[R8_WARPS * R8_RING];
   __shared__ int32_t ok_s[R8_WARPS * R8_RING], wsum[R8_WARPS];
@@ -72,7 +79,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(con
   griddep_wait();
   const int G = a.n_q / a.n_kv;
   // ---- items of every sequence
-  auto chunks_of = [&](const AttnSeq& s) { return (s.q_len * G + 8 * MT - 1) / (8 * MT); };
+  auto chunks_of = [&](const AttnSeq& s) { return (s.q_len * G + ROWS - 1) / ROWS; };
   auto splits_of = [&](const AttnSeq& s) { return (s.kv_len + a.split - 1) / a.split; };
   int carry = 0;
   for (int base = 0; base < a.n_seqs; base += R8_THREADS) {
@@ -118,7 +125,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(con
     it.split = local - it.chunk * n_splits;
     it.tok0 = it.split * a.split;
     int end = min(it.sq.kv_len, it.tok0 + a.split);
-    if (a.tree == nullptr) end = min(end, it.sq.kv_len - it.sq.q_len + min((it.chunk + 1) * 8 * MT - 1, it.sq.q_len * G - 1) / G + 1);
+    if (a.tree == nullptr) end = min(end, it.sq.kv_len - it.sq.q_len + min((it.chunk + 1) * ROWS - 1, it.sq.q_len * G - 1) / G + 1);
     it.n_tok = max(end - it.tok0, 0);
     return it;
   };
@@ -174,52 +181,46 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(con
   for (; alive && f < n_flat; f += n_slots) {
     const RowsItem it = item_at(f);
     const int n_rows = it.sq.q_len * G, prefix_len = it.sq.kv_len - it.sq.q_len;
-    // ---- this thread's rows: fragments, scale into the exp2 domain, what they see
-    uint32_t qa[MT][4][4];
-    float q_mul[MT], m_r[MT], l_r[MT];
-    uint64_t o[MT][16];                       // two dims each
-    int row_q[MT], head[MT], lim[MT];         // lim: causal, last token seen
-    unsigned long long word[MT];
+    // ---- Q^T as B fragments: this thread has row g of each tile, of sixteen dims 4 t4 .. 4 t4 + 3
+    uint32_t qb[NT][HEAD_DIM / 16][2];
+    float q_mul[NT][2], m_r[NT][2], l_r[NT][2], o[NT][HEAD_DIM / 16][4];   // of rows 2 t4, 2 t4 + 1
+    int lim[NT][2];                           // causal: last token seen
+    unsigned long long word[NT][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int rr = it.chunk * 8 * MT + mt * 8 + g, i = rr / G;
-      row_q[mt] = rr < n_rows ? it.sq.q_start + i : -1;
-      head[mt] = it.kvh * G + rr - i * G;
-      lim[mt] = prefix_len + i;
-      word[mt] = 0;
-      if (a.tree != nullptr && row_q[mt] >= 0) word[mt] = a.tree[row_q[mt]];
-      uint32_t w[4][4];                       // k-step, (dims 4 t4 .. of its first 16, of its second 16): two words each
+    for (int n = 0; n < NT; ++n) {
+      const int rr = it.chunk * ROWS + n * 8 + g, i = rr / G;
+      const __nv_bfloat16* src = a.q + (size_t)(it.sq.q_start + i) * a.ldq + (size_t)(it.kvh * G + rr - i * G) * HEAD_DIM + 4 * t4;
+      uint2 w[HEAD_DIM / 16];
       uint32_t top = 0;
-      const __nv_bfloat16* src = a.q + (size_t)max(row_q[mt], 0) * a.ldq + (size_t)head[mt] * HEAD_DIM + 4 * t4;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint2 v = row_q[mt] >= 0 ? *reinterpret_cast<const uint2*>(src + ks * 32 + h * 16) : make_uint2(0, 0);
-          w[ks][2 * h] = v.x;
-          w[ks][2 * h + 1] = v.y;
-          top = max(max(top, max(v.x << 16 & 0x7fff0000u, v.x & 0x7fff0000u)), max(v.y << 16 & 0x7fff0000u, v.y & 0x7fff0000u));
-        }
+      for (int c = 0; c < HEAD_DIM / 16; ++c) {
+        w[c] = rr < n_rows ? *reinterpret_cast<const uint2*>(src + c * 16) : make_uint2(0, 0);
+        top = max(max(top, max(w[c].x << 16 & 0x7fff0000u, w[c].x & 0x7fff0000u)), max(w[c].y << 16 & 0x7fff0000u, w[c].y & 0x7fff0000u));
+      }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^e that brings the largest number to [128, 256); a row that is not finite: NaN, which its scores and sums then are
-      const float up = power_up(top);
-      q_mul[mt] = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * 1.4426950408889634f / up;
+      const float up = power_up(top), mul = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * 1.4426950408889634f * one_over(up);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
+      for (int c = 0; c < HEAD_DIM / 16; ++c) {
+        qb[n][c][0] = f16x2(__uint_as_float(w[c].x << 16) * up, __uint_as_float(w[c].x & 0xffff0000u) * up);
+        qb[n][c][1] = f16x2(__uint_as_float(w[c].y << 16) * up, __uint_as_float(w[c].y & 0xffff0000u) * up);
+      }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = w[ks][2 * h], y = w[ks][2 * h + 1];
-          split4(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, __uint_as_float(y << 16) * up, __uint_as_float(y & 0xffff0000u) * up,
-                 qa[mt][ks][2 * h], qa[mt][ks][2 * h + 1]);
-        }
-      m_r[mt] = -INFINITY;
-      l_r[mt] = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        const int r2 = it.chunk * ROWS + n * 8 + 2 * t4 + e, i2 = r2 / G;
+        q_mul[n][e] = __shfl_sync(0xffffffffu, mul, 4 * (2 * t4 + e));
+        lim[n][e] = prefix_len + i2;
+        word[n][e] = a.tree != nullptr && r2 < n_rows ? a.tree[it.sq.q_start + i2] : 0;
+        m_r[n][e] = -INFINITY;
+        l_r[n][e] = 0.f;
+      }
 #pragma unroll
-      for (int n = 0; n < 16; ++n) o[mt][n] = 0;
+      for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][0] = o[n][md][1] = o[n][md][2] = o[n][md][3] = 0.f;
     }
     // every row of the chunk sees the tokens below this one
-    const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * 8 * MT / G + 1 : 0);
+    const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * ROWS / G + 1 : 0);
+    float ref_v = 0x1p-118f;                  // r
     const int n_blk = it.n_blk();
     for (int jb = 0; jb < n_blk; ++jb) {
       if (!bounded_wait(&full[c_st], c_ph)) {
@@ -229,103 +230,126 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(con
       const bool ok = page_ok[c_st] != 0;
       if (ok) {
         const uint32_t k_base = ring_base + c_st * KV8_PAGE, v_base = k_base + KV8_CODES;
-        const float* k_scale = reinterpret_cast<const float*>(ring + c_st * KV8_PAGE + KV8_K_SCALES);
+        const float* k_scale = reinterpret_cast<const float*>(ring + c_st * KV8_PAGE + KV8_K_SCALES) + g;
         const float* v_scale = k_scale + KV_BLOCK;
         const int tok_b = it.tok0 + jb * KV_BLOCK;
         const bool open = tok_b + KV_BLOCK > min(seen_by_all, it.sq.kv_len);   // some row may not see some token
-        // ---- S = Q K^T: 4 tiles of 8 tokens x 4 steps of 32 dims
-        float s[MT][4][4];
+        // ---- S^T = K Q^T: 2 tiles of 16 tokens x 8 steps of 16 dims.  A register of codes is dims 4 t4 .. 4 t4 + 3 of a chunk: the step's
+        // k places 2 t4, 2 t4 + 1 and 2 t4 + 8, 2 t4 + 9, in Q^T as in K
+        float s[NT][2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int kp = 0; kp < 2; ++kp) {
-            uint32_t kb[4];
-            ldsm_x4(kb, k_base + (8 * j + ri) * HEAD_DIM + (((4 * kp + mi) ^ ri) << 4));
+          for (int cp = 0; cp < HEAD_DIM / 32; ++cp) {
+            uint32_t k[4];                    // (tokens 0 .. 7, 8 .. 15 of the tile) x (chunk 2 cp, 2 cp + 1)
+            ldsm_x4(k, k_base + (16 * mt + (mi & 1) * 8 + ri) * HEAD_DIM + (((2 * cp + (mi >> 1)) ^ ri) << 4));
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              if (kp == 0) mma_e4m3_first(s[mt][j], qa[mt][0], kb[0], kb[1]);
-              else mma_e4m3(s[mt][j], qa[mt][2 * kp], kb[0], kb[1]);
-              mma_e4m3(s[mt][j], qa[mt][2 * kp + 1], kb[2], kb[3]);
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t a0 = e4m3x2_to_f16x2(k[2 * c]), a1 = e4m3x2_to_f16x2(k[2 * c + 1]), a2 = e4m3x2_to_f16x2(k[2 * c] >> 16),
+                             a3 = e4m3x2_to_f16x2(k[2 * c + 1] >> 16);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if (cp + c == 0) mma_f16_first(s[n][mt], a0, a1, a2, a3, qb[n][0][0], qb[n][0][1]);
+                else mma_f16(s[n][mt], a0, a1, a2, a3, qb[n][2 * cp + c][0], qb[n][2 * cp + c][1]);
+              }
             }
           }
-        // ---- softmax: this thread has tokens 8 j + 2 t4 + e of its rows
-        uint32_t pa[MT][4];
-        uint64_t keep2[MT], add_hi[MT], add_lo[MT];   // what the row's sums are multiplied by, and this block's products
+        // ---- the largest value scale that is a number
+        {
+          const float v = (v_scale - g)[lane];
+          const uint32_t u = __reduce_max_sync(0xffffffffu, tok_b + lane < it.sq.kv_len && v < INFINITY ? __float_as_uint(v) : 0u);
+          if (u > __float_as_uint(ref_v)) {
+            const float to = power_above(u), ratio = ref_v * one_over(to);
+            ref_v = to;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float x[4][2], top = -INFINITY;
-          uint32_t hid = 0;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 ks = *reinterpret_cast<const float2*>(k_scale + 8 * j + 2 * t4);
-            x[j][0] = (s[mt][j][0] + s[mt][j][2] * (1.f / KV8_LO)) * (ks.x * q_mul[mt]);
-            x[j][1] = (s[mt][j][1] + s[mt][j][3] * (1.f / KV8_LO)) * (ks.y * q_mul[mt]);
+              for (int md = 0; md < HEAD_DIM / 16; ++md)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][md][i] *= ratio;
           }
-          if (open) {
+        }
+        const float v_mul = R8_HELD * one_over(ref_v);
+        // ---- softmax: this thread has tokens g + 8 i of its rows, score (i, e) in s[n][i / 2][2 (i % 2) + e]
+        float top[NT][2];
+        uint32_t hid = 0;
+        bool grows = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int i = 0; i < 4; ++i) {
+          const float ks = k_scale[8 * i];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) s[n][i >> 1][2 * (i & 1) + e] *= ks * q_mul[n][e];
+        }
+        if (open) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int tok = tok_b + 8 * j + 2 * t4 + e, node = tok - prefix_len;
-                const bool sees = tok < it.sq.kv_len && (a.tree == nullptr ? tok <= lim[mt] : node < 0 || (word[mt] >> node & 1) != 0);
+                const int tok = tok_b + 8 * i + g, node = tok - prefix_len;
+                const bool sees = tok < it.sq.kv_len && (a.tree == nullptr ? tok <= lim[n][e] : node < 0 || (word[n][e] >> node & 1) != 0);
                 if (!sees) {
-                  x[j][e] = -INFINITY;
-                  hid |= 1u << (2 * j + e);
+                  s[n][i >> 1][2 * (i & 1) + e] = -INFINITY;
+                  hid |= 1u << (n * 8 + 2 * i + e);
                 }
               }
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(x[j][0], x[j][1]));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const float m_new = fmaxf(m_r[mt], top);
-          const float here = top == -INFINITY ? 0.f : top;   // (no score above -inf: every probability is 0, not the NaN of inf - inf)
-          const float part = top == -INFINITY ? 0.f : ex2(top - m_new);
-          const float keep = m_r[mt] == -INFINITY ? 0.f : ex2(m_r[mt] - m_new);
-          keep2[mt] = pack2(keep, keep);
-          m_r[mt] = m_new;
-          float sum = 0.f, most = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 vs = *reinterpret_cast<const float2*>(v_scale + 8 * j + 2 * t4);
-            x[j][0] = ex2(x[j][0] - here);
-            x[j][1] = ex2(x[j][1] - here);
-            sum += x[j][0] + x[j][1];
-            x[j][0] *= vs.x;
-            x[j][1] *= vs.y;
-          }
-          if (open) {                         // (a hidden row's scale may be NaN)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (hid >> (2 * j + e) & 1) x[j][e] = 0.f;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) most = fmaxf(most, fmaxf(x[j][0], x[j][1]));
-          l_r[mt] = l_r[mt] * keep + sum * (sum == 0.f ? 0.f : part);
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const float up = power_up(__float_as_uint(most));
-          const float add = part * one_over(up);
-          add_hi[mt] = pack2(add, add);
-          add_lo[mt] = pack2(add * (1.f / KV8_LO), add * (1.f / KV8_LO));
-          split4(x[0][0] * up, x[0][1] * up, x[1][0] * up, x[1][1] * up, pa[mt][0], pa[mt][1]);
-          split4(x[2][0] * up, x[2][1] * up, x[3][0] * up, x[3][1] * up, pa[mt][2], pa[mt][3]);
         }
-        // ---- O += P V: 16 tiles of 8 dims, all 32 tokens in one step
 #pragma unroll
-        for (int n = 0; n < 16; n += 2) {
-          uint32_t vb[4];
-          ldsm_x4(vb, v_base + (mi & 1) * (KV8_CODES / 2) + (8 * (n + (mi >> 1)) + ri) * 16);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int e = 0; e < 2; ++e) {
+            float x = max3(fmaxf(s[n][0][e], s[n][0][2 + e]), s[n][1][e], s[n][1][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            top[n][e] = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            grows |= top[n][e] > m_r[n][e] + R8_SLACK;
+          }
+        if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float c[4];
-              mma_e4m3_first(c, pa[mt], vb[2 * h], vb[2 * h + 1]);
-              o[mt][n + h] = fma2(pack2(c[2], c[3]), add_lo[mt], fma2(pack2(c[0], c[1]), add_hi[mt], mul2(o[mt][n + h], keep2[mt])));
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const bool up = top[n][e] > m_r[n][e] + R8_SLACK;
+              const float corr = up ? ex2(m_r[n][e] - top[n][e]) : 1.f;
+              if (up) m_r[n][e] = top[n][e];
+              l_r[n][e] *= corr;
+#pragma unroll
+              for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][e] *= corr, o[n][md][2 + e] *= corr;
             }
+        }
+        uint32_t p[NT][4];                    // P^T as B fragments: tokens 8 i + 2 t4, 2 t4 + 1 of row g
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float vs = v_scale[8 * i] * v_mul;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float ref = m_r[n][e] == -INFINITY ? 0.f : m_r[n][e];   // (no score above -inf: every probability is 0, not the NaN of inf - inf)
+              x[e] = ex2(s[n][i >> 1][2 * (i & 1) + e] - ref);
+              l_r[n][e] += x[e];
+              x[e] *= vs;
+              if (open && (hid >> (n * 8 + 2 * i + e) & 1)) x[e] = 0.f;     // (a hidden row's scale may be NaN)
+            }
+            p[n][i] = movmatrix_trans(f16x2(x[0], x[1]));
+          }
+        }
+        // ---- O^T += V^T P^T: 8 tiles of 16 dims x 2 steps of 16 tokens; a register of codes is tokens 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of a dim
+#pragma unroll
+        for (int md = 0; md < HEAD_DIM / 16; ++md) {
+          uint32_t v[4];                      // (dims 0 .. 7, 8 .. 15 of the tile) x (tokens 0 .. 15, 16 .. 31)
+          ldsm_x4(v, v_base + (mi >> 1) * (KV8_CODES / 2) + (16 * md + (mi & 1) * 8 + ri) * 16);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a0 = e4m3x2_to_f16x2(v[2 * h]), a1 = e4m3x2_to_f16x2(v[2 * h + 1]), a2 = e4m3x2_to_f16x2(v[2 * h] >> 16),
+                           a3 = e4m3x2_to_f16x2(v[2 * h + 1] >> 16);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(o[n][md], a0, a1, a2, a3, p[n][2 * h], p[n][2 * h + 1]);
+          }
         }
       }
       __syncwarp();
@@ -335,30 +359,36 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(MT)) attn8_rows_kernel(con
     if (!alive) break;
     // ---- the item's rows
     const int n_splits = splits_of(it.sq);
+    const float unit = ref_v * (1.f / R8_HELD);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float l = l_r[mt];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (row_q[mt] < 0) continue;
-      if (n_splits == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + (size_t)row_q[mt] * a.ldo + (size_t)head[mt] * HEAD_DIM) + t4;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < 16; ++n) {
-          float x, y;
-          unpack2(o[mt][n], x, y);
-          dst[n * 4] = cvt2(x * inv, y * inv);
+      for (int e = 0; e < 2; ++e) {
+        float l = l_r[n][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int rr = it.chunk * ROWS + n * 8 + 2 * t4 + e, i = rr / G, row = it.sq.q_start + i, head = it.kvh * G + rr - i * G;
+        if (rr >= n_rows) continue;
+        if (n_splits == 1) {
+          const float inv = l == 0.f ? 0.f : unit / l;
+          __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)head * HEAD_DIM + g;
+#pragma unroll
+          for (int md = 0; md < HEAD_DIM / 16; ++md) {
+            dst[md * 16] = __float2bfloat16_rn(o[n][md][e] * inv);
+            dst[md * 16 + 8] = __float2bfloat16_rn(o[n][md][2 + e] * inv);
+          }
+        } else {
+          const size_t at = ((size_t)row * a.n_q + head) * a.max_splits + it.split;
+          float* dst = a.part_o + at * HEAD_DIM + g;
+#pragma unroll
+          for (int md = 0; md < HEAD_DIM / 16; ++md) {
+            dst[md * 16] = o[n][md][e] * unit;
+            dst[md * 16 + 8] = o[n][md][2 + e] * unit;
+          }
+          if (g == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_r[n][e], l);
         }
-      } else {
-        const size_t at = ((size_t)row_q[mt] * a.n_q + head[mt]) * a.max_splits + it.split;
-        float2* dst = reinterpret_cast<float2*>(a.part_o + at * HEAD_DIM) + t4;
-#pragma unroll
-        for (int n = 0; n < 16; ++n)
-          reinterpret_cast<uint64_t*>(dst)[n * 4] = o[mt][n];
-        if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_r[mt], l);
       }
-    }
   }
   if (!alive) {
     // a copy never landed: say so; those in flight are done long before this millisecond is over
@@ -430,16 +460,16 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
 }
 
 struct RowsPlan {
-  int mt, split, max_splits, most_splits;     // most_splits: no call with the same rows and fewer keys has more
+  int rows, split, max_splits, most_splits;     // most_splits: no call with the same rows and fewer keys has more
   bool prompt;                                // attention8_prompt.cu
 };
 RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   RowsPlan p{};
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
   p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
-  p.mt = rows > 8 ? 2 : 1;
+  p.rows = rows > 8 ? 16 : 8;
   // Splits: the shortest with which all items run at once; where they do not, the longest that leaves three rounds of them
-  const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + 8 * p.mt - 1) / (8 * p.mt)), slots = 148. * R8_CTAS(p.mt) * R8_WARPS;
+  const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS * R8_WARPS;
   auto rounds = [&](int split) { return items * ((max_kv + split - 1) / split) / slots; };
   p.split = 64;
   while (p.split < 512 && rounds(p.split) > 1.) p.split *= 2;
@@ -452,19 +482,19 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   return p;
 }
 
-template <int MT>
+template <int ROWS>
 cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
   const int smem = R8_WARPS * R8_RING * KV8_PAGE + a.n_seqs * 4;
   static OncePerDevice once;
   cudaError_t e = once([] {
-    return cudaFuncSetAttribute(attn8_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, R8_WARPS * R8_RING * KV8_PAGE + TGIS_KV8_MAX_SEQS * 4);
+    return cudaFuncSetAttribute(attn8_rows_kernel<ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, R8_WARPS * R8_RING * KV8_PAGE + TGIS_KV8_MAX_SEQS * 4);
   });
   if (e != cudaSuccess) return e;
   const long long rows = (long long)a.max_q * (a.n_q / a.n_kv);
-  const long long most = (long long)a.n_seqs * a.n_kv * a.max_splits * ((rows + 8 * MT - 1) / (8 * MT));
+  const long long most = (long long)a.n_seqs * a.n_kv * a.max_splits * ((rows + ROWS - 1) / ROWS);
   if (most >= 1ll << 31) return cudaErrorInvalidValue;
-  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_CTAS(MT) * num_sms, (most + R8_WARPS - 1) / R8_WARPS));
-  return launch_k(attn8_rows_kernel<MT>, dim3(grid), dim3(R8_THREADS), smem, stream, a);
+  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_CTAS * num_sms, (most + R8_WARPS - 1) / R8_WARPS));
+  return launch_k(attn8_rows_kernel<ROWS>, dim3(grid), dim3(R8_THREADS), smem, stream, a);
 }
 
 }  // namespace
@@ -487,7 +517,7 @@ cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cu
   a.max_splits = p.max_splits;
   a.part_o = reinterpret_cast<float*>(workspace);
   a.part_ml = a.part_o + (size_t)a.T * a.n_q * a.max_splits * HEAD_DIM;
-  cudaError_t e = p.mt == 1 ? rows_launch<1>(a, num_sms, stream) : rows_launch<2>(a, num_sms, stream);
+  cudaError_t e = p.rows == 8 ? rows_launch<8>(a, num_sms, stream) : rows_launch<16>(a, num_sms, stream);
   if (launches != nullptr && p.max_splits == 1) *launches = 1;
   if (e != cudaSuccess || p.max_splits == 1) return e;
   const int per_cta = p.max_splits > 16 ? 1 : M8_WARPS, y = (int)std::min<long long>(((long long)args.max_q * args.n_q + per_cta - 1) / per_cta, 1024);

@@ -9,7 +9,7 @@
 // the device.
 //
 // Both products are f16 x f16 -> fp32 (kind::f16).  Four warps widen K and V as they multiply them by their rows' scales (a code has 4 bits,
-// so a product rounded to f16's 11 is off by 2^-12; a key's scale is applied as two f16 numbers, for an error of the whole row's
+// so a product rounded to f16's 11 is off by 2^-11; a key's scale is applied as two f16 numbers, for an error of the whole row's
 // would be one of its score); both are held relative to a power of two at or above the scales, the tile's for K, that of the keys so far
 // for V.  A query row is exact in f16 but for numbers 2^-22 of its largest and below.  A probability is one f16 number of 11 bits,
 // held times 2^7; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
@@ -200,11 +200,6 @@ struct Walk {
 
 // C fp32, A and B f16, K-major
 __device__ __forceinline__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ uint32_t hmul2(uint32_t x, uint32_t y) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
@@ -223,14 +218,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-// power of two at or above a number > 0 (its bits)
-__device__ __forceinline__ float power_above(uint32_t bits) { return __uint_as_float((bits + 0x7fffffu) & 0x7f800000u); }
-
 __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __grid_constant__ PromptArgs a) {
   extern __shared__ uint8_t smem_raw[];
   P8Smem& sm = *reinterpret_cast<P8Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));

@@ -44,26 +44,6 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return f;
 }
 
-constexpr float KV8_LO = 16.f;                                 // lo parts are held times this
-// four numbers of at most 256 as hi parts and as lo parts, by way of f16 (11 bits: 2^-12 of a number; what follows is exact but for lo)
-__device__ __forceinline__ void split4(float x0, float x1, float x2, float x3, uint32_t& hi, uint32_t& lo) {
-  auto two = [](float x, float y, uint32_t& h, uint32_t& l) {
-    uint16_t c, d;
-    uint32_t v, t;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(v));
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(t) : "r"(v), "r"(e4m3x2_to_f16x2(c)));
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(t) : "r"(t), "r"(0x4c004c00u));   // KV8_LO, twice
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(d) : "r"(t));
-    h = c;
-    l = d;
-  };
-  uint32_t h0, l0, h1, l1;
-  two(x0, x1, h0, l0);
-  two(x2, x3, h1, l1);
-  hi = __byte_perm(h0, h1, 0x5410);
-  lo = __byte_perm(l0, l1, 0x5410);
-}
 // 2^e that brings a magnitude (the bits of a number >= 0) to [128, 256); no more than 2^126
 __device__ __forceinline__ float power_up(uint32_t bits) {
   const int ex = min(max((int)(bits >> 23), 8), 254);
@@ -71,6 +51,18 @@ __device__ __forceinline__ float power_up(uint32_t bits) {
 }
 // of a power of two from 2^-126 to 2^126
 __device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
+// power of two at or above a number > 0 (its bits)
+__device__ __forceinline__ float power_above(uint32_t bits) { return __uint_as_float((bits + 0x7fffffu) & 0x7f800000u); }
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
 // cudaFuncSetAttribute once a device
 struct OncePerDevice {
   static constexpr int MAX = 64;
