@@ -9,9 +9,10 @@
 // scales so far; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
 // most) and nothing above 2^-31 of the largest is lost.
 //
-// Work item = (sequence, 8 or 16 rows, kv head, split of the keys); row = token * G + head of the group.  Every warp walks its own items
-// alone, its blocks of 32 tokens (one bulk copy each) requested RING blocks ahead across items; sequence lengths and pages are read
-// on the device, so the list of items is made by every CTA for itself: a prefix sum over the sequences.
+// Work item = (sequence, 8 or 16 rows, kv head, split of the keys); row = token * G + head of the group.  A CTA's four warps take the
+// item's blocks of 32 tokens in turn (one bulk copy each, requested RING blocks ahead across items) and join their sums in shared memory;
+// a sequence of several splits leaves them in the workspace to attn8_merge_kernel.  Sequence lengths and pages are read on the device,
+// so the list of items is made by every CTA for itself: a prefix sum over the sequences.
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -26,13 +27,19 @@ namespace tgis {
 namespace {
 
 constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
-constexpr int R8_CTAS = 3;                    // per SM
+constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
 constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a score may exceed its row's reference; what probabilities are held times
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
-  int max_splits, split;                      // split: tokens (a multiple of KV_BLOCK)
+  int max_splits, split;                      // split: most tokens of one (a multiple of KV_BLOCK)
 };
+// a sequence's splits are of equal length but for the last
+__device__ __forceinline__ int splits_of(const RowsArgs& a, const AttnSeq& s) { return (s.kv_len + a.split - 1) / a.split; }
+__device__ __forceinline__ int split_blocks(const RowsArgs& a, const AttnSeq& s) {
+  const int n = splits_of(a, s);
+  return ((s.kv_len + KV_BLOCK - 1) / KV_BLOCK + n - 1) / max(n, 1);
+}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -61,11 +68,13 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {   // 8 x 8 f16
 }
 
 template <int ROWS>
-__global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(const __grid_constant__ RowsArgs a) {
   constexpr int NT = ROWS / 8;                // column tiles of the products
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full_s[R8_WARPS * R8_RING];
   __shared__ int32_t ok_s[R8_WARPS * R8_RING], wsum[R8_WARPS];
+  __shared__ float2 stat_s[R8_WARPS][ROWS];
+  __shared__ float4 hand_s[R8_WARPS][ROWS / 8][2][32];
   const int warp = threadIdx.x >> 5, lane = (int)lane_id();
   uint8_t* ring = smem + warp * (R8_RING * KV8_PAGE);
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + R8_WARPS * R8_RING * KV8_PAGE);   // items ahead of sequence s, per kv head
@@ -80,14 +89,13 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
   const int G = a.n_q / a.n_kv;
   // ---- items of every sequence
   auto chunks_of = [&](const AttnSeq& s) { return (s.q_len * G + ROWS - 1) / ROWS; };
-  auto splits_of = [&](const AttnSeq& s) { return (s.kv_len + a.split - 1) / a.split; };
   int carry = 0;
   for (int base = 0; base < a.n_seqs; base += R8_THREADS) {
     const int s = base + threadIdx.x;
     int n = 0;
     if (s < a.n_seqs) {
       const AttnSeq sq = load_seq(a, s);
-      if (seq_fits(a, sq)) n = chunks_of(sq) * splits_of(sq);
+      if (seq_fits(a, sq)) n = chunks_of(sq) * splits_of(a, sq);
       else if (blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
     }
     int sum = n;
@@ -108,7 +116,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
     carry += total;
     __syncthreads();
   }
-  const uint32_t n_flat = (uint32_t)carry * a.n_kv, n_slots = gridDim.x * R8_WARPS;   // (host: no more than 2^31)
+  const uint32_t n_flat = (uint32_t)carry * a.n_kv, n_slots = gridDim.x;   // (host: no more than 2^31)
   auto item_at = [&](uint32_t f) {
     RowsItem it;
     const int e = (int)(f / (uint32_t)a.n_kv);
@@ -120,20 +128,23 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
       else hi = mid;
     }
     it.sq = load_seq(a, lo);
-    const int n_splits = splits_of(it.sq), local = e - prefix[lo];
+    const int n_splits = splits_of(a, it.sq), local = e - prefix[lo];
     it.chunk = local / n_splits;
     it.split = local - it.chunk * n_splits;
-    it.tok0 = it.split * a.split;
-    int end = min(it.sq.kv_len, it.tok0 + a.split);
+    const int len = split_blocks(a, it.sq) * KV_BLOCK;
+    it.tok0 = it.split * len;
+    int end = min(it.sq.kv_len, it.tok0 + len);
     if (a.tree == nullptr) end = min(end, it.sq.kv_len - it.sq.q_len + min((it.chunk + 1) * ROWS - 1, it.sq.q_len * G - 1) / G + 1);
     it.n_tok = max(end - it.tok0, 0);
     return it;
   };
-  auto page_of = [&](const RowsItem& it, int jb) {   // this lane's page of blocks jb .. jb + 31
-    const int b = jb + lane;
+  // a warp's blocks of an item: warp, warp + R8_WARPS, ...
+  auto blocks_of = [&](const RowsItem& it) { return (it.n_blk() - warp + R8_WARPS - 1) / R8_WARPS; };
+  auto page_of = [&](const RowsItem& it, int jb) {   // the pages of its blocks jb .. jb + 31, one a lane
+    const int b = (jb + lane) * R8_WARPS + warp;
     return b < it.n_blk() ? a.block_table[(size_t)it.sq.block_row * a.bt_stride + it.tok0 / KV_BLOCK + b] : 0;
   };
-  uint32_t f = warp * gridDim.x + blockIdx.x;   // consecutive items land on different SMs
+  uint32_t f = blockIdx.x;
   if (f >= n_flat) return;
   // ---- issue cursor: RING blocks ahead of the consumer; the item after its own is decoded when it enters its own
   uint32_t i_f = f;
@@ -146,8 +157,9 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
     }
   };
   ahead();
+  bool alive = true;                          // no wait has run out; after one the warp goes on without copies, for the others wait for it
   auto issue = [&]() {
-    while (i_f < n_flat && i_jb >= i_it.n_blk()) {
+    while (i_f < n_flat && i_jb >= blocks_of(i_it)) {
       i_f += n_slots;
       if (i_f >= n_flat) return;
       i_it = i_nxt;
@@ -155,7 +167,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
       i_jb = 0;
       ahead();
     }
-    if (i_f >= n_flat) return;
+    if (i_f >= n_flat || !alive) return;
     const int page = __shfl_sync(0xffffffffu, i_pages, i_jb & 31);
     if (lane == 0) {
       const bool ok = page >= 0 && page < a.n_pages;
@@ -169,7 +181,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
       }
     }
     i_st = i_st == R8_RING - 1 ? 0 : i_st + 1;
-    if ((++i_jb & 31) == 0 && i_jb < i_it.n_blk()) i_pages = page_of(i_it, i_jb);
+    if ((++i_jb & 31) == 0 && i_jb < blocks_of(i_it)) i_pages = page_of(i_it, i_jb);
   };
   for (int i = 0; i < R8_RING; ++i) issue();
 
@@ -177,8 +189,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
   const uint32_t ring_base = smem_u32(ring);
   int c_st = 0;
   uint32_t c_ph = 0;
-  bool alive = true;
-  for (; alive && f < n_flat; f += n_slots) {
+  for (; f < n_flat; f += n_slots) {
     const RowsItem it = item_at(f);
     const int n_rows = it.sq.q_len * G, prefix_len = it.sq.kv_len - it.sq.q_len;
     // ---- Q^T as B fragments: this thread has row g of each tile, of sixteen dims 4 t4 .. 4 t4 + 3
@@ -221,18 +232,15 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
     // every row of the chunk sees the tokens below this one
     const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * ROWS / G + 1 : 0);
     float ref_v = 0x1p-118f;                  // r
-    const int n_blk = it.n_blk();
+    const int n_blk = blocks_of(it);
     for (int jb = 0; jb < n_blk; ++jb) {
-      if (!bounded_wait(&full[c_st], c_ph)) {
-        alive = false;
-        break;
-      }
-      const bool ok = page_ok[c_st] != 0;
+      alive = alive && bounded_wait(&full[c_st], c_ph);
+      const bool ok = alive && page_ok[c_st] != 0;
       if (ok) {
         const uint32_t k_base = ring_base + c_st * KV8_PAGE, v_base = k_base + KV8_CODES;
         const float* k_scale = reinterpret_cast<const float*>(ring + c_st * KV8_PAGE + KV8_K_SCALES) + g;
         const float* v_scale = k_scale + KV_BLOCK;
-        const int tok_b = it.tok0 + jb * KV_BLOCK;
+        const int tok_b = it.tok0 + (jb * R8_WARPS + warp) * KV_BLOCK;
         const bool open = tok_b + KV_BLOCK > min(seen_by_all, it.sq.kv_len);   // some row may not see some token
         // ---- S^T = K Q^T: 2 tiles of 16 tokens x 8 steps of 16 dims.  A register of codes is dims 4 t4 .. 4 t4 + 3 of a chunk: the step's
         // k places 2 t4, 2 t4 + 1 and 2 t4 + 8, 2 t4 + 9, in Q^T as in K
@@ -356,10 +364,10 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
       issue();
       if (++c_st == R8_RING) c_st = 0, c_ph ^= 1;
     }
-    if (!alive) break;
-    // ---- the item's rows
-    const int n_splits = splits_of(it.sq);
-    const float unit = ref_v * (1.f / R8_HELD);
+    // ---- the item's rows: the warps' sums joined, each warp then having two of the eight tiles of dims.  In step k a warp hands the warp
+    // k places on what that one has to have
+    const int n_splits = splits_of(a, it.sq);
+    float m_all[NT][2], by[NT][2], l_all[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -368,25 +376,82 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS) attn8_rows_kernel(const _
         l += __shfl_xor_sync(0xffffffffu, l, 4);
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (g == 0) stat_s[warp][n * 8 + 2 * t4 + e] = make_float2(m_r[n][e], l);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float2 ml[R8_WARPS];
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < R8_WARPS; ++w) {
+          ml[w] = stat_s[w][n * 8 + 2 * t4 + e];
+          m = fmaxf(m, ml[w].x);
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < R8_WARPS; ++w) l += ml[w].y * ex2(ml[w].x - ref);
+        m_all[n][e] = m;
+        l_all[n][e] = l;
+        by[n][e] = ex2(m_r[n][e] - ref) * (ref_v * (1.f / R8_HELD));
+      }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int md = 0; md < HEAD_DIM / 16; ++md)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][md][i] *= by[n][i & 1];
+    static_assert(R8_WARPS == 4 && HEAD_DIM == 128, "a warp's share is two tiles of dims");
+    float mine[NT][2][4];
+    auto tiles_of = [&](int w, auto&& f2) {   // (registers are not indexed by variables)
+#pragma unroll
+      for (int c = 0; c < R8_WARPS; ++c)
+        if (w == c) f2(c);
+    };
+    tiles_of(warp, [&](int c) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) mine[n][x >> 2][x & 3] = o[n][2 * c + (x >> 2)][x & 3];
+    });
+#pragma unroll
+    for (int k = 1; k < R8_WARPS; ++k) {
+      const int to = (warp + k) % R8_WARPS;
+      tiles_of(to, [&](int c) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) hand_s[c][n][x][lane] = make_float4(o[n][2 * c + x][0], o[n][2 * c + x][1], o[n][2 * c + x][2], o[n][2 * c + x][3]);
+      });
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float4 v = hand_s[warp][n][x][lane];
+          mine[n][x][0] += v.x; mine[n][x][1] += v.y; mine[n][x][2] += v.z; mine[n][x][3] += v.w;
+        }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
         const int rr = it.chunk * ROWS + n * 8 + 2 * t4 + e, i = rr / G, row = it.sq.q_start + i, head = it.kvh * G + rr - i * G;
         if (rr >= n_rows) continue;
         if (n_splits == 1) {
-          const float inv = l == 0.f ? 0.f : unit / l;
-          __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)head * HEAD_DIM + g;
+          const float inv = l_all[n][e] == 0.f ? 0.f : 1.f / l_all[n][e];
+          __nv_bfloat16* dst = a.out + (size_t)row * a.ldo + (size_t)head * HEAD_DIM + warp * 32 + g;
 #pragma unroll
-          for (int md = 0; md < HEAD_DIM / 16; ++md) {
-            dst[md * 16] = __float2bfloat16_rn(o[n][md][e] * inv);
-            dst[md * 16 + 8] = __float2bfloat16_rn(o[n][md][2 + e] * inv);
-          }
+          for (int x = 0; x < 4; ++x) dst[x * 8] = __float2bfloat16_rn(mine[n][x >> 1][2 * (x & 1) + e] * inv);
         } else {
           const size_t at = ((size_t)row * a.n_q + head) * a.max_splits + it.split;
-          float* dst = a.part_o + at * HEAD_DIM + g;
+          float* dst = a.part_o + at * HEAD_DIM + warp * 32 + g;
 #pragma unroll
-          for (int md = 0; md < HEAD_DIM / 16; ++md) {
-            dst[md * 16] = o[n][md][e] * unit;
-            dst[md * 16 + 8] = o[n][md][2 + e] * unit;
-          }
-          if (g == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_r[n][e], l);
+          for (int x = 0; x < 4; ++x) dst[x * 8] = mine[n][x >> 1][2 * (x & 1) + e];
+          if (g == 0 && warp == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_all[n][e], l_all[n][e]);
         }
       }
   }
@@ -407,7 +472,7 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
   griddep_wait();
   const AttnSeq sq = load_seq(a, blockIdx.x);
   if (!seq_fits(a, sq)) return;
-  const int lane = (int)lane_id(), warp = threadIdx.x >> 5, n_splits = (sq.kv_len + a.split - 1) / a.split;
+  const int lane = (int)lane_id(), warp = threadIdx.x >> 5, n_splits = splits_of(a, sq);
   if (n_splits <= 1) return;
   const int n_rows = sq.q_len * a.n_q, step = gridDim.y * (M8_WARPS / PARTS);
   for (int base = blockIdx.y * (M8_WARPS / PARTS); base < n_rows; base += step) {
@@ -468,17 +533,18 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
   p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   p.rows = rows > 8 ? 16 : 8;
-  // Splits: the shortest with which all items run at once; where they do not, the longest that leaves three rounds of them
-  const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS * R8_WARPS;
+  // Splits: one where 1024 tokens hold the sequence (the second launch takes longer than eight more blocks a warp); else the shortest
+  // with which all items run at once, and where they do not the longest that leaves three rounds of them
+  const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS(p.rows);
   auto rounds = [&](int split) { return items * ((max_kv + split - 1) / split) / slots; };
-  p.split = 64;
-  while (p.split < 512 && rounds(p.split) > 1.) p.split *= 2;
+  p.split = 256;
+  while (p.split < 2048 && rounds(p.split) > 1.) p.split *= 2;
   if (rounds(p.split) > 1.)
-    while (p.split > 128 && rounds(p.split) < 3.) p.split /= 2;
-  if (rows > 16) p.split = 512;               // (many rows and few columns that attention8_prompt.cu does not take)
+    while (p.split > 512 && rounds(p.split) < 3.) p.split /= 2;
+  if (max_kv <= 1024) p.split = 1024;
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
-  // (splits of 64 and more for one round; 128 and more where twice as long ones leave less than three)
-  p.most_splits = std::max(p.max_splits, (int)std::min((max_kv + 63) / 64 + 0., 6. * slots / items + 2.));
+  // (splits of 256 and more for one round; 512 and more where twice as long ones leave less than three)
+  p.most_splits = std::max(p.max_splits, max_kv <= 1024 ? 1 : (int)std::min((max_kv + 255) / 256 + 0., 6. * slots / items + 2.));
   return p;
 }
 
@@ -493,7 +559,7 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
   const long long rows = (long long)a.max_q * (a.n_q / a.n_kv);
   const long long most = (long long)a.n_seqs * a.n_kv * a.max_splits * ((rows + ROWS - 1) / ROWS);
   if (most >= 1ll << 31) return cudaErrorInvalidValue;
-  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_CTAS * num_sms, (most + R8_WARPS - 1) / R8_WARPS));
+  const int grid = (int)std::max<long long>(1, std::min<long long>((long long)R8_CTAS(ROWS) * num_sms, most));
   return launch_k(attn8_rows_kernel<ROWS>, dim3(grid), dim3(R8_THREADS), smem, stream, a);
 }
 
