@@ -14,6 +14,7 @@
 // a sequence of several splits leaves them in the workspace to attn8_merge_kernel.  Sequence lengths and pages are read on the device,
 // so the list of items is made by every CTA for itself: a prefix sum over the sequences.
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 
@@ -533,18 +534,14 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
   p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   p.rows = rows > 8 ? 16 : 8;
-  // Splits: one where 1024 tokens hold the sequence (the second launch takes longer than eight more blocks a warp); else the shortest
-  // with which all items run at once, and where they do not the longest that leaves three rounds of them
+  // Splits: one where 1024 tokens hold the sequence (the second launch takes longer than eight more blocks a warp); else as many as run
+  // at once, of 256 to 2048 tokens (the bounds are those of the longest sequence, so a tenth more do); else three rounds of them.
   const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS(p.rows);
-  auto rounds = [&](int split) { return items * ((max_kv + split - 1) / split) / slots; };
-  p.split = 256;
-  while (p.split < 2048 && rounds(p.split) > 1.) p.split *= 2;
-  if (rounds(p.split) > 1.)
-    while (p.split > 512 && rounds(p.split) < 3.) p.split /= 2;
-  if (max_kv <= 1024) p.split = 1024;
+  auto length = [&](double n) { return (int)std::ceil(max_kv / std::max(n, 1.) / 128.) * 128; };
+  const int at_once = length(std::floor(1.1 * slots / items));
+  p.split = max_kv <= 1024 ? 1024 : items <= 1.1 * slots && at_once <= 2048 ? std::max(at_once, 256) : std::min(std::max(length(std::ceil(3. * slots / items)), 512), 2048);
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
-  // (splits of 256 and more for one round; 512 and more where twice as long ones leave less than three)
-  p.most_splits = std::max(p.max_splits, max_kv <= 1024 ? 1 : (int)std::min((max_kv + 255) / 256 + 0., 6. * slots / items + 2.));
+  p.most_splits = std::max(p.max_splits, max_kv <= 1024 ? 1 : (int)std::min((max_kv + 255) / 256 + 0., std::max(3. * slots / items + 2., max_kv / 2048. + 1.)));
   return p;
 }
 
