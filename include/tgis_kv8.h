@@ -2,7 +2,8 @@
  * tgis_kv8.h -- the 8-bit paged cache of libtgis_engine.so and the attention that reads it, on the caller's stream.
  *
  * A stored row (one token, one key / value head, 128 numbers x) is 128 e4m3 codes c and one fp32 scale s:
- *     s = max(max |x| / 448, 2^-126),   c = e4m3(x / s) (nearest, ties to even),   the row stands for c * s.
+ *     s = max(max |x| * (1 / 448), 2^-126),   c = e4m3(x / s) (nearest, ties to even),   the row stands for c * s,
+ * with 1 / 448, the product and the quotient rounded to fp32.
  * A row that holds a NaN or an infinity is stored with a NaN for its scale and zeros for codes: whoever sees it gets NaN, whoever does
  * not gets what it would have got without it.
  *

@@ -62,6 +62,12 @@ def pages_natural(cache: Cache8):
     return out
 
 
+def scales_natural(cache: Cache8, i: int):
+    """fp32 scales of every slot's key (0) or value (1) row, in 64 bits [slots, n_kv]."""
+    raw = cache.pages.view(cache.n_pages * cache.n_kv, PAGE_BYTES)[:, 8192 + 128 * i:8320 + 128 * i].contiguous()
+    return raw.view(torch.float32).double().view(cache.n_pages, cache.n_kv, PAGE).transpose(1, 2).reshape(-1, cache.n_kv)
+
+
 def filled(n_pages, n_kv, seed, spread=0.5):
     g = gen(seed)
     cache = Cache8.empty(n_pages, n_kv)
@@ -98,9 +104,7 @@ def reference(cache, q, seqs, bt, scale, tree=None):
 
 def floor_of(cache, seqs, bt, T, n_q):
     """2^-30 max s * sum |c| over the tokens of a row's sequence."""
-    raw = cache.pages.view(cache.n_pages * cache.n_kv, PAGE_BYTES)
-    s = raw[:, 8320:].contiguous().view(torch.float32).double().view(cache.n_pages, cache.n_kv, PAGE).transpose(1, 2).reshape(-1, cache.n_kv)
-    v = pages_natural(cache)[1]
+    s, v = scales_natural(cache, 1), pages_natural(cache)[1]
     low = torch.zeros(T, cache.n_kv, D, dtype=torch.float64, device="cuda")
     for start, new, all_, row in seqs:
         if new:
@@ -173,8 +177,9 @@ def test_rows_are_rotated_quantised_and_read_back(T, n_q, n_kv):
         assert q is None
     nat = pages_natural(cache)
     at = ints(slots).long()
-    for got, stored, rows in ((k, nat[0][at], turned[:, n_q:n_q + n_kv]), (v, nat[1][at], x.reshape(T, -1, D)[:, n_q + n_kv:])):
-        s = (rows.abs().amax(-1) / 448.0).clamp(min=TINY)[..., None]
+    for i, (got, stored, rows) in enumerate(((k, nat[0][at], turned[:, n_q:n_q + n_kv]), (v, nat[1][at], x.reshape(T, -1, D)[:, n_q + n_kv:]))):
+        s = scales_natural(cache, i)[at][..., None]
+        assert bool((s / (rows.abs().amax(-1, keepdim=True) / 448.0).clamp(min=TINY) - 1).abs().max() < 2.0 ** -21)
         # half a step of the code; 2^-15 of that and 2^-22 of the largest number for the fp32 rotation, scale and quotient
         assert bool(((stored - rows).abs() <= torch.maximum(rows.abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -15) + 448 * s * 2.0 ** -22).all())
         near = to_e4m3(rows / s) * s
@@ -195,8 +200,7 @@ def test_codes_of_values_are_those_of_torch():
     cache = Cache8.empty(2, 1)
     cache.write(x, ints([0] * 64), ints(list(range(64))), still())
     rows = x.float().view(64, 2, D)
-    # (by a tensor: torch multiplies by the reciprocal of a plain number)
-    s = (rows.abs().amax(-1) / torch.tensor(448.0, device="cuda")).clamp(min=TINY)
+    s = (rows.abs().amax(-1) * torch.tensor(1.0 / 448.0, device="cuda")).clamp(min=TINY)
     want = (rows / s[..., None]).to(torch.float8_e4m3fn).double() * s.double()[..., None]
     k, v = pages_natural(cache)
     assert torch.equal(k[:, 0], want[:, 0]) and torch.equal(v[:, 0], want[:, 1])

@@ -31,7 +31,7 @@ __device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
 }
 // Scale of a row whose largest magnitude has these bits: NaN where the row holds a number that is not finite
 __device__ __forceinline__ float scale_of(uint32_t m) {
-  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__fdiv_rn(__uint_as_float(m), KV8_TOP), KV8_TINY);
+  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(m) * (1.f / KV8_TOP), KV8_TINY);
 }
 // Codes of x / s; zeros where the scale is NaN.  An IEEE division is a call of some forty instructions, so the quotients are products with
 // the scale's reciprocal, which are within 2 ulp of them, and are divided again only where that could change a code: within 3 ulp of the
