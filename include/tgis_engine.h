@@ -112,6 +112,11 @@ typedef struct tgis_engine tgis_engine;
  *          Single GPU, no LoRA slots. */
 #define TGIS_ARCH_LUDELIX 7
 
+/* What the Llama family's keys and values are stored as.  E4M3: 8-bit rows with an fp32 scale each (include/tgis_kv8.h), about half the
+ * bytes of a token; queries, softmax and sums are as exact as over the cache in the model's type. */
+#define TGIS_KV_MODEL 0
+#define TGIS_KV_E4M3 1
+
 /* Model + runtime configuration (bf16 decoder-only transformer; see TGIS_ARCH_*). */
 typedef struct tgis_config {
   int32_t abi_version; /* must be TGIS_ABI_VERSION */
@@ -147,7 +152,7 @@ typedef struct tgis_config {
   int32_t max_loras;
   int32_t max_lora_rank;
   int32_t arch;               /* TGIS_ARCH_LLAMA / TGIS_ARCH_OPT */
-  int32_t reserved0;
+  int32_t kv_cache_dtype;     /* TGIS_KV_* (vLLM: --kv-cache-dtype) */
 } tgis_config;
 
 /* Per-layer geometry for architectures whose layers are listed one by one (TGIS_ARCH_PONENEX); tgis_config carries hidden,

@@ -88,3 +88,30 @@ def test_workspace_grows_with_the_bounds(lib):
 def test_binding_refuses_tensors_off_the_device():
     with pytest.raises(ValueError, match="pages"):
         cache8.Cache8(torch.zeros(2, 1, cache8.PAGE_BYTES, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("change,says", [(dict(kv_cache_dtype=7), "kv_cache_dtype"), (dict(kv_cache_dtype=1, arch=_lib.ARCH_OPT, head_dim=64, hidden=64), "Llama"),
+                                         (dict(kv_cache_dtype=1, max_num_seqs=5000), "sequences")])
+def test_engine_refuses(lib, change, says):
+    cfg = _lib.TgisConfig()
+    cfg.abi_version = _lib.ABI_VERSION
+    values = dict(n_layers=1, hidden=128, n_q_heads=1, n_kv_heads=1, head_dim=128, ffn=128, vocab=64, max_model_len=64, max_num_seqs=1, max_batched_tokens=64, tp_size=1)
+    for name, value in {**values, **change}.items():
+        setattr(cfg, name, value)
+    handle = C.c_void_p()
+    assert lib.tgis_engine_create(C.byref(cfg), C.byref(handle)) != 0
+    assert says in lib.tgis_last_error().decode()
+
+
+def test_flag_and_block_bytes():
+    from vllm_tgis_adapter_b200.engine.core import PRESETS, EngineError, NativeEngine, cache_block_bytes
+    from vllm_tgis_adapter_b200.tgis_utils.args import parse_args
+
+    assert parse_args(["--model", "tiny"]).kv_cache_dtype == "auto"
+    assert parse_args(["--model", "tiny", "--kv-cache-dtype", "fp8"]).kv_cache_dtype == "fp8"
+    with pytest.raises(SystemExit):
+        parse_args(["--model", "tiny", "--kv-cache-dtype", "int4"])
+    mc = PRESETS["llama3-8b"]
+    assert cache_block_bytes(mc) == 2 * 32 * 8 * 32 * 128 * 2 and cache_block_bytes(mc, "fp8") == 32 * 8 * 8448
+    with pytest.raises(EngineError, match="kv_cache_dtype"):
+        NativeEngine(mc, kv_cache_dtype="int4")

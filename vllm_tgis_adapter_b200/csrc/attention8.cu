@@ -33,7 +33,7 @@ constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a sco
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
-  int max_splits, split;                      // split: most tokens of one (a multiple of KV_BLOCK)
+  int max_splits, split, rows_of_seq;         // split: most tokens of one (a multiple of KV_BLOCK)
 };
 // a sequence's splits are of equal length but for the last
 __device__ __forceinline__ int splits_of(const RowsArgs& a, const AttnSeq& s) { return (s.kv_len + a.split - 1) / a.split; }
@@ -58,7 +58,7 @@ __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
 }
 struct RowsItem {
   AttnSeq sq;
-  int kvh, chunk, split, tok0, n_tok;         // keys tok0 .. tok0 + n_tok - 1 of the sequence (of the split, and seen by a row of the chunk)
+  int seq, kvh, chunk, split, tok0, n_tok;         // keys tok0 .. tok0 + n_tok - 1 of the sequence (of the split, and seen by a row of the chunk)
   __device__ int n_blk() const { return (n_tok + KV_BLOCK - 1) / KV_BLOCK; }
 };
 
@@ -96,7 +96,8 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
     int n = 0;
     if (s < a.n_seqs) {
       const AttnSeq sq = load_seq(a, s);
-      if (seq_fits(a, sq)) n = chunks_of(sq) * splits_of(a, sq);
+      if (!seq_picked(a, sq)) n = 0;
+      else if (seq_fits(a, sq)) n = chunks_of(sq) * splits_of(a, sq);
       else if (blockIdx.x == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
     }
     int sum = n;
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
       if (prefix[mid] <= e) lo = mid;
       else hi = mid;
     }
+    it.seq = lo;
     it.sq = load_seq(a, lo);
     const int n_splits = splits_of(a, it.sq), local = e - prefix[lo];
     it.chunk = local / n_splits;
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
 #pragma unroll
           for (int x = 0; x < 4; ++x) dst[x * 8] = __float2bfloat16_rn(mine[n][x >> 1][2 * (x & 1) + e] * inv);
         } else {
-          const size_t at = ((size_t)row * a.n_q + head) * a.max_splits + it.split;
+          const size_t at = (((size_t)it.seq * a.rows_of_seq + i) * a.n_q + head) * a.max_splits + it.split;
           float* dst = a.part_o + at * HEAD_DIM + warp * 32 + g;
 #pragma unroll
           for (int x = 0; x < 4; ++x) dst[x * 8] = mine[n][x >> 1][2 * (x & 1) + e];
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
   }
   if (!alive) {
     // a copy never landed: say so; those in flight are done long before this millisecond is over
-    if (lane == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_STALLED);
+    if (lane == 0) say_stalled(a);
     for (const long long t0 = clock64(); clock64() - t0 < 2000000ll;) {}
   }
 }
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
   griddep_launch();
   griddep_wait();
   const AttnSeq sq = load_seq(a, blockIdx.x);
-  if (!seq_fits(a, sq)) return;
+  if (!seq_picked(a, sq) || !seq_fits(a, sq)) return;
   const int lane = (int)lane_id(), warp = threadIdx.x >> 5, n_splits = splits_of(a, sq);
   if (n_splits <= 1) return;
   const int n_rows = sq.q_len * a.n_q, step = gridDim.y * (M8_WARPS / PARTS);
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
     float m = -INFINITY, l = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < n_rows && s0 < s1) {
-      const size_t at = ((size_t)t * a.n_q + head) * a.max_splits;
+      const size_t at = (((size_t)blockIdx.x * a.rows_of_seq + i / a.n_q) * a.n_q + head) * a.max_splits;
       for (int s = s0 + lane; s < s1; s += 32) m = fmaxf(m, a.part_ml[(at + s) * 2]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -565,21 +567,22 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   const RowsPlan p = rows_plan(T, n_seqs, n_q, n_kv, max_q, max_kv);
   if (p.prompt) return attn8_prompt_workspace(ATTN8_MAX_SMS);
-  return p.most_splits > 1 ? (size_t)T * n_q * p.most_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
+  return p.most_splits > 1 ? (size_t)n_seqs * max_q * n_q * p.most_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
 }
 
-cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches) {
+cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches, bool prompts) {
   if (args.n_seqs <= 0 || args.T <= 0) return cudaSuccess;
   num_sms = std::min(num_sms, ATTN8_MAX_SMS);
   const RowsPlan p = rows_plan(args.T, args.n_seqs, args.n_q, args.n_kv, args.max_q, args.max_kv);
   if (launches != nullptr) *launches = 2;
-  if (p.prompt) return attn8_prompt_launch(args, workspace, num_sms, stream);
+  if (p.prompt || prompts) return attn8_prompt_launch(args, workspace, num_sms, stream);
   RowsArgs a;
   static_cast<Attn8Args&>(a) = args;
   a.split = p.split;
   a.max_splits = p.max_splits;
+  a.rows_of_seq = a.max_q;
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_ml = a.part_o + (size_t)a.T * a.n_q * a.max_splits * HEAD_DIM;
+  a.part_ml = a.part_o + (size_t)a.n_seqs * a.max_q * a.n_q * a.max_splits * HEAD_DIM;
   cudaError_t e = p.rows == 8 ? rows_launch<8>(a, num_sms, stream) : rows_launch<16>(a, num_sms, stream);
   if (launches != nullptr && p.max_splits == 1) *launches = 1;
   if (e != cudaSuccess || p.max_splits == 1) return e;

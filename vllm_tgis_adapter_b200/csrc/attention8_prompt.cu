@@ -102,7 +102,7 @@ struct SeqUnits {
 __device__ __forceinline__ SeqUnits units_of(const PromptArgs& a, int s) {
   SeqUnits u;
   u.sq = load_seq(a, s);
-  if (!seq_fits(a, u.sq)) u.sq.q_len = 0;
+  if (!seq_picked(a, u.sq) || !seq_fits(a, u.sq)) u.sq.q_len = 0;
   u.n_units = (u.sq.q_len + 2 * a.TM - 1) / (2 * a.TM);
   u.tokens = u.n_units > 0 ? (u.sq.q_len + u.n_units - 1) / u.n_units : 0;
   return u;
@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t lay_out(const PromptArgs& a, uint32_t* prefi
       const SeqUnits u = units_of(a, s);
       for (int i = 0; i < u.n_units; ++i) n += P8_COST + (uint32_t)steps_of(a, u, i);
       n *= (uint32_t)a.n_kv;
-      if (u.n_units == 0 && blockIdx.x == 0 && a.status != nullptr && !seq_fits(a, load_seq(a, s))) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
+      if (u.n_units == 0 && blockIdx.x == 0 && a.status != nullptr && seq_picked(a, load_seq(a, s)) && !seq_fits(a, load_seq(a, s))) atomicOr(a.status, TGIS_KV8_BAD_SEQ);
     }
     uint32_t sum = n;
 #pragma unroll
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
   __syncthreads();
   // after a wait that ran out copies and MMAs of the other roles may be in flight; they are done long before this millisecond is over
   if (*reinterpret_cast<volatile int*>(&sm.gave_up)) {
-    if (threadIdx.x == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_STALLED);
+    if (threadIdx.x == 0) say_stalled(a);
     for (const long long t0 = clock64(); clock64() - t0 < 2000000ll;) {}
   }
   __syncthreads();

@@ -101,11 +101,21 @@ struct Attn8Args {
   __nv_bfloat16* out;
   int64_t ldo;
   int32_t* status;
+  int lo_q = -0x7fffffff - 1, hi_q = 0x7fffffff;   // sequences with fewer or more queries are another launch's
+  int* stalled = nullptr;            // host memory: set to one where a wait ran out
 };
 // whether a record agrees with what the call said
 __device__ __forceinline__ bool seq_fits(const Attn8Args& a, const AttnSeq& s) {
   return s.q_len >= 0 && s.q_len <= a.max_q && s.kv_len >= s.q_len && s.kv_len <= a.max_kv && s.q_start >= 0 && s.q_start <= a.T - s.q_len &&
          s.block_row >= 0 && s.block_row < a.bt_rows && (s.kv_len + KV_BLOCK - 1) / KV_BLOCK <= a.bt_stride && (a.tree == nullptr || s.q_len <= TGIS_KV8_MAX_TREE);
+}
+__device__ __forceinline__ bool seq_picked(const Attn8Args& a, const AttnSeq& s) { return s.q_len >= a.lo_q && s.q_len <= a.hi_q; }
+__device__ __forceinline__ void say_stalled(const Attn8Args& a) {
+  if (a.status != nullptr) atomicOr(a.status, TGIS_KV8_STALLED);
+  if (a.stalled != nullptr) {
+    *reinterpret_cast<volatile int*>(a.stalled) = 1;
+    __threadfence_system();
+  }
 }
 __device__ __forceinline__ AttnSeq load_seq(const Attn8Args& a, int s) {
   const int4 v = reinterpret_cast<const int4*>(a.seqs)[s];
@@ -118,6 +128,7 @@ bool attn8_prompt_takes(int T, int n_seqs, int n_q, int n_kv, int max_q, int max
 constexpr int ATTN8_MAX_SMS = 160;             // what workspaces are sized for, so that their size asks no device
 size_t attn8_prompt_workspace(int num_sms);
 cudaError_t attn8_prompt_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream);
-cudaError_t attn8_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream, int* launches = nullptr);
+// prompts: by attention8_prompt.cu whatever the bounds say (the caller has left single tokens to another launch)
+cudaError_t attn8_launch(const Attn8Args& a, void* workspace, int num_sms, cudaStream_t stream, int* launches = nullptr, bool prompts = false);
 
 }  // namespace tgis

@@ -41,6 +41,7 @@
 #include <unistd.h>
 
 #include "../../include/tgis_engine.h"
+#include "cache8.cuh"
 #include "kernels.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -385,6 +386,9 @@ struct tgis_engine {
   std::string pnx_dump_path;                         // TGIS_DUMP_RESID: append the residual stream after every layer (debug)
   // kv cache
   DevBuf<bf16> k_cache, v_cache;
+  bool kv8 = false;                                  // tgis_config.kv_cache_dtype: e4m3 rows with a scale each (cache8.cuh) in place of these
+  DevBuf<uint8_t> kv8_pages, kv8_ws;                 // all layers'; partial sums of the attention
+  size_t kv8_layer_bytes = 0;
   size_t kv_layer_elems = 0;
   int num_blocks = 0;
   std::vector<int32_t> free_blocks;
@@ -584,6 +588,7 @@ struct tgis_engine {
     Fl = c.ffn / tp;
     Vl = c.vocab / tp;
     opt = c.arch == TGIS_ARCH_OPT;
+    kv8 = c.kv_cache_dtype == TGIS_KV_E4M3;
     pnx_on = c.arch == TGIS_ARCH_PONENEX || c.arch == TGIS_ARCH_FALERAX || c.arch == TGIS_ARCH_REVEPEL || c.arch == TGIS_ARCH_SIKAZEN ||
              c.arch == TGIS_ARCH_BISUZEN || c.arch == TGIS_ARCH_LUDELIX;  // the layer-list architectures
     if (pnx_on) logits_bf16 = false;  // fp32 logits straight from the accumulators
@@ -812,17 +817,26 @@ struct tgis_engine {
       const float frac = c.gpu_mem_fraction > 0 ? c.gpu_mem_fraction : 0.85f;
       kv_bytes = (size_t)(free_b * (double)frac);
     }
-    const size_t bytes_per_block = 2 * L * block_elems * sizeof(bf16);
+    const size_t bytes_per_block = kv8 ? L * nkv * (size_t)KV8_PAGE : 2 * L * block_elems * sizeof(bf16);
     size_t nb = kv_bytes / bytes_per_block;
     const size_t nb_cap = (size_t)S_max * bt_stride + 1;  // more can never be used
     nb = std::min(nb, nb_cap);
     if (nb < (size_t)bt_stride) throw CudaError("KV cache too small for one max_model_len sequence");
     num_blocks = (int)nb;
     kv_layer_elems = nb * block_elems;
-    k_cache.alloc(L * kv_layer_elems);
-    v_cache.alloc(L * kv_layer_elems);
-    k_cache.zero();  // finite garbage invariant: masked slots must never hold NaN/Inf (see attention.cu)
-    v_cache.zero();
+    if (kv8) {
+      kv8_layer_bytes = nb * nkv * (size_t)KV8_PAGE;
+      kv8_pages.alloc(L * kv8_layer_bytes);
+      kv8_pages.zero();  // every code is a number (tgis_kv8.h)
+      size_t ws = attn8_prompt_workspace(ATTN8_MAX_SMS);
+      for (int n = 1; n <= S_max; ++n) ws = std::max(ws, attn8_workspace(n, n, nq, nkv, 1, bt_stride * KV_BLOCK + DECODE_SPLIT));
+      kv8_ws.alloc(ws);
+    } else {
+      k_cache.alloc(L * kv_layer_elems);
+      v_cache.alloc(L * kv_layer_elems);
+      k_cache.zero();  // finite garbage invariant: masked slots must never hold NaN/Inf (see attention.cu)
+      v_cache.zero();
+    }
     free_blocks.resize(num_blocks);
     for (int i = 0; i < num_blocks; ++i) free_blocks[i] = num_blocks - 1 - i;
     free_slots.resize(S_max);
@@ -3284,7 +3298,7 @@ struct tgis_engine {
       return g;
     };
     if (lora) ++lora_steps;
-    const bool rope_wanted = !pnx_on && !lora && fuse_rope && !cfg.debug_gemm_ref && gemm_even_split(T, qkv_dim, H, num_sms) >= 2 &&
+    const bool rope_wanted = !pnx_on && !kv8 && !lora && fuse_rope && !cfg.debug_gemm_ref && gemm_even_split(T, qkv_dim, H, num_sms) >= 2 &&
                              T <= (qkv_cluster > 0 ? std::max(rope_fuse_max_t, rope_fuse_cluster_max_t) : rope_fuse_max_t);
     // residual add + RMSNorm inside the GEMMs either side of it (single GPU, small steps, both row-"producers" reduced
     // on chip): o-proj -> [post-attention norm] -> gate_up and down-proj -> [next layer's input norm] -> qkv
@@ -3341,24 +3355,28 @@ struct tgis_engine {
         if (late) lora_shrink(g, xn.p, H, true);
         if (lora) lora_expand(g, qkv.p, qkv_dim);
       }
-      bf16* kc = k_cache.p + (size_t)li * kv_layer_elems;
-      bf16* vc = v_cache.p + (size_t)li * kv_layer_elems;
-      if (!rope_fused) {
-        CK(rope_kvwrite_launch(qkv.p, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, kc, vc, T, nq, nkv,
-                               stream));
-        ++n_launches;
-      }
-      if (n_dec > 0) {
-        const int max_splits = (max_dec_kv + DECODE_SPLIT - 1) / DECODE_SPLIT;
-        CK(attn_decode_launch(qkv.p, qkv_dim, kc, vc, ds<DecItem>(items_off(S)), n_dec * max_splits, d_seqs,
-                              ds<int32_t>(off_decids), n_dec, max_splits, part_o.p, part_ml.p, attn_out.p, q_dim, nq,
-                              nkv, scale, num_sms, stream, attn_arrive.p));
-        n_launches += (max_splits > 1 && !attn_inkernel_merge) ? 2 : 1;
-      }
-      if (n_tiles > 0) {
-        CK(attn_prefill_launch(qkv.p, qkv_dim, kc, vc, num_blocks, ds<PrefillUnit>(off_units), n_tiles, step_short_blocks,
-                               d_bt, bt_stride, attn_out.p, q_dim, T, nq, nkv, scale, num_sms, stream));
-        ++n_launches;
+      if (kv8) {
+        kv8_attend(li, T, S, n_dec, n_tiles, max_dec_kv);
+      } else {
+        bf16* kc = k_cache.p + (size_t)li * kv_layer_elems;
+        bf16* vc = v_cache.p + (size_t)li * kv_layer_elems;
+        if (!rope_fused) {
+          CK(rope_kvwrite_launch(qkv.p, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, kc, vc, T, nq, nkv,
+                                 stream));
+          ++n_launches;
+        }
+        if (n_dec > 0) {
+          const int max_splits = (max_dec_kv + DECODE_SPLIT - 1) / DECODE_SPLIT;
+          CK(attn_decode_launch(qkv.p, qkv_dim, kc, vc, ds<DecItem>(items_off(S)), n_dec * max_splits, d_seqs,
+                                ds<int32_t>(off_decids), n_dec, max_splits, part_o.p, part_ml.p, attn_out.p, q_dim, nq,
+                                nkv, scale, num_sms, stream, attn_arrive.p));
+          n_launches += (max_splits > 1 && !attn_inkernel_merge) ? 2 : 1;
+        }
+        if (n_tiles > 0) {
+          CK(attn_prefill_launch(qkv.p, qkv_dim, kc, vc, num_blocks, ds<PrefillUnit>(off_units), n_tiles, step_short_blocks,
+                                 d_bt, bt_stride, attn_out.p, q_dim, T, nq, nkv, scale, num_sms, stream));
+          ++n_launches;
+        }
       }
       const bool late_o = lora_late(H, q_dim), late_gu = lora_late(2 * F, H), late_d = lora_late(H, F);
       if (lora && !late_o) lora_shrink(lora_one(lora_layers[li].A_o, lora_layers[li].B_o, q_dim, H, LR), attn_out.p, q_dim, false);
@@ -3428,6 +3446,31 @@ struct tgis_engine {
       }
     }
     CK(stl_marker_launch(22, stream));  // timeline builds: step end (after the result copy)
+  }
+
+  // Rotary embedding, storing and attention of a layer over the 8-bit cache: single tokens, then prompts and their portions.  Bounds are
+  // those of the step's graph (single tokens) or of the engine: they choose launches, not results that depend on the batch's lengths.
+  void kv8_attend(int li, int T, int S, int n_dec, int n_tiles, int max_dec_kv) {
+    uint8_t* pages = kv8_pages.p + (size_t)li * kv8_layer_bytes;
+    CK(kv8_write_launch(pages, num_blocks, nkv, qkv.p, qkv_dim, T, nq, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, cfg.max_model_len, qkv.p,
+                        qkv_dim, nullptr, stream));
+    ++n_launches;
+    Attn8Args a{pages, num_blocks, nkv, qkv.p, qkv_dim, T, nq, ds<AttnSeq>(off_seqs), S, ds<int32_t>(off_bt), S, bt_stride, nullptr, attn_scale,
+                1, (max_dec_kv + DECODE_SPLIT - 1) / DECODE_SPLIT * DECODE_SPLIT, attn_out.p, q_dim, nullptr};
+    CK(gemm_pair_word(&a.stalled));
+    int launches = 0;
+    if (n_dec > 0) {
+      a.hi_q = 1;
+      CK(attn8_launch(a, kv8_ws.p, num_sms, stream, &launches));
+      n_launches += launches;
+    }
+    if (n_tiles > 0) {
+      a.lo_q = 2;
+      a.hi_q = a.max_q = T;
+      a.max_kv = cfg.max_model_len;
+      CK(attn8_launch(a, kv8_ws.p, num_sms, stream, &launches, true));
+      n_launches += launches;
+    }
   }
 
   // OPT layer stack (vllm model_executor/models/opt.py:170-197, do_layer_norm_before): the tcgen05 GEMMs write their fp32
@@ -4310,6 +4353,11 @@ int tgis_engine_create(const tgis_config* cfg, tgis_engine** out) {
     if (cfg->max_lora_rank < 8 || cfg->max_lora_rank > 64 || cfg->max_lora_rank % 8)
       return fail("max_lora_rank must be a multiple of 8 in [8, 64]");
   }
+  if (cfg->kv_cache_dtype != TGIS_KV_MODEL && cfg->kv_cache_dtype != TGIS_KV_E4M3) return fail("unknown kv_cache_dtype");
+  if (cfg->kv_cache_dtype == TGIS_KV_E4M3) {
+    if (cfg->arch != TGIS_ARCH_LLAMA) return fail("the 8-bit cache serves the Llama family only");
+    if (cfg->max_num_seqs > TGIS_KV8_MAX_SEQS) return fail("the 8-bit cache serves at most " + std::to_string(TGIS_KV8_MAX_SEQS) + " sequences at a time");
+  }
   int ndev = 0;
   if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0)
     return fail("no CUDA device: the TGIS engine has no CPU fallback");
@@ -4337,6 +4385,7 @@ int tgis_engine_create_spec(const tgis_config* cfg, const tgis_model_spec* spec,
   if (cfg->hidden < 1 || cfg->hidden > 12288 || cfg->vocab < 1) return fail("bad hidden / vocab");
   if (cfg->tp_size > 1) return fail("this architecture runs on a single GPU only (tp_size must be 1)");
   if (cfg->max_loras > 0) return fail("LoRA adapter slots are not supported for this architecture");
+  if (cfg->kv_cache_dtype != TGIS_KV_MODEL) return fail("the 8-bit cache serves the Llama family only");
   if (cfg->max_batched_tokens < 1 || cfg->max_num_seqs < 1 || cfg->max_model_len < 2) return fail("bad limits");
   for (int i = 0; i < spec->n_layers; ++i) {
     const tgis_layer_spec& s = spec->layers[i];

@@ -73,8 +73,16 @@ PRESETS: dict[str, ModelConfig] = {
 KV_BLOCK_TOKENS = 32   # tokens per cache block (csrc/kernels.h KV_BLOCK)
 
 
-def cache_block_bytes(mc: ModelConfig) -> int:
+# --kv-cache-dtype -> tgis_config.kv_cache_dtype
+KV_CACHE_DTYPES = {"auto": _lib.KV_MODEL, "bfloat16": _lib.KV_MODEL, "fp8": _lib.KV_E4M3, "fp8_e4m3": _lib.KV_E4M3}
+
+
+def cache_block_bytes(mc: ModelConfig, kv_cache_dtype: str = "auto") -> int:
     """Bytes one cache block takes over all layers (what `kv_cache_bytes` is divided by)."""
+    if KV_CACHE_DTYPES[kv_cache_dtype] == _lib.KV_E4M3:
+        from .cache8 import PAGE_BYTES
+
+        return mc.n_layers * mc.n_kv_heads * PAGE_BYTES
     if mc.arch == "ponenex":
         esz = 4 if mc.dtype == "float32" else 2
         return KV_BLOCK_TOKENS * esz * sum(l.kv_rank + l.rot_dim for l in mc.layers)
@@ -164,7 +172,8 @@ class NativeEngine:
     def __init__(self, model: ModelConfig, *, max_num_seqs: int = 64, max_batched_tokens: int = 2048,
                  kv_cache_bytes: int = 0, gpu_mem_fraction: float = 0.85, device: int = 0, seed: int = 0,
                  debug_gemm_ref: bool = False, use_cuda_graphs: bool | None = None, tp_size: int = 1, tp_rank: int = 0,
-                 nccl_id: bytes | None = None, shm_name: str = "", max_loras: int = 0, max_lora_rank: int = 16):
+                 nccl_id: bytes | None = None, shm_name: str = "", max_loras: int = 0, max_lora_rank: int = 16,
+                 kv_cache_dtype: str = "auto"):
         self.lib = _lib.load_library()
         self.model = model
         if use_cuda_graphs is None:   # default on; TGIS_CUDA_GRAPHS=0 turns decode-step graph replay off
@@ -188,6 +197,9 @@ class NativeEngine:
             cfg.shm_name = shm_name.encode()
         cfg.use_cuda_graphs, cfg.debug_gemm_ref, cfg.seed = int(use_cuda_graphs), 1 if debug_gemm_ref else 0, seed
         cfg.max_loras, cfg.max_lora_rank = int(max_loras), int(max_lora_rank) if max_loras else 0
+        if kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise EngineError(f"unknown kv_cache_dtype {kv_cache_dtype!r}: one of {', '.join(KV_CACHE_DTYPES)}")
+        cfg.kv_cache_dtype = KV_CACHE_DTYPES[kv_cache_dtype]
         archs = {"llama": _lib.ARCH_LLAMA, "opt": _lib.ARCH_OPT, "ponenex": _lib.ARCH_PONENEX, "falerax": _lib.ARCH_FALERAX,
                  "revepel": _lib.ARCH_REVEPEL, "sikazen": _lib.ARCH_SIKAZEN, "bisuzen": _lib.ARCH_BISUZEN,
                  "ludelix": _lib.ARCH_LUDELIX}
