@@ -52,7 +52,7 @@ int64_t tgis_kv8_attention_workspace(int32_t T, int32_t n_seqs, int32_t n_q, int
  * tokens, whose pages are block_table[block_row][0 .. (kv_len - 1) / 32].  tree NULL: query i sees tokens 0 .. kv_len - q_len + i.
  * tree [T]: the last q_len (<= 64) tokens are a draft; query t sees tokens 0 .. kv_len - q_len - 1 and those nodes j of the draft whose
  * bit j is set in tree[t] (its own has to be set to be seen).  A query that sees nothing gives zeros.  Rows of q and out [T, ld*] bf16
- * that no sequence names are not touched.  max_q, max_kv: no sequence has more queries / tokens (host; they choose kernels and
+ * that no sequence names are not touched; no two sequences name the same.  max_q, max_kv: no sequence has more queries / tokens (host; they choose kernels and
  * shapes, so a captured call can be replayed for any lengths within them).  Calls that may run at the same time need workspaces of their own. */
 int tgis_kv8_attention(const void* pages, int32_t n_pages, int32_t n_kv, const void* q, int64_t ldq, int32_t T, int32_t n_q, const int32_t* seqs,
                        int32_t n_seqs, const int32_t* block_table, int32_t bt_rows, int32_t bt_stride, const uint64_t* tree, float scale,

@@ -13,6 +13,8 @@ weight by a factor between exp(-2 d) and exp(2 d) for the largest d of the row.
 """
 import math
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -264,6 +266,75 @@ def test_single_tokens(n_q, n_kv):
 @pytest.mark.parametrize("n_q,n_kv", HEADS)
 def test_portions_of_prompts(n_q, n_kv):
     attend_case([(2, 0), (7, 3), (33, 0), (31, 1), (64, 64), (5, 300), (1, 40), (130, 0), (70, 131)], n_q, n_kv, n_q + 1, gap=2, extra_rows=3)
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(64, 1), (40, 1), (128, 1), (150, 1), (34, 2)])
+def test_wide_groups(n_q, n_kv):
+    """More query heads than a tile of rows, than half an accumulator, than one."""
+    attend_case([(1, 0), (1, 90), (3, 200), (1, 300), (9, 0)], n_q, n_kv, n_q)
+    attend_case([(1, 0), (1, 90), (1, 700)], n_q, n_kv, n_q + 1)
+    attend_case([(3, 40), (7, 200)], n_q, n_kv, n_q + 2, tree=branches)
+
+
+def test_many_sequences():
+    """More sequences than a CTA has threads, most of them empty or bad; pages shared by many."""
+    cache, rng = filled(40, 2, 77), random.Random(5)
+    for most_q, n in ((1, 3000), (40, 1500)):
+        seqs, bt, row = [], [], 0
+        for i in range(n):
+            new = rng.randint(1, most_q) if i % 3 else 0
+            old = rng.randint(0, 150)
+            seqs.append([row, new, new + old, i])
+            row += new
+            bt.append([rng.randrange(40) for _ in range(6)])
+        q = torch.randn(row, 4 * D, device="cuda", generator=gen(n)).to(torch.bfloat16)
+        out = torch.full_like(q, 7.0)
+        cache.attend(q, ints(seqs), ints(bt), D ** -0.5, most_q, 190, out=out)
+        cache.check()
+        some = rng.sample([s for s in seqs if s[1]], 40) + [s for s in seqs if s[1]][-3:]
+        want, size, most = reference(cache, q, some, bt, D ** -0.5)
+        named = ~want.isnan().all(dim=1)
+        may = (TOL + torch.expm1(2 * 2.0 ** -11 * most[named])) * size[named] + 1e-6
+        assert int(named.sum()) > 40 and bool(((out[named].double() - want[named]).abs() <= may).all())
+
+
+def test_a_step_captured_before_any_call_and_replayed_on_two_streams(tmp_path):
+    """A process whose first calls are captured; two graphs with workspaces of their own at the same time."""
+    code = f"""
+import sys; sys.path[:0] = {sys.path[:2]!r}
+import torch
+from vllm_tgis_adapter_b200.engine.cache8 import Cache8
+cache = Cache8.empty(64, 2)
+still = torch.tensor([1.0] * 64 + [0.0] * 64, device="cuda").bfloat16().view(1, 128)
+n = 64 * 32
+rows = torch.randn(n, 512, device="cuda").bfloat16()
+zero, every = torch.zeros(n, device="cuda", dtype=torch.int32), torch.arange(n, device="cuda", dtype=torch.int32)
+bt = torch.arange(64, device="cuda", dtype=torch.int32).view(1, 64)
+jobs = []
+for new in (1, 90):
+    q = torch.randn(new, 512, device="cuda").bfloat16()
+    seqs = torch.tensor([[0, new, 2000, 0]], device="cuda", dtype=torch.int32)
+    jobs.append((q, seqs, new, torch.zeros_like(q), torch.cuda.Stream(), torch.cuda.CUDAGraph()))
+first = torch.cuda.CUDAGraph()
+with torch.cuda.graph(first):
+    cache.write(rows, zero, every, still)
+for q, seqs, new, out, stream, graph in jobs:
+    with torch.cuda.graph(graph, stream=stream):
+        cache.attend(q, seqs, bt, 0.1, new, 2048, out=out)
+first.replay()
+torch.cuda.synchronize()
+for _ in range(50):
+    for q, seqs, new, out, stream, graph in jobs:
+        with torch.cuda.stream(stream):
+            graph.replay()
+torch.cuda.synchronize()
+for q, seqs, new, out, stream, graph in jobs:
+    assert torch.equal(out, cache.attend(q, seqs, bt, 0.1, new, 2048)) and bool(out.isfinite().all()) and bool((out != 0).any())
+cache.check()
+print("right")
+"""
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert "right" in got.stdout, got.stderr[-2000:]
 
 
 def chains(seqs, T, seed):

@@ -167,8 +167,9 @@ struct Walk {
       if (left < all || i >= u.n_units - 1) break;
       left -= all;
     }
-    kvh = (int)(left / (steps + P8_COST));
-    return left - kvh * (steps + P8_COST);
+    // (the bounds hold unless sequences name rows twice, so many that the counts overflow: then results are wrong, and nothing else)
+    kvh = min((int)(left / (steps + P8_COST)), a.n_kv - 1);
+    return min(left - kvh * (steps + P8_COST), steps + P8_COST - 1);
   }
   __device__ bool next() {
     do {
@@ -179,8 +180,10 @@ struct Walk {
       } else if (++kvh == a.n_kv) {   // the stretch goes on: the unit before ended
         kvh = 0;
         if (++i == u.n_units) {
-          do u = units_of(a, ++s);
-          while (u.n_units == 0);
+          do {
+            if (++s >= a.n_seqs) return false;
+            u = units_of(a, s);
+          } while (u.n_units == 0);
           i = 0;
         }
         steps = steps_of(a, u, i);
@@ -813,7 +816,7 @@ __global__ void __launch_bounds__(J8_WARPS * 32) attn8_join_kernel(const __grid_
 bool attn8_prompt_takes(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   const int G = n_q / n_kv, TM = 128 / std::max(G, 1);
   if (TM < 1) return false;
-  const double steps = ((double)T / TM + n_seqs) * ((double)max_kv / P8_KV + 1) * n_kv;
+  const double steps = ((double)T / TM + n_seqs) * ((double)max_kv / P8_KV + 1 + P8_COST) * n_kv;
   return steps < 2e9;
 }
 
