@@ -563,47 +563,48 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       unsigned long long word = 0;
       if (!mine) lim = 0x7fffffff;
       else if (a.tree != nullptr) lim = t.before - 1, word = a.tree[t.row0 + in_unit] & ((unsigned long long)t.word_mask_hi << 32 | t.word_mask_lo);
-      // ---- Q, every row's largest number at 128 to 256.  Eight lanes read a half row of 128 bytes, four rows at a time
+      // ---- Q, every row's largest number at 128 to 256.  The half rows of this warp come as they are to the place of its part of the operand
+      // (eight lanes copy 128 bytes of one); then a thread turns its own into f16 there.  (Loops, for code that runs once a unit is
+      // fetched as it runs: unrolled this took six thousand clocks.)
       const int sub = lane >> 3, at = lane & 7;
-      auto row_of = [&](int i, int& global_row, int& qhead) {   // the i-th of this lane's eight rows; whether it is one
-        const int rr = quarter * 32 + i * 4 + sub, tk = (int)(rr * a.per_g >> 16), iu = g * t.half + tk;
-        global_row = t.row0 + iu;
-        qhead = t.kvh * a.G + rr - tk * a.G;
-        return tk < t.half && iu < t.tokens;
+      const int copied = min(t.half, t.tokens - g * t.half), row0 = t.row0 + g * t.half, head0 = t.kvh * a.G;
+      auto row_of = [&](int i, int& global_row, int& qhead) {   // the i-th of the eight rows that this lane copies; whether it is one
+        const int rr = quarter * 32 + i * 4 + sub, tk = (int)(rr * a.per_g >> 16);
+        global_row = row0 + tk;
+        qhead = head0 + rr - tk * a.G;
+        return tk < copied;
       };
-      float qm;
+      __syncwarp();                                             // the last unit's rows have been read there
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        int grow, qhead;
+        const bool there = row_of(i, grow, qhead);
+        const __nv_bfloat16* from = there ? a.q + (size_t)grow * a.ldq + (size_t)qhead * HEAD_DIM + h * 64 + at * 8 : a.q;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.q[g] + p8_at(quarter * 32 + i * 4 + sub, h * 8 + at))), "l"(from),
+                     "r"(there ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      uint32_t q_top = 0;
+#pragma unroll 2
+      for (int c = 0; c < 8; ++c) {
+        const uint4 x = *reinterpret_cast<const uint4*>(sm.q[g] + p8_at(r, h * 8 + c));
+        q_top = max(q_top, max(max(max(x.x << 16 & 0x7fff0000u, x.x & 0x7fff0000u), max(x.y << 16 & 0x7fff0000u, x.y & 0x7fff0000u)),
+                               max(max(x.z << 16 & 0x7fff0000u, x.z & 0x7fff0000u), max(x.w << 16 & 0x7fff0000u, x.w & 0x7fff0000u))));
+      }
+      q_top = max(q_top, __float_as_uint(pair_up(__uint_as_float(q_top))));
+      if (!ok) break;
+      // (hidden scores are -inf before they are scaled; a row that is not finite: NaN, which its scores and sums then are)
+      const float qm = q_top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f * one_over(power_up(q_top));
       {
-        uint4 x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          int grow, qhead;
-          x[i] = row_of(i, grow, qhead) ? *reinterpret_cast<const uint4*>(a.q + (size_t)grow * a.ldq + (size_t)qhead * HEAD_DIM + h * 64 + at * 8) : make_uint4(0, 0, 0, 0);
-        }
-        float(*say)[128] = sm.pair[met & 1][g];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t top = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(v[k] << 16 & 0x7fff0000u, v[k] & 0x7fff0000u));
-#pragma unroll
-          for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (at == 0) say[h][quarter * 32 + i * 4 + sub] = __uint_as_float(top);
-        }
-        meet();
-        if (!ok) break;
-        auto top_of = [&](int row) { return max(__float_as_uint(say[0][row]), __float_as_uint(say[1][row])); };
-        const uint32_t top = top_of(r);
-        qm = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(fabsf(a.scale), 1e-30f) * 1.4426950408889634f / power_up(top);   // (hidden scores are -inf before they are scaled)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int rr = quarter * 32 + i * 4 + sub;
-          const float up = a.scale < 0.f ? -power_up(top_of(rr)) : power_up(top_of(rr));
-          const uint32_t v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = f16x2(__uint_as_float(v[k] << 16) * up, __uint_as_float(v[k] & 0xffff0000u) * up);
-          *reinterpret_cast<uint4*>(sm.q[g] + p8_at(rr, h * 8 + at)) = make_uint4(w[0], w[1], w[2], w[3]);
+        const float up = a.scale < 0.f ? -power_up(q_top) : power_up(q_top);
+#pragma unroll 2
+        for (int c = 0; c < 8; ++c) {
+          uint4* at_c = reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c));
+          const uint4 x = *at_c;
+          auto turn = [&](uint32_t w) { return f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
+          *at_c = make_uint4(turn(x.x), turn(x.y), turn(x.z), turn(x.w));
         }
       }
       fence_proxy_async();
@@ -730,7 +731,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c)) = make_uint4(x, y, z, w); };
       auto send = [&](auto&& to) {
         __syncwarp();
-#pragma unroll 2
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           int grow, qhead;
           if (row_of(i, grow, qhead)) *to(quarter * 32 + i * 4 + sub, grow, qhead) = *reinterpret_cast<const uint4*>(sm.q[g] + p8_at(quarter * 32 + i * 4 + sub, h * 8 + at));
