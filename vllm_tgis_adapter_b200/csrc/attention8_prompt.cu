@@ -35,7 +35,7 @@ constexpr int P8_THREADS = 768;                             // warps 0..7, 8..15
 constexpr int P8_WARP_COPY = 16, P8_WARP_MMA = 17, P8_WARP_WIDEN = 20, P8_WIDEN = 4;
 constexpr int P8_REGS_SOFTMAX = 88, P8_REGS_OTHER = 64;     // 512 x 88 + 256 x 64 = 768 x 80, what the launch gives every thread
 constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
-constexpr int P8_STAGES = 2;                                // tiles as they come from the cache
+constexpr int P8_NOTES = 4;
 constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile of K or V, of one accumulator's Q, in f16
 constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
 constexpr float P8_HELD = 7.f;                              // exp2 domain: probabilities and their sums are held times 2^7
@@ -63,21 +63,23 @@ struct Task {
 constexpr int P8_TASKS = 4;
 struct P8Smem {
   // K-major operands under the 128-byte swizzle, p8_at
-  uint8_t q[2][P8_TILE], k[P8_TILE], v[P8_TILE];
-  uint8_t raw[P8_STAGES][P8_BLOCKS * KV8_PAGE];
+  // (two of K: a tile of it is widened while the scores of the one before wait for their probabilities)
+  uint8_t q[2][P8_TILE], k[2][P8_TILE], v[P8_TILE];
+  uint8_t raw_k[P8_BLOCKS][KV8_CODES], raw_v[P8_BLOCKS][KV8_CODES];   // as they come from the cache
+  float scales[P8_BLOCKS][2 * KV_BLOCK];   // a block's keys', then its values'
   // scales of value rows as f16 multipliers at their places, of even and odd tiles, a copy for every warp that uses them
   __align__(16) uint16_t v_mul[P8_WIDEN][2][P8_KV];
-  TileNotes notes[2];          // of even and odd tiles
+  TileNotes notes[P8_NOTES];   // tile t's: t % P8_NOTES
   Task task[P8_TASKS];
   float pair[2][2][2][128];    // what the two threads of a row tell one another: of even and odd times, accumulator, half, row
-  uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_full[P8_STAGES], raw_empty[P8_STAGES], q_full[2], note_full[2], pair_full[2][4], k_full, k_empty, v_full, v_empty, s_full[2],
-      p_full[2], o_full[2];
-  uint32_t absent[P8_STAGES];  // by the copying warp
+  uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_k_full, raw_k_empty, raw_v_full, raw_v_empty, q_full[2], note_full[P8_NOTES], pair_full[2][4],
+      k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full[2], o_full[2];
+  uint32_t absent;  // by the copying warp
   uint32_t tmem_base;
   int gave_up;
   uint32_t prefix[1];          // steps ahead of each sequence
 };
-static_assert((2 * P8_TILE + 2 * P8_TILE) % 1024 == 0 && sizeof(((P8Smem*)0)->raw[0]) % 128 == 0 && offsetof(P8Smem, raw) % 128 == 0 && KV8_PAGE % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, raw_full) % 8 == 0, "");
+static_assert(offsetof(P8Smem, raw_k) % 1024 == 0 && offsetof(P8Smem, scales) % 128 == 0 && offsetof(P8Smem, notes) % 16 == 0 && offsetof(P8Smem, task_full) % 8 == 0, "");
 
 // eight numbers (16 bytes) of a row: [2 halves of 64 numbers][128 rows][8 groups, group g at place g ^ (row & 7)]
 __device__ __forceinline__ int p8_at(int row, int group) { return (group >> 3) * (P8_TILE / 2) + row * 128 + (((group & 7) ^ (row & 7)) << 4); }
@@ -229,22 +231,22 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
     if (elect_one()) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sm.q_full[i], 8);
-        mbar_init(&sm.note_full[i], P8_WIDEN);
+        mbar_init(&sm.k_full[i], P8_WIDEN);
+        mbar_init(&sm.k_empty[i], 1);
         mbar_init(&sm.s_full[i], 1);
         mbar_init(&sm.p_full[i], 8);
         for (int k = 0; k < 4; ++k) mbar_init(&sm.pair_full[i][k], 2);
         mbar_init(&sm.o_full[i], 1);
       }
-      for (int i = 0; i < P8_STAGES; ++i) {
-        mbar_init(&sm.raw_full[i], 1);
-        mbar_init(&sm.raw_empty[i], P8_WIDEN);
-      }
+      for (int i = 0; i < P8_NOTES; ++i) mbar_init(&sm.note_full[i], P8_WIDEN);
       for (int i = 0; i < P8_TASKS; ++i) {
         mbar_init(&sm.task_full[i], 1);
         mbar_init(&sm.task_empty[i], 16 + 1 + P8_WIDEN);
       }
-      mbar_init(&sm.k_full, P8_WIDEN);
-      mbar_init(&sm.k_empty, 1);
+      mbar_init(&sm.raw_k_full, 1);
+      mbar_init(&sm.raw_k_empty, P8_WIDEN);
+      mbar_init(&sm.raw_v_full, 1);
+      mbar_init(&sm.raw_v_empty, P8_WIDEN);
       mbar_init(&sm.v_full, P8_WIDEN);
       mbar_init(&sm.v_empty, 1);
       sm.gave_up = 0;
@@ -279,8 +281,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       const uint32_t total = lay_out(a, sm.prefix);
       const uint32_t n = min(gridDim.x, total), b = min(blockIdx.x, n);   // (no stretch of the first n is empty)
       Walk w(a, sm.prefix, n > 0 ? stretch_begin(total, b, n) : 0u, n > 0 ? stretch_begin(total, min(b + 1, n), n) : 0u);
-      int st = 0;
-      uint32_t ph = 1;         // the first pass over the rings finds them empty
+      uint32_t k_ph = 1, v_ph = 1;   // the first time the buffers are empty
       tph = 1;
       CutUnit cut{};
       for (;;) {
@@ -318,6 +319,16 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           return b < n_blk ? a.block_table[(size_t)w.u.sq.block_row * a.bt_stride + b] : 0;
         };
         int page = page_of(w.tile0);
+        const uint8_t* v_src = nullptr;
+        int v_nb = 0;
+        auto copy_v = [&]() {
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_v_empty, v_ph));
+          if (!ok) return;
+          v_ph ^= 1;
+          if (lane == 0) mbar_arrive_expect_tx(&sm.raw_v_full, v_nb * KV8_CODES);
+          __syncwarp();
+          if (lane < v_nb) bulk_load_1d(sm.raw_v[lane], v_src, KV8_CODES, &sm.raw_v_full);
+        };
         for (int j = w.tile0; j < w.tile1; ++j) {
           const int nb = w.blocks(j);
           const bool there = page >= 0 && page < a.n_pages;
@@ -325,33 +336,48 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           if (absent != 0 && lane == 0 && a.status != nullptr) atomicOr(a.status, TGIS_KV8_BAD_PAGE);
           // (an absent page's keys are not seen; some page's codes stand in for it, for they are numbers)
           const uint8_t* src = a.pages + ((size_t)(there ? page : 0) * a.n_kv + w.kvh) * KV8_PAGE;
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_empty[st], ph));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_k_empty, k_ph));
           if (!ok) break;
+          k_ph ^= 1;
           if (lane == 0) {
-            sm.absent[st] = absent;
-            mbar_arrive_expect_tx(&sm.raw_full[st], nb * KV8_PAGE);
+            sm.absent = absent;
+            mbar_arrive_expect_tx(&sm.raw_k_full, nb * (KV8_CODES + (int)sizeof(sm.scales[0])));
           }
           __syncwarp();
-          if (lane < nb) bulk_load_1d(sm.raw[st] + lane * KV8_PAGE, src, KV8_PAGE, &sm.raw_full[st]);
-          if (++st == P8_STAGES) st = 0, ph ^= 1;
+          if (lane < nb) {
+            bulk_load_1d(sm.scales[lane], src + KV8_K_SCALES, sizeof(sm.scales[0]), &sm.raw_k_full);
+            bulk_load_1d(sm.raw_k[lane], src, KV8_CODES, &sm.raw_k_full);
+          }
           if (j + 1 < w.tile1) page = page_of(j + 1);
+          // (K is widened a tile ahead of V, so its copy goes first)
+          if (j > w.tile0) copy_v();
+          if (!ok) break;
+          v_src = src + KV8_CODES;
+          v_nb = nb;
         }
+        if (ok) copy_v();
         if (!ok) break;
       }
       if (lane == 0) a.cut[blockIdx.x] = cut;
     } else if (warp == P8_WARP_MMA) {
       // ===================== MMAs =====================
-      uint32_t kph = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
-      auto operand = [](const uint8_t* p, int ks) { return make_smem_desc_sw128(smem_u32(p) + (ks >> 2) * (P8_TILE / 2) + (ks & 3) * 32); };   // 16 numbers along k
+      uint32_t kt = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};   // kt: tile of the CTA whose K is next
+      // descriptors of 16 numbers along k (their first field counts 16 bytes).  One thread issues an MMA each 64 clocks at best: nothing
+      // but the issue stands between them
+      const uint64_t q_desc = make_smem_desc_sw128(smem_u32(sm.q[0])), k_desc = make_smem_desc_sw128(smem_u32(sm.k[0])), v_desc = make_smem_desc_sw128(smem_u32(sm.v));
+      auto along = [](int ks) { return (uint64_t)((ks >> 2) * (P8_TILE / 2 / 16) + (ks & 3) * 2); };
       auto scores = [&](int g, int nb) {
         const uint32_t idesc = idesc_of(128, nb * KV_BLOCK);
-#pragma unroll 2
-        for (int ks = 0; ks < HEAD_DIM / 16; ++ks) tc_mma_f16(tmem_base + g * 128, operand(sm.q[g], ks), operand(sm.k, ks), idesc, ks > 0);
+        const uint64_t q = q_desc + g * (P8_TILE / 16), k = k_desc + (kt & 1) * (P8_TILE / 16);
+#pragma unroll
+        for (int ks = 0; ks < HEAD_DIM / 16; ++ks) tc_mma_f16(tmem_base + g * 128, q + along(ks), k + along(ks), idesc, ks > 0);
         tc_commit(&sm.s_full[g]);
       };
       auto values = [&](int g, int nb, bool first) {
-        const uint32_t idesc = idesc_of(128, HEAD_DIM);
-        for (int ks = 0; ks < 2 * nb; ++ks) mma_ts(tmem_base + 256 + g * 128, tmem_base + g * 128 + (ks >> 2) * 64 + (ks & 3) * 8, operand(sm.v, ks), idesc, !(first && ks == 0));
+        const uint32_t idesc = idesc_of(128, HEAD_DIM), p = tmem_base + g * 128, o = p + 256;
+#pragma unroll
+        for (int ks = 0; ks < P8_KV / 16; ++ks)
+          if (ks < 2 * nb) mma_ts(o, p + (ks >> 2) * 64 + (ks & 3) * 8, v_desc + along(ks), idesc, ks > 0 || !first);
       };
       while (const Task* tp = take()) {
         const int groups = tp->two() ? 2 : 1, tile0 = tp->tile0, tile1 = tp->tile1;
@@ -360,15 +386,15 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.q_full[g], qph[g]));
           qph[g] ^= 1;
         }
-        ok = ok && __all_sync(0xffffffffu, bounded_wait(&sm.k_full, kph));
+        ok = ok && __all_sync(0xffffffffu, bounded_wait(&sm.k_full[kt & 1], kt >> 1 & 1));
         if (!ok) break;
-        kph ^= 1;
         tc_fence_after();
         if (elect_one()) {
           for (int g = 0; g < groups; ++g) scores(g, task.blocks(tile0));
-          tc_commit(&sm.k_empty);
+          tc_commit(&sm.k_empty[kt & 1]);
         }
         __syncwarp();
+        ++kt;
         for (int j = tile0; j < tile1 && ok; ++j) {
           const bool more = j + 1 < tile1;
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_full, vph));
@@ -386,17 +412,17 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
             __syncwarp();
             if (!more) continue;
             if (g == 0) {
-              ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_full, kph));
-              kph ^= 1;
+              ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_full[kt & 1], kt >> 1 & 1));
               if (!ok) break;
               tc_fence_after();
             }
             if (elect_one()) {
               scores(g, task.blocks(j + 1));
-              if (g == groups - 1) tc_commit(&sm.k_empty);
+              if (g == groups - 1) tc_commit(&sm.k_empty[kt & 1]);
             }
             __syncwarp();
           }
+          if (more) ++kt;
         }
         if (!ok) break;
         done_with();
@@ -405,9 +431,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       // ===================== K, V to f16: thread = token, then dim =====================
       const int mine = warp - P8_WARP_WIDEN, part = mine * 32 + lane;
       const uint32_t swizzle = (uint32_t)(lane & 7) << 4, out_row = (uint32_t)part * 128 + swizzle;
-      const uint32_t k_out = smem_u32(sm.k) + out_row, v_out = smem_u32(sm.v) + out_row, v_mul = smem_u32(sm.v_mul[mine]);
-      int st = 0, odd_tile = 0;               // of the tile whose K is next
-      uint32_t full = 0, k_empty = 1, v_empty = 1;
+      const uint32_t k_out0 = smem_u32(sm.k[0]) + out_row, v_out = smem_u32(sm.v) + out_row, v_mul = smem_u32(sm.v_mul[mine]);
+      uint32_t kt = 0;                        // tile of the CTA whose K is next
+      uint32_t v_full = 0;
       while (const Task* tp = take()) {
         const int tile0 = tp->tile0, tile1 = tp->tile1, kv_len = tp->kv_len;
         float r = 0.f;
@@ -417,14 +443,14 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         // come once a step and all at once
         auto scales = [&](int j) {
           const int nb = tp->blocks(j);
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_full[st], full));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_k_full, kt & 1));
           if (!ok) return;
-          const uint32_t absent = sm.absent[st];
+          const uint32_t absent = sm.absent;
           float my_k = 0.f, vs[P8_BLOCKS], top_k = 0.f, top_v = 0.f;
           uint32_t any_odd = 0;
 #pragma unroll
           for (int b = 0; b < P8_BLOCKS; ++b) {
-            const float* sc = reinterpret_cast<const float*>(sm.raw[st] + b * KV8_PAGE + KV8_K_SCALES);
+            const float* sc = sm.scales[b];
             const bool there = b < nb && !(absent >> b & 1) && j * P8_KV + b * KV_BLOCK + lane < kv_len;
             float k = there ? sc[lane] : 0.f;
             vs[b] = there ? sc[KV_BLOCK + lane] : 0.f;
@@ -442,18 +468,18 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           hi = f16x2(k, k);
           lo = f16x2(k - f16x2_to_f32x2(hi).x, k - f16x2_to_f32x2(hi).x);
 #pragma unroll
-          for (int b = 0; b < P8_BLOCKS; ++b) sm.v_mul[mine][odd_tile][b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * v_to, 0.f);
+          for (int b = 0; b < P8_BLOCKS; ++b) sm.v_mul[mine][kt & 1][b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * v_to, 0.f);
           mem.special = absent | (any_odd != 0 ? 1u << P8_BLOCKS : 0u);
           mem.k_unit = k_top * (1.f / P8_K_TOP);
           mem.v_unit = r * (1.f / P8_V_TOP);
         };
         // K: sixteen dims at a time -> two groups of eight numbers.  (A block that a last tile does not have is not read.)
         auto widen_k = [&](int j) {
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty, k_empty));
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.k_empty[kt & 1], (kt >> 1 & 1) ^ 1));
           if (!ok) return;
-          k_empty ^= 1;
-          // (the scores of the tile before are done, so who reads the notes of the one before that has finished)
-          TileNotes& t = sm.notes[odd_tile];
+          // (the scores of the tile before the last are done, so who reads the notes of the one before that has finished)
+          TileNotes& t = sm.notes[kt % P8_NOTES];
+          const uint32_t k_out = k_out0 + (kt & 1) * P8_TILE;
           if (lane == 0) {
             t.poison[mine] = mem.poison[0];
             if (mine == 0) t.special = mem.special, t.k_unit = mem.k_unit, t.v_unit = mem.v_unit;
@@ -463,7 +489,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
             return hfma2(h, hi, hmul2(h, lo));
           };
           if (mine < tp->blocks(j)) {
-            const uint32_t from = smem_u32(sm.raw[st]) + (uint32_t)mine * KV8_PAGE + (uint32_t)lane * HEAD_DIM + swizzle;
+            const uint32_t from = smem_u32(sm.raw_k[mine]) + (uint32_t)lane * HEAD_DIM + swizzle;
 #pragma unroll 1
             for (int d0 = 0; d0 < HEAD_DIM / 16; d0 += 2) {
               uint4 x[2];
@@ -480,23 +506,25 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&sm.note_full[odd_tile]);
-            mbar_arrive(&sm.k_full);
+            mbar_arrive(&sm.note_full[kt % P8_NOTES]);
+            mbar_arrive(&sm.k_full[kt & 1]);
+            mbar_arrive(&sm.raw_k_empty);
           }
+          ++kt;
         };
         // V: sixteen tokens at a time
-        auto widen_v = [&](int j, int stage, int odd) {
-          ok = __all_sync(0xffffffffu, bounded_wait(&sm.v_empty, v_empty));
+        auto widen_v = [&](int j, int odd) {
+          ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_v_full, v_full) && bounded_wait(&sm.v_empty, v_full ^ 1));
           if (!ok) return;
-          v_empty ^= 1;
+          v_full ^= 1;
           const int nh = 2 * tp->blocks(j);
-          const uint32_t from = smem_u32(sm.raw[stage]) + KV8_CODES + (uint32_t)part * 16, mul = v_mul + odd * (P8_KV * 2);
+          const uint32_t from = smem_u32(sm.raw_v[0]) + (uint32_t)part * 16, mul = v_mul + odd * (P8_KV * 2);
 #pragma unroll 1
           for (int h0 = 0; h0 < nh; h0 += 2) {
             uint4 x[2], m[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              x[h] = lds128(from + (h0 >> 1) * KV8_PAGE + h * (KV8_CODES / 2));
+              x[h] = lds128(from + (h0 >> 1) * KV8_CODES + h * (KV8_CODES / 2));
               m[2 * h] = lds128(mul + (h0 + h) * 32);
               m[2 * h + 1] = lds128(mul + (h0 + h) * 32 + 16);
             }
@@ -513,18 +541,18 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           __syncwarp();
           if (lane == 0) {
             mbar_arrive(&sm.v_full);
-            mbar_arrive(&sm.raw_empty[stage]);
+            mbar_arrive(&sm.raw_v_empty);
           }
         };
         scales(tile0);
         if (ok) widen_k(tile0);
         for (int j = tile0; j < tile1 && ok; ++j) {
-          const int stage = st, odd = odd_tile;
-          if (++st == P8_STAGES) st = 0, full ^= 1;
-          odd_tile ^= 1;
-          if (j + 1 < tile1) scales(j + 1);
-          if (ok) widen_v(j, stage, odd);
-          if (ok && j + 1 < tile1) widen_k(j + 1);
+          const int odd = (int)(kt - 1) & 1;
+          if (j + 1 < tile1) {
+            scales(j + 1);
+            if (ok) widen_k(j + 1);
+          }
+          if (ok) widen_v(j, odd);
         }
         if (!ok) break;
         done_with();
@@ -615,11 +643,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       for (int j = tile0; j < tile1; ++j) {
         const int nb = t.blocks(j) - 2 * h;                 // of this thread's half
         // (in this order: with its scores there, a tile's notes are, and the next tile's in their place are not)
-        ok = __all_sync(0xffffffffu, bounded_wait(&sm.s_full[g], sph) && bounded_wait(&sm.note_full[tile & 1], tile >> 1 & 1));
+        ok = __all_sync(0xffffffffu, bounded_wait(&sm.s_full[g], sph) && bounded_wait(&sm.note_full[tile % P8_NOTES], tile / P8_NOTES & 1));
         if (!ok) break;
         sph ^= 1;
         tc_fence_after();
-        const TileNotes& sc = sm.notes[tile & 1];
+        const TileNotes& sc = sm.notes[tile % P8_NOTES];
         ++tile;
         const int seen = lim - j * P8_KV - h * 64;          // last column seen (of the keys before a draft)
         const uint32_t special = sc.special;
