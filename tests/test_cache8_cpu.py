@@ -115,3 +115,16 @@ def test_flag_and_block_bytes():
     assert cache_block_bytes(mc) == 2 * 32 * 8 * 32 * 128 * 2 and cache_block_bytes(mc, "fp8") == 32 * 8 * 8448
     with pytest.raises(EngineError, match="kv_cache_dtype"):
         NativeEngine(mc, kv_cache_dtype="int4")
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(32, 8), (6, 2), (64, 8), (8, 1)])
+@pytest.mark.parametrize("max_q", [1, 4, 12])
+def test_workspace_grows_with_sequences_and_their_lengths(lib, n_q, n_kv, max_q):
+    """A workspace for the largest call holds every smaller one (what a server allocates once)."""
+    ask = lambda n, kv: lib.tgis_kv8_attention_workspace(n * max_q, n, n_q, n_kv, max_q, kv)
+    for n in (1, 7, 12, 56, 256):
+        sizes = [ask(n, kv) for kv in [*range(16, 5000, 61), 8192, 32768, 131072]]
+        assert sizes == sorted(sizes)
+    for kv in (600, 1000, 3000, 8192):
+        sizes = [ask(n, kv) for n in range(1, 200)]
+        assert sizes == sorted(sizes)

@@ -29,6 +29,12 @@ namespace {
 
 constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
 constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
+// Rows of a sequence (its queries times heads of a group) up to which this kernel reads its pages once for each 16 of them, instead of one
+// unit of attention8_prompt.cu; and keys up to which it takes more rows, where all run at once.  Microseconds here and there, 32 / 8 heads:
+// 8 queries behind 500: 10.3 and 17.8; 32 x 8 behind 1000: 35 and 65; 32 x 12: 51 and 65; 32 x 16: 68 and 67; a prompt of 64: 7.2 and 11.4, of
+// 128: 7.9 and 12.7; 64 behind 500: 12.6 and 18.9, 128: 13.1 and 20.9; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
+// 11.1, of 48 (not): 13.3 and 11.7.
+constexpr int R8_MOST_ROWS = 48, R8_MORE_KEYS = 1024;
 constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a score may exceed its row's reference; what probabilities are held times
 
 struct RowsArgs : Attn8Args {
@@ -528,22 +534,27 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
 }
 
 struct RowsPlan {
-  int rows, split, max_splits, most_splits;     // most_splits: no call with the same rows and fewer keys has more
+  int rows, split, max_splits;
+  double most_splits;                         // as many or more, no fewer for more keys, and no fewer of all sequences for more of these
   bool prompt;                                // attention8_prompt.cu
 };
 RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   RowsPlan p{};
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
-  p.prompt = rows > 16 && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   p.rows = rows > 8 ? 16 : 8;
-  // Splits: one where 1024 tokens hold the sequence (the second launch takes longer than eight more blocks a warp); else as many as run
-  // at once, of 256 to 2048 tokens (the bounds are those of the longest sequence, so a tenth more do); else three rounds of them.
   const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS(p.rows);
+  p.prompt = rows > R8_MOST_ROWS && (items > slots || max_kv > R8_MORE_KEYS) && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
+  // Splits (the bounds are those of the longest sequence): one for few tokens, which the second launch costs more than it saves; else as
+  // many as run at once, of 256 to 4096 tokens; else one for 2048 tokens or three rounds of them, of 1024 to 2048.  Microseconds, 32 / 8 heads,
+  // one single token behind 600: one split 8.4, of 256 tokens 8.5; 1024: 10.8 and 8.6; 12 behind 2048: four (all at once) 14.2, six 19.9,
+  // two 18.9; 12 behind 8192: four 41.9, eight 42.7, sixteen 50.0; 32 behind 4096: one 50.3, two 68.5, four 62.8; 64 behind 4096 (more than
+  // run at once): one 112, of 1024 tokens 106, of 256 147; 64 behind 2048: one 61, two 66.
   auto length = [&](double n) { return (int)std::ceil(max_kv / std::max(n, 1.) / 128.) * 128; };
-  const int at_once = length(std::floor(1.1 * slots / items));
-  p.split = max_kv <= 1024 ? 1024 : items <= 1.1 * slots && at_once <= 2048 ? std::max(at_once, 256) : std::min(std::max(length(std::ceil(3. * slots / items)), 512), 2048);
+  const int at_once = std::max(length(std::floor(slots / items)), 256);
+  const bool few = max_kv <= 768;
+  p.split = few ? 768 : items <= slots && at_once <= 4096 ? at_once : max_kv <= 2048 ? 2048 : std::min(std::max(length(std::ceil(3. * slots / items)), 1024), 2048);
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
-  p.most_splits = std::max(p.max_splits, max_kv <= 1024 ? 1 : (int)std::min((max_kv + 255) / 256 + 0., std::max(3. * slots / items + 2., max_kv / 2048. + 1.)));
+  p.most_splits = few ? 1. : std::min(max_kv / 256. + 1., std::max(3. * slots / items + 2., max_kv / 2048. + 1.));
   return p;
 }
 
@@ -567,7 +578,7 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   const RowsPlan p = rows_plan(T, n_seqs, n_q, n_kv, max_q, max_kv);
   if (p.prompt) return attn8_prompt_workspace(ATTN8_MAX_SMS);
-  return p.most_splits > 1 ? (size_t)n_seqs * max_q * n_q * p.most_splits * (HEAD_DIM + 2) * sizeof(float) : 0;
+  return p.most_splits > 1. ? ((size_t)std::ceil(n_seqs * p.most_splits) * max_q * n_q * (HEAD_DIM + 2) * sizeof(float) + 15) / 16 * 16 : 0;
 }
 
 cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches, bool prompts) {
@@ -586,9 +597,12 @@ cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cu
   cudaError_t e = p.rows == 8 ? rows_launch<8>(a, num_sms, stream) : rows_launch<16>(a, num_sms, stream);
   if (launches != nullptr && p.max_splits == 1) *launches = 1;
   if (e != cudaSuccess || p.max_splits == 1) return e;
-  const int per_cta = p.max_splits > 16 ? 1 : M8_WARPS, y = (int)std::min<long long>(((long long)args.max_q * args.n_q + per_cta - 1) / per_cta, 1024);
-  return p.max_splits > 16 ? launch_k(attn8_merge_kernel<M8_WARPS>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a)
-                           : launch_k(attn8_merge_kernel<1>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a);
+  // a warp a row joins four splits as fast as eight warps do (32 tokens behind 4096: 64 us both); eight splits: 69 and 62, 32 of one token behind
+  // 8192: 18 and 12
+  const bool wide = p.max_splits > 4;
+  const int per_cta = wide ? 1 : M8_WARPS, y = (int)std::min<long long>(((long long)args.max_q * args.n_q + per_cta - 1) / per_cta, 1024);
+  return wide ? launch_k(attn8_merge_kernel<M8_WARPS>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a)
+              : launch_k(attn8_merge_kernel<1>, dim3(a.n_seqs, y), dim3(M8_WARPS * 32), 0, stream, a);
 }
 
 }  // namespace tgis

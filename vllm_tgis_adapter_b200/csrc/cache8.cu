@@ -337,7 +337,7 @@ kv8_read_kernel(const uint8_t* __restrict__ pages, int n_pages, int n_kv, const 
 // Rows (tokens times heads) up to which a warp has one: single tokens of many sequences lie on as many pages, and a window would store or read
 // its sixteen rows byte by byte in one CTA.  Microseconds of a store, a row a warp against windows, 32 + 8 heads: 96 single tokens 3.5 and
 // 8.2; neighbours 16: 2.8 and 4.0, 256: 4.9 and 6.5, 512: 8.3 and 7.9, 1024: 12.5 and 8.7, 2614: 28.8 and 16.2; reading back 2614: 7.6 and 4.5.
-constexpr int W8_SINGLE = 4096, W8_ALL_AT_ONCE = 8192;
+constexpr int W8_SINGLE = 4096, W8_ALL_AT_ONCE = 4096;
 long long v_ctas(int T, int n_kv, bool single) {
   return single ? ((long long)T * n_kv + W8_WARPS - 1) / W8_WARPS : (long long)(T + W8_WINDOW - 1) / W8_WINDOW * n_kv;
 }
@@ -350,6 +350,7 @@ cudaError_t kv8_write_launch(uint8_t* pages, int n_pages, int n_kv, const __nv_b
   if (T <= 0) return cudaSuccess;
   const int first = q_out != nullptr ? 0 : n_q, quads = (n_q + n_kv - first + 3) / 4;
   // a warp a quad while there are few of them; two warps a token (whose cos and sin they then have for several heads) otherwise
+  // (ten quads a token: 256 tokens 4.9 us and 5.9, 512: 8.1 and 7.7, 1024: 10.2 and 8.5, 4000: 32.7 and 24.8)
   const int parts = (long long)T * quads <= W8_ALL_AT_ONCE ? quads : std::min(quads, 2);
   const bool single = (long long)T * n_kv <= W8_SINGLE;
   const long long qk = ((long long)T * parts + W8_WARPS - 1) / W8_WARPS, ctas = qk + v_ctas(T, n_kv, single);

@@ -52,11 +52,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
   return d;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-  return d;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
