@@ -594,3 +594,44 @@ def test_a_conversation_over_the_cache():
 
 def q_all(cache, qkv, cs, total):
     return Cache8.empty(6, cache.n_kv).write(qkv, ints(list(range(total))), ints([-1] * total), cs)
+
+
+# ------------------------------------------------------- the kernel of long prompts on short sequences (bounds choose between the two)
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+def test_portions_in_bounds_of_long_prompts(n_q, n_kv):
+    attend_case([(2, 0), (7, 3), (33, 0), (31, 1), (64, 64), (5, 300), (1, 40), (130, 0), (70, 131), (1, 0), (1, 127), (1, 128)], n_q, n_kv, n_q + 1, gap=2, extra_rows=3, max_more=2000)
+
+
+@pytest.mark.parametrize("n_q,n_kv", HEADS)
+@pytest.mark.parametrize("tree", [chains, branches, any_words])
+def test_trees_in_bounds_of_long_contexts(n_q, n_kv, tree):
+    attend_case([(1, 0), (2, 0), (8, 24), (24, 200), (64, 0), (63, 300), (5, 127), (3, 128), (64, 64)], n_q, n_kv, n_q + 2, tree=tree, gap=1, extra_rows=2, max_more=2000)
+
+
+@pytest.mark.parametrize("tree", [None, chains])
+def test_large_scores_in_bounds_of_long_prompts(tree):
+    for scale, size in ((1.0, 4.0), (-0.2, 1.0), (0.0, 1.0), (0.1, 1e-30), (1e-30, 1e30), (1e-3, 3.0)):
+        attend_case([(6, 40), (1, 200), (20, 0), (64, 9)], 4, 2, 9, tree=tree, scale=scale, q_size=size, max_more=2000)
+
+
+@pytest.mark.parametrize("spread", [0.0, 6.0, 20.0])
+def test_rows_of_very_different_sizes_in_bounds_of_long_prompts(spread):
+    seqs, bt, n_pages, T = batch([(1, 500), (6, 300), (40, 60)], 11)
+    cache = filled(n_pages, 2, 12, spread)
+    attend_case([(1, 500), (6, 300), (40, 60)], 4, 2, 11, cache=cache, scale=1e-3 if spread < 10 else 1e-9, max_more=2000)
+
+
+@pytest.mark.parametrize("case", [test_rows_whose_mask_leaves_nothing_are_zeros, test_numbers_that_are_not_finite_stay_with_the_rows_that_see_them,
+                                  test_queries_that_are_not_finite])
+def test_empty_rows_and_no_numbers_in_bounds_of_long_prompts(case, monkeypatch):
+    attend = Cache8.attend
+    monkeypatch.setattr(Cache8, "attend", lambda self, q, seqs, bt, scale, max_q, max_kv, **more: attend(self, q, seqs, bt, scale, max(max_q, 64), max(max_kv, 2000), **more))
+    case()
+
+
+@pytest.mark.parametrize("n_q,n_kv", [(4, 1), (32, 8), (3, 3)])
+def test_a_few_queries_behind_long_contexts(n_q, n_kv):
+    """17 to 48 rows a sequence and splits: several chunks of rows, each joined over its splits."""
+    most = 48 // (n_q // n_kv)
+    attend_case([(most, 1500), (most - 3, 900), (1, 2100), (2, 0), (5, 770)], n_q, n_kv, 31)
+    attend_case([(most, 1100), (most - 3, 900), (1, 40)], n_q, n_kv, 32, tree=branches)
