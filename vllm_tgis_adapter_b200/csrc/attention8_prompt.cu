@@ -14,10 +14,17 @@
 // for V.  A query row is exact in f16 but for numbers 2^-22 of its largest and below.  A probability is one f16 number of 11 bits,
 // held times 2^7; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
 // most) and nothing above 2^-31 of the largest is lost.  (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the
-// products cost the same and every score takes a multiplication by its key's scale, every probability one by its value's:
-// 361 against XXX us for 1859 tokens behind 6144, 32 / 8 heads.)
-// Scores and probabilities of a row are one thread's; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are written in that
-// order.  A row with a NaN for its scale gets zeros here and a bit; who sees it gets NaN for its sum.
+// products cost the same and every score takes a multiplication by its key's scale, every probability one by its value's: as first
+// built both took 380 us for 1859 tokens behind 6144, 32 / 8 heads, and each later step, to 263, needed the multiplications gone.)
+// Two threads share a row, half of a step's columns each; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are
+// written in that order.  A row with a NaN for its scale gets zeros here and a bit; who sees it gets NaN for its sum.
+//
+// What bounds it: the chain of a step.  Of its 4900 clocks an accumulator spends 3100 in the softmax (scores read 600, the two threads'
+// maximum 300, exponentials 2000, 1024 of them the least that 16 a clock take) and 1700 in its two products, which wait for those of
+// the other one; the two take turns.  Without the exponentials a step is 4500, without the widening 4550: nothing alone is the bound.
+// 1859 tokens behind 6144: 263 us, 820 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
+// prompt of 2048: 75; six prompts of 90 to 593 (1679 tokens): 39; 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 80.
+// A unit's beginning and end take as much as three and a half steps (Q copied and turned, the first pages, O): what short prompts consist of.
 //
 // No wait is unbounded: after about two seconds a role gives up, the call's status says so; copies and MMAs in flight land first and TMEM is
 // freed on every path.
@@ -40,7 +47,7 @@ constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile o
 constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
 constexpr float P8_HELD = 7.f;                              // exp2 domain: probabilities and their sums are held times 2^7
 constexpr float P8_V_TOP = 64.f, P8_K_TOP = 16.f;           // largest scale that a code (448 at most) is multiplied by
-constexpr uint32_t P8_COST = 2;                             // what the beginning and the end of a unit take, in steps
+constexpr uint32_t P8_COST = 2;                             // what the beginning and the end of a unit count for, in steps (they overlap the next unit's)
 
 // What the softmax has to know of a tile, beside its scores
 struct TileNotes {
