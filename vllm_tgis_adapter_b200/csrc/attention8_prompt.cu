@@ -64,7 +64,7 @@ struct Task {
   int row0, kvh, cut;          // row of the first token; bits: 1 begins behind the unit's first step, 2 ends ahead of its last
   uint32_t word_mask_lo, word_mask_hi;   // nodes of the draft
   uint32_t pad[3];
-  __device__ bool two() const { return tokens > 1; }
+  __device__ bool two() const { return tokens > half; }
   __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
 };
 constexpr int P8_TASKS = 4;
@@ -206,7 +206,7 @@ struct Walk {
   }
   __device__ int keys() const { return keys_of(a, u, i); }
   __device__ int tokens() const { return min(u.tokens, u.sq.q_len - i * u.tokens); }
-  __device__ int half() const { return (tokens() + 1) / 2; }   // tokens of the first accumulator; the second has the others
+  __device__ int half() const { return tokens() <= a.TM ? tokens() : (tokens() + 1) / 2; }   // tokens of the first accumulator; the second has the others
   __device__ int blocks(int j) const { return min(P8_BLOCKS, (keys() + KV_BLOCK - 1) / KV_BLOCK - j * P8_BLOCKS); }
 };
 
@@ -602,21 +602,15 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       // (eight lanes copy 128 bytes of one); then a thread turns its own into f16 there.  (Loops, for code that runs once a unit is
       // fetched as it runs: unrolled this took six thousand clocks.)
       const int sub = lane >> 3, at = lane & 7;
-      const int copied = min(t.half, t.tokens - g * t.half), row0 = t.row0 + g * t.half, head0 = t.kvh * a.G;
-      auto row_of = [&](int i, int& global_row, int& qhead) {   // the i-th of the eight rows that this lane copies; whether it is one
-        const int rr = quarter * 32 + i * 4 + sub, tk = (int)(rr * a.per_g >> 16);
-        global_row = row0 + tk;
-        qhead = head0 + rr - tk * a.G;
-        return tk < copied;
-      };
+      // (where a row of 32 lies is its thread's to say: numbers ahead of it in q or out, -1: there is none)
+      auto row_at = [&](int64_t ld) { return mine ? (long long)(t.row0 + in_unit) * ld + (t.kvh * a.G + r - tok * a.G) * HEAD_DIM : -1ll; };
+      const long long q_at = row_at(a.ldq);
       __syncwarp();                                             // the last unit's rows have been read there
 #pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        int grow, qhead;
-        const bool there = row_of(i, grow, qhead);
-        const __nv_bfloat16* from = there ? a.q + (size_t)grow * a.ldq + (size_t)qhead * HEAD_DIM + h * 64 + at * 8 : a.q;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.q[g] + p8_at(quarter * 32 + i * 4 + sub, h * 8 + at))), "l"(from),
-                     "r"(there ? 16 : 0)
+      for (int i = 0; i < 32; i += 4) {
+        const long long from = __shfl_sync(0xffffffffu, q_at, i + sub);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.q[g] + p8_at(quarter * 32 + i + sub, h * 8 + at))),
+                     "l"(a.q + (from < 0 ? 0 : from + h * 64 + at * 8)), "r"(from < 0 ? 0 : 16)
                      : "memory");
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -764,12 +758,13 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       if (!ok) break;
       // the rows leave through shared memory, where this warp's part of Q was (the last scores are done): eight lanes then write 128 bytes of one
       auto put = [&](int c, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { *reinterpret_cast<uint4*>(sm.q[g] + p8_at(r, h * 8 + c)) = make_uint4(x, y, z, w); };
-      auto send = [&](auto&& to) {
+      auto send = [&](auto&& to) {   // to(row, what its thread says of it): where its 16 bytes go, NULL: nowhere
         __syncwarp();
+        const long long o_at = row_at(a.ldo);
 #pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-          int grow, qhead;
-          if (row_of(i, grow, qhead)) *to(quarter * 32 + i * 4 + sub, grow, qhead) = *reinterpret_cast<const uint4*>(sm.q[g] + p8_at(quarter * 32 + i * 4 + sub, h * 8 + at));
+        for (int i = 0; i < 32; i += 4) {
+          uint4* dst = to(quarter * 32 + i + sub, __shfl_sync(0xffffffffu, o_at, i + sub));
+          if (dst != nullptr) *dst = *reinterpret_cast<const uint4*>(sm.q[g] + p8_at(quarter * 32 + i + sub, h * 8 + at));
         }
         __syncwarp();
       };
@@ -793,10 +788,10 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) put(i, o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
-          send([&](int rr, int, int) { return reinterpret_cast<uint4*>(a.frag_o + (slot + rr) * HEAD_DIM + h * 64 + c * 32) + at; });
+          send([&](int rr, long long o) { return o < 0 ? nullptr : reinterpret_cast<uint4*>(a.frag_o + (slot + rr) * HEAD_DIM + h * 64 + c * 32) + at; });
         }
       }
-      if (t.cut == 0) send([&](int, int grow, int qhead) { return reinterpret_cast<uint4*>(a.out + (size_t)grow * a.ldo + (size_t)qhead * HEAD_DIM + h * 64) + at; });
+      if (t.cut == 0) send([&](int, long long o) { return o < 0 ? nullptr : reinterpret_cast<uint4*>(a.out + o + h * 64) + at; });
       else if (mine && h == 0) *reinterpret_cast<float2*>(a.frag_ml + (slot + r) * 2) = make_float2(m, l);
       tc_fence_before();
       done_with();
