@@ -37,9 +37,9 @@ constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
 constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
 // Rows of a sequence (its queries times heads of a group) up to which this kernel reads its pages once for each 16 of them, instead of one
 // unit of attention8_prompt.cu; and keys up to which it takes more rows, where all run at once.  Microseconds here and there, 32 / 8 heads:
-// 8 queries behind 500: 10.3 and 17.8; 32 x 8 behind 1000: 35 and 65; 32 x 12: 51 and 65; 32 x 16: 68 and 67; a prompt of 64: 7.2 and 11.4, of
-// 128: 7.9 and 12.7; 64 behind 500: 12.6 and 18.9, 128: 13.1 and 20.9; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
-// 11.1, of 48 (not): 13.3 and 11.7.
+// 8 queries behind 500: 10.2 and 15.8; 32 x 8 behind 1000: 35 and 57; 32 x 12: 51 and 58; 32 x 16: 67 and 59; a prompt of 64: 7.4 and 11.1, of
+// 128: 8.0 and 12.3; 64 behind 500: 12.6 and 19.2, 128: 13.1 and 21.0; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
+// 9.2, of 48 (not): 13.3 and 11.4.
 constexpr int R8_MOST_ROWS = 48, R8_MORE_KEYS = 1024;
 constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a score may exceed its row's reference; what probabilities are held times
 

@@ -1,8 +1,9 @@
 // Attention over the 8-bit paged cache (include/tgis_kv8.h; layout and number format: cache8.cuh) of prompts, their portions and wide
 // drafted trees, on tcgen05.
 //
-// A unit is up to 2 TM query tokens of one sequence and one kv head, half of them in each of two accumulators (row = token * G + head of the
-// group, TM = 128 / G); a step is one tile of 128 keys of a unit.  All steps of the call lie in one row, sequence after sequence,
+// A unit is up to 2 TM query tokens of one sequence and one kv head (row = token * G + head of the group, TM = 128 / G), half of them in each
+// of two accumulators, or all in one that holds them (whose step is shorter: 16 drafts of 5 to 24 behind 200 to 1500, 34 us; halved, 39); a
+// step is one tile of 128 keys of a unit.  All steps of the call lie in one row, sequence after sequence,
 // and every CTA takes an equal stretch of them: a stretch that begins or ends inside a unit leaves that unit's sums (o, m, l) in
 // the workspace, and attn8_join_kernel joins them in order.  So a long prompt, many short ones and a few drafts over long contexts
 // all keep every SM busy to the end, and the workspace is two units a CTA whatever the lengths are.  Lengths and pages are read on
