@@ -23,7 +23,7 @@
 // What bounds it: the chain of a step.  Of its 4900 clocks an accumulator spends 3100 in the softmax (scores read 600, the two threads'
 // maximum 300, exponentials 2000, 1024 of them the least that 16 a clock take) and 1700 in its two products, which wait for those of
 // the other one; the two take turns.  Without the exponentials a step is 4500, without the widening 4550: nothing alone is the bound.
-// 1859 tokens behind 6144: 263 us, 820 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
+// 1859 tokens behind 6144: 264 us, 815 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
 // prompt of 2048: 75; six prompts of 90 to 593 (1679 tokens): 39; 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 80.
 // A unit's beginning and end take as much as three and a half steps (Q copied and turned, the first pages, O): what short prompts consist of.
 //
@@ -48,7 +48,9 @@ constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile o
 constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
 constexpr float P8_HELD = 7.f;                              // exp2 domain: probabilities and their sums are held times 2^7
 constexpr float P8_V_TOP = 64.f, P8_K_TOP = 16.f;           // largest scale that a code (448 at most) is multiplied by
-constexpr uint32_t P8_COST = 2;                             // what the beginning and the end of a unit count for, in steps (they overlap the next unit's)
+// What the beginning and the end of a unit count for, in steps.  As 1, 2, 3: 2048 tokens 85, 75, 72 us; six prompts of 90 to 593 38.8, 38.6, 40.4;
+// 16 drafts of 5 to 24 behind 200 to 1500 36, 33.5, 35
+constexpr uint32_t P8_COST = 2;
 
 // What the softmax has to know of a tile, beside its scores
 struct TileNotes {
