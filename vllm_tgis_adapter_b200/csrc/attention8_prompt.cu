@@ -686,7 +686,10 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
-        const float qk = qm * sc.k_unit;
+        // (a unit that is no normal number would make hidden scores, -inf, times 0 NaN; scores of 2^24 units at most are nothing beside 2^-126 of
+        // them.  A NaN fails the comparison and stays)
+        float qk = qm * sc.k_unit;
+        if (qk < 0x1p-126f) qk = 0x1p-126f;
         uint64_t qm2 = pack2(qk, qk);
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         top = fmaxf(top, pair_up(top)) * qk;
