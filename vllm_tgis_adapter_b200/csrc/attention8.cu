@@ -6,10 +6,10 @@
 // Both products are mma.sync f16 x f16 -> fp32, K and V widened in registers (exact) as their fragments leave shared memory; mma.sync on
 // e4m3 itself, with queries and probabilities as two e4m3 numbers each, costs the same tensor work and fifteen instructions each
 // (64 tokens behind 8000, 32 / 8 heads: 211 us, against 194).  A query row (bf16) times the power of two that brings its largest number to
-// [128, 256) is exact in f16 but for numbers 2^-22 of the largest and below.  Scores are multiplied by their key's scale in fp32; a
-// probability times its value row's scale is one f16 number of 11 bits, held times 2^7 / r, r the power of two at or above the
-// scales so far; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
-// most) and nothing above 2^-31 of the largest is lost.
+// [128, 256) is exact in f16 but for numbers 2^-22 of the largest and below.  Scores are multiplied by their key's scale in fp32; a row's
+// weight, probability times value's scale, is one f16 number of 11 bits, held times 2^7 / r.  The reference m of a row's exponentials moves
+// only when a score passes it by 2^8, and r, a power of two and the row's own, only when a weight passes it by 2^8: it fits f16 (2^15 at
+// most), and nothing above 2^-31 of the row's largest weight is lost, whatever tokens hold that it does not see or gives no weight.
 //
 // Work item = (sequence, 8 or 16 rows, kv head, split of the keys); row = token * G + head of the group.  A CTA's four warps take the
 // item's blocks of 32 tokens in turn (one bulk copy each, requested RING blocks ahead across items) and join their sums in shared memory;
@@ -41,7 +41,9 @@ constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
 // 128: 8.0 and 12.3; 64 behind 500: 12.6 and 19.2, 128: 13.1 and 21.0; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
 // 9.2, of 48 (not): 13.3 and 11.4.
 constexpr int R8_MOST_ROWS = 48, R8_MORE_KEYS = 1024;
-constexpr float R8_SLACK = 8.f, R8_HELD = 128.f;   // exp2 domain: how far a score may exceed its row's reference; what probabilities are held times
+constexpr float R8_SLACK = 8.f;                    // exp2 domain: how far a score may exceed its row's reference
+constexpr float R8_HELD = 128.f, R8_ROOM = 256.f;  // weights are held times 2^7 / r; how often r fits into the largest of them before it moves
+constexpr float R8_LEAST = 0x1p-118f;              // smallest r
 
 struct RowsArgs : Attn8Args {
   float *part_o, *part_ml;
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
     const int n_rows = it.sq.q_len * G, prefix_len = it.sq.kv_len - it.sq.q_len;
     // ---- Q^T as B fragments: this thread has row g of each tile, of sixteen dims 4 t4 .. 4 t4 + 3
     uint32_t qb[NT][HEAD_DIM / 16][2];
-    float q_mul[NT][2], m_r[NT][2], l_r[NT][2], o[NT][HEAD_DIM / 16][4];   // of rows 2 t4, 2 t4 + 1
+    float q_mul[NT][2], m_r[NT][2], l_r[NT][2], r_r[NT][2], o[NT][HEAD_DIM / 16][4];   // of rows 2 t4, 2 t4 + 1
     int lim[NT][2];                           // causal: last token seen
     unsigned long long word[NT][2];
 #pragma unroll
@@ -240,13 +242,13 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
         word[n][e] = a.tree != nullptr && r2 < n_rows ? a.tree[it.sq.q_start + i2] : 0;
         m_r[n][e] = -INFINITY;
         l_r[n][e] = 0.f;
+        r_r[n][e] = R8_LEAST;
       }
 #pragma unroll
       for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][0] = o[n][md][1] = o[n][md][2] = o[n][md][3] = 0.f;
     }
     // every row of the chunk sees the tokens below this one
     const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * ROWS / G + 1 : 0);
-    float ref_v = 0x1p-118f;                  // r
     const int n_blk = blocks_of(it);
     for (int jb = 0; jb < n_blk; ++jb) {
       alive = alive && bounded_wait(&full[c_st], c_ph);
@@ -277,22 +279,6 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
               }
             }
           }
-        // ---- the largest value scale that is a number
-        {
-          const float v = (v_scale - g)[lane];
-          const uint32_t u = __reduce_max_sync(0xffffffffu, tok_b + lane < it.sq.kv_len && v < INFINITY ? __float_as_uint(v) : 0u);
-          if (u > __float_as_uint(ref_v)) {
-            const float to = power_above(u), ratio = ref_v * one_over(to);
-            ref_v = to;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int md = 0; md < HEAD_DIM / 16; ++md)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[n][md][i] *= ratio;
-          }
-        }
-        const float v_mul = R8_HELD * one_over(ref_v);
         // ---- softmax: this thread has tokens g + 8 i of its rows, score (i, e) in s[n][i / 2][2 (i % 2) + e]
         float top[NT][2];
         uint32_t hid = 0;
@@ -339,27 +325,53 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
               const float corr = up ? ex2(m_r[n][e] - top[n][e]) : 1.f;
               if (up) m_r[n][e] = top[n][e];
               l_r[n][e] *= corr;
+              // (the weights so far shrink, and r with them: a power of two at or above)
+              const float now = r_r[n][e] * corr, to = fmaxf(power_above(__float_as_uint(now)), R8_LEAST), f = now * one_over(to);
+              r_r[n][e] = to;
 #pragma unroll
-              for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][e] *= corr, o[n][md][2 + e] *= corr;
+              for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][e] *= f, o[n][md][2 + e] *= f;
             }
         }
-        uint32_t p[NT][4];                    // P^T as B fragments: tokens 8 i + 2 t4, 2 t4 + 1 of row g
+        // ---- weights: probabilities times their values' scales, none where the row does not see the token (whose scale may be NaN)
+        float most[NT][2];
+        bool more = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float vs = v_scale[8 * i] * v_mul;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float x[2];
+          for (int e = 0; e < 2; ++e) {
+            const float ref = m_r[n][e] == -INFINITY ? 0.f : m_r[n][e];   // (no score above -inf: every probability is 0, not the NaN of inf - inf)
+            most[n][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float& x = s[n][i >> 1][2 * (i & 1) + e];
+              x = ex2(x - ref);
+              l_r[n][e] += x;
+              x *= v_scale[8 * i];
+              if (open && (hid >> (n * 8 + 2 * i + e) & 1)) x = 0.f;
+              most[n][e] = fmaxf(most[n][e], x);
+            }
+            more |= most[n][e] > r_r[n][e] * R8_ROOM;
+          }
+        if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float ref = m_r[n][e] == -INFINITY ? 0.f : m_r[n][e];   // (no score above -inf: every probability is 0, not the NaN of inf - inf)
-              x[e] = ex2(s[n][i >> 1][2 * (i & 1) + e] - ref);
-              l_r[n][e] += x[e];
-              x[e] *= vs;
-              if (open && (hid >> (n * 8 + 2 * i + e) & 1)) x[e] = 0.f;     // (a hidden row's scale may be NaN)
+              float x = fmaxf(most[n][e], __shfl_xor_sync(0xffffffffu, most[n][e], 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              const float to = x > r_r[n][e] * R8_ROOM ? fminf(power_above(__float_as_uint(x)), 0x1p126f) : r_r[n][e], f = r_r[n][e] * one_over(to);
+              r_r[n][e] = to;
+#pragma unroll
+              for (int md = 0; md < HEAD_DIM / 16; ++md) o[n][md][e] *= f, o[n][md][2 + e] *= f;
             }
-            p[n][i] = movmatrix_trans(f16x2(x[0], x[1]));
-          }
+        }
+        uint32_t p[NT][4];                    // weights^T as B fragments: tokens 8 i + 2 t4, 2 t4 + 1 of row g
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float h0 = R8_HELD * one_over(r_r[n][0]), h1 = R8_HELD * one_over(r_r[n][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[n][i] = movmatrix_trans(f16x2(s[n][i >> 1][2 * (i & 1)] * h0, s[n][i >> 1][2 * (i & 1) + 1] * h1));
         }
         // ---- O^T += V^T P^T: 8 tiles of 16 dims x 2 steps of 16 tokens; a register of codes is tokens 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9 of a dim
 #pragma unroll
@@ -410,7 +422,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
         for (int w = 0; w < R8_WARPS; ++w) l += ml[w].y * ex2(ml[w].x - ref);
         m_all[n][e] = m;
         l_all[n][e] = l;
-        by[n][e] = ex2(m_r[n][e] - ref) * (ref_v * (1.f / R8_HELD));
+        by[n][e] = ex2(m_r[n][e] - ref) * (r_r[n][e] * (1.f / R8_HELD));
       }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
