@@ -7,8 +7,8 @@ from cache8_checks import D, PAGE, attend, branches, cache_of, check, layout, sl
 
 pytestmark = pytest.mark.gpu
 N_Q, N_KV = 8, 2
-DRAFTS = [("rows", [(12, 300), (5, 60), (1, 40), (12, 0)])]
-CASES = [c + (t,) for c in DRAFTS for t in (None, branches)]
+DRAFTS = [("rows", [(12, 300), (5, 60), (1, 40), (12, 0)]), ("prompt", [(12, 300), (5, 60), (1, 40), (12, 0)]), ("prompt", [(64, 100), (40, 0), (61, 3), (64, 300)])]
+CASES = [c + (t,) for c in DRAFTS for t in (None, branches)] + [("prompt", [(300, 0), (129, 171), (200, 0)], None)]
 
 
 def rows(n_pages, seed, q_rows):

@@ -11,10 +11,12 @@
 //
 // Both products are f16 x f16 -> fp32 (kind::f16).  Four warps widen K and V as they multiply them by their rows' scales (a code has 4 bits,
 // so a product rounded to f16's 11 is off by 2^-11; a key's scale is applied as two f16 numbers, for an error of the whole row's
-// would be one of its score); both are held relative to a power of two at or above the scales, the tile's for K, that of the keys so far
-// for V.  A query row is exact in f16 but for numbers 2^-22 of its largest and below.  A probability is one f16 number of 11 bits,
-// held times 2^7; the reference m of a row's exponentials moves only when a score passes it by 2^8, so that it fits f16 (2^15 at
-// most) and nothing above 2^-31 of the largest is lost.  (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the
+// would be one of its score); both are held relative to a power of two at or above the tile's scales.  A query row is exact in f16 but for
+// numbers 2^-22 of its largest and below.  A weight (a probability times the tile's unit of V) is one f16 number of 11 bits, held times 2^7;
+// a row has one reference of its exponentials and one of its weights, which move only when something passes them by 2^8, so that it
+// fits f16 (2^15 at most) and nothing above 2^-31 of the row's largest is lost.  A tile whose scales lie further apart than 2^12 has no unit
+// that serves a row which sees its small ones alone: its codes stay as they are, exact, and the softmax multiplies scores and probabilities by
+// the scales, in fp32 and in steps.  So what a row does not see, or gives no weight, never costs it its own tokens' bits.  (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the
 // products cost the same and every score takes a multiplication by its key's scale, every probability one by its value's: as first
 // built both took 380 us for 1859 tokens behind 6144, 32 / 8 heads, and each later step, to 263, needed the multiplications gone.)
 // Two threads share a row, half of a step's columns each; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are
@@ -23,8 +25,8 @@
 // What bounds it: the chain of a step.  Of its 4900 clocks an accumulator spends 3100 in the softmax (scores read 600, the two threads'
 // maximum 300, exponentials 2000, 1024 of them the least that 16 a clock take) and 1700 in its two products, which wait for those of
 // the other one; the two take turns.  Without the exponentials a step is 4500, without the widening 4550: nothing alone is the bound.
-// 1859 tokens behind 6144: 264 us, 815 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
-// prompt of 2048: 75; six prompts of 90 to 593 (1679 tokens): 39; 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 80.
+// 1859 tokens behind 6144: 274 us, 788 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
+// prompt of 2048: 76; six prompts of 90 to 593 (1679 tokens): 39; 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 82.
 // A unit's beginning and end take as much as three and a half steps (Q copied and turned, the first pages, O): what short prompts consist of.
 //
 // No wait is unbounded: after about two seconds a role gives up, the call's status says so; copies and MMAs in flight land first and TMEM is
@@ -46,8 +48,14 @@ constexpr int P8_KV = 128, P8_BLOCKS = P8_KV / KV_BLOCK;    // keys of a step
 constexpr int P8_NOTES = 4;
 constexpr int P8_TILE = P8_KV * HEAD_DIM * 2;               // bytes of a tile of K or V, of one accumulator's Q, in f16
 constexpr float P8_SLACK = 8.f;                             // exp2 domain: how far a score may exceed its row's reference
-constexpr float P8_HELD = 7.f;                              // exp2 domain: probabilities and their sums are held times 2^7
+constexpr float P8_HELD = 7.f, P8_HELD_TIMES = 128.f;       // exp2 domain: weights and sums are held times 2^7
+constexpr float P8_LEAST = -118.f;                          // exp2 domain: smallest unit of weights
 constexpr float P8_V_TOP = 64.f, P8_K_TOP = 16.f;           // largest scale that a code (448 at most) is multiplied by
+constexpr int P8_V_TOP_LOG = 6;
+// A tile's scales lie within this of its largest (the power of two above it), or its codes stay without them: what is held relative to
+// one unit would lose the small rows' bits, and a row may see those alone.  (Scales of a layer's rows differ by 2^2 to 2^5, those of a prompt's first
+// token by up to 2^8.  The smallest scale of all, that of rows of zeros, does not count.)
+constexpr float P8_BAND = 0x1p-12f;
 // What the beginning and the end of a unit count for, in steps.  As 1, 2, 3: 2048 tokens 85, 75, 72 us; six prompts of 90 to 593 38.8, 38.6, 40.4;
 // 16 drafts of 5 to 24 behind 200 to 1500 36, 33.5, 35
 constexpr uint32_t P8_COST = 2;
@@ -55,10 +63,11 @@ constexpr uint32_t P8_COST = 2;
 // What the softmax has to know of a tile, beside its scores
 struct TileNotes {
   uint32_t poison[P8_BLOCKS];  // tokens whose key or value row is not a number
-  uint32_t special;            // bits 0..3: blocks whose page does not exist; bit 4: there are poisoned tokens
-  float k_unit, v_unit;        // what a number of K, of V is in units of
+  uint32_t special;            // bits 0..3: blocks whose page does not exist; bit 4: there are poisoned tokens; bit 5: codes without their scales
+  float k_unit, v_log;         // what a number of K is in units of; log2 of what one of V is
   uint32_t pad;
 };
+constexpr uint32_t P8_ODD = 1u << P8_BLOCKS, P8_WIDE = 2u << P8_BLOCKS;
 // Steps [tile0, tile1) of a unit: the copying warp walks the row of steps, the others take from its list
 struct Task {
   int tile0, tile1;            // tile1 0: no more
@@ -80,6 +89,7 @@ struct P8Smem {
   // scales of value rows as f16 multipliers at their places, of even and odd tiles, a copy for every warp that uses them
   __align__(16) uint16_t v_mul[P8_WIDEN][2][P8_KV];
   TileNotes notes[P8_NOTES];   // tile t's: t % P8_NOTES
+  float row_scales[P8_NOTES][2][P8_KV];    // of keys, of values, where a tile's codes are without them
   Task task[P8_TASKS];
   float pair[2][2][2][128];    // what the two threads of a row tell one another: of even and odd times, accumulator, half, row
   uint64_t task_full[P8_TASKS], task_empty[P8_TASKS], raw_k_full, raw_k_empty, raw_v_full, raw_v_empty, q_full[2], note_full[P8_NOTES], pair_full[2][4],
@@ -233,6 +243,69 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+
+// ---- a thread's scores in steps, 16 at a time, for tiles that need it.  Calls: in line they took 8 % of all other tiles' time, called 3 %
+// (a unit that is no normal number would make scores of nothing 0 * -inf where they are hidden, or 0 * inf: NaN; scores of 2^24 units at most are
+// nothing beside 2^-126 of them.  A NaN fails both comparisons and stays)
+__device__ __forceinline__ float p8_normal(float x) { return x < 0x1p-126f ? 0x1p-126f : x > 0x1.fffffep127f ? 0x1.fffffep127f : x; }
+// scores 16 c .. 16 c + 15, -inf where hidden; ks: scales of their keys, NULL: `times` has them
+__device__ __forceinline__ void p8_scores(float (&x)[16], uint32_t s_t, int c, uint32_t vis0, uint32_t vis1, float times, const float* ks) {
+  uint32_t s[16];
+  tmem_ld_32x32b_x16(s_t + c * 16, s);
+  const uint32_t seen = (c < 2 ? vis0 : vis1) >> (c & 1) * 16;
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = seen >> i & 1 ? __uint_as_float(s[i]) * (ks != nullptr ? p8_normal(times * ks[c * 16 + i]) : times) : -INFINITY;
+}
+__device__ __noinline__ float p8_top(uint32_t s_t, int nb, uint32_t vis0, uint32_t vis1, float times, const float* ks) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < 2 * min(nb, 2); ++c) {
+    float x[16];
+    p8_scores(x, s_t, c, vis0, vis1, times, ks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+  }
+  return top;
+}
+// the largest probability times its value's scale (vs NULL: 2^v_log)
+__device__ __noinline__ float p8_most(uint32_t s_t, int nb, uint32_t vis0, uint32_t vis1, float times, const float* ks, float ref, const float* vs, float v_log) {
+  float most = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 2 * min(nb, 2); ++c) {
+    float x[16];
+    p8_scores(x, s_t, c, vis0, vis1, times, ks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, ex2(x[i] - ref) * (vs != nullptr ? vs[c * 16 + i] : ex2(v_log)));
+  }
+  return most;
+}
+// weights to where the product reads them; the sum of the probabilities, times 2^7
+__device__ __noinline__ float p8_weights(uint32_t s_t, int nb, uint32_t vis0, uint32_t vis1, float times, const float* ks, float ref, const float* vs, float v_log,
+                                         float unit) {
+  const float hold = ex2(P8_HELD - unit);
+  float l = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 2 * min(nb, 2); ++c) {
+    float x[16];
+    uint32_t p[8];
+    p8_scores(x, s_t, c, vis0, vis1, times, ks);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] = ex2(x[i] - ref);
+      l += x[i] * P8_HELD_TIMES;
+      x[i] = x[i] * (vs != nullptr ? vs[c * 16 + i] : ex2(v_log)) * hold;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int col = 2 * (4 * (i & 1) + (i >> 1));   // as in the kernel
+      p[i] = f16x2(x[col], x[col + 1]);
+    }
+    tmem_st_x8(s_t + c * 8, p);   // (over scores that have been read)
+  }
+  return l;
+}
+
 __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __grid_constant__ PromptArgs a) {
   extern __shared__ uint8_t smem_raw[];
   P8Smem& sm = *reinterpret_cast<P8Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -446,8 +519,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       uint32_t v_full = 0;
       while (const Task* tp = take()) {
         const int tile0 = tp->tile0, tile1 = tp->tile1, kv_len = tp->kv_len;
-        float r = 0.f;
         uint32_t hi = 0, lo = 0;              // this thread's key scale as two f16 numbers, each twice
+        float row_k = 0.f, row_v = 0.f;       // its scales as they are
         TileNotes mem;                        // (poison[0]: of this warp's block)
         // Scales of tile j, which every warp looks at all of (lane = token of a block).  Done ahead of the waits for buffers, which
         // come once a step and all at once
@@ -456,7 +529,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           ok = __all_sync(0xffffffffu, bounded_wait(&sm.raw_k_full, kt & 1));
           if (!ok) return;
           const uint32_t absent = sm.absent;
-          float my_k = 0.f, vs[P8_BLOCKS], top_k = 0.f, top_v = 0.f;
+          float vs[P8_BLOCKS], top_k = 0.f, top_v = 0.f, low_k = INFINITY, low_v = INFINITY;
           uint32_t any_odd = 0;
 #pragma unroll
           for (int b = 0; b < P8_BLOCKS; ++b) {
@@ -470,18 +543,23 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
             any_odd |= odd;
             top_k = fmaxf(top_k, k);
             top_v = fmaxf(top_v, vs[b]);
-            if (b == mine) my_k = k, mem.poison[0] = odd;
+            if (k > KV8_TINY) low_k = fminf(low_k, k);
+            if (vs[b] > KV8_TINY) low_v = fminf(low_v, vs[b]);
+            if (b == mine) row_k = k, row_v = vs[b], mem.poison[0] = odd;
           }
-          const float k_top = fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_k))), 0x1p-118f);
-          r = fmaxf(r, fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v))), 0x1p-118f));
-          const float v_to = P8_V_TOP * one_over(r), k = my_k * (P8_K_TOP * one_over(k_top));
-          hi = f16x2(k, k);
-          lo = f16x2(k - f16x2_to_f32x2(hi).x, k - f16x2_to_f32x2(hi).x);
+          auto above = [](float top) { return fmaxf(power_above(__reduce_max_sync(0xffffffffu, __float_as_uint(top))), 0x1p-118f); };
+          auto least = [](float low) { return __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low))); };
+          const float k_top = above(top_k), v_top = above(top_v);
+          const bool wide = least(low_k) < k_top * P8_BAND || least(low_v) < v_top * P8_BAND;
+          const float v_to = P8_V_TOP * one_over(v_top), k = row_k * (P8_K_TOP * one_over(k_top));
+          hi = wide ? f16x2(1.f, 1.f) : f16x2(k, k);
+          lo = wide ? 0u : f16x2(k - f16x2_to_f32x2(hi).x, k - f16x2_to_f32x2(hi).x);
 #pragma unroll
-          for (int b = 0; b < P8_BLOCKS; ++b) sm.v_mul[mine][kt & 1][b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(vs[b] * v_to, 0.f);
-          mem.special = absent | (any_odd != 0 ? 1u << P8_BLOCKS : 0u);
+          for (int b = 0; b < P8_BLOCKS; ++b)
+            sm.v_mul[mine][kt & 1][b * KV_BLOCK + (lane & 16) + v8_place(lane & 15)] = (uint16_t)f16x2(wide ? 1.f : vs[b] * v_to, 0.f);
+          mem.special = absent | (any_odd != 0 ? P8_ODD : 0u) | (wide ? P8_WIDE : 0u);
           mem.k_unit = k_top * (1.f / P8_K_TOP);
-          mem.v_unit = r * (1.f / P8_V_TOP);
+          mem.v_log = wide ? 0.f : (float)((int)(__float_as_uint(v_top) >> 23) - 127 - P8_V_TOP_LOG);
         };
         // K: sixteen dims at a time -> two groups of eight numbers.  (A block that a last tile does not have is not read.)
         auto widen_k = [&](int j) {
@@ -492,7 +570,11 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           const uint32_t k_out = k_out0 + (kt & 1) * P8_TILE;
           if (lane == 0) {
             t.poison[mine] = mem.poison[0];
-            if (mine == 0) t.special = mem.special, t.k_unit = mem.k_unit, t.v_unit = mem.v_unit;
+            if (mine == 0) t.special = mem.special, t.k_unit = mem.k_unit, t.v_log = mem.v_log;
+          }
+          if (mem.special & P8_WIDE) {
+            sm.row_scales[kt % P8_NOTES][0][part] = row_k;
+            sm.row_scales[kt % P8_NOTES][1][part] = row_v;
           }
           auto wide = [&](uint32_t two) {
             const uint32_t h = e4m3x2_to_f16x2(two);
@@ -642,7 +724,9 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[g]);
-      float m = 0.f, l = 0.f, unit = 0.f;
+      float m = 0.f, l = 0.f, unit = 0.f;                       // unit: log2 of what O is in units of, 2^m apart
+      float most_unit = 0.f;                                    // no row's is larger
+      bool large = false;                                       // some row's reference is
       const int tile0 = t.tile0, tile1 = t.tile1;
       for (int j = tile0; j < tile1; ++j) {
         const int nb = t.blocks(j) - 2 * h;                 // of this thread's half
@@ -651,11 +735,12 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         if (!ok) break;
         sph ^= 1;
         tc_fence_after();
-        const TileNotes& sc = sm.notes[tile % P8_NOTES];
+        const int at_note = tile % P8_NOTES;
+        const TileNotes& sc = sm.notes[at_note];
         ++tile;
         const int seen = lim - j * P8_KV - h * 64;          // last column seen (of the keys before a draft)
         const uint32_t special = sc.special;
-        const bool mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || special != 0);
+        const bool wide = (special & P8_WIDE) != 0, mask = __any_sync(0xffffffffu, seen < nb * KV_BLOCK - 1 || (special & ~P8_WIDE) != 0);
         uint32_t vis[2] = {0xffffffffu, 0xffffffffu};       // columns that the row sees
         if (mask) {
 #pragma unroll
@@ -674,35 +759,74 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           for (int i = 0; i < 32; ++i)
             if (!(seen_of_it >> i & 1)) s[i] = __float_as_uint(-INFINITY);
         };
+        const float qk = p8_normal(qm * sc.k_unit);
+        auto k_scales = [&]() { return wide ? sm.row_scales[at_note][0] + h * 64 : nullptr; };
+        auto v_scales = [&]() { return wide ? sm.row_scales[at_note][1] + h * 64 : nullptr; };
         // The scores are read twice, 32 at a time: once for their maximum, once for the probabilities (all at once spill).  The loops are not
         // unrolled: the instruction cache does not hold the roles' code if they are
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (__builtin_expect(!wide, 1)) {
 #pragma unroll 1
-        for (int c = 0; c < min(nb, 2); ++c) {
-          uint32_t s[32];
-          tmem_ld_x32(s_t + c * 32, s);
-          tmem_ld_wait();
-          if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
+          for (int c = 0; c < min(nb, 2); ++c) {
+            uint32_t s[32];
+            tmem_ld_x32(s_t + c * 32, s);
+            tmem_ld_wait();
+            if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            for (int i = 0; i < 32; i += 2) mx[i >> 1 & 3] = max3(mx[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+          }
+        } else {
+          mx[0] = p8_top(s_t, nb, vis[0], vis[1], qm, k_scales());
         }
-        // (a unit that is no normal number would make hidden scores, -inf, times 0 NaN; scores of 2^24 units at most are nothing beside 2^-126 of
-        // them.  A NaN fails the comparison and stays)
-        float qk = qm * sc.k_unit;
-        if (qk < 0x1p-126f) qk = 0x1p-126f;
-        uint64_t qm2 = pack2(qk, qk);
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        top = fmaxf(top, pair_up(top)) * qk;
+        top = fmaxf(top, pair_up(top));
+        if (!wide) top *= qk;
+        else if (!(qm < INFINITY)) top = qm;                 // (the maximum of NaN and -inf)
         if (!ok) break;
-        const float unit_now = sc.v_unit;
+        // A row's weights, probabilities times what their values are in units of, have a reference of their own, 2^(m + unit): the row's largest one
+        // may belong to another token than its largest probability.  Both move only when something passes them by 2^8
+        const float v_log = sc.v_log;
+        float f = 1.f;                                       // what O is multiplied by
+        bool moved = false;                                  // some row's is not 1
+        auto reference = [&]() { return m == -INFINITY ? 0.f : m; };   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
         if (j == tile0) {
           m = top;
-        } else if (__any_sync(0xffffffffu, top > m + P8_SLACK) || unit_now != unit) {
+          unit = most_unit = v_log;
+          large = __any_sync(0xffffffffu, fabsf(reference()) > 0x1p20f);
+        } else if (__any_sync(0xffffffffu, top > m + P8_SLACK || (!wide && top - m + v_log > unit + P8_SLACK))) {
+          const bool up = top > m + P8_SLACK;
+          const float by = up ? m - top : 0.f;
+          if (up) m = top;
+          // (a row without a score above -inf so far has nothing in O, whatever its unit is)
+          const float to = fmaxf(ceilf(unit + by), wide ? P8_LEAST : v_log + ceilf(top - reference()));
+          l *= ex2(by);
+          f = ex2(by + unit - to);
+          unit = to;
+          most_unit = fmaxf(most_unit, v_log + P8_SLACK);
+          moved = true;
+          large = __any_sync(0xffffffffu, fabsf(reference()) > 0x1p20f);
+        }
+        const float ref = reference();
+        // One product and one addition make an exponent, and a row's sum is that of its weights, unless its scales differ, its values are so much
+        // smaller than earlier ones that the sum would lose what they do, or its scores are so large that an exact product less a rounded one
+        // may be far from zero: then in steps, which costs such a tile five to seven times its time (2048 tokens 381 us, not 76)
+        const bool in_steps = wide || large || (most_unit - v_log > 64.f && __any_sync(0xffffffffu, unit - v_log > 64.f));
+        if (__builtin_expect(in_steps, 0)) {
+          float most = p8_most(s_t, nb, vis[0], vis[1], wide ? qm : qk, k_scales(), ref, v_scales(), v_log);
+          most = fmaxf(most, pair_up(most));
+          if (!ok) break;
+          // exponent of the power of two at or above it
+          float to = fmaxf((float)((int)(__float_as_uint(power_above(__float_as_uint(most))) >> 23) - 127), P8_LEAST);
+          if (j != tile0) {
+            to = fmaxf(to, unit);
+            f *= ex2(unit - to);
+            moved = true;
+          }
+          unit = to;
+          most_unit = INFINITY;
+        }
+        if (moved) {
           // the products that wrote O retired before these scores did
-          float f = top > m + P8_SLACK ? ex2(m - top) : 1.f;
-          if (top > m + P8_SLACK) m = top;
-          l *= f;
-          f *= unit / unit_now;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[16];
@@ -713,39 +837,35 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
             tmem_st_x16(o_t + c * 16, o);
           }
         }
-        unit = unit_now;
-        const float ref = m == -INFINITY ? 0.f : m;   // (no score above -inf so far: every probability is 0, not the NaN of inf - inf)
-        const uint64_t neg_m = pack2(P8_HELD - ref, P8_HELD - ref);
-        // an exact product less a rounded one may be far from zero where both are large: such scores are rounded first, as their maximum was
-        const bool large = fabsf(ref) > 0x1p20f;
-        if (large) qm2 = pack2(1.f, 1.f);
         uint64_t sum0 = 0, sum1 = 0;
+        if (__builtin_expect(!in_steps, 1)) {
+          const float add = P8_HELD + (v_log - unit) - ref;
+          const uint64_t qm2 = pack2(qk, qk), neg_m = pack2(add, add);
 #pragma unroll 1
-        for (int c = 0; c < min(nb, 2); ++c) {
-          uint32_t s[32];
-          tmem_ld_x32(s_t + c * 32, s);
-          tmem_ld_wait();
-          if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
-          if (large) {
+          for (int c = 0; c < min(nb, 2); ++c) {
+            uint32_t s[32];
+            tmem_ld_x32(s_t + c * 32, s);
+            tmem_ld_wait();
+            if (mask) hide(s, c == 0 ? vis[0] : vis[1]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(__uint_as_float(s[i]) * qk);
-          }
+            for (int k = 0; k < 2; ++k) {
+              uint32_t p[8];
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int col = k * 16 + 2 * (4 * (i & 1) + (i >> 1));   // places 2 i, 2 i + 1 of half a block (cache8.cuh v8_place)
-              float x, y;
-              unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
-              x = ex2(x);
-              y = ex2(y);
-              if (i & 1) sum1 = add2(sum1, pack2(x, y));
-              else sum0 = add2(sum0, pack2(x, y));
-              p[i] = f16x2(x, y);
+              for (int i = 0; i < 8; ++i) {
+                const int col = k * 16 + 2 * (4 * (i & 1) + (i >> 1));   // places 2 i, 2 i + 1 of half a block (cache8.cuh v8_place)
+                float x, y;
+                unpack2(fma2(pack2(__uint_as_float(s[col]), __uint_as_float(s[col + 1])), qm2, neg_m), x, y);
+                x = ex2(x);
+                y = ex2(y);
+                if (i & 1) sum1 = add2(sum1, pack2(x, y));
+                else sum0 = add2(sum0, pack2(x, y));
+                p[i] = f16x2(x, y);
+              }
+              tmem_st_x8(s_t + c * 16 + k * 8, p);   // (over scores that have been read)
             }
-            tmem_st_x8(s_t + c * 16 + k * 8, p);   // (over scores that have been read)
           }
+        } else {
+          l += p8_weights(s_t, nb, vis[0], vis[1], wide ? qm : qk, k_scales(), ref, v_scales(), v_log, unit);
         }
         tmem_st_wait();
         tc_fence_before();
@@ -753,7 +873,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         if (lane == 0) mbar_arrive(&sm.p_full[g]);
         float x, y;
         unpack2(add2(sum0, sum1), x, y);
-        l += x + y;
+        if (!in_steps) l += (x + y) * ex2(unit - v_log);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, bounded_wait(&sm.o_full[g], oph));
@@ -774,7 +894,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
         }
         __syncwarp();
       };
-      const float by = t.cut != 0 ? unit : l == 0.f ? 0.f : unit / l;
+      // (in two steps, for values next to fp32's largest)
+      const float by = t.cut != 0 ? ex2(unit) : l == 0.f ? 0.f : ex2(unit - 8.f) / (l * 0x1p-8f);
       const size_t slot = ((size_t)blockIdx.x * 2 + ((t.cut & 1) == 0)) * 256 + g * 128;
 #pragma unroll 1
       for (int c = 0; c < 2; ++c) {
