@@ -675,7 +675,7 @@ int tgis_kv8_write(void* pages, int32_t n_pages, int32_t n_kv, const void* qkv, 
   if (T == 0) return 0;
   if (check_rows("qkv", qkv, ld, (int64_t)n_q + 2 * n_kv) != 0) return -1;
   if (q_out != nullptr && n_q > 0 && check_rows("q_out", q_out, ldq, n_q) != 0) return -1;
-  if (q_out == qkv && q_out != nullptr && ldq != ld) return fail("queries rotated in place keep their rows: ldq %lld, ld %lld", (long long)ldq, (long long)ld);
+  if (T > 1 && q_out == qkv && q_out != nullptr && ldq != ld) return fail("queries rotated in place keep their rows: ldq %lld, ld %lld", (long long)ldq, (long long)ld);
   if (positions == nullptr || slots == nullptr || !aligned(positions, 4) || !aligned(slots, 4)) return fail("positions, slots: int32 pointers are wanted");
   if (cos_sin == nullptr || !aligned(cos_sin, 16) || n_positions < 1) return fail("cos_sin: a 16-byte aligned table of at least one position is wanted");
   return done(tgis::kv8_write_launch((uint8_t*)pages, n_pages, n_kv, (const __nv_bfloat16*)qkv, ld, T, n_q, positions, slots, (const __nv_bfloat16*)cos_sin,
