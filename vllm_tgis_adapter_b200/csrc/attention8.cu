@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
     const int seen_by_all = prefix_len + (a.tree == nullptr ? it.chunk * ROWS / G + 1 : 0);
     const int n_blk = blocks_of(it);
     for (int jb = 0; jb < n_blk; ++jb) {
-      alive = alive && bounded_wait(&full[c_st], c_ph);
+      alive = alive && warp_wait(&full[c_st], c_ph);
       const bool ok = alive && page_ok[c_st] != 0;
       if (ok) {
         const uint32_t k_base = ring_base + c_st * KV8_PAGE, v_base = k_base + KV8_CODES;

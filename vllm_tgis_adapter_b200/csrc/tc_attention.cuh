@@ -72,19 +72,26 @@ __device__ __forceinline__ void set_regs() {
   if constexpr (UP) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
-// false: the wait ran out
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity) {
+// about two seconds: no wait of a working pipeline is that long
+constexpr long long WAIT_LIMIT = 4000000000ll;
+// false: the wait ran out.  Lanes count for themselves: a copy that lands as they give up is seen by some of a warp, so whatever goes on by
+// the result asks the whole warp (warp_wait, __all_sync)
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, long long limit = WAIT_LIMIT) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > 4000000000ll) return false;   // about two seconds: no wait of a working pipeline is that long
+    if (clock64() - t0 > limit) return false;
   return true;
+}
+// false in all lanes: the wait of one ran out
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, long long limit = WAIT_LIMIT) {
+  return __all_sync(0xffffffffu, bounded_wait(bar, parity, limit));
 }
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, int* err) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > 4000000000ll) {   // about two seconds: no wait of a working pipeline is that long
+    if (clock64() - t0 > WAIT_LIMIT) {
       *reinterpret_cast<volatile int*>(err) = 1;
       __threadfence_system();
       return false;

@@ -7,6 +7,8 @@
 
 #include "../../include/tgis_kernels.h"
 #include "kernels.h"
+#include "ptx.cuh"
+#include "tc_attention.cuh"
 
 using namespace tgis;
 using bf16 = __nv_bfloat16;
@@ -40,6 +42,22 @@ int product_end() {
   return gemm_pair_failed() ? kfail("a product's pipeline wait ran out") : 0;
 }
 
+// lanes whose bit is set wait for a barrier that has been arrived at, the others for one that never is; what each was told
+__global__ void warp_wait_kernel(uint32_t arrived, long long limit, uint32_t* told) {
+  __shared__ uint64_t bar[2];
+  const int lane = threadIdx.x;
+  if (lane == 0) {
+    mbar_init(&bar[0], 1);
+    mbar_init(&bar[1], 1);
+    fence_barrier_init();
+    mbar_arrive(&bar[0]);
+  }
+  __syncwarp();
+  const bool ok = warp_wait(&bar[arrived >> lane & 1 ? 0 : 1], 0, limit);
+  const uint32_t all = __ballot_sync(0xffffffffu, ok);
+  if (lane == 0) *told = all;
+}
+
 int test_num_sms() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -63,6 +81,16 @@ struct Tmp {
 }  // namespace
 
 extern "C" {
+
+int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told) {
+  if (told == nullptr || limit < 0 || limit > WAIT_LIMIT) return kfail("told is NULL, or the limit is above that of the kernels");
+  Tmp<uint32_t> d;
+  KCK(d.alloc(1));
+  warp_wait_kernel<<<1, 32>>>(arrived, limit, d.p);
+  KCK(cudaGetLastError());
+  KCK(cudaMemcpy(told, d.p, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  return 0;
+}
 
 int tgis_k_pair_fault(int32_t nth) { return gemm_pair_fault(nth); }
 
