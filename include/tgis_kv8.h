@@ -44,7 +44,8 @@ int tgis_kv8_write(void* pages, int32_t n_pages, int32_t n_kv, const void* qkv, 
 int tgis_kv8_read(const void* pages, int32_t n_pages, int32_t n_kv, const int32_t* slots, int32_t T, void* k_out, int64_t ldk, void* v_out,
                   int64_t ldv, int32_t* status, void* stream);
 
-/* Bytes of workspace that tgis_kv8_attention needs for these bounds (host only); < 0: bad arguments */
+/* Bytes of workspace that tgis_kv8_attention needs for these bounds (host only); < 0: bad arguments.  No fewer for more sequences, for more queries
+ * of a sequence or for longer ones, and 43 MB at most: one for the largest of each that a program calls with serves all its calls. */
 int64_t tgis_kv8_attention_workspace(int32_t T, int32_t n_seqs, int32_t n_q, int32_t n_kv, int32_t max_q, int32_t max_kv);
 
 /* out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j over the rows that the query sees, h's head being h / (n_q / n_kv).

@@ -41,6 +41,7 @@ constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
 // 128: 8.0 and 12.3; 64 behind 500: 12.6 and 19.2, 128: 13.1 and 21.0; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
 // 9.2, of 48 (not): 13.3 and 11.4.
 constexpr int R8_MOST_ROWS = 48, R8_MORE_KEYS = 1024;
+constexpr int R8_ONE_SPLIT = 768;                  // keys of a sequence that are not split
 constexpr float R8_SLACK = 8.f;                    // exp2 domain: how far a score may exceed its row's reference
 constexpr float R8_HELD = 128.f, R8_ROOM = 256.f;  // weights are held times 2^7 / r; how often r fits into the largest of them before it moves
 constexpr float R8_LEAST = 0x1p-118f;              // smallest r
@@ -551,17 +552,24 @@ __global__ void __launch_bounds__(M8_WARPS * 32) attn8_merge_kernel(const __grid
   }
 }
 
+// Partial sums of a (query, head) and split; what those of a call take at most, which is what attention8_prompt.cu takes (43 MB, which stay in the L2):
+// splits that would need more are fewer.  Microseconds with all of them and with those that fit, 32 / 8 heads: 256 x 8 queries behind 8100
+// (4 and 1) 1408 and 1157, behind 4000 (2 and 1) 716 and 619; 64 x 12 behind 8100 (4 and 3) 540 and 515; 256 x 12 (4 and 1) 2115 and 1706.
+constexpr size_t R8_PART = (HEAD_DIM + 2) * sizeof(float);
+size_t parts_room() { return attn8_prompt_workspace(ATTN8_MAX_SMS); }
+
 struct RowsPlan {
   int rows, split, max_splits;
-  double most_splits;                         // as many or more, no fewer for more keys, and no fewer of all sequences for more of these
-  bool prompt;                                // attention8_prompt.cu
+  bool wide, prompt;                          // more than this kernel is for; attention8_prompt.cu takes them
 };
 RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   RowsPlan p{};
   const int rows = (int)std::min<long long>((long long)max_q * (n_q / n_kv), 1 << 30);
   p.rows = rows > 8 ? 16 : 8;
+  // (a B200's SMs, whatever the device has: a workspace's size is asked for without one)
   const double items = (double)std::max(n_seqs, 1) * n_kv * ((rows + p.rows - 1) / p.rows), slots = 148. * R8_CTAS(p.rows);
-  p.prompt = rows > R8_MOST_ROWS && (items > slots || max_kv > R8_MORE_KEYS) && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
+  p.wide = rows > R8_MOST_ROWS && (items > slots || max_kv > R8_MORE_KEYS);
+  p.prompt = p.wide && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   // Splits (the bounds are those of the longest sequence): one for few tokens, which the second launch costs more than it saves; else as
   // many as run at once, of 256 to 4096 tokens; else one for 2048 tokens or three rounds of them, of 1024 to 2048.  Microseconds, 32 / 8 heads,
   // one single token behind 600: one split 8.4, of 256 tokens 8.5; 1024: 10.8 and 8.6; 12 behind 2048: four (all at once) 14.2, six 19.9,
@@ -569,10 +577,10 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   // run at once): one 112, of 1024 tokens 106, of 256 147; 64 behind 2048: one 61, two 66.
   auto length = [&](double n) { return (int)std::ceil(max_kv / std::max(n, 1.) / 128.) * 128; };
   const int at_once = std::max(length(std::floor(slots / items)), 256);
-  const bool few = max_kv <= 768;
-  p.split = few ? 768 : items <= slots && at_once <= 4096 ? at_once : max_kv <= 2048 ? 2048 : std::min(std::max(length(std::ceil(3. * slots / items)), 1024), 2048);
+  p.split = max_kv <= R8_ONE_SPLIT ? R8_ONE_SPLIT : items <= slots && at_once <= 4096 ? at_once : max_kv <= 2048 ? 2048 : std::min(std::max(length(std::ceil(3. * slots / items)), 1024), 2048);
+  const double room = std::max(1., std::floor((double)parts_room() / ((double)std::max(n_seqs, 1) * std::max(max_q, 1) * n_q * R8_PART)));
+  if ((max_kv + p.split - 1) / p.split > room) p.split = length(room);
   p.max_splits = std::max(1, (max_kv + p.split - 1) / p.split);
-  p.most_splits = few ? 1. : std::min(max_kv / 256. + 1., std::max(3. * slots / items + 2., max_kv / 2048. + 1.));
   return p;
 }
 
@@ -593,10 +601,16 @@ cudaError_t rows_launch(const RowsArgs& a, int num_sms, cudaStream_t stream) {
 
 }  // namespace
 
+// No fewer bytes for more sequences, more of their queries or longer ones: whoever keeps one workspace asks for the largest of each.  Splits are at
+// most one for 256 tokens, and at most three rounds of items and two more, or one for 2048 tokens (rows_plan); a round has 296 items of 16 rows or
+// 444 of 8, so that splits times rows of all sequences are 3 * 4736 and two of each row at most.
 size_t attn8_workspace(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) {
   const RowsPlan p = rows_plan(T, n_seqs, n_q, n_kv, max_q, max_kv);
-  if (p.prompt) return attn8_prompt_workspace(ATTN8_MAX_SMS);
-  return p.most_splits > 1. ? ((size_t)std::ceil(n_seqs * p.most_splits) * max_q * n_q * (HEAD_DIM + 2) * sizeof(float) + 15) / 16 * 16 : 0;
+  if (p.wide) return parts_room();
+  const double rows = (double)n_seqs * n_q * max_q;
+  if (max_kv <= R8_ONE_SPLIT) return 0;
+  const double parts = std::min(rows * (max_kv / 256. + 1.), std::max(3. * 4736. + 2. * rows, rows * (max_kv / 2048. + 1.)));
+  return std::min((size_t)std::ceil(parts) * R8_PART, parts_room());
 }
 
 cudaError_t attn8_launch(const Attn8Args& args, void* workspace, int num_sms, cudaStream_t stream, int* launches, bool prompts) {

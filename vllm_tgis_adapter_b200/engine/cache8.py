@@ -130,7 +130,7 @@ class Cache8:
         return k_out, v_out
 
     def workspace_bytes(self, T: int, n_seqs: int, n_q: int, max_q: int, max_kv: int) -> int:
-        """What `attend` needs for these bounds (no fewer for more sequences, nor for longer ones)."""
+        """What `attend` needs for these bounds (no fewer for more sequences, more queries of one or longer ones; 43 MB at most)."""
         n = self._workspace(T, n_seqs, n_q, self.n_kv, max_q, max_kv)
         if n < 0:
             raise ValueError(self._error())
