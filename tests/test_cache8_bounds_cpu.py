@@ -2,7 +2,7 @@
 import pytest
 from test_cache8_cpu import AT, WRITE
 
-from vllm_tgis_adapter_b200.engine import _lib
+from vllm_tgis_adapter_b200.engine import _lib, cache8
 
 
 @pytest.fixture(scope="module")
@@ -29,3 +29,11 @@ def test_workspace_of_the_largest_call_serves_every_smaller_one(lib, n_q, n_kv):
         assert 0 <= here <= 160 * (2 * 256 * 130 * 4 + 32)
         for smaller in ((counts[max(counts.index(n) - 1, 0)], q, kv), (n, queries[max(queries.index(q) - 1, 0)], kv), (n, q, lengths[max(lengths.index(kv) - 1, 0)])):
             assert size[smaller] <= here, (smaller, (n, q, kv))
+
+
+@pytest.mark.parametrize("max_q,max_kv,says", [(1 << 32 | 5, 100, "31 bits"), (5, 1 << 32 | 100, "31 bits"), (5, 1 << 31, "31 bits"), (-1, 100, "31 bits"), (5, (1 << 31) - 1, "max_kv")])
+def test_bounds_are_not_cut_to_32_bits(lib, max_q, max_kv, says):
+    cache = object.__new__(cache8.Cache8)   # (as far as sizes go: one with pages needs a device)
+    cache._lib, cache._workspace, cache.n_kv = lib, lib.tgis_kv8_attention_workspace, 2
+    with pytest.raises(ValueError, match=says):
+        cache.workspace_bytes(5, 1, 4, max_q, max_kv)

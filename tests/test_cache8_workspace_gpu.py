@@ -28,3 +28,13 @@ def test_one_workspace_for_all_calls(n_q, n_kv, most_seqs, longest):
         some = {(s, i) for s in {0, n // 2, n - 1} for i in {0, new - 1}}
         check(cache, q, seqs, bt, 0.5 * D ** -0.5, "rows" if new * n_q // n_kv <= 48 else "prompt", got=got, only=some)
         assert bool((room[size:] == 0x5a).all())
+
+
+def test_bounds_are_not_cut_to_32_bits():
+    cache = cache_of(1, 1, *torch.ones(2, PAGE, 1, D, device="cuda"))
+    q, seqs, bt = torch.ones(1, D, device="cuda", dtype=torch.bfloat16), ints([[0, 1, 1, 0]]), ints([[0]])
+    ws = torch.zeros(64, dtype=torch.uint8, device="cuda")
+    for max_q, max_kv in ((1 << 32 | 1, 1), (1, 1 << 32 | 1), (1, 1 << 31), (-1, 1)):
+        for workspace in (None, ws):
+            with pytest.raises(ValueError, match="31 bits"):
+                cache.attend(q, seqs, bt, 1.0, max_q, max_kv, workspace=workspace)

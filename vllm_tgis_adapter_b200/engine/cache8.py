@@ -131,6 +131,8 @@ class Cache8:
 
     def workspace_bytes(self, T: int, n_seqs: int, n_q: int, max_q: int, max_kv: int) -> int:
         """What `attend` needs for these bounds (no fewer for more sequences, more queries of one or longer ones; 43 MB at most)."""
+        if max_q >> 31 or max_kv >> 31:   # (a longer number would be cut to 32 bits on its way)
+            raise ValueError(f"max_q {max_q}, max_kv {max_kv}: numbers of 31 bits are wanted")
         n = self._workspace(T, n_seqs, n_q, self.n_kv, max_q, max_kv)
         if n < 0:
             raise ValueError(self._error())
@@ -164,6 +166,8 @@ class Cache8:
             if tree.dtype not in (torch.int64, torch.uint64) or tree.dim() != 1 or tree.shape[0] != T or tree.device != device or not tree.is_contiguous():
                 raise ValueError(f"tree: {T} contiguous 64-bit words on {device} are wanted")
             words = tree.data_ptr()
+        if max_q >> 31 or max_kv >> 31:
+            raise ValueError(f"max_q {max_q}, max_kv {max_kv}: numbers of 31 bits are wanted")
         n_seqs, room, space = seqs.shape[0], 0, None
         if workspace is None:
             room = self.workspace_bytes(T, n_seqs, n_q, max_q, max_kv)
