@@ -113,7 +113,8 @@ typedef struct tgis_engine tgis_engine;
 #define TGIS_ARCH_LUDELIX 7
 
 /* What the Llama family's keys and values are stored as.  E4M3: 8-bit rows with an fp32 scale each (include/tgis_kv8.h), about half the
- * bytes of a token; queries, softmax and sums are as exact as over the cache in the model's type. */
+ * bytes of a token.  Sums and softmax are in fp32; a probability is one number of 11 bits where the 16-bit cache's kernels hold two of 8, and a prompt's keys
+ * and values are rounded to 11 bits once more: the results' own rounding (bf16, 8 bits) covers either but for a few percent of it. */
 #define TGIS_KV_MODEL 0
 #define TGIS_KV_E4M3 1
 

@@ -16,9 +16,9 @@
 // a sequence of several splits leaves them in the workspace to attn8_merge_kernel.  Sequence lengths and pages are read on the device,
 // so the list of items is made by every CTA for itself: a prefix sum over the sequences.
 //
-// What bounds it: reading the pages where they are many (64 tokens behind 8000: 194 us, 5.6 TB/s, 85% of a copy's rate); below that the
-// chain of a block in a warp (copy, scores, softmax, output: about 0.5 us) and the launch: one token behind 16: 4.6 us, behind 511: 7.5,
-// behind 8191: 11.6 (32 splits and their join); 32 behind 511 to 639: 12.3.
+// What bounds it: reading the pages where they are many (64 tokens behind 8000: 201 us, 5.4 TB/s, 82% of a copy's rate); below that the
+// chain of a block in a warp (copy, scores, softmax, output: about 0.5 us) and the launch: one token behind 16: 4.7 us, behind 511: 7.6,
+// behind 8191: 11.9 (32 splits and their join); 32 behind 511 to 639: 12.5.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -37,9 +37,9 @@ constexpr int R8_WARPS = 4, R8_THREADS = R8_WARPS * 32, R8_RING = 2;
 constexpr int R8_CTAS(int rows) { return rows == 8 ? 3 : 2; }   // per SM
 // Rows of a sequence (its queries times heads of a group) up to which this kernel reads its pages once for each 16 of them, instead of one
 // unit of attention8_prompt.cu; and keys up to which it takes more rows, where all run at once.  Microseconds here and there, 32 / 8 heads:
-// 8 queries behind 500: 10.2 and 15.8; 32 x 8 behind 1000: 35 and 57; 32 x 12: 51 and 58; 32 x 16: 67 and 59; a prompt of 64: 7.4 and 11.1, of
-// 128: 8.0 and 12.3; 64 behind 500: 12.6 and 19.2, 128: 13.1 and 21.0; 96 behind 2000: 28 and 24; four prompts of 32 (all at once): 8.0 and
-// 9.2, of 48 (not): 13.3 and 11.4.
+// 8 queries behind 500: 10.4 and 15.8; 32 x 8 behind 1000: 35 and 59; 32 x 12: 52 and 60; 32 x 16: 69 and 60; a prompt of 64: 7.5 and 11.2, of
+// 128: 8.1 and 12.4; 64 behind 500: 12.7 and 19.3, 128: 13.5 and 21.3; 96 behind 2000: 29 and 24; four prompts of 32 (all at once): 8.2 and
+// 9.3, of 48 (not): 13.6 and 11.5.
 constexpr int R8_MOST_ROWS = 48, R8_MORE_KEYS = 1024;
 constexpr int R8_ONE_SPLIT = 768;                  // keys of a sequence that are not split
 constexpr float R8_SLACK = 8.f;                    // exp2 domain: how far a score may exceed its row's reference
@@ -572,9 +572,9 @@ RowsPlan rows_plan(int T, int n_seqs, int n_q, int n_kv, int max_q, int max_kv) 
   p.prompt = p.wide && attn8_prompt_takes(T, n_seqs, n_q, n_kv, max_q, max_kv);
   // Splits (the bounds are those of the longest sequence): one for few tokens, which the second launch costs more than it saves; else as
   // many as run at once, of 256 to 4096 tokens; else one for 2048 tokens or three rounds of them, of 1024 to 2048.  Microseconds, 32 / 8 heads,
-  // one single token behind 600: one split 8.4, of 256 tokens 8.5; 1024: 10.8 and 8.6; 12 behind 2048: four (all at once) 14.2, six 19.9,
-  // two 18.9; 12 behind 8192: four 41.9, eight 42.7, sixteen 50.0; 32 behind 4096: one 50.3, two 68.5, four 62.8; 64 behind 4096 (more than
-  // run at once): one 112, of 1024 tokens 106, of 256 147; 64 behind 2048: one 61, two 66.
+  // one single token behind 600: one split 8.5, of 256 tokens 8.3; 1024: 11.1 and 9.1; 12 behind 2048: four (all at once) 15.1, eight 18.2, one
+  // 21.6; 12 behind 8192: four 43.4, eight 43.7, sixteen 51.4; 32 behind 4096: one 51.3, two 65.4, four 64.7; 64 behind 4096 (more than
+  // run at once): one 115, three rounds of them 117, of 1024 tokens 123, of 2048 108, of 256 151; 64 behind 2048: one 63, two 65.
   auto length = [&](double n) { return (int)std::ceil(max_kv / std::max(n, 1.) / 128.) * 128; };
   const int at_once = std::max(length(std::floor(slots / items)), 256);
   p.split = max_kv <= R8_ONE_SPLIT ? R8_ONE_SPLIT : items <= slots && at_once <= 4096 ? at_once : max_kv <= 2048 ? 2048 : std::min(std::max(length(std::ceil(3. * slots / items)), 1024), 2048);

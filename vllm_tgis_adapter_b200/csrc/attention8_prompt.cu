@@ -16,17 +16,19 @@
 // a row has one reference of its exponentials and one of its weights, which move only when something passes them by 2^8, so that it
 // fits f16 (2^15 at most) and nothing above 2^-31 of the row's largest is lost.  A tile whose scales lie further apart than 2^12 has no unit
 // that serves a row which sees its small ones alone: its codes stay as they are, exact, and the softmax multiplies scores and probabilities by
-// the scales, in fp32 and in steps.  So what a row does not see, or gives no weight, never costs it its own tokens' bits.  (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the
-// products cost the same and every score takes a multiplication by its key's scale, every probability one by its value's: as first
-// built both took 380 us for 1859 tokens behind 6144, 32 / 8 heads, and each later step, to 263, needed the multiplications gone.)
+// the scales, in fp32 and in steps.  So what a row does not see, or gives no weight, never costs it its own tokens' bits.
+// (With K as the cache holds it and queries as two e4m3 numbers on kind::f8f6f4 the products cost the same and every score takes a
+// multiplication by its key's scale, every probability one by its value's: as first built both took 380 us for 1859 tokens behind 6144, 32 / 8
+// heads, and each later step, to 263, needed the multiplications gone.)
 // Two threads share a row, half of a step's columns each; tokens of a page lie in V's columns as cache8.cuh says, so P's columns are
 // written in that order.  A row with a NaN for its scale gets zeros here and a bit; who sees it gets NaN for its sum.
 //
 // What bounds it: the chain of a step.  Of its 4900 clocks an accumulator spends 3100 in the softmax (scores read 600, the two threads'
 // maximum 300, exponentials 2000, 1024 of them the least that 16 a clock take) and 1700 in its two products, which wait for those of
-// the other one; the two take turns.  Without the exponentials a step is 4500, without the widening 4550: nothing alone is the bound.
+// the other one; the two take turns.  Without the exponentials a step is 4500, without the widening 4550: nothing alone is the bound.  (References of
+// weights, which came after that, are 150 more.)
 // 1859 tokens behind 6144: 274 us, 788 TFLOP/s of the 1660 that a product of matrices reaches (the 16-bit cache's kernel: 345 us);
-// prompt of 2048: 76; six prompts of 90 to 593 (1679 tokens): 39; 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 82.
+// prompt of 2048: 76 (61); six prompts of 90 to 593 (1679 tokens): 39 (2048 tokens in six: 30); 4 drafts of 64 behind 4000 to 8000, 64 / 8 heads: 82.
 // A unit's beginning and end take as much as three and a half steps (Q copied and turned, the first pages, O): what short prompts consist of.
 //
 // No wait is unbounded: after about two seconds a role gives up, the call's status says so; copies and MMAs in flight land first and TMEM is
@@ -53,8 +55,8 @@ constexpr float P8_LEAST = -118.f;                          // exp2 domain: smal
 constexpr float P8_V_TOP = 64.f, P8_K_TOP = 16.f;           // largest scale that a code (448 at most) is multiplied by
 constexpr int P8_V_TOP_LOG = 6;
 // A tile's scales lie within this of its largest (the power of two above it), or its codes stay without them: what is held relative to
-// one unit would lose the small rows' bits, and a row may see those alone.  (Scales of a layer's rows differ by 2^2 to 2^5, those of a prompt's first
-// token by up to 2^8.  The smallest scale of all, that of rows of zeros, does not count.)
+// one unit would lose the small rows' bits, and a row may see those alone.  At 2^-12 of it a key's scale as two f16 numbers is off by 2^-17 (their last
+// step is 2^-24 of 16), a value's by 2^-11 like any other.  (The smallest scale of all, that of rows of zeros, does not count.)
 constexpr float P8_BAND = 0x1p-12f;
 // What the beginning and the end of a unit count for, in steps.  As 1, 2, 3: 2048 tokens 85, 75, 72 us; six prompts of 90 to 593 38.8, 38.6, 40.4;
 // 16 drafts of 5 to 24 behind 200 to 1500 36, 33.5, 35
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       if (lane == 0) mbar_arrive(&sm.q_full[g]);
       float m = 0.f, l = 0.f, unit = 0.f;                       // unit: log2 of what O is in units of, 2^m apart
       float most_unit = 0.f;                                    // no row's is larger
-      bool large = false;                                       // some row's reference is
+      bool large = false;                                       // some row's m is far from 0
       const int tile0 = t.tile0, tile1 = t.tile1;
       for (int j = tile0; j < tile1; ++j) {
         const int nb = t.blocks(j) - 2 * h;                 // of this thread's half
@@ -815,8 +817,8 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
           float most = p8_most(s_t, nb, vis[0], vis[1], wide ? qm : qk, k_scales(), ref, v_scales(), v_log);
           most = fmaxf(most, pair_up(most));
           if (!ok) break;
-          // exponent of the power of two at or above it
-          float to = fmaxf((float)((int)(__float_as_uint(power_above(__float_as_uint(most))) >> 23) - 127), P8_LEAST);
+          // exponent of the power of two at or above it; 2^127 has room for the largest
+          float to = fminf(fmaxf((float)((int)(__float_as_uint(power_above(__float_as_uint(most))) >> 23) - 127), P8_LEAST), 127.f);
           if (j != tile0) {
             to = fmaxf(to, unit);
             f *= ex2(unit - to);

@@ -3449,7 +3449,8 @@ struct tgis_engine {
   }
 
   // Rotary embedding, storing and attention of a layer over the 8-bit cache: single tokens, then prompts and their portions.  Bounds are
-  // those of the step's graph (single tokens) or of the engine: they choose launches, not results that depend on the batch's lengths.
+  // those of the step's graph (single tokens) or of the engine.  Sums are split by what else is in the step (attention8.cu by the number of sequences and
+  // their longest, attention8_prompt.cu by all steps of the call), so a row's last bits depend on its neighbours, as they do not over the 16-bit cache.
   void kv8_attend(int li, int T, int S, int n_dec, int n_tiles, int max_dec_kv) {
     uint8_t* pages = kv8_pages.p + (size_t)li * kv8_layer_bytes;
     CK(kv8_write_launch(pages, num_blocks, nkv, qkv.p, qkv_dim, T, nq, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, cfg.max_model_len, qkv.p,
