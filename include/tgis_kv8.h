@@ -6,6 +6,7 @@
  * with 1 / 448, the product and the quotient rounded to fp32.
  * A row that holds a NaN or an infinity is stored with a NaN for its scale and zeros for codes: whoever sees it gets NaN, whoever does
  * not gets what it would have got without it.  Finite rows of any size cost those that do not see them, or give them no weight, nothing either.
+ * Numbers of a query count to 2^-39 of its row's largest.
  *
  * Memory of one layer: `pages` [n_pages][n_kv][TGIS_KV8_PAGE_BYTES], 16-byte aligned, 32 tokens a page; slot = page * 32 + place.  It is
  * filled with zeros before the first use and written by tgis_kv8_write (or copied from another such cache) alone: that keeps

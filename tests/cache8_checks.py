@@ -9,8 +9,12 @@
              largest weight: half of f16's smallest step is 2^-25, so each is off by 2^-31 of that, times |c|.
   "prompt"   (csrc/attention8_prompt.cu): 2^-9 of sum p |v| (a probability, a value's scale and their code's product in f16, 2^-11
              each, and fp32).  A key's number is off by 2^-11 of itself (2^-16 of it for the two f16 numbers of its scale and the
-             fp32 sum) and by half of f16's smallest step of the tile's unit, 2^-25 * 2^13 / 16 = 2^-16 of its scale.  Values: 2^-25 * 2^13 / 64 =
+             fp32 sum) and (but for zeros) by half of f16's smallest step of the tile's unit, 2^-25 * 2^13 / 16 = 2^-16 of its scale.  Values: 2^-25 * 2^13 / 64 =
              2^-18 of the scale; probabilities: 2^-31 of what the row's largest one stands for, whose unit may be 2^12 above its own scale.
+
+A query's number is held in f16 where the largest of its row is 2^14 at least.  It is exact there from 2^-17 on (bf16 has 8 bits, f16's smallest step is
+2^-24), which 2^-31 of the largest is; a smaller one is off by half a step, 2^-25, which is 2^-39 of the largest.  A score is off by that times |scale| sum |k|
+over such numbers, in both.
 
 A score off by d changes a weight by exp(d) and the sum that all is divided by as well: two tokens' d together, those of the two largest among tokens
 whose p is not below 2^-40 (a lone one's does not matter, and one far below them stays there).
@@ -131,8 +135,10 @@ def check(cache, q, seqs, bt, scale, kernel, words=None, got=None, only=None):
             if kernel == "rows":
                 d, plain, floor = 2.0 ** -19 * most, 2.0 ** -10, 2.0 ** -31 * low
             else:
-                d = (2.0 ** -11 + 2.0 ** -16) * most + 2.0 ** -16 * abs(scale) * qq.abs().sum(-1, keepdim=True) * s[..., 0].t()[:, None]
+                d = (2.0 ** -11 + 2.0 ** -16) * most + 2.0 ** -16 * abs(scale) * torch.einsum("hgd,khd->hgk", qq.abs(), (c != 0).double()) * s[..., 0].t()[:, None]
                 plain, floor = 2.0 ** -9, 2.0 ** -19 * low + 2.0 ** -18 * weight.sum(-1, keepdim=True)
+            top = qq.abs().amax(-1, keepdim=True)
+            d = d + 2.0 ** -39 * abs(scale) * top * torch.einsum("hgd,khd->hgk", (qq.abs() < 2.0 ** -31 * top).double(), k.abs())
             d = torch.where(p > 2.0 ** -40, d, 0.0)
             two = d.topk(min(2, d.shape[-1]), dim=-1).values.sum(-1, keepdim=True)
             two = torch.where((p > 2.0 ** -40).sum(-1, keepdim=True) > 1, two, 0.0)

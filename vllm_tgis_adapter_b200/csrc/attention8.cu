@@ -6,7 +6,7 @@
 // Both products are mma.sync f16 x f16 -> fp32, K and V widened in registers (exact) as their fragments leave shared memory; mma.sync on
 // e4m3 itself, with queries and probabilities as two e4m3 numbers each, costs the same tensor work and fifteen instructions each
 // (64 tokens behind 8000, 32 / 8 heads: 211 us, against 194).  A query row (bf16) times the power of two that brings its largest number to
-// [128, 256) is exact in f16 but for numbers 2^-22 of the largest and below.  Scores are multiplied by their key's scale in fp32; a row's
+// [2^14, 2^15) is exact in f16 but for numbers 2^-31 of the largest and below (off by 2^-39 of it).  Scores are multiplied by their key's scale in fp32; a row's
 // weight, probability times value's scale, is one f16 number of 11 bits, held times 2^7 / r.  The reference m of a row's exponentials moves
 // only when a score passes it by 2^8, and r, a power of two and the row's own, only when a weight passes it by 2^8: it fits f16 (2^15 at
 // most), and nothing above 2^-31 of the row's largest weight is lost, whatever tokens hold that it does not see or gives no weight.
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e that brings the largest number to [128, 256); a row that is not finite: NaN, which its scores and sums then are
+      // 2^e that brings the largest number to [2^14, 2^15); a row that is not finite: NaN, which its scores and sums then are
       const float up = power_up(top), mul = top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : a.scale * 1.4426950408889634f * one_over(up);
 #pragma unroll
       for (int c = 0; c < HEAD_DIM / 16; ++c) {

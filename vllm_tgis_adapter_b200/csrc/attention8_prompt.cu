@@ -12,7 +12,7 @@
 // Both products are f16 x f16 -> fp32 (kind::f16).  Four warps widen K and V as they multiply them by their rows' scales (a code has 4 bits,
 // so a product rounded to f16's 11 is off by 2^-11; a key's scale is applied as two f16 numbers, for an error of the whole row's
 // would be one of its score); both are held relative to a power of two at or above the tile's scales.  A query row is exact in f16 but for
-// numbers 2^-22 of its largest and below.  A weight (a probability times the tile's unit of V) is one f16 number of 11 bits, held times 2^7;
+// numbers 2^-31 of its largest and below.  A weight (a probability times the tile's unit of V) is one f16 number of 11 bits, held times 2^7;
 // a row has one reference of its exponentials and one of its weights, which move only when something passes them by 2^8, so that it
 // fits f16 (2^15 at most) and nothing above 2^-31 of the row's largest is lost.  A tile whose scales lie further apart than 2^12 has no unit
 // that serves a row which sees its small ones alone: its codes stay as they are, exact, and the softmax multiplies scores and probabilities by
@@ -247,7 +247,7 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t x, uint32_t y, ui
 }
 
 // ---- a thread's scores in steps, 16 at a time, for tiles that need it.  Calls: in line they took 8 % of all other tiles' time, called 3 %
-// (a unit that is no normal number would make scores of nothing 0 * -inf where they are hidden, or 0 * inf: NaN; scores of 2^24 units at most are
+// (a unit that is no normal number would make scores of nothing 0 * -inf where they are hidden, or 0 * inf: NaN; scores of 2^35 units at most are
 // nothing beside 2^-126 of them.  A NaN fails both comparisons and stays)
 __device__ __forceinline__ float p8_normal(float x) { return x < 0x1p-126f ? 0x1p-126f : x > 0x1.fffffep127f ? 0x1.fffffep127f : x; }
 // scores 16 c .. 16 c + 15, -inf where hidden; ks: scales of their keys, NULL: `times` has them
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1) attn8_prompt_kernel(const __gri
       unsigned long long word = 0;
       if (!mine) lim = 0x7fffffff;
       else if (a.tree != nullptr) lim = t.before - 1, word = a.tree[t.row0 + in_unit] & ((unsigned long long)t.word_mask_hi << 32 | t.word_mask_lo);
-      // ---- Q, every row's largest number at 128 to 256.  The half rows of this warp come as they are to the place of its part of the operand
+      // ---- Q, every row's largest number at 2^14 to 2^15.  The half rows of this warp come as they are to the place of its part of the operand
       // (eight lanes copy 128 bytes of one); then a thread turns its own into f16 there.  (Loops, for code that runs once a unit is
       // fetched as it runs: unrolled this took six thousand clocks.)
       const int sub = lane >> 3, at = lane & 7;

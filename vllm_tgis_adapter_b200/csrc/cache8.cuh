@@ -44,10 +44,10 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return f;
 }
 
-// 2^e that brings a magnitude (the bits of a number >= 0) to [128, 256); no more than 2^126
+// 2^e that brings a magnitude (the bits of a number >= 0) to [2^14, 2^15), the most that f16 has room for; no more than 2^126
 __device__ __forceinline__ float power_up(uint32_t bits) {
-  const int ex = min(max((int)(bits >> 23), 8), 254);
-  return __uint_as_float((uint32_t)(261 - ex) << 23);   // 2^(134 - ex)
+  const int ex = min(max((int)(bits >> 23), 15), 254);
+  return __uint_as_float((uint32_t)(268 - ex) << 23);   // 2^(141 - ex)
 }
 // of a power of two from 2^-126 to 2^126
 __device__ __forceinline__ float one_over(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
