@@ -13,7 +13,7 @@
              2^-18 of the scale; probabilities: 2^-31 of what the row's largest one stands for, whose unit may be 2^12 above its own scale.
 
 A query's number is held in f16 where the largest of its row is 2^14 at least.  It is exact there from 2^-17 on (bf16 has 8 bits, f16's smallest step is
-2^-24), which 2^-31 of the largest is; a smaller one is off by half a step, 2^-25, which is 2^-39 of the largest.  A score is off by that times |scale| sum |k|
+2^-24), which 2^-31 of the largest is; a smaller one, if it is not zero, is off by half a step, 2^-25, which is 2^-39 of the largest.  A score is off by that times |scale| sum |k|
 over such numbers, in both.
 
 A score off by d changes a weight by exp(d) and the sum that all is divided by as well: two tokens' d together, those of the two largest among tokens
@@ -138,7 +138,7 @@ def check(cache, q, seqs, bt, scale, kernel, words=None, got=None, only=None):
                 d = (2.0 ** -11 + 2.0 ** -16) * most + 2.0 ** -16 * abs(scale) * torch.einsum("hgd,khd->hgk", qq.abs(), (c != 0).double()) * s[..., 0].t()[:, None]
                 plain, floor = 2.0 ** -9, 2.0 ** -19 * low + 2.0 ** -18 * weight.sum(-1, keepdim=True)
             top = qq.abs().amax(-1, keepdim=True)
-            d = d + 2.0 ** -39 * abs(scale) * top * torch.einsum("hgd,khd->hgk", (qq.abs() < 2.0 ** -31 * top).double(), k.abs())
+            d = d + 2.0 ** -39 * abs(scale) * top * torch.einsum("hgd,khd->hgk", ((qq.abs() < 2.0 ** -31 * top) & (qq != 0)).double(), k.abs())
             d = torch.where(p > 2.0 ** -40, d, 0.0)
             two = d.topk(min(2, d.shape[-1]), dim=-1).values.sum(-1, keepdim=True)
             two = torch.where((p > 2.0 ** -40).sum(-1, keepdim=True) > 1, two, 0.0)

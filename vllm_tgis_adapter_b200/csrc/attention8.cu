@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(R8_THREADS, R8_CTAS(ROWS)) attn8_rows_kernel(c
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) s[n][i >> 1][2 * (i & 1) + e] *= ks * q_mul[n][e];
+            for (int e = 0; e < 2; ++e) s[n][i >> 1][2 * (i & 1) + e] *= min_nan(ks * q_mul[n][e], 0x1.fffffep127f);   // (0 * inf: a zero is one)
         }
         if (open) {
 #pragma unroll

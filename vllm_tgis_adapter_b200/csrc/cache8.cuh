@@ -63,6 +63,12 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
+// the smaller number, NaN where one is
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
 // cudaFuncSetAttribute once a device
 struct OncePerDevice {
   static constexpr int MAX = 64;
