@@ -23,45 +23,6 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&x)[8]) {
   x[0] = lo_f(v.x); x[1] = hi_f(v.x); x[2] = lo_f(v.y); x[3] = hi_f(v.y); x[4] = lo_f(v.z); x[5] = hi_f(v.z); x[6] = lo_f(v.w); x[7] = hi_f(v.w);
 }
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) { return make_uint4(pack_bf(x[0], x[1]), pack_bf(x[2], x[3]), pack_bf(x[4], x[5]), pack_bf(x[6], x[7])); }
-// magnitudes as whole numbers order as their values do, with infinities and NaN above all
-__device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  return m;
-}
-// Scale of a row whose largest magnitude has these bits: NaN where the row holds a number that is not finite
-__device__ __forceinline__ float scale_of(uint32_t m) {
-  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(m) * (1.f / KV8_TOP), KV8_TINY);
-}
-// Codes of x / s; zeros where the scale is NaN.  An IEEE division is a call of some forty instructions, so the quotients are products with
-// the scale's reciprocal, which are within 2 ulp of them, and are divided again only where that could change a code: within 3 ulp of the
-// middle of two e4m3 numbers (one in 200,000), or below 2^-6, where the middles lie elsewhere.
-template <int N>
-__device__ __forceinline__ void codes(const float (&x)[N], float s, uint32_t (&out)[N / 4]) {
-  const bool fine = s < INFINITY;
-  const float by = fine ? __frcp_rn(s) : 0.f;
-  float q[N];
-  bool close = false;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = fine ? x[i] * by : 0.f;
-    const int off = (int)(__float_as_uint(q[i]) & 0xfffffu) - 0x80000;
-    close |= (off >= -3 && off <= 3) || (fabsf(q[i]) < 0.015625f && q[i] != 0.f);
-  }
-  if (close) {
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {   // (one division in the code)
-      float xi = x[0];
-#pragma unroll
-      for (int j = 1; j < N; ++j) xi = i == j ? x[j] : xi;
-      const float d = __fdiv_rn(xi, s);
-#pragma unroll
-      for (int j = 0; j < N; ++j) q[j] = i == j ? d : q[j];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < N / 4; ++i) out[i] = e4m3x2(q[4 * i], q[4 * i + 1]) | e4m3x2(q[4 * i + 2], q[4 * i + 3]) << 16;
-}
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float s) {
   uint32_t c[2];
   codes(x, s, c);

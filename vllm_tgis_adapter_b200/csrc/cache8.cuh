@@ -44,6 +44,46 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return f;
 }
 
+// magnitudes as whole numbers order as their values do, with infinities and NaN above all
+__device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  return m;
+}
+// Scale of a row (or another group that is quantised together) whose largest magnitude has these bits: NaN where it holds a number that is not finite
+__device__ __forceinline__ float scale_of(uint32_t m) {
+  return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(m) * (1.f / KV8_TOP), KV8_TINY);
+}
+// Codes of x / s; zeros where the scale is NaN.  An IEEE division is a call of some forty instructions, so the quotients are products with
+// the scale's reciprocal, which are within 2 ulp of them, and are divided again only where that could change a code: within 3 ulp of the
+// middle of two e4m3 numbers (one in 200,000), or below 2^-6, where the middles lie elsewhere.
+template <int N>
+__device__ __forceinline__ void codes(const float (&x)[N], float s, uint32_t (&out)[N / 4]) {
+  const bool fine = s < INFINITY;
+  const float by = fine ? __frcp_rn(s) : 0.f;
+  float q[N];
+  bool close = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    q[i] = fine ? x[i] * by : 0.f;
+    const int off = (int)(__float_as_uint(q[i]) & 0xfffffu) - 0x80000;
+    close |= (off >= -3 && off <= 3) || (fabsf(q[i]) < 0.015625f && q[i] != 0.f);
+  }
+  if (close) {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {   // (one division in the code)
+      float xi = x[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) xi = i == j ? x[j] : xi;
+      const float d = __fdiv_rn(xi, s);
+#pragma unroll
+      for (int j = 0; j < N; ++j) q[j] = i == j ? d : q[j];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i) out[i] = e4m3x2(q[4 * i], q[4 * i + 1]) | e4m3x2(q[4 * i + 2], q[4 * i + 3]) << 16;
+}
+
 // 2^e that brings a magnitude (the bits of a number >= 0) to [2^14, 2^15), the most that f16 has room for; no more than 2^126
 __device__ __forceinline__ float power_up(uint32_t bits) {
   const int ex = min(max((int)(bits >> 23), 15), 254);

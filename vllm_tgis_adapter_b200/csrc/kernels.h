@@ -12,6 +12,8 @@ namespace tgis {
 // ---- gemm_tcgen05.cu --------------------------------------------------------------------------------------------
 int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld_elems,
                       uint32_t box_rows, uint32_t box_cols);
+// rows of bytes (ld a multiple of 16), 128-byte swizzle
+int make_tmap_u8_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols);
 int make_tmap_bf16_3d(CUtensorMap* out, const void* base, const uint64_t (&dims)[3], const uint64_t (&stride_bytes)[2],
                       const uint32_t (&box)[3], bool swizzle128);
 int gemm_pick_bt(int T);

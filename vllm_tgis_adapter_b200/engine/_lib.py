@@ -159,6 +159,18 @@ KERNEL_SYMBOLS = [
 # ... and include/tgis_kv8.h
 KV8_SYMBOLS = ["tgis_kv8_write", "tgis_kv8_read", "tgis_kv8_attention_workspace", "tgis_kv8_attention", "tgis_kv8_last_error"]
 
+# ... and include/tgis_w8.h
+W8_SYMBOLS = ["tgis_w8_quantise_rows", "tgis_w8_quantise_weight", "tgis_w8_product", "tgis_w8_gated", "tgis_w8_feed_forward", "tgis_w8_last_error"]
+
+
+class TgisW8Matrix(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("ld", C.c_int64), ("n", C.c_int32), ("k", C.c_int32)]
+
+
+class TgisW8Rows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("ld", C.c_int64), ("lds", C.c_int64), ("t", C.c_int32), ("k", C.c_int32)]
+
+
 _LIB: C.CDLL | None = None
 
 
@@ -272,6 +284,12 @@ def load_library() -> C.CDLL:
     lib.tgis_kv8_attention_workspace.restype = i64
     lib.tgis_kv8_attention_workspace.argtypes = [i32] * 6
     lib.tgis_kv8_attention.argtypes = [vp, i32, i32, vp, i64, i32, i32, vp, i32, vp, i32, i32, vp, f32, i32, i32, vp, i64, vp, i64, vp, vp]
+    lib.tgis_w8_last_error.restype = C.c_char_p
+    lib.tgis_w8_quantise_rows.argtypes = [vp, i32, i64, vp, f32, vp, i64, vp, i64, vp, vp]   # (records by address)
+    lib.tgis_w8_quantise_weight.argtypes = [vp, i32, i64, vp, vp]
+    lib.tgis_w8_product.argtypes = [vp, vp, vp, i32, i64, vp, vp]
+    lib.tgis_w8_gated.argtypes = [vp, vp, vp, vp, vp, vp]
+    lib.tgis_w8_feed_forward.argtypes = [vp, vp, vp, vp, vp, vp, i32, i64, vp, vp]
     _LIB = lib
     return lib
 

@@ -1,0 +1,239 @@
+"""Products with 8-bit weights (csrc/rows8.cu, csrc/gemm8.cu; C ABI: include/tgis_w8.h).
+
+    layer = Linear8.from_weight(w)                    # w [n, k]: every block of 128 x 128 as e4m3 codes with one fp32 scale
+    rows = quantise(x)                                # x [T, k]: every 128 neighbours of a row as e4m3 codes with one fp32 scale
+    rows = quantise(x, norm=w_norm, residual=res)     # ... of the RMS norm of x + residual, which is updated
+    y = layer(rows)                                   # [T, n]
+    y = FeedForward8(gate, up, down)(rows)            # silu(gate x) * (up x) in 8-bit rows, then the down projection
+
+`Linear8(codes, scales)` takes a checkpoint's block-scaled matrix as it is.  Calls go to the current stream of their tensors' device and return
+after the launch; they may be captured into CUDA graphs and, having no workspace, run at the same time.  Arguments that the host
+can check raise ValueError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import TgisW8Matrix, TgisW8Rows
+
+GROUP, MAX_K, MAX_ROWS = 128, 131072, 1 << 22
+TYPES = {torch.bfloat16: 0, torch.float32: 1}
+_functions = None
+
+
+class _Functions:
+    def __init__(self):
+        lib = _lib.load_library()
+        self.rows, self.weight, self.product, self.gated, self.feed_forward = (
+            lib.tgis_w8_quantise_rows, lib.tgis_w8_quantise_weight, lib.tgis_w8_product, lib.tgis_w8_gated, lib.tgis_w8_feed_forward)
+        self.error = lib.tgis_w8_last_error
+
+
+def _load() -> _Functions:
+    global _functions
+    if _functions is None:
+        _functions = _Functions()
+    return _functions
+
+
+def _run(function, device: torch.device, *args) -> None:
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        raise ValueError((_load().error() or b"").decode(errors="replace"))
+
+
+def _pitch(name: str, x: torch.Tensor, device: torch.device | None = None) -> int:
+    """Row pitch of a 2-D bf16 or fp32 CUDA tensor with contiguous rows."""
+    if x.dtype not in TYPES or x.dim() != 2 or not x.is_cuda or (device is not None and x.device != device):
+        raise ValueError(f"{name}: a bf16 or fp32 tensor [rows, numbers] on {device or 'a CUDA device'} is wanted")
+    rows, width = x.shape
+    pitch, step = x.stride()
+    if step != 1 and width > 1:
+        raise ValueError(f"{name}: contiguous rows are wanted")
+    return pitch if rows > 1 else width
+
+
+class Rows8:
+    """T rows of k numbers in 8 bits: `codes` e4m3 [T, k], `scales` fp32 [groups, T]; views of tensors whose rows are as long as whole groups are."""
+
+    __slots__ = ("codes", "scales", "device", "record", "at")
+
+    def __init__(self, T: int, k: int, device: torch.device):
+        groups = -(-k // GROUP)
+        codes = torch.empty((T, groups * GROUP), dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty((groups, T), dtype=torch.float32, device=device)
+        self.device = codes.device
+        self.record = TgisW8Rows(codes.data_ptr(), scales.data_ptr(), groups * GROUP, T, T, k)
+        self.at = C.addressof(self.record)
+        self.codes, self.scales = codes if k == groups * GROUP else codes[:, :k], scales
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.record.t, self.record.k
+
+    def values(self) -> torch.Tensor:
+        """What the rows stand for, fp32 [T, k]."""
+        return self.codes.float() * self.scales.t().repeat_interleave(GROUP, dim=1)[:, : self.codes.shape[1]]
+
+
+def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-5, residual: torch.Tensor | None = None,
+             residual_out: torch.Tensor | None = None, out: Rows8 | None = None) -> Rows8:
+    """Rows of x [T, k] (bf16 or fp32) in 8 bits.  `residual` (like x): x + residual, rounded to their type, takes the place of x and is stored in
+    `residual_out` (None: residual itself).  `norm` (bf16 [k]): the RMS norm's weight, v = r * norm / sqrt(mean r^2 + eps)."""
+    ld = _pitch("x", x)
+    device, (T, k) = x.device, x.shape
+    if k < 1 or k > MAX_K or T > MAX_ROWS:
+        raise ValueError(f"x: at most {MAX_ROWS} rows of 1 to {MAX_K} numbers are wanted, not {T} of {k}")
+    norm_at = res_at = to_at = None
+    ldr = ldt = 0
+    if norm is not None:
+        if norm.dtype != torch.bfloat16 or norm.dim() != 1 or norm.shape[0] != k or norm.device != device or not norm.is_contiguous():
+            raise ValueError(f"norm: {k} contiguous bf16 numbers on {device} are wanted")
+        norm_at = norm.data_ptr()
+    if residual is not None:
+        ldr = _pitch("residual", residual, device)
+        if residual_out is None:
+            residual_out, ldt = residual, ldr
+        else:
+            ldt = _pitch("residual_out", residual_out, device)
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual_out.shape != x.shape or residual_out.dtype != x.dtype:
+            raise ValueError(f"residual, residual_out: {x.dtype} tensors [{T}, {k}] are wanted")
+        res_at, to_at = residual.data_ptr(), residual_out.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out: there is no residual")
+    if out is None:
+        out = Rows8(T, k, device)
+    elif out.shape != (T, k) or out.device != device:
+        raise ValueError(f"out: {T} rows of {k} numbers on {device} are wanted")
+    if T or norm is not None:
+        _run(_load().rows, device, x.data_ptr(), TYPES[x.dtype], ld, norm_at, eps, res_at, ldr, to_at, ldt, out.at)
+    return out
+
+
+class Linear8:
+    """A weight matrix in 8 bits: `codes` e4m3 [n, k], `scales` fp32 [blocks of 128 rows, groups of 128].  Codes whose rows do not start on
+    16 bytes are copied once."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype != torch.float8_e4m3fn or codes.dim() != 2 or not codes.is_cuda or codes.numel() == 0:
+            raise ValueError("codes: a torch.float8_e4m3fn CUDA tensor [n, k] is wanted")
+        n, k = codes.shape
+        blocks = (-(-n // GROUP), -(-k // GROUP))
+        if k > MAX_K or n > MAX_ROWS:
+            raise ValueError(f"codes: at most {MAX_ROWS} rows of {MAX_K} numbers are wanted, not {n} of {k}")
+        if scales.dtype != torch.float32 or tuple(scales.shape) != blocks or scales.device != codes.device or not scales.is_contiguous():
+            raise ValueError(f"scales: a contiguous fp32 tensor {list(blocks)} on {codes.device} is wanted")
+        pitch, step = codes.stride()
+        if n == 1:
+            pitch = -(-k // 16) * 16
+        if (step != 1 and k > 1) or pitch < k or pitch % 16 or codes.data_ptr() % 16:
+            rows = torch.zeros((n, blocks[1] * GROUP), dtype=torch.uint8, device=codes.device)
+            rows[:, :k] = codes.view(torch.uint8)
+            codes, pitch = rows.view(torch.float8_e4m3fn)[:, :k], blocks[1] * GROUP
+        self.codes, self.scales, self.device, self.n, self.k = codes, scales, codes.device, n, k
+        self.record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), pitch, n, k)
+        self.at = C.addressof(self.record)
+        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status_at, self._product = self.status.data_ptr(), _load().product
+
+    @classmethod
+    def from_weight(cls, w: torch.Tensor) -> "Linear8":
+        """w [n, k] (bf16 or fp32) in 8 bits."""
+        ld = _pitch("w", w)
+        n, k = w.shape
+        if w.numel() == 0 or k > MAX_K or n > MAX_ROWS:
+            raise ValueError(f"w: 1 to {MAX_ROWS} rows of 1 to {MAX_K} numbers are wanted, not {n} of {k}")
+        groups = -(-k // GROUP)
+        codes = torch.empty((n, groups * GROUP), dtype=torch.float8_e4m3fn, device=w.device)
+        scales = torch.empty((-(-n // GROUP), groups), dtype=torch.float32, device=w.device)
+        record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), groups * GROUP, n, k)
+        _run(_load().weight, w.device, w.data_ptr(), TYPES[w.dtype], ld, C.addressof(record))
+        return cls(codes if k == groups * GROUP else codes[:, :k], scales)
+
+    def values(self) -> torch.Tensor:
+        """What the matrix stands for, fp32 [n, k]."""
+        s = self.scales.repeat_interleave(GROUP, dim=0)[: self.n].repeat_interleave(GROUP, dim=1)[:, : self.k]
+        return self.codes.float() * s
+
+    def __call__(self, x: Rows8, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """x w^T [T, n], in `dtype` (bf16 or fp32) or into `out`."""
+        T, k = x.record.t, x.record.k
+        if k != self.k or x.device != self.device:
+            raise ValueError(f"x: rows of {self.k} numbers on {self.device} are wanted, not of {k} on {x.device}")
+        out, ld = _result(out, dtype, T, self.n, self.device)
+        if T:
+            _run(self._product, self.device, x.at, self.at, out.data_ptr(), TYPES[out.dtype], ld, self._status_at)
+        return out
+
+    def check(self) -> None:
+        """Waits for the device and raises if a call since the last check gave up."""
+        _check(self.status)
+
+
+def _result(out: torch.Tensor | None, dtype: torch.dtype, T: int, n: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    if out is None:
+        if dtype not in TYPES:
+            raise ValueError("dtype: torch.bfloat16 or torch.float32 is wanted")
+        return torch.empty((T, n), dtype=dtype, device=device), n
+    ld = _pitch("out", out, device)
+    if out.shape[0] != T or out.shape[1] != n:
+        raise ValueError(f"out: [{T}, {n}] is wanted")
+    return out, ld
+
+
+def _check(status: torch.Tensor) -> None:
+    with torch.cuda.device(status.device):
+        torch.cuda.synchronize()
+    if int(status.item()):
+        status.zero_()
+        raise RuntimeError("a wait inside a kernel ran out")
+
+
+class FeedForward8:
+    """y = down h, h = silu(gate x) * (up x) held in 8-bit rows between the two launches."""
+
+    def __init__(self, gate: Linear8, up: Linear8, down: Linear8):
+        if up.n != gate.n or up.k != gate.k or down.k != gate.n or up.device != gate.device or down.device != gate.device:
+            raise ValueError(f"gate [{gate.n}, {gate.k}], up [{up.n}, {up.k}], down [{down.n}, {down.k}] on one device do not make a feed-forward block")
+        if gate.n > MAX_K:
+            raise ValueError(f"gate: at most {MAX_K} rows are wanted")
+        self.gate, self.up, self.down, self.device, self.status = gate, up, down, gate.device, gate.status
+        self._status_at, self._call = gate.status.data_ptr(), _load().feed_forward
+
+    def hidden(self, x: Rows8, out: Rows8 | None = None) -> Rows8:
+        """h alone."""
+        self._fits(x)
+        T = x.record.t
+        if out is None:
+            out = Rows8(T, self.gate.n, self.device)
+        elif out.shape != (T, self.gate.n) or out.device != self.device:
+            raise ValueError(f"out: {T} rows of {self.gate.n} numbers on {self.device} are wanted")
+        if T:
+            _run(_load().gated, self.device, x.at, self.gate.at, self.up.at, out.at, self._status_at)
+        return out
+
+    def _fits(self, x: Rows8) -> None:
+        if x.record.k != self.gate.k or x.device != self.device:
+            raise ValueError(f"x: rows of {self.gate.k} numbers on {self.device} are wanted, not of {x.record.k} on {x.device}")
+
+    def __call__(self, x: Rows8, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """[T, down's n], in `dtype` (bf16 or fp32) or into `out`."""
+        self._fits(x)
+        T = x.record.t
+        out, ld = _result(out, dtype, T, self.down.n, self.device)
+        if T:
+            h = Rows8(T, self.gate.n, self.device)   # (the stream's: the next call's may be the same memory)
+            _run(self._call, self.device, x.at, self.gate.at, self.up.at, self.down.at, h.at, out.data_ptr(), TYPES[out.dtype], ld, self._status_at)
+        return out
+
+    def check(self) -> None:
+        """Waits for the device and raises if a call since the last check gave up."""
+        _check(self.status)
