@@ -331,3 +331,22 @@ def test_refusals(lib):
                 lib.quantise(torch.randn(4, 130, device=dev))), "x:")]:
         with pytest.raises(ValueError, match=says):
             call()
+
+
+def test_codes_of_bf16_numbers_by_many_scales(lib):
+    """Quotients are made by corrections, not by a division: every bf16 number against scales of all kinds and sizes."""
+    gen = torch.Generator().manual_seed(1)
+    top = torch.cat([torch.randint(0x0001, 0x7f80, (300,), generator=gen), torch.arange(0x3f80, 0x4000), torch.arange(0x0001, 0x0100, 7), torch.arange(0x7f00, 0x7f80, 3)])
+    every = torch.randint(0, 0x7f80, (len(top), 127 * 40), generator=gen)
+    every = torch.minimum(every % (0x0700) + (top[:, None] - 0x0700).clamp(min=0), top[:, None])   # (within 2^14 of the group's largest)
+    x = torch.cat([every.view(-1, 127), top.repeat_interleave(40)[:, None]], dim=1).to(torch.int16).view(torch.bfloat16)
+    x = (x * (1 - 2 * torch.randint(0, 2, x.shape, generator=gen)).to(torch.bfloat16)).cuda()
+    rows = lib.quantise(x)
+    codes, scales = checks.groups_of(x.float(), 1)
+    same_groups(rows.codes, rows.scales, codes, scales.t())
+    assert torch.equal(rows.codes.float().signbit(), x.signbit())
+    more = x.float() * (1 + 2.0 ** -8 * torch.rand(x.shape, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda"))
+    more = torch.where(more.isfinite(), more, x.float())
+    codes, scales = checks.groups_of(more, 1)
+    rows = lib.quantise(more)
+    same_groups(rows.codes, rows.scales, codes, scales.t())

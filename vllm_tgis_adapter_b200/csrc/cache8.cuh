@@ -11,6 +11,7 @@
 
 #include "../../include/tgis_kv8.h"
 #include "kernels.h"
+#include "tc_attention.cuh"
 
 namespace tgis {
 
@@ -44,44 +45,47 @@ __device__ __forceinline__ float2 f16x2_to_f32x2(uint32_t h) {
   return f;
 }
 
-// magnitudes as whole numbers order as their values do, with infinities and NaN above all
+// bits of the largest magnitude (and of m's), those of a NaN where one is among them: as whole numbers they order as magnitudes do
 __device__ __forceinline__ uint32_t largest(const float (&x)[8], uint32_t m) {
+  float f = __uint_as_float(m);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-  return m;
+  for (int i = 0; i < 8; i += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(f) : "f"(x[i]), "f"(x[i + 1]));
+  return __float_as_uint(f);
 }
 // Scale of a row (or another group that is quantised together) whose largest magnitude has these bits: NaN where it holds a number that is not finite
 __device__ __forceinline__ float scale_of(uint32_t m) {
   return m >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(m) * (1.f / KV8_TOP), KV8_TINY);
 }
-// Codes of x / s; zeros where the scale is NaN.  An IEEE division is a call of some forty instructions, so the quotients are products with
-// the scale's reciprocal, which are within 2 ulp of them, and are divided again only where that could change a code: within 3 ulp of the
-// middle of two e4m3 numbers (one in 200,000), or below 2^-6, where the middles lie elsewhere.
+// Codes of x / s; zeros where the scale is NaN.  An IEEE division is a call of some forty instructions, and numbers of bf16 lie in the middle
+// of two codes often enough that no quotient that is off by a bit will do.  q = x * (1 / s) is within 1.5 ulp; x - q s is exact in a fused
+// multiply-add, a first correction by it leaves less than an ulp, and after a second one q is the rounded quotient (Markstein's theorem: the
+// reciprocal is the rounded one).  What lies below the least normal number is not exact: tiny groups are taken times 2^64, which no quotient sees.
 template <int N>
-__device__ __forceinline__ void codes(const float (&x)[N], float s, uint32_t (&out)[N / 4]) {
+__device__ __forceinline__ void codes(const float (&v)[N], float s, uint32_t (&out)[N / 4]) {
   const bool fine = s < INFINITY;
-  const float by = fine ? __frcp_rn(s) : 0.f;
+  uint64_t x[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) x[i] = pack2(v[2 * i], v[2 * i + 1]);
+  if (s < 0x1p-60f) {
+    const uint64_t up = pack2(0x1p64f, 0x1p64f);
+    s *= 0x1p64f;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) x[i] = mul2(x[i], up);
+  }
+  const float one = __frcp_rn(s);
+  const uint64_t by = pack2(one, one), minus = pack2(-s, -s);
   float q[N];
-  bool close = false;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = fine ? x[i] * by : 0.f;
-    const int off = (int)(__float_as_uint(q[i]) & 0xfffffu) - 0x80000;
-    close |= (off >= -3 && off <= 3) || (fabsf(q[i]) < 0.015625f && q[i] != 0.f);
-  }
-  if (close) {
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {   // (one division in the code)
-      float xi = x[0];
-#pragma unroll
-      for (int j = 1; j < N; ++j) xi = i == j ? x[j] : xi;
-      const float d = __fdiv_rn(xi, s);
-#pragma unroll
-      for (int j = 0; j < N; ++j) q[j] = i == j ? d : q[j];
-    }
+  for (int i = 0; i < N / 2; ++i) {
+    uint64_t d = mul2(x[i], by);
+    d = fma2(fma2(d, minus, x[i]), by, d);
+    d = fma2(fma2(d, minus, x[i]), by, d);
+    unpack2(d, q[2 * i], q[2 * i + 1]);
+    q[2 * i] = copysignf(q[2 * i], v[2 * i]);   // (of a zero, the sum has lost it)
+    q[2 * i + 1] = copysignf(q[2 * i + 1], v[2 * i + 1]);
   }
 #pragma unroll
-  for (int i = 0; i < N / 4; ++i) out[i] = e4m3x2(q[4 * i], q[4 * i + 1]) | e4m3x2(q[4 * i + 2], q[4 * i + 3]) << 16;
+  for (int i = 0; i < N / 4; ++i) out[i] = fine ? e4m3x2(q[4 * i], q[4 * i + 1]) | e4m3x2(q[4 * i + 2], q[4 * i + 3]) << 16 : 0u;
 }
 
 // 2^e that brings a magnitude (the bits of a number >= 0) to [2^14, 2^15), the most that f16 has room for; no more than 2^126

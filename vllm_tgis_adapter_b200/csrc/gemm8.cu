@@ -7,10 +7,11 @@
 // in the other half of TMEM.  A tile's weights have one scale a k-block and a column has one, so a warp of its own puts their product where
 // the epilogue reads it.  K is split over the CTAs of a cluster, whose sums meet in distributed shared memory in the order of k.
 //
-// Roles: warp 0 TMA producer, warp 1 MMA issuer and TMEM owner, warp 2 scales, warps 4..11 epilogue.  No wait is unbounded.
+// Roles: warps 0..7 epilogue, warp 8 TMA producer, warp 9 MMA issuer and TMEM owner, warp 10 scales.  No wait is unbounded.
 #include <stdarg.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "launch.cuh"
 #include "linear8.cuh"
@@ -19,9 +20,11 @@
 namespace tgis {
 namespace {
 
-constexpr int G8_THREADS = 384, G8_WARPS = 12, G8_EPI = 4;   // epilogue: warps 4 .. 11
+constexpr int G8_EPI = 8, G8_WARPS = 11, G8_THREADS = G8_WARPS * 32;   // epilogue: warps 0 .. 7
+constexpr int G8_LOAD = 8, G8_MMA = 9, G8_SCALE = 10;
 constexpr int G8_W_BYTES = 128 * W8_GROUP;                   // a k-block of a weight tile
 constexpr int G8_SLOTS = 4;                                  // k-blocks whose scales are there
+constexpr int G8_ENDS = 6;
 
 // D[tmem] (+)= A[smem] B[smem], e4m3, fp32 sums
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -32,42 +35,6 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// kind::f8f6f4: C = F32, A = B = E4M3, both K-major
-__host__ __device__ constexpr uint32_t idesc_f8(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
-
-__device__ __forceinline__ void tmem_ld_x8(uint32_t at, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(at));
-}
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t* r) {
-  if constexpr (N == 8) {
-    tmem_ld_x8(at, r);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i += 16) tmem_ld_32x32b_x16(at + i, r + i);
-  }
-}
-
-__device__ __forceinline__ void say_stalled8(const Gemm8Args& a) {
-  if (a.status != nullptr) atomicOr(a.status, TGIS_W8_STALLED);
-  if (a.stalled != nullptr) {
-    *reinterpret_cast<volatile int*>(a.stalled) = 1;
-    __threadfence_system();
-  }
-}
-__device__ __forceinline__ bool wait8(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > 4000000000ll) return false;   // about two seconds: no wait of a working pipeline is that long
-  }
-  return true;
-}
-
-__device__ __forceinline__ float swiglu(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
-
 // Tokens of a tile, and what follows from them.  Two CTAs share an SM while their accumulators (TMEM has 512 columns) and registers allow.
 template <int NT, bool GATED>
 struct Form {
@@ -107,16 +74,16 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_at + 1);
 
   const int warp = threadIdx.x >> 5, lane = (int)lane_id();
-  const int rank = (int)cluster_ctarank(), S = (int)gridDim.z;        // cluster: the CTAs of blockIdx.z
+  const int rank = (int)cluster_ctarank(), S = (int)gridDim.z, log_s = __ffs(S) - 1;   // cluster: the CTAs of blockIdx.z, one, two, four or eight
   const int nb = (int)blockIdx.x, t0 = (int)blockIdx.y * NT;
   const int kb0 = (int)((long long)rank * a.G / S), kb1 = (int)((long long)(rank + 1) * a.G / S);
 
-  if (warp == 0 && elect_one()) {
+  if (warp == G8_LOAD && elect_one()) {
     tma_prefetch_desc(&wmap);
     if (GATED) tma_prefetch_desc(&wmap2);
     tma_prefetch_desc(&xmap);
   }
-  if (warp == 1) {
+  if (warp == G8_MMA) {
     if (elect_one()) {
       for (int i = 0; i < F::STAGES; ++i) {
         mbar_init(&full[i], 1);
@@ -124,11 +91,11 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&tmem_full[i], 1);
-        mbar_init(&tmem_empty[i], G8_WARPS - G8_EPI);
+        mbar_init(&tmem_empty[i], G8_EPI);
       }
       for (int i = 0; i < G8_SLOTS; ++i) {
         mbar_init(&scale_full[i], 1);
-        mbar_init(&scale_empty[i], G8_WARPS - G8_EPI);
+        mbar_init(&scale_empty[i], G8_EPI);
       }
       *gave_up = 0;
       fence_barrier_init();
@@ -140,9 +107,9 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
-  griddep_launch();
+  if (!a.late) griddep_launch();
 
-  if (warp == 0) {
+  if (warp == G8_LOAD) {
     // ===================== TMA producer =====================
     if (elect_one()) {
       const uint64_t once = policy_evict_first();
@@ -157,6 +124,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       if (!a.early) griddep_wait();
       for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
       if (a.early) griddep_wait();
+      if (a.late) griddep_launch_after();
       for (int i = 0; i < pre; ++i) load_x(i, kb0 + i);
       int s = pre % F::STAGES;
       uint32_t phase = pre == F::STAGES ? 1 : 0;
@@ -170,7 +138,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         if (++s == F::STAGES) s = 0, phase ^= 1;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == G8_MMA) {
     // ===================== MMA issuer =====================
     if (elect_one()) {
       constexpr uint32_t idesc = idesc_f8(128, NT);
@@ -197,40 +165,58 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         if (++s == F::STAGES) s = 0, phase ^= 1;
       }
     }
-  } else if (warp == 2) {
+  } else if (warp == G8_SCALE) {
     // ===================== scales: sx[t] sw of the k-blocks to come =====================
     griddep_wait();
     const float* sw = a.sw + (size_t)nb * a.G;
     const float* sw2 = GATED ? a.sw2 + (size_t)nb * a.G : nullptr;
-    constexpr int EACH = (NT + 31) / 32;
-    float x[EACH], w = 0.f, w2 = 0.f;
-    auto load = [&](int kb) {
-      w = sw[kb];
-      if (GATED) w2 = sw2[kb];
+    // (AHEAD k-blocks at a time, asked for while those before them are handed out: one at a time took the L2's latency for each)
+    constexpr int EACH = (NT + 31) / 32, AHEAD = NT > 128 ? 4 : 8;
+    float x[AHEAD][EACH], w[AHEAD], w2[AHEAD];
+    auto load = [&](int from) {
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) x[i] = i * 32 + lane < NT && t0 + i * 32 + lane < a.T ? a.sx[(size_t)kb * a.lds + t0 + i * 32 + lane] : 0.f;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int kb = min(from + u, kb1 - 1);
+        w[u] = sw[kb];
+        w2[u] = GATED ? sw2[kb] : 0.f;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) x[u][j] = j * 32 + lane < NT && t0 + j * 32 + lane < a.T ? a.sx[(size_t)kb * a.lds + t0 + j * 32 + lane] : 0.f;
+      }
     };
     load(kb0);
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int i = kb - kb0, slot = i % G8_SLOTS;
-      if (!__all_sync(0xffffffffu, wait8(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1))) {
-        if (lane == 0) *gave_up = 1;
-        break;
-      }
-      float* to = scale + slot * F::HALVES * NT;
+    bool ok = true;
+    for (int at = kb0; at < kb1 && ok; at += AHEAD) {
+      float f[AHEAD][F::HALVES][EACH];
 #pragma unroll
-      for (int j = 0; j < EACH; ++j)
-        if (j * 32 + lane < NT) {
-          to[j * 32 + lane] = x[j] * w;
-          if (GATED) to[NT + j * 32 + lane] = x[j] * w2;
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+          f[u][0][j] = x[u][j] * w[u];
+          if (GATED) f[u][F::HALVES - 1][j] = x[u][j] * w2[u];
         }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&scale_full[slot]);
-      if (kb + 1 < kb1) load(kb + 1);
+      if (at + AHEAD < kb1) load(at + AHEAD);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (at + u >= kb1) break;
+        const int i = at + u - kb0, slot = i % G8_SLOTS;
+        if (!__all_sync(0xffffffffu, wait8(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1))) {
+          if (lane == 0) *gave_up = 1;
+          ok = false;
+          break;
+        }
+        float* to = scale + slot * F::HALVES * NT;
+#pragma unroll
+        for (int h = 0; h < F::HALVES; ++h)
+#pragma unroll
+          for (int j = 0; j < EACH; ++j)
+            if (j * 32 + lane < NT) to[h * NT + j * 32 + lane] = f[u][h][j];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scale_full[slot]);
+      }
     }
-  } else if (warp >= G8_EPI) {
+  } else {
     // ===================== epilogue: lane = weight row, column = token =====================
-    const int quarter = warp & 3, half = (warp - G8_EPI) >> 2, col0 = half * F::NC;   // gated: the other half is the other matrix
+    const int quarter = warp & 3, half = warp >> 2, col0 = half * F::NC;   // gated: the other half is the other matrix
     float acc[F::NC];
 #pragma unroll
     for (int j = 0; j < F::NC; ++j) acc[j] = 0.f;
@@ -245,60 +231,66 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       tc_fence_after();
       const uint32_t at = tmem + buf * F::COLS + col0 + ((uint32_t)(quarter * 32) << 16);
       const float4* sc = reinterpret_cast<const float4*>(scale + slot * F::HALVES * NT + col0);
-      constexpr int STEP = F::NC < 32 ? F::NC : 32;
+      constexpr int STEP = F::NC < 16 ? F::NC : 16;
+      uint32_t r[2][STEP];
+      tmem_ld<STEP>(at, r[0]);
 #pragma unroll
       for (int c = 0; c < F::NC; c += STEP) {
-        uint32_t r[STEP];
-        tmem_ld<STEP>(at + c, r);
         tmem_ld_wait();
-        if (c + STEP == F::NC) {
+        if (c + STEP < F::NC) {   // (on its way while this one is added)
+          tmem_ld<STEP>(at + c + STEP, r[(c / STEP + 1) & 1]);
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&tmem_empty[buf]);
         }
+        const uint32_t* now = r[(c / STEP) & 1];
 #pragma unroll
         for (int j = 0; j < STEP; j += 4) {
           const float4 f = sc[(c + j) / 4];
-          acc[c + j] += __uint_as_float(r[j]) * f.x;
-          acc[c + j + 1] += __uint_as_float(r[j + 1]) * f.y;
-          acc[c + j + 2] += __uint_as_float(r[j + 2]) * f.z;
-          acc[c + j + 3] += __uint_as_float(r[j + 3]) * f.w;
+          add_scaled(acc[c + j], acc[c + j + 1], now[j], now[j + 1], f.x, f.y);
+          add_scaled(acc[c + j + 2], acc[c + j + 3], now[j + 2], now[j + 3], f.z, f.w);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&scale_empty[slot]);
     }
-    // the ring is done with once the last accumulator is there: the sums take its place, [matrix][token][weight row]
+    if (S > 1) cluster_sync_all();   // every CTA's ring is done with: the sums take its place
+    // Token t is the CTA's of rank t mod S: sums [CTA that they come from][matrix][token / S][weight row].  (Stores that nobody waits for: with sums kept here
+    // and read from there, 64 tokens' latency was 1400 to 3900 clocks.)
     if (!*gave_up) {
-      float* to = reinterpret_cast<float*>(smem) + (size_t)col0 * 128 + quarter * 32 + lane;
+      const uint32_t mine = smem_u32(smem) + (uint32_t)(((rank * F::HALVES + (GATED ? half : 0)) * (NT >> log_s)) * 512 + (quarter * 32 + lane) * 4);
 #pragma unroll
-      for (int j = 0; j < F::NC; ++j) to[j * 128] = acc[j];
+      for (int j = 0; j < F::NC; ++j) {
+        const int t = (GATED ? 0 : col0) + j;
+        if (t0 + t < a.T) st_dsmem_f32(dsmem_addr(mine + (uint32_t)(t >> log_s) * 512, t & (S - 1)), acc[j]);
+      }
     }
   }
+  __syncwarp();
+  if (warp >= G8_EPI && S > 1) cluster_sync_all();   // (the epilogue's first)
   tc_fence_before();
-  __syncthreads();
+  if (S > 1) cluster_sync_all();
+  else __syncthreads();
   if (*gave_up) {   // copies and MMAs in flight, all issued by now, are done long before this millisecond is over
     for (const long long t1 = clock64(); clock64() - t1 < 2000000ll;) {}
     if (threadIdx.x == 0) say_stalled8(a);
+    __syncthreads();
   }
-  cluster_sync_all();
-  if (warp == 1) {
+  if (warp == G8_MMA) {
     tc_fence_after();
     tmem_dealloc<F::TMEM>(tmem);
   }
   // ===================== the cluster's sums -> y or h: a warp a token, four weight rows a lane =====================
   griddep_wait();
-  const uint32_t mine = smem_u32(smem) + lane * 16;
-  for (int t = rank * G8_WARPS + warp; t < NT && t0 + t < a.T; t += S * G8_WARPS) {
+  for (int i = warp, t; t = (i << log_s) + rank, t < NT && t0 + t < a.T; i += G8_WARPS) {
     float v[F::HALVES][4] = {};
-    for (int r = 0; r < S; ++r) {
-      const uint32_t from = dsmem_addr(mine, r);
+    for (int r = 0; r < S; ++r)
 #pragma unroll
       for (int h = 0; h < F::HALVES; ++h) {
-        const float4 p = ld_dsmem_f4(from + (uint32_t)(h * NT + t) * 512);
+        const float4 p = *reinterpret_cast<const float4*>(smem + (size_t)((r * F::HALVES + h) * (NT >> log_s) + i) * 512 + lane * 16);
         v[h][0] += p.x; v[h][1] += p.y; v[h][2] += p.z; v[h][3] += p.w;
       }
-    }
     const int n = nb * 128 + lane * 4;
     if constexpr (GATED) {
       float h[4];
@@ -309,7 +301,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         m = max(m, __float_as_uint(h[i]) & 0x7fffffffu);
       }
       const float s = scale_of(__reduce_max_sync(0xffffffffu, m));
-      codes(h, s, c);
+      codes_near(h, s, c);
       *reinterpret_cast<uint32_t*>(a.codes + (size_t)(t0 + t) * a.ldc + n) = c[0];
       if (lane == 0) a.sh[(size_t)nb * a.ldh + t0 + t] = s;
     } else {
@@ -329,12 +321,6 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       }
     }
   }
-  cluster_sync_all();   // nobody leaves while its sums are read
-}
-
-// K-major operand rows of 128 codes a box
-cudaError_t map8(CUtensorMap* out, const void* codes, int64_t rows, int64_t cols, int64_t ld, int box) {
-  return make_tmap_u8_2d(out, codes, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint32_t)box, W8_GROUP) == 0 ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 template <int NT, bool GATED, class OT>
@@ -345,9 +331,18 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
   if (e != cudaSuccess) return e;
   const int tiles = (a.N + 127) / 128, x_tiles = (a.T + NT - 1) / NT;
   if (x_tiles > 65535) return cudaErrorInvalidValue;
-  // as many CTAs as run at once, and two k-blocks for each at least
+  // The pieces of k whose waves take the fewest k-blocks: a wave's beginning and end take about G8_ENDS of them.  (A tenth of a wave too many costs less than
+  // a wave, for the memory is what all wait for: 32 x 4096 x 14336 in 32 clusters of eight where 30 run at once 14.4 us, of four 15.5, of two 20.7)
+  static ClustersAtOnce at_once;
   int S = 1;
-  while (S < 8 && (long long)tiles * x_tiles * S * 2 <= (long long)num_sms * F::CTAS && a.G >= S * 4) S *= 2;
+  float least = -1.f;
+  for (int s = 1; s <= 8 && s * 2 <= std::max(a.G, 2); s *= 2) {
+    int n = 0;
+    if ((e = at_once(gemm8_kernel<NT, GATED, OT>, G8_THREADS, F::SMEM, s, &n)) != cudaSuccess) return e;
+    const float waves = (float)tiles * (float)x_tiles / (float)(n * F::CTAS);   // (the answer is for one CTA an SM)
+    const float cost = std::max(std::ceil(waves - 0.1f), 1.f) * (float)((a.G + s - 1) / s + G8_ENDS);
+    if (least < 0.f || cost < least) S = s, least = cost;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)tiles, (unsigned)x_tiles, (unsigned)S);
   cfg.blockDim = dim3(G8_THREADS);
@@ -367,7 +362,7 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
 
 template <bool GATED, class OT>
 cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgis_w8_rows& x, const Gemm8Args& a, int num_sms, cudaStream_t stream) {
-  const int nt = a.T <= 16 ? 16 : a.T <= 32 ? 32 : a.T <= 64 ? 64 : a.T <= 128 || GATED ? 128 : 256;
+  const int nt = a.T <= 16 ? 16 : a.T <= 32 ? 32 : a.T <= 64 ? 64 : 128;
   const int box = std::min(nt, a.T);
   CUtensorMap xm;
   cudaError_t e = map8(&xm, x.codes, x.t, x.k, x.ld, box);
@@ -376,36 +371,35 @@ cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgi
     case 16: return launch8<16, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
     case 32: return launch8<32, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
     case 64: return launch8<64, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
-    case 128: return launch8<128, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
-    default:
-      if constexpr (GATED) return cudaErrorInvalidValue;
-      else return launch8<256, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
+    default: return launch8<128, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
   }
 }
 
 }  // namespace
 
-cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, int32_t* status, int* stalled, bool early,
-                         int num_sms, cudaStream_t stream) {
+cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, const Gemm8Call& call, int num_sms,
+                         cudaStream_t stream) {
   if (x.t <= 0 || w.n <= 0) return cudaSuccess;
   Gemm8Args a{};
   a.sx = x.scales; a.lds = x.lds; a.sw = w.scales;
   a.T = x.t; a.N = w.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
-  a.y = y; a.ldy = ldy; a.status = status; a.stalled = stalled; a.early = early;
+  a.y = y; a.ldy = ldy; a.status = call.status; a.stalled = call.stalled; a.early = call.early; a.late = call.late;
+  if (gemm8_pair_takes(a.T)) return gemm8_pair_launch(x, w, a, f32, num_sms, stream);
   CUtensorMap wm;
   cudaError_t e = map8(&wm, w.codes, w.n, w.k, w.ld, 128);
   if (e != cudaSuccess) return e;
   return f32 ? launch_tokens<false, float>(wm, wm, x, a, num_sms, stream) : launch_tokens<false, __nv_bfloat16>(wm, wm, x, a, num_sms, stream);
 }
 
-cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const tgis_w8_rows& out, int32_t* status,
-                               int* stalled, bool early, int num_sms, cudaStream_t stream) {
+cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const tgis_w8_rows& out,
+                               const Gemm8Call& call, int num_sms, cudaStream_t stream) {
   if (x.t <= 0 || gate.n <= 0) return cudaSuccess;
   Gemm8Args a{};
   a.sx = x.scales; a.lds = x.lds; a.sw = gate.scales; a.sw2 = up.scales;
   a.T = x.t; a.N = gate.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
   a.codes = (uint8_t*)out.codes; a.ldc = out.ld; a.sh = out.scales; a.ldh = out.lds;
-  a.status = status; a.stalled = stalled; a.early = early;
+  a.status = call.status; a.stalled = call.stalled; a.early = call.early; a.late = call.late;
+  if (gemm8_pair_takes(a.T)) return gemm8_pair_gated_launch(x, gate, up, a, num_sms, stream);
   CUtensorMap wm, wm2;
   cudaError_t e = map8(&wm, gate.codes, gate.n, gate.k, gate.ld, 128);
   if (e == cudaSuccess) e = map8(&wm2, up.codes, up.n, up.k, up.ld, 128);
@@ -453,6 +447,12 @@ int check_rows(const char* name, const tgis_w8_rows* x, bool made) {
   if (x->lds < x->t) return fail("%s: scales of %lld rows where %d are", name, (long long)x->lds, x->t);
   return check_codes(name, x->codes, x->scales, x->ld, made ? (x->k + 127ll) / 128 * 128 : x->k);
 }
+int check_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out) {
+  if (check_rows("x", x, false) != 0 || check_matrix("gate", gate, false) != 0 || check_matrix("up", up, false) != 0 || check_rows("out", out, true) != 0) return -1;
+  if (x->k != gate->k || x->k != up->k || gate->n != up->n) return fail("x has rows of %d numbers, gate is %d x %d, up %d x %d", x->k, gate->n, gate->k, up->n, up->k);
+  if (out->t != x->t || out->k != gate->n) return fail("out: %d x %d is wanted, not %d x %d", x->t, gate->n, out->t, out->k);
+  return 0;
+}
 int check_type(int32_t type) { return type == TGIS_W8_BF16 || type == TGIS_W8_F32 ? 0 : fail("type %d is not TGIS_W8_BF16 or TGIS_W8_F32", type); }
 int check_plain(const char* name, const void* p, int32_t type, int64_t ld, int64_t k) {
   if (p == nullptr || !aligned(p, type == TGIS_W8_F32 ? 4 : 2) || ld < k) return fail("%s: rows of %lld numbers of the type are wanted", name, (long long)k);
@@ -498,27 +498,31 @@ int tgis_w8_product(const tgis_w8_rows* x, const tgis_w8_matrix* w, void* y, int
   if (check_plain("y", y, type, ldy, w->n) != 0) return -1;
   int sms = 0;
   if (sms_of_device(&sms) != 0) return -1;
-  return done(tgis::gemm8_launch(*x, *w, y, type == TGIS_W8_F32, ldy, status, nullptr, false, sms, (cudaStream_t)stream), "tgis_w8_product");
+  return done(tgis::gemm8_launch(*x, *w, y, type == TGIS_W8_F32, ldy, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_product");
 }
 
 int tgis_w8_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out, int32_t* status, void* stream) {
-  if (check_rows("x", x, false) != 0 || check_matrix("gate", gate, false) != 0 || check_matrix("up", up, false) != 0 || check_rows("out", out, true) != 0) return -1;
-  if (x->k != gate->k || x->k != up->k || gate->n != up->n) return fail("x has rows of %d numbers, gate is %d x %d, up %d x %d", x->k, gate->n, gate->k, up->n, up->k);
-  if (out->t != x->t || out->k != gate->n) return fail("out: %d x %d is wanted, not %d x %d", x->t, gate->n, out->t, out->k);
+  if (check_gated(x, gate, up, out) != 0) return -1;
   if (x->t == 0) return 0;
   int sms = 0;
   if (sms_of_device(&sms) != 0) return -1;
-  return done(tgis::gemm8_gated_launch(*x, *gate, *up, *out, status, nullptr, false, sms, (cudaStream_t)stream), "tgis_w8_gated");
+  return done(tgis::gemm8_gated_launch(*x, *gate, *up, *out, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_gated");
 }
 
 int tgis_w8_feed_forward(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_matrix* down,
                          const tgis_w8_rows* hidden, void* y, int32_t type, int64_t ldy, int32_t* status, void* stream) {
-  // (all of it is checked before the first launch)
-  if (check_type(type) != 0 || check_matrix("down", down, false) != 0 || check_rows("hidden", hidden, true) != 0) return -1;
+  if (check_type(type) != 0 || check_gated(x, gate, up, hidden) != 0 || check_matrix("down", down, false) != 0) return -1;
   if (hidden->k != down->k) return fail("hidden has rows of %d numbers, down of %d", hidden->k, down->k);
-  if (hidden->t > 0 && check_plain("y", y, type, ldy, down->n) != 0) return -1;
-  if (tgis_w8_gated(x, gate, up, hidden, status, stream) != 0) return -1;
-  return tgis_w8_product(hidden, down, y, type, ldy, status, stream);
+  if (x->t == 0) return 0;
+  if (check_plain("y", y, type, ldy, down->n) != 0) return -1;
+  int sms = 0;
+  if (sms_of_device(&sms) != 0) return -1;
+  // The second launch begins once the kernels before the first are complete, so the down projection's weights, which the first does not write, are
+  // asked for while it runs.
+  tgis::Gemm8Call first{status}, second{status};
+  first.late = second.early = true;
+  const int rc = done(tgis::gemm8_gated_launch(*x, *gate, *up, *hidden, first, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
+  return rc != 0 ? rc : done(tgis::gemm8_launch(*hidden, *down, y, type == TGIS_W8_F32, ldy, second, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
 }
 
 }  // extern "C"

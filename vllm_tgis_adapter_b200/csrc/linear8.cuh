@@ -1,8 +1,11 @@
 // Products with 8-bit weights (include/tgis_w8.h): arguments and launchers shared by rows8.cu, gemm8.cu and the engine.  The number format
 // (scale_of, codes) is the 8-bit cache's.
 #pragma once
+#include <atomic>
+
 #include "../../include/tgis_w8.h"
 #include "cache8.cuh"
+#include "ptx.cuh"
 
 namespace tgis {
 
@@ -41,12 +44,119 @@ struct Gemm8Args {
   float* sh;
   int32_t* status;
   int* stalled = nullptr;        // host memory: set to one where a wait ran out
-  int early = 0;                 // the weights were written before the kernels in flight began: they may be read ahead of those
+  int early = 0, late = 0;       // Gemm8Call
 };
+struct Gemm8Call {
+  int32_t* status = nullptr;
+  int* stalled = nullptr;
+  bool early = false;            // what wrote the weights was complete when the kernel before this one began: they may be read ahead of its end
+  bool late = false;             // the next kernel begins once the kernels before this one are complete (its weights may be read early)
+};
+// ---- what the products share
+// kind::f8f6f4: C = F32, A = B = E4M3, both K-major
+__host__ __device__ constexpr uint32_t idesc_f8(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+__device__ __forceinline__ void tmem_ld_x8(uint32_t at, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(at));
+}
+// a0 += d0 s0, a1 += d1 s1
+__device__ __forceinline__ void add_scaled(float& a0, float& a1, uint32_t d0, uint32_t d1, float s0, float s1) {
+  unpack2(fma2(pack2(__uint_as_float(d0), __uint_as_float(d1)), pack2(s0, s1), pack2(a0, a1)), a0, a1);
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t* r) {
+  if constexpr (N == 8) {
+    tmem_ld_x8(at, r);
+  } else if constexpr (N % 32 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 32) tmem_ld_x32(at + i, r + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 16) tmem_ld_32x32b_x16(at + i, r + i);
+  }
+}
+
+__device__ __forceinline__ void say_stalled8(const Gemm8Args& a) {
+  if (a.status != nullptr) atomicOr(a.status, TGIS_W8_STALLED);
+  if (a.stalled != nullptr) {
+    *reinterpret_cast<volatile int*>(a.stalled) = 1;
+    __threadfence_system();
+  }
+}
+__device__ __forceinline__ bool wait8(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - t0 > 4000000000ll) return false;   // about two seconds: no wait of a working pipeline is that long
+  }
+  return true;
+}
+
+// silu(g) u: exp and quotient are the approximate ones, within some steps of 2^-23 of what is rounded to 2^-4 next
+__device__ __forceinline__ float swiglu(float g, float u) {
+  float e, q;
+  e = ex2(g * -1.4426950408889634f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(1.f + e));   // (no denormal goes in, and what comes out as zero is below 2^-126)
+  return g * q * u;
+}
+// codes() of sums, which are no exact numbers: their quotients are products with the scale's reciprocal (1.5 ulp; a code differs where a sum lies that near
+// to the middle of two, one in a million)
+template <int N>
+__device__ __forceinline__ void codes_near(const float* v, float s, uint32_t (&out)[N]) {
+  const bool fine = s < INFINITY;
+  const float by = __frcp_rn(s);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w = e4m3x2(v[4 * i] * by, v[4 * i + 1] * by) | e4m3x2(v[4 * i + 2] * by, v[4 * i + 3] * by) << 16;
+    out[i] = fine ? w : 0u;
+  }
+}
+
+// K-major operand rows of 128 codes, `box` rows at a time
+inline cudaError_t map8(CUtensorMap* out, const void* codes, int64_t rows, int64_t cols, int64_t ld, int box) {
+  return make_tmap_u8_2d(out, codes, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint32_t)box, W8_GROUP) == 0 ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// Clusters of a kernel that run at once, asked once a device and size: an SM's share of a GPC is not always a whole number of clusters
+struct ClustersAtOnce {
+  std::atomic<int> known[OncePerDevice::MAX][4] = {};
+  template <class K>
+  cudaError_t operator()(K kernel, int threads, int smem, int cluster, int* out) {   // cluster: 1, 2, 4 or 8
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const int at = cluster == 8 ? 3 : cluster / 2;
+    if (dev < OncePerDevice::MAX && (*out = known[dev][at].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(cluster * 1024));
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
+    if (e == cudaSuccess && *out < 1) e = cudaErrorLaunchOutOfResources;
+    if (e == cudaSuccess && dev < OncePerDevice::MAX) known[dev][at].store(*out, std::memory_order_relaxed);
+    return e;
+  }
+};
+
 // y = x w^T (y bf16, or fp32: f32), and h of both matrices
-cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, int32_t* status, int* stalled, bool early,
-                         int num_sms, cudaStream_t stream);
-cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const tgis_w8_rows& out, int32_t* status,
-                               int* stalled, bool early, int num_sms, cudaStream_t stream);
+cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, const Gemm8Call& call, int num_sms,
+                         cudaStream_t stream);
+cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const tgis_w8_rows& out,
+                               const Gemm8Call& call, int num_sms, cudaStream_t stream);
+
+// ---- gemm8_pair.cu: prompts
+bool gemm8_pair_takes(int T);
+cudaError_t gemm8_pair_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, const Gemm8Args& g, bool f32, int num_sms, cudaStream_t stream);
+cudaError_t gemm8_pair_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const Gemm8Args& g, int num_sms,
+                                    cudaStream_t stream);
 
 }  // namespace tgis

@@ -10,7 +10,7 @@
 namespace tgis {
 namespace {
 
-constexpr int R8_WARPS = 8, R8_THREADS = R8_WARPS * 32;
+constexpr int R8_WARPS = 8, R8_THREADS = R8_WARPS * 32;   // of a block of weights
 
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -23,24 +23,43 @@ __device__ __forceinline__ float rounded(float v) {
   if constexpr (sizeof(X) == 2) return bf16_round(v);
   else return v;
 }
-// Eight neighbours at k of a row of K; zeros behind it.  VEC: rows start on 16 bytes and K is a multiple of 8.
+// Eight neighbours at k of a row of K, as they lie in memory; zeros behind it.  VEC: rows start on 16 bytes and K is a multiple of 8.
+template <class X>
+struct alignas(16) Eight {
+  X v[8];
+};
+template <>
+struct alignas(16) Eight<__nv_bfloat16> {
+  uint32_t v[4];
+};
 template <class X, bool VEC>
-__device__ __forceinline__ void load8(const X* row, int k, int K, float (&v)[8]) {
+__device__ __forceinline__ Eight<X> load8(const X* row, int k, int K) {
+  Eight<X> e = {};
   if constexpr (VEC) {
-    if (k >= K) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    } else if constexpr (sizeof(X) == 2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + k);
-      v[0] = bf_lo(u.x); v[1] = bf_hi(u.x); v[2] = bf_lo(u.y); v[3] = bf_hi(u.y); v[4] = bf_lo(u.z); v[5] = bf_hi(u.z); v[6] = bf_lo(u.w); v[7] = bf_hi(u.w);
-    } else {
-      const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    if (k < K) {
+      const uint4* p = reinterpret_cast<const uint4*>(row + k);
+      *reinterpret_cast<uint4*>(e.v) = p[0];
+      if constexpr (sizeof(X) == 4) *reinterpret_cast<uint4*>(e.v + 4) = p[1];
     }
+  } else if constexpr (sizeof(X) == 2) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) e.v[i / 2] |= (uint32_t)p[k + i] << (i % 2 * 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (float)row[k + i] : 0.f;
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) e.v[i] = row[k + i];
   }
+  return e;
+}
+__device__ __forceinline__ void unpack(const Eight<float>& e, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = e.v[i];
+}
+__device__ __forceinline__ void unpack(const Eight<__nv_bfloat16>& e, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = i % 2 ? bf_hi(e.v[i / 2]) : bf_lo(e.v[i / 2]);
 }
 template <class X, bool VEC>
 __device__ __forceinline__ void store8(X* row, int k, int K, const float (&v)[8]) {
@@ -64,72 +83,83 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s) {
   return make_uint2(c[0], c[1]);
 }
 
-// WARPS warps a row, R8_WARPS / WARPS rows a CTA.  The scales of a row wait in shared memory for its sum of squares (NORM).
+// A CTA: a row, two of its groups a warp at a time; what the next two need is on its way before these are stored (a compiler cannot know that
+// outputs and inputs are apart).  The row's scales wait in shared memory for its sum of squares (NORM).
 template <class X, bool VEC, bool NORM, int WARPS>
-__global__ void __launch_bounds__(R8_THREADS) rows8_kernel(const Rows8Args a) {
-  constexpr int ROWS = R8_WARPS / WARPS;
-  extern __shared__ float held[];                // NORM: [ROWS][groups]
-  __shared__ float sums[R8_WARPS];
+__global__ void __launch_bounds__(WARPS * 32) rows8_kernel(const Rows8Args a) {
+  extern __shared__ float held[];                // NORM: [groups]
+  __shared__ float sums[WARPS];
   griddep_launch();
   griddep_wait();
-  const int warp = threadIdx.x >> 5, lane = (int)lane_id(), half = lane >> 4, c = lane & 15;
-  const int r = warp / WARPS, part = warp % WARPS, G = (a.K + W8_GROUP - 1) / W8_GROUP;
-  const int64_t t = (int64_t)blockIdx.x * ROWS + r;
+  const int warp = threadIdx.x >> 5, lane = (int)lane_id(), half = lane >> 4, c = lane & 15, G = (a.K + W8_GROUP - 1) / W8_GROUP;
+  const int64_t t = blockIdx.x;
+  const X* x = reinterpret_cast<const X*>(a.x) + t * a.ldx;
+  const X* res = a.residual != nullptr ? reinterpret_cast<const X*>(a.residual) + t * a.ldr : nullptr;
+  X* to = reinterpret_cast<X*>(a.residual_out) + (res != nullptr ? t * a.ldro : 0);
+  uint8_t* code = a.codes + t * a.ldc;
   float ss = 0.f;
-  if (t < a.T) {
-    const X* x = reinterpret_cast<const X*>(a.x) + t * a.ldx;
-    const X* res = reinterpret_cast<const X*>(a.residual);
-    if (res != nullptr) res += t * a.ldr;
-    X* to = reinterpret_cast<X*>(a.residual_out) + (res != nullptr ? t * a.ldro : 0);
-    uint8_t* code = a.codes + t * a.ldc;
-#pragma unroll 2
-    for (int g0 = part * 2; g0 < G; g0 += WARPS * 2) {
-      const int g = g0 + half, k = g * W8_GROUP + c * 8;
-      float v[8];
-      load8<X, VEC>(x, k, a.K, v);
-      if (res != nullptr) {
-        float o[8];
-        load8<X, VEC>(res, k, a.K, o);
+  struct Raw {
+    Eight<X> x, res;
+    Eight<__nv_bfloat16> norm;
+  };
+  auto load = [&](int g0) {
+    const int k = (g0 + half) * W8_GROUP + c * 8;
+    Raw raw = {};
+    raw.x = load8<X, VEC>(x, k, a.K);
+    if (res != nullptr) raw.res = load8<X, VEC>(res, k, a.K);
+    if constexpr (NORM) raw.norm = load8<__nv_bfloat16, VEC>(a.norm, k, a.K);
+    return raw;
+  };
+  auto work = [&](int g0, const Raw& raw) {
+    const int g = g0 + half, k = g * W8_GROUP + c * 8;
+    float xv[8];
+    unpack(raw.x, xv);
+    if (res != nullptr) {
+      float ov[8];
+      unpack(raw.res, ov);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = rounded<X>(v[i] + o[i]);
-        store8<X, VEC>(to, k, a.K, v);
-      }
-      if constexpr (NORM) {
-        float w[8];
-        load8<__nv_bfloat16, VEC>(a.norm, k, a.K, w);
+      for (int i = 0; i < 8; ++i) xv[i] = rounded<X>(xv[i] + ov[i]);
+      store8<X, VEC>(to, k, a.K, xv);
+    }
+    float wv[8];
+    if constexpr (NORM) unpack(raw.norm, wv);
+    if constexpr (NORM) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          ss += v[i] * v[i];
-          v[i] *= w[i];
-        }
-      }
-      uint32_t m = largest(v, 0);
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float s = scale_of(m);
-      if (g < G) {
-        *reinterpret_cast<uint2*>(code + k) = codes_of(v, s);
-        if (c == 0) {
-          if constexpr (NORM) held[r * G + g] = s;
-          else a.scales[(size_t)g * a.lds + t] = s;
-        }
+      for (int i = 0; i < 8; ++i) {
+        ss += xv[i] * xv[i];
+        xv[i] *= wv[i];
       }
     }
+    uint32_t m = largest(xv, 0);
+#pragma unroll
+    for (int s = 1; s < 16; s <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, s));
+    const float s = scale_of(m);
+    if (g < G) {
+      *reinterpret_cast<uint2*>(code + k) = codes_of(xv, s);
+      if (c == 0) {
+        if constexpr (NORM) held[g] = s;
+        else a.scales[(size_t)g * a.lds + t] = s;
+      }
+    }
+  };
+  constexpr int STEP = WARPS * 2;
+  for (int g0 = warp * 2; g0 < G; g0 += 2 * STEP) {
+    const bool more = g0 + STEP < G;
+    Raw first = load(g0), second = {};
+    if (more) second = load(g0 + STEP);
+    work(g0, first);
+    if (more) work(g0 + STEP, second);
   }
   if constexpr (NORM) {
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    for (int s = 16; s >= 1; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
     if (lane == 0) sums[warp] = ss;
     __syncthreads();
-    // (neighbouring threads have neighbouring rows: a CTA's eight scales of a group are one sector)
-    for (int i = threadIdx.x; i < G * ROWS; i += R8_THREADS) {
-      const int g = i / ROWS, row = i % ROWS;
-      const int64_t at = (int64_t)blockIdx.x * ROWS + row;
-      float all = 0.f;
+    float all = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) all += sums[row * WARPS + w];
-      if (at < a.T) a.scales[(size_t)g * a.lds + at] = held[row * G + g] * (1.f / sqrtf(all / (float)a.K + a.eps));
-    }
+    for (int i = 0; i < WARPS; ++i) all += sums[i];
+    const float by = 1.f / sqrtf(all / (float)a.K + a.eps);
+    for (int g = threadIdx.x; g < G; g += WARPS * 32) a.scales[(size_t)g * a.lds + t] = held[g] * by;
   }
 }
 
@@ -144,20 +174,19 @@ __global__ void __launch_bounds__(R8_THREADS) weight8_kernel(const X* __restrict
   const int warp = threadIdx.x >> 5, lane = (int)lane_id(), G = (K + W8_GROUP - 1) / W8_GROUP;
   const int nb = (int)(blockIdx.x / (uint32_t)G), g = (int)(blockIdx.x % (uint32_t)G), k = g * W8_GROUP + (lane & 15) * 8;
   const int n0 = nb * W8_GROUP + warp * 2 + (lane >> 4);
-  float v[EACH][8];
+  Eight<X> raw[EACH];   // (as it lies in memory: half the registers of fp32)
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int n = n0 + i * 2 * R8_WARPS;
-    if (n < N) {
-      load8<X, VEC>(w + (int64_t)n * ldw, k, K, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+    raw[i] = n < N ? load8<X, VEC>(w + (int64_t)n * ldw, k, K) : Eight<X>{};
   }
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) m = largest(v[i], m);
+  for (int i = 0; i < EACH; ++i) {
+    float v[8];
+    unpack(raw[i], v);
+    m = largest(v, m);
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if (lane == 0) most[warp] = m;
   __syncthreads();
@@ -168,7 +197,9 @@ __global__ void __launch_bounds__(R8_THREADS) weight8_kernel(const X* __restrict
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int n = n0 + i * 2 * R8_WARPS;
-    if (n < N) *reinterpret_cast<uint2*>(codes_out + (int64_t)n * ldc + k) = codes_of(v[i], s);
+    float v[8];
+    unpack(raw[i], v);
+    if (n < N) *reinterpret_cast<uint2*>(codes_out + (int64_t)n * ldc + k) = codes_of(v, s);
   }
 }
 
@@ -177,13 +208,10 @@ bool on16(const void* p, int64_t ld, int size) { return (reinterpret_cast<uintpt
 template <class X, bool VEC, bool NORM>
 cudaError_t rows8_some(const Rows8Args& a, int num_sms, cudaStream_t stream) {
   const int G = (a.K + W8_GROUP - 1) / W8_GROUP;
-  // a CTA a row while that leaves no SM with more than a few, a warp a row from there
-  const bool split = a.T <= 4 * num_sms;
-  const int rows = split ? 1 : R8_WARPS;
-  const unsigned ctas = (unsigned)(((long long)a.T + rows - 1) / rows);
-  const size_t smem = NORM ? (size_t)rows * G * sizeof(float) : 0;
-  return split ? launch_k(rows8_kernel<X, VEC, NORM, R8_WARPS>, dim3(ctas), dim3(R8_THREADS), smem, stream, a)
-               : launch_k(rows8_kernel<X, VEC, NORM, 1>, dim3(ctas), dim3(R8_THREADS), smem, stream, a);
+  // Two groups a warp: few rows want all of theirs at once, many rows small CTAs
+  const int warps = G <= 8 ? 4 : G <= 16 || a.T > 4 * num_sms ? 8 : 16;
+  auto go = [&](auto kernel) { return launch_k(kernel, dim3((unsigned)a.T), dim3((unsigned)warps * 32), NORM ? (size_t)G * sizeof(float) : 0, stream, a); };
+  return warps == 4 ? go(rows8_kernel<X, VEC, NORM, 4>) : warps == 8 ? go(rows8_kernel<X, VEC, NORM, 8>) : go(rows8_kernel<X, VEC, NORM, 16>);
 }
 template <class X>
 cudaError_t rows8_typed(const Rows8Args& a, int num_sms, cudaStream_t stream) {

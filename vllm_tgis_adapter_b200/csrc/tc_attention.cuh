@@ -1,4 +1,4 @@
-// What the tcgen05 attention kernels share beyond ptx.cuh: products with an operand in TMEM, TMEM rows to and from registers, packed fp32
+// What the tcgen05 attention kernels (and the 8-bit formats) share beyond ptx.cuh: products with an operand in TMEM, TMEM rows to and from registers, packed fp32
 // arithmetic, register shares, waits that end.
 #pragma once
 #include "ptx.cuh"
@@ -50,6 +50,11 @@ __device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("m
 __device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
   return d;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {

@@ -61,16 +61,36 @@ def _pitch(name: str, x: torch.Tensor, device: torch.device | None = None) -> in
     return pitch if rows > 1 else width
 
 
+class _Device:
+    """What calls on a device share: the status word, and tensors whose new_empty costs half of torch.empty's time."""
+
+    def __init__(self, device: torch.device):
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.status_at = self.status.data_ptr()
+        self.fp32, self.bf16, self.codes, self.bytes = (torch.empty(0, dtype=t, device=device) for t in (torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8))
+
+
+_devices: dict[int, _Device] = {}
+
+
+def _of(device: torch.device) -> _Device:
+    got = _devices.get(device.index)
+    if got is None:
+        got = _devices[device.index] = _Device(device)
+    return got
+
+
 class Rows8:
     """T rows of k numbers in 8 bits: `codes` e4m3 [T, k], `scales` fp32 [groups, T]; views of tensors whose rows are as long as whole groups are."""
 
     __slots__ = ("codes", "scales", "device", "record", "at")
 
     def __init__(self, T: int, k: int, device: torch.device):
-        groups = -(-k // GROUP)
-        codes = torch.empty((T, groups * GROUP), dtype=torch.float8_e4m3fn, device=device)
-        scales = torch.empty((groups, T), dtype=torch.float32, device=device)
-        self.device = codes.device
+        if device.index is None:
+            device = torch.device(device.type, torch.cuda.current_device())
+        groups, on = -(-k // GROUP), _of(device)
+        codes, scales = on.codes.new_empty((T, groups * GROUP)), on.fp32.new_empty((groups, T))
+        self.device = device
         self.record = TgisW8Rows(codes.data_ptr(), scales.data_ptr(), groups * GROUP, T, T, k)
         self.at = C.addressof(self.record)
         self.codes, self.scales = codes if k == groups * GROUP else codes[:, :k], scales
@@ -141,8 +161,7 @@ class Linear8:
         self.codes, self.scales, self.device, self.n, self.k = codes, scales, codes.device, n, k
         self.record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), pitch, n, k)
         self.at = C.addressof(self.record)
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._status_at, self._product = self.status.data_ptr(), _load().product
+        self._on, self._product = _of(self.device), _load().product
 
     @classmethod
     def from_weight(cls, w: torch.Tensor) -> "Linear8":
@@ -152,8 +171,8 @@ class Linear8:
         if w.numel() == 0 or k > MAX_K or n > MAX_ROWS:
             raise ValueError(f"w: 1 to {MAX_ROWS} rows of 1 to {MAX_K} numbers are wanted, not {n} of {k}")
         groups = -(-k // GROUP)
-        codes = torch.empty((n, groups * GROUP), dtype=torch.float8_e4m3fn, device=w.device)
-        scales = torch.empty((-(-n // GROUP), groups), dtype=torch.float32, device=w.device)
+        on = _of(w.device)
+        codes, scales = on.codes.new_empty((n, groups * GROUP)), on.fp32.new_empty((-(-n // GROUP), groups))
         record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), groups * GROUP, n, k)
         _run(_load().weight, w.device, w.data_ptr(), TYPES[w.dtype], ld, C.addressof(record))
         return cls(codes if k == groups * GROUP else codes[:, :k], scales)
@@ -168,21 +187,21 @@ class Linear8:
         T, k = x.record.t, x.record.k
         if k != self.k or x.device != self.device:
             raise ValueError(f"x: rows of {self.k} numbers on {self.device} are wanted, not of {k} on {x.device}")
-        out, ld = _result(out, dtype, T, self.n, self.device)
+        out, ld = _result(out, dtype, T, self.n, self._on, self.device)
         if T:
-            _run(self._product, self.device, x.at, self.at, out.data_ptr(), TYPES[out.dtype], ld, self._status_at)
+            _run(self._product, self.device, x.at, self.at, out.data_ptr(), TYPES[out.dtype], ld, self._on.status_at)
         return out
 
     def check(self) -> None:
-        """Waits for the device and raises if a call since the last check gave up."""
-        _check(self.status)
+        """Waits for the device and raises if a call on it has given up since the last check."""
+        _check(self._on.status)
 
 
-def _result(out: torch.Tensor | None, dtype: torch.dtype, T: int, n: int, device: torch.device) -> tuple[torch.Tensor, int]:
+def _result(out: torch.Tensor | None, dtype: torch.dtype, T: int, n: int, on: _Device, device: torch.device) -> tuple[torch.Tensor, int]:
     if out is None:
         if dtype not in TYPES:
             raise ValueError("dtype: torch.bfloat16 or torch.float32 is wanted")
-        return torch.empty((T, n), dtype=dtype, device=device), n
+        return (on.bf16 if dtype == torch.bfloat16 else on.fp32).new_empty((T, n)), n
     ld = _pitch("out", out, device)
     if out.shape[0] != T or out.shape[1] != n:
         raise ValueError(f"out: [{T}, {n}] is wanted")
@@ -205,8 +224,9 @@ class FeedForward8:
             raise ValueError(f"gate [{gate.n}, {gate.k}], up [{up.n}, {up.k}], down [{down.n}, {down.k}] on one device do not make a feed-forward block")
         if gate.n > MAX_K:
             raise ValueError(f"gate: at most {MAX_K} rows are wanted")
-        self.gate, self.up, self.down, self.device, self.status = gate, up, down, gate.device, gate.status
-        self._status_at, self._call = gate.status.data_ptr(), _load().feed_forward
+        self.gate, self.up, self.down, self.device = gate, up, down, gate.device
+        self._on, self._call = _of(gate.device), _load().feed_forward
+        self._groups = -(-gate.n // GROUP)
 
     def hidden(self, x: Rows8, out: Rows8 | None = None) -> Rows8:
         """h alone."""
@@ -217,7 +237,7 @@ class FeedForward8:
         elif out.shape != (T, self.gate.n) or out.device != self.device:
             raise ValueError(f"out: {T} rows of {self.gate.n} numbers on {self.device} are wanted")
         if T:
-            _run(_load().gated, self.device, x.at, self.gate.at, self.up.at, out.at, self._status_at)
+            _run(_load().gated, self.device, x.at, self.gate.at, self.up.at, out.at, self._on.status_at)
         return out
 
     def _fits(self, x: Rows8) -> None:
@@ -228,12 +248,15 @@ class FeedForward8:
         """[T, down's n], in `dtype` (bf16 or fp32) or into `out`."""
         self._fits(x)
         T = x.record.t
-        out, ld = _result(out, dtype, T, self.down.n, self.device)
+        out, ld = _result(out, dtype, T, self.down.n, self._on, self.device)
         if T:
-            h = Rows8(T, self.gate.n, self.device)   # (the stream's: the next call's may be the same memory)
-            _run(self._call, self.device, x.at, self.gate.at, self.up.at, self.down.at, h.at, out.data_ptr(), TYPES[out.dtype], ld, self._status_at)
+            width = self._groups * GROUP
+            room = self._on.bytes.new_empty(T * (width + self._groups * 4))   # (the stream's: the next call's may be the same memory)
+            at = room.data_ptr()
+            h = TgisW8Rows(at, at + T * width, width, T, T, self.gate.n)
+            _run(self._call, self.device, x.at, self.gate.at, self.up.at, self.down.at, C.addressof(h), out.data_ptr(), TYPES[out.dtype], ld, self._on.status_at)
         return out
 
     def check(self) -> None:
-        """Waits for the device and raises if a call since the last check gave up."""
-        _check(self.status)
+        """Waits for the device and raises if a call on it has given up since the last check."""
+        _check(self._on.status)
