@@ -118,6 +118,12 @@ typedef struct tgis_engine tgis_engine;
 #define TGIS_KV_MODEL 0
 #define TGIS_KV_E4M3 1
 
+/* What the Llama family's projections (q, k, v, o, gate, up, down; not embeddings and head) are held as.  E4M3: blocks of 128 x 128 with an
+ * fp32 scale each, made from the tensors that tgis_engine_load_weight gets, times rows in 8 bits (include/tgis_w8.h): half the bytes that a
+ * decode step reads.  One GPU, no adapter slots. */
+#define TGIS_WEIGHTS_MODEL 0
+#define TGIS_WEIGHTS_E4M3 1
+
 /* Model + runtime configuration (bf16 decoder-only transformer; see TGIS_ARCH_*). */
 typedef struct tgis_config {
   int32_t abi_version; /* must be TGIS_ABI_VERSION */
@@ -389,6 +395,8 @@ const char* tgis_last_error(void);
 int tgis_abi_version(void);
 
 int tgis_engine_create(const tgis_config* cfg, tgis_engine** out);
+/* the same with weights held as TGIS_WEIGHTS_* (vLLM: --quantization fp8) */
+int tgis_engine_create_weights(const tgis_config* cfg, int32_t weights, tgis_engine** out);
 /* Layer-list architectures.  cfg->arch == TGIS_ARCH_PONENEX; parameter names: "embed", "head", "final.norm", "l<i>.norm1|norm1b|norm2|norm2b",
  * "l<i>.mix.dq|dq.norm|uq|dkv|dkv.norm|uk|uv|g|o", "l<i>.mlp.router|router.b|e<j>.gate|e<j>.up|e<j>.down|shared.gate|
  * shared.up|shared.down|shared.sg" (bf16 [out, in]; the engine widens them for TGIS_DTYPE_F32). */

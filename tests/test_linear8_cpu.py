@@ -117,3 +117,31 @@ def test_binding_refuses_tensors_off_the_device():
         linear8.Linear8(torch.zeros(2, 128).to(torch.float8_e4m3fn), torch.zeros(1, 1))
     with pytest.raises(ValueError, match="w:"):
         linear8.Linear8.from_weight(torch.zeros(2, 128))
+
+
+@pytest.mark.parametrize("weights,change,says", [(7, {}, "weights"), (1, dict(arch=_lib.ARCH_OPT, head_dim=64, hidden=64), "Llama"), (1, dict(tp_size=2, n_kv_heads=2, n_q_heads=2), "single GPU"),
+                                                 (1, dict(max_loras=1, max_lora_rank=8), "LoRA"), (1, dict(debug_gemm_ref=1), "debug_gemm_ref"), (1, dict(ffn=131136), "131072")])
+def test_engine_refuses(lib, weights, change, says):
+    cfg = _lib.TgisConfig()
+    cfg.abi_version = _lib.ABI_VERSION
+    values = dict(n_layers=1, hidden=128, n_q_heads=1, n_kv_heads=1, head_dim=128, ffn=128, vocab=64, max_model_len=64, max_num_seqs=1, max_batched_tokens=64, tp_size=1)
+    for name, value in {**values, **change}.items():
+        setattr(cfg, name, value)
+    handle = C.c_void_p()
+    assert lib.tgis_engine_create_weights(C.byref(cfg), weights, C.byref(handle)) != 0
+    assert says in lib.tgis_last_error().decode()
+
+
+def test_flag():
+    from vllm_tgis_adapter_b200.engine.core import PRESETS, EngineError, NativeEngine
+    from vllm_tgis_adapter_b200.engine.ponenex import PRESETS as LISTS
+    from vllm_tgis_adapter_b200.tgis_utils.args import parse_args
+
+    assert parse_args(["--model", "tiny"]).quantization is None
+    assert parse_args(["--model", "tiny", "--quantization", "fp8"]).quantization == "fp8"
+    with pytest.raises(SystemExit):
+        parse_args(["--model", "tiny", "--quantization", "int4"])
+    with pytest.raises(EngineError, match="quantization"):
+        NativeEngine(PRESETS["tiny"], quantization="int4")
+    with pytest.raises(EngineError, match="Llama"):
+        NativeEngine(LISTS["ponenex-1k"], quantization="fp8")

@@ -44,6 +44,7 @@
 #include "cache8.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "linear8.cuh"
 #include "ptx.cuh"
 
 namespace {
@@ -147,6 +148,7 @@ struct DevBuf {
 
 struct LayerW {
   bf16 *wqkv, *wo, *wgu, *wd, *ln1, *ln2;
+  tgis_w8_matrix qkv8{}, o8{}, gate8{}, up8{}, d8{};   // in place of the first four: TGIS_WEIGHTS_E4M3
   // OPT only (tgis_config.arch == TGIS_ARCH_OPT): wgu holds fc1 [ffn, hidden] (not interleaved), wd holds fc2; biases of
   // the four projections (q/k/v concatenated, head-padded like wqkv) and of the two LayerNorms
   bf16 *b_qkv = nullptr, *b_o = nullptr, *b_fc1 = nullptr, *b_fc2 = nullptr, *ln1_b = nullptr, *ln2_b = nullptr;
@@ -388,6 +390,10 @@ struct tgis_engine {
   DevBuf<bf16> k_cache, v_cache;
   bool kv8 = false;                                  // tgis_config.kv_cache_dtype: e4m3 rows with a scale each (cache8.cuh) in place of these
   DevBuf<uint8_t> kv8_pages, kv8_ws;                 // all layers'; partial sums of the attention
+  bool w8 = false;                                   // TGIS_WEIGHTS_E4M3: the layers' projections on linear8.cuh
+  DevBuf<uint8_t> w8_codes, x8_codes, h8_codes;      // all layers' weights; a step's rows, before the projections and inside the feed-forward block
+  DevBuf<float> w8_scales, x8_scales, h8_scales;
+  DevBuf<bf16> w8_load;                              // a tensor on its way into 8 bits (until start)
   size_t kv8_layer_bytes = 0;
   size_t kv_layer_elems = 0;
   int num_blocks = 0;
@@ -633,7 +639,7 @@ struct tgis_engine {
     const size_t H = c.hidden, F = Fl, V = c.vocab, L = c.n_layers;  // F: this rank's ffn shard
     if (!pnx_on) {
     // ---- weights: one arena
-    const size_t per_layer = (size_t)qkv_dim * H + H * q_dim + 2 * F * H + H * F + 2 * H;
+    const size_t per_layer = (w8 ? 0 : (size_t)qkv_dim * H + H * q_dim + 2 * F * H + H * F) + 2 * H;
     const size_t opt_extra = opt ? (size_t)pos_rows * H + H + L * ((size_t)qkv_dim + 4 * H + F) + 64 * (6 * L + 4) : 0;
     const size_t total = V * H /*embed*/ + V * H /*lm_head*/ + H /*norm*/ + (size_t)c.max_model_len * HEAD_DIM +
                          L * per_layer + 64 * (6 * L + 8) + opt_extra;
@@ -651,10 +657,10 @@ struct tgis_engine {
     cos_sin = take((size_t)c.max_model_len * HEAD_DIM);
     layers.resize(L);
     for (auto& l : layers) {
-      l.wqkv = take((size_t)qkv_dim * H);
-      l.wo = take(H * q_dim);
-      l.wgu = take(2 * F * H);
-      l.wd = take(H * F);
+      l.wqkv = w8 ? nullptr : take((size_t)qkv_dim * H);
+      l.wo = w8 ? nullptr : take(H * q_dim);
+      l.wgu = w8 ? nullptr : take(2 * F * H);
+      l.wd = w8 ? nullptr : take(H * F);
       l.ln1 = take(H);
       l.ln2 = take(H);
       if (opt) {
@@ -789,6 +795,7 @@ struct tgis_engine {
       if (make_tmap_bf16_2d(m, w, rows, cols, cols, 128, 64) != 0) throw CudaError("cuTensorMapEncodeTiled(weight) failed");
     };
     for (auto& l : layers) {
+      if (w8) break;   // (their maps are made by the launches)
       wmap(&l.m_qkv, l.wqkv, qkv_dim, H);
       wmap(&l.m_o, l.wo, H, q_dim);
       wmap(&l.m_gu, l.wgu, opt ? F : 2 * F, H);  // OPT: fc1
@@ -807,6 +814,8 @@ struct tgis_engine {
       xmap(&xm_act[i], act.p, T_alloc, F);
       xmap(&xm_last[i], last_hidden.p, S_alloc, H);
     }
+
+    if (w8) w8_alloc();
 
     // ---- KV cache
     const size_t block_elems = (size_t)nkv * KV_BLOCK * HEAD_DIM;  // per layer, per K or V (this rank's kv heads)
@@ -1098,6 +1107,61 @@ struct tgis_engine {
     return fail("unknown layer weight " + full_name);
   }
 
+  // ---- the layers' projections in 8 bits (one GPU): a matrix's blocks of 128 x 128 in the order of its rows; k and v behind q as in wqkv
+  void w8_alloc() {
+    const size_t H = cfg.hidden, F = cfg.ffn, T = std::max(T_max, 256);
+    auto up = [](size_t n) { return (n + W8_GROUP - 1) / W8_GROUP * W8_GROUP; };
+    size_t codes = 0, scales = 0;
+    auto each = [&](auto fn) {   // (twice: the sizes, then the places)
+      codes = scales = 0;
+      for (auto& l : layers) {
+        auto one = [&](tgis_w8_matrix& m, size_t n, size_t k) {
+          fn(m, n, k);
+          codes += up(n) * up(k);
+          scales += up(n) / W8_GROUP * (up(k) / W8_GROUP);
+        };
+        one(l.qkv8, qkv_dim, H);
+        one(l.o8, H, q_dim);
+        one(l.gate8, F, H);
+        one(l.up8, F, H);
+        one(l.d8, H, F);
+      }
+    };
+    each([](tgis_w8_matrix&, size_t, size_t) {});
+    w8_codes.alloc(codes);
+    w8_scales.alloc(scales);
+    each([&](tgis_w8_matrix& m, size_t n, size_t k) { m = {w8_codes.p + codes, w8_scales.p + scales, (int64_t)up(k), (int32_t)n, (int32_t)k}; });
+    w8_load.alloc(std::max({H * F, H * (size_t)q_dim}));
+    const size_t x = up(std::max(H, (size_t)q_dim));
+    x8_codes.alloc(T * x);
+    x8_scales.alloc(T * (x / W8_GROUP));
+    h8_codes.alloc(T * up(F));
+    h8_scales.alloc(T * (up(F) / W8_GROUP));
+  }
+  int w8_load_weight(LayerW& l, const std::string& sub, const std::string& name, const void* ptr, int64_t rows, int64_t cols) {
+    const int64_t H = cfg.hidden, F = cfg.ffn, kvd = (int64_t)nkv * HEAD_DIM;
+    if (w8_load.p == nullptr) return fail("weights are loaded before the engine starts: " + name);
+    const tgis_w8_matrix* m = nullptr;
+    int64_t first = 0, n = 0;   // rows of m
+    if (sub == "self_attn.q_proj.weight") m = &l.qkv8, n = q_dim;
+    else if (sub == "self_attn.k_proj.weight") m = &l.qkv8, first = q_dim, n = kvd;
+    else if (sub == "self_attn.v_proj.weight") m = &l.qkv8, first = q_dim + kvd, n = kvd;
+    else if (sub == "self_attn.o_proj.weight") m = &l.o8, n = H;
+    else if (sub == "mlp.gate_proj.weight") m = &l.gate8, n = F;
+    else if (sub == "mlp.up_proj.weight") m = &l.up8, n = F;
+    else if (sub == "mlp.down_proj.weight") m = &l.d8, n = H;
+    else return fail("unknown layer weight " + name);
+    if (rows * cols != n * m->k) return fail("shape mismatch for " + name + ": got " + std::to_string(rows) + "x" + std::to_string(cols) + " expected " +
+                                             std::to_string(n) + "x" + std::to_string(m->k));
+    cudaError_t e = cudaMemcpy(w8_load.p, ptr, (size_t)(n * m->k) * sizeof(bf16), cudaMemcpyDefault);
+    if (e == cudaSuccess)   // (heads are 128 rows: q, k and v begin at blocks)
+      e = weight8_launch(w8_load.p, false, m->k, (int)n, m->k, (uint8_t*)m->codes + (size_t)first * m->ld, m->ld,
+                         m->scales + first / W8_GROUP * ((m->k + W8_GROUP - 1) / W8_GROUP), cudaStreamLegacy);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    if (e != cudaSuccess) return fail(std::string("weight in 8 bits failed: ") + cudaGetErrorString(e));
+    return 0;
+  }
+
   int load_weight(const std::string& name, const void* ptr, int64_t rows, int64_t cols, int dtype) {
     if (dtype != 0) {
       if (pnx_on && dtype == 1) return pnx_load_table(name, static_cast<const int32_t*>(ptr), rows, cols);
@@ -1133,6 +1197,7 @@ struct tgis_engine {
       LayerW& l = layers[li];
       const std::string sub = name.substr(dot + 1);
       const int64_t kvd = (int64_t)nkv * HEAD_DIM;  // local
+      if (w8 && sub.find("_proj.weight") != std::string::npos) return w8_load_weight(l, sub, name, ptr, rows, cols);
       if (sub == "self_attn.q_proj.weight") rows_shard(l.wqkv, (int64_t)c.n_q_heads * HEAD_DIM, H, q_dim);
       else if (sub == "self_attn.k_proj.weight") rows_shard(l.wqkv + (size_t)q_dim * H, (int64_t)c.n_kv_heads * HEAD_DIM, H, kvd);
       else if (sub == "self_attn.v_proj.weight") rows_shard(l.wqkv + (size_t)(q_dim + kvd) * H, (int64_t)c.n_kv_heads * HEAD_DIM, H, kvd);
@@ -3298,14 +3363,14 @@ struct tgis_engine {
       return g;
     };
     if (lora) ++lora_steps;
-    const bool rope_wanted = !pnx_on && !kv8 && !lora && fuse_rope && !cfg.debug_gemm_ref && gemm_even_split(T, qkv_dim, H, num_sms) >= 2 &&
+    const bool rope_wanted = !pnx_on && !kv8 && !w8 && !lora && fuse_rope && !cfg.debug_gemm_ref && gemm_even_split(T, qkv_dim, H, num_sms) >= 2 &&
                              T <= (qkv_cluster > 0 ? std::max(rope_fuse_max_t, rope_fuse_cluster_max_t) : rope_fuse_max_t);
     // residual add + RMSNorm inside the GEMMs either side of it (single GPU, small steps, both row-"producers" reduced
     // on chip): o-proj -> [post-attention norm] -> gate_up and down-proj -> [next layer's input norm] -> qkv
-    const bool norm_fused = !pnx_on && !lora && fuse_norm && tp == 1 && !cfg.debug_gemm_ref && T <= GEMM_NORM_MAX_T && H % 128 == 0 && H / 128 <= GEMM_NORM_MAX_PARTS &&
+    const bool norm_fused = !pnx_on && !w8 && !lora && fuse_norm && tp == 1 && !cfg.debug_gemm_ref && T <= GEMM_NORM_MAX_T && H % 128 == 0 && H / 128 <= GEMM_NORM_MAX_PARTS &&
                             gemm_cluster_split(T, H, q_dim, num_sms) > 0 && gemm_cluster_split(T, H, F, num_sms) > 0;
     // ... and between the register products of a small model's steps of a few tokens
-    const bool skinny_norm = !pnx_on && !opt && !lora && !norm_fused && tp == 1 && !cfg.debug_gemm_ref && !profiling && gemm_skinny_norm_takes(T, H, q_dim, qkv_dim, F);
+    const bool skinny_norm = !pnx_on && !w8 && !opt && !lora && !norm_fused && tp == 1 && !cfg.debug_gemm_ref && !profiling && gemm_skinny_norm_takes(T, H, q_dim, qkv_dim, F);
     float* ssq_o = skinny_ssq.p;                                       // left by the o and by the down projection
     float* ssq_d = skinny_ssq.p + (size_t)8 * (H / 8);
     const int n_parts = H / 128;
@@ -3315,6 +3380,17 @@ struct tgis_engine {
     const GemmNorm prod_mlp{resid.p, ssq_mlp, nullptr, nullptr, nullptr, 0, 0.f};
     for (int li = 0; li < ((opt || pnx_on) ? 0 : c.n_layers); ++li) {  // Llama stack (OPT: opt_layers() above)
       LayerW& l = layers[li];
+      if (w8) {   // rows of the norm in 8 bits -> qkv -> attention -> rows -> o; rows of the norm -> the block
+        const tgis_w8_rows x = w8_rows(li == 0 ? resid.p : tmp.p, H, T, l.ln1, li > 0);
+        w8_product(x, l.qkv8, qkv.p, qkv_dim);
+        attend(li, T, S, n_dec, n_tiles, max_dec_kv, false);
+        w8_product(w8_rows(attn_out.p, q_dim, T, nullptr, false), l.o8, tmp.p, H);
+        const tgis_w8_rows h{h8_codes.p, h8_scales.p, l.d8.ld, T, T, F};
+        CK(gemm8_gated_launch(w8_rows(tmp.p, H, T, l.ln2, true), l.gate8, l.up8, h, w8_call(), num_sms, stream));
+        ++n_launches;
+        w8_product(h, l.d8, tmp.p, H);
+        continue;
+      }
       const GemmNorm cons_qkv{nullptr, nullptr, resid.p, ssq_mlp, l.ln1, n_parts, c.rms_eps};
       const GemmNorm cons_gu{nullptr, nullptr, resid.p, ssq_attn, l.ln2, n_parts, c.rms_eps};
       const bool qkv_norm_in = norm_fused && li > 0;
@@ -3355,29 +3431,7 @@ struct tgis_engine {
         if (late) lora_shrink(g, xn.p, H, true);
         if (lora) lora_expand(g, qkv.p, qkv_dim);
       }
-      if (kv8) {
-        kv8_attend(li, T, S, n_dec, n_tiles, max_dec_kv);
-      } else {
-        bf16* kc = k_cache.p + (size_t)li * kv_layer_elems;
-        bf16* vc = v_cache.p + (size_t)li * kv_layer_elems;
-        if (!rope_fused) {
-          CK(rope_kvwrite_launch(qkv.p, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, kc, vc, T, nq, nkv,
-                                 stream));
-          ++n_launches;
-        }
-        if (n_dec > 0) {
-          const int max_splits = (max_dec_kv + DECODE_SPLIT - 1) / DECODE_SPLIT;
-          CK(attn_decode_launch(qkv.p, qkv_dim, kc, vc, ds<DecItem>(items_off(S)), n_dec * max_splits, d_seqs,
-                                ds<int32_t>(off_decids), n_dec, max_splits, part_o.p, part_ml.p, attn_out.p, q_dim, nq,
-                                nkv, scale, num_sms, stream, attn_arrive.p));
-          n_launches += (max_splits > 1 && !attn_inkernel_merge) ? 2 : 1;
-        }
-        if (n_tiles > 0) {
-          CK(attn_prefill_launch(qkv.p, qkv_dim, kc, vc, num_blocks, ds<PrefillUnit>(off_units), n_tiles, step_short_blocks,
-                                 d_bt, bt_stride, attn_out.p, q_dim, T, nq, nkv, scale, num_sms, stream));
-          ++n_launches;
-        }
-      }
+      attend(li, T, S, n_dec, n_tiles, max_dec_kv, rope_fused);
       const bool late_o = lora_late(H, q_dim), late_gu = lora_late(2 * F, H), late_d = lora_late(H, F);
       if (lora && !late_o) lora_shrink(lora_one(lora_layers[li].A_o, lora_layers[li].B_o, q_dim, H, LR), attn_out.p, q_dim, false);
       if (skinny_norm) {   // o projection, norm, gate and up projection in two launches
@@ -3446,6 +3500,55 @@ struct tgis_engine {
       }
     }
     CK(stl_marker_launch(22, stream));  // timeline builds: step end (after the result copy)
+  }
+
+  // Rotary embedding, storing and attention of a layer; rope_fused: the qkv product has done the first two
+  void attend(int li, int T, int S, int n_dec, int n_tiles, int max_dec_kv, bool rope_fused) {
+    const AttnSeq* d_seqs = ds<AttnSeq>(off_seqs);
+    const int32_t* d_bt = ds<int32_t>(off_bt);
+    const float scale = attn_scale;
+    if (kv8) {
+      kv8_attend(li, T, S, n_dec, n_tiles, max_dec_kv);
+    } else {
+      bf16* kc = k_cache.p + (size_t)li * kv_layer_elems;
+      bf16* vc = v_cache.p + (size_t)li * kv_layer_elems;
+      if (!rope_fused) {
+        CK(rope_kvwrite_launch(qkv.p, ds<int32_t>(off_pos), ds<int32_t>(off_slotmap), cos_sin, kc, vc, T, nq, nkv,
+                               stream));
+        ++n_launches;
+      }
+      if (n_dec > 0) {
+        const int max_splits = (max_dec_kv + DECODE_SPLIT - 1) / DECODE_SPLIT;
+        CK(attn_decode_launch(qkv.p, qkv_dim, kc, vc, ds<DecItem>(items_off(S)), n_dec * max_splits, d_seqs,
+                              ds<int32_t>(off_decids), n_dec, max_splits, part_o.p, part_ml.p, attn_out.p, q_dim, nq,
+                              nkv, scale, num_sms, stream, attn_arrive.p));
+        n_launches += (max_splits > 1 && !attn_inkernel_merge) ? 2 : 1;
+      }
+      if (n_tiles > 0) {
+        CK(attn_prefill_launch(qkv.p, qkv_dim, kc, vc, num_blocks, ds<PrefillUnit>(off_units), n_tiles, step_short_blocks,
+                               d_bt, bt_stride, attn_out.p, q_dim, T, nq, nkv, scale, num_sms, stream));
+        ++n_launches;
+      }
+    }
+  }
+
+  // ---- the projections in 8 bits: T rows of x [T, k], of the residual stream plus x (which it becomes) or of either's norm
+  tgis_w8_rows w8_rows(const bf16* x, int k, int T, const bf16* norm, bool add) {
+    const tgis_w8_rows r{x8_codes.p, x8_scales.p, (k + W8_GROUP - 1) / W8_GROUP * W8_GROUP, T, T, k};
+    const Rows8Args a{x, k, norm, cfg.rms_eps, add ? resid.p : nullptr, k, resid.p, k, x8_codes.p, x8_scales.p, r.ld, T, T, k};
+    CK(rows8_launch(a, false, num_sms, stream));
+    ++n_launches;
+    return r;
+  }
+  Gemm8Call w8_call() {
+    Gemm8Call call;
+    CK(gemm_pair_word(&call.stalled));
+    call.early = true;   // (weights are static)
+    return call;
+  }
+  void w8_product(const tgis_w8_rows& x, const tgis_w8_matrix& w, bf16* y, int ldy) {
+    CK(gemm8_launch(x, w, y, false, ldy, w8_call(), num_sms, stream));
+    ++n_launches;
   }
 
   // Rotary embedding, storing and attention of a layer over the 8-bit cache: single tokens, then prompts and their portions.  Bounds are
@@ -4322,7 +4425,9 @@ static_assert(sizeof(tgis_sampling_params) == 120, "ctypes mirror: engine/_lib.p
 static_assert(sizeof(tgis_config) == 304, "ctypes mirror: engine/_lib.py TgisConfig");
 int tgis_abi_version(void) { return TGIS_ABI_VERSION; }
 
-int tgis_engine_create(const tgis_config* cfg, tgis_engine** out) {
+int tgis_engine_create(const tgis_config* cfg, tgis_engine** out) { return tgis_engine_create_weights(cfg, TGIS_WEIGHTS_MODEL, out); }
+
+int tgis_engine_create_weights(const tgis_config* cfg, int32_t weights, tgis_engine** out) {
   if (!cfg || !out) return fail("null argument");
   if (cfg->abi_version != TGIS_ABI_VERSION) return fail("ABI version mismatch");
   if (cfg->arch == TGIS_ARCH_PONENEX || cfg->arch == TGIS_ARCH_FALERAX || cfg->arch == TGIS_ARCH_REVEPEL || cfg->arch == TGIS_ARCH_SIKAZEN ||
@@ -4359,11 +4464,20 @@ int tgis_engine_create(const tgis_config* cfg, tgis_engine** out) {
     if (cfg->arch != TGIS_ARCH_LLAMA) return fail("the 8-bit cache serves the Llama family only");
     if (cfg->max_num_seqs > TGIS_KV8_MAX_SEQS) return fail("the 8-bit cache serves at most " + std::to_string(TGIS_KV8_MAX_SEQS) + " sequences at a time");
   }
+  if (weights != TGIS_WEIGHTS_MODEL && weights != TGIS_WEIGHTS_E4M3) return fail("unknown weights");
+  if (weights == TGIS_WEIGHTS_E4M3) {
+    if (cfg->arch != TGIS_ARCH_LLAMA) return fail("8-bit weights serve the Llama family only");
+    if (tpv > 1) return fail("8-bit weights are supported on a single GPU only (tp_size must be 1)");
+    if (cfg->max_loras > 0) return fail("LoRA adapter slots are not supported over 8-bit weights (max_loras must be 0)");
+    if (cfg->debug_gemm_ref) return fail("debug_gemm_ref has no product of 8-bit weights");
+    if (cfg->ffn > TGIS_W8_MAX_K || cfg->n_q_heads * HEAD_DIM > TGIS_W8_MAX_K) return fail("8-bit weights: rows of more than " + std::to_string(TGIS_W8_MAX_K) + " numbers");
+  }
   int ndev = 0;
   if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0)
     return fail("no CUDA device: the TGIS engine has no CPU fallback");
   auto* e = new tgis_engine();
   e->cfg = *cfg;
+  e->w8 = weights == TGIS_WEIGHTS_E4M3;
   try {
     e->init();
   } catch (const std::exception& ex) {

@@ -21,6 +21,7 @@ LAYER_SHARED_KV, LAYER_FULL_QK_NORM, LAYER_HEAD_GATE = 64, 128, 256
 STYLE_POST_NORM, STYLE_TIED_HEAD, STYLE_PARALLEL_GATED, STYLE_PARALLEL_PAIR, STYLE_PRE_DYT, STYLE_PRE_RMS = 1, 2, 4, 8, 16, 32
 DTYPE_BF16, DTYPE_F32 = 0, 1
 KV_MODEL, KV_E4M3 = 0, 1
+WEIGHTS_MODEL, WEIGHTS_E4M3 = 0, 1
 MAX_REQUEST_ID = 96
 MAX_TOPN = 12
 MAX_STOP_TOKEN_IDS = 8
@@ -146,7 +147,7 @@ class TgisStatus(C.Structure):
 
 # Every symbol include/tgis_engine.h and include/tgis_kernels.h declare (tests/test_abi_cpu.py checks the export list)
 ENGINE_SYMBOLS = [
-    "tgis_last_error", "tgis_abi_version", "tgis_engine_create", "tgis_engine_create_spec", "tgis_engine_trace_step", "tgis_engine_load_weight", "tgis_engine_start",
+    "tgis_last_error", "tgis_abi_version", "tgis_engine_create", "tgis_engine_create_weights", "tgis_engine_create_spec", "tgis_engine_trace_step", "tgis_engine_load_weight", "tgis_engine_start",
     "tgis_engine_add_request", "tgis_engine_abort", "tgis_engine_set_mask_provider", "tgis_engine_load_adapter_weight", "tgis_engine_clear_adapter", "tgis_engine_poll", "tgis_engine_status",
     "tgis_engine_max_model_len", "tgis_engine_set_profiling", "tgis_nccl_unique_id", "tgis_engine_worker_run", "tgis_engine_shutdown", "tgis_engine_destroy", "tgis_engine_run_until_idle",
 ]
@@ -204,6 +205,7 @@ def load_library() -> C.CDLL:
     lib.tgis_k_tp_wait.argtypes = [vp, vp, vp, i32, C.c_uint64, C.c_double]
     lib.tgis_k_warp_wait.argtypes = [C.c_uint32, i64, C.POINTER(C.c_uint32)]
     lib.tgis_engine_create.argtypes = [C.POINTER(TgisConfig), C.POINTER(vp)]
+    lib.tgis_engine_create_weights.argtypes = [C.POINTER(TgisConfig), i32, C.POINTER(vp)]
     lib.tgis_engine_create_spec.argtypes = [C.POINTER(TgisConfig), C.POINTER(TgisModelSpec), C.POINTER(vp)]
     lib.tgis_engine_trace_step.argtypes = [vp, C.POINTER(TgisTraceEntry), i32, C.POINTER(C.c_char_p), i32, C.POINTER(f32)]
     lib.tgis_engine_load_weight.argtypes = [vp, C.c_char_p, vp, i64, i64, i32]

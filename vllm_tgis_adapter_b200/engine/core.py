@@ -73,7 +73,8 @@ PRESETS: dict[str, ModelConfig] = {
 KV_BLOCK_TOKENS = 32   # tokens per cache block (csrc/kernels.h KV_BLOCK)
 
 
-# --kv-cache-dtype -> tgis_config.kv_cache_dtype
+# --kv-cache-dtype -> tgis_config.kv_cache_dtype; --quantization -> the weights of tgis_engine_create_weights
+WEIGHTS = {None: _lib.WEIGHTS_MODEL, "fp8": _lib.WEIGHTS_E4M3}
 KV_CACHE_DTYPES = {"auto": _lib.KV_MODEL, "bfloat16": _lib.KV_MODEL, "fp8": _lib.KV_E4M3, "fp8_e4m3": _lib.KV_E4M3}
 
 
@@ -173,7 +174,7 @@ class NativeEngine:
                  kv_cache_bytes: int = 0, gpu_mem_fraction: float = 0.85, device: int = 0, seed: int = 0,
                  debug_gemm_ref: bool = False, use_cuda_graphs: bool | None = None, tp_size: int = 1, tp_rank: int = 0,
                  nccl_id: bytes | None = None, shm_name: str = "", max_loras: int = 0, max_lora_rank: int = 16,
-                 kv_cache_dtype: str = "auto"):
+                 kv_cache_dtype: str = "auto", quantization: str | None = None):
         self.lib = _lib.load_library()
         self.model = model
         if use_cuda_graphs is None:   # default on; TGIS_CUDA_GRAPHS=0 turns decode-step graph replay off
@@ -200,6 +201,8 @@ class NativeEngine:
         if kv_cache_dtype not in KV_CACHE_DTYPES:
             raise EngineError(f"unknown kv_cache_dtype {kv_cache_dtype!r}: one of {', '.join(KV_CACHE_DTYPES)}")
         cfg.kv_cache_dtype = KV_CACHE_DTYPES[kv_cache_dtype]
+        if quantization not in WEIGHTS:
+            raise EngineError(f"unknown quantization {quantization!r}: fp8 or none")
         archs = {"llama": _lib.ARCH_LLAMA, "opt": _lib.ARCH_OPT, "ponenex": _lib.ARCH_PONENEX, "falerax": _lib.ARCH_FALERAX,
                  "revepel": _lib.ARCH_REVEPEL, "sikazen": _lib.ARCH_SIKAZEN, "bisuzen": _lib.ARCH_BISUZEN,
                  "ludelix": _lib.ARCH_LUDELIX}
@@ -209,12 +212,14 @@ class NativeEngine:
         self.max_loras, self.max_lora_rank = int(max_loras), int(max_lora_rank)
         self._h = C.c_void_p()
         if model.arch in LAYER_LIST_ARCHS:
+            if quantization is not None:
+                raise EngineError("8-bit weights serve the Llama family only")
             family = importlib.import_module("." + model.arch, __package__)   # one module per layer-list family
             spec, _keep = family.model_spec(model)   # _keep: the ctypes arrays the spec points into
             if self.lib.tgis_engine_create_spec(C.byref(cfg), C.byref(spec), C.byref(self._h)) != 0:
                 raise EngineError(f"tgis_engine_create_spec failed: {_lib.last_error(self.lib)}")
-        elif self.lib.tgis_engine_create(C.byref(cfg), C.byref(self._h)) != 0:
-            raise EngineError(f"tgis_engine_create failed: {_lib.last_error(self.lib)}")
+        elif self.lib.tgis_engine_create_weights(C.byref(cfg), WEIGHTS[quantization], C.byref(self._h)) != 0:
+            raise EngineError(f"tgis_engine_create_weights failed: {_lib.last_error(self.lib)}")
         self._poll_buf = (TgisStepOutput * 512)()
         self._unread: list[StepOutput] = []
 

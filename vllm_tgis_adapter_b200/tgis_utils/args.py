@@ -82,6 +82,8 @@ def make_engine_arg_parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", type=str, default="auto", choices=["auto", "bfloat16", "bf16", "float32", "fp32"])
     p.add_argument("--kv-cache-dtype", type=str, default="auto", choices=["auto", "bfloat16", "fp8", "fp8_e4m3"],
                    help="what the Llama family's keys and values are stored as; fp8: e4m3 rows with a scale each, half the bytes")
+    p.add_argument("--quantization", "-q", type=str, default=None, choices=["fp8"],
+                   help="what the Llama family's projections are held as; fp8: e4m3 blocks of 128 x 128 with a scale each, half the bytes (one GPU, no LoRA)")
     p.add_argument("--tensor-parallel-size", "-tp", type=int, default=None)
     p.add_argument("--max-num-seqs", type=int, default=256)
     p.add_argument("--max-num-batched-tokens", type=int, default=8192)
