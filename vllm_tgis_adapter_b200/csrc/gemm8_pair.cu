@@ -126,15 +126,16 @@ __global__ void __launch_bounds__(P8_THREADS, 1)
 gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wmap2, const __grid_constant__ CUtensorMap xmap,
                   const __grid_constant__ Pair8Args pa) {
   constexpr int NH = 32 * CH, N_TILE = GATED ? 128 : 2 * NH;   // columns of a half; weight rows (features) of a tile
+  constexpr int BUFS = 512 / NH;   // accumulators of a half in TMEM, the halves in turn: 4, 5 or 8
   static_assert(!GATED || CH == 4, "");
   extern __shared__ uint8_t smem_raw[];
   const Gemm8Args& a = pa.g;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + P8_RING);
   uint64_t* empty = full + P8_STAGES;
-  uint64_t* tmem_full = empty + P8_STAGES;       // [buffer][half]
-  uint64_t* tmem_empty = tmem_full + 4;
-  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(tmem_empty + 4);
+  uint64_t* tmem_full = empty + P8_STAGES;
+  uint64_t* tmem_empty = tmem_full + BUFS;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(tmem_empty + BUFS);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_at + 1);
   uint32_t* most = reinterpret_cast<uint32_t*>(smem + P8_RING + P8_BARS);
 
@@ -154,7 +155,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
         mbar_init(&full[i], 1);    // the leader's expect_tx (both CTAs' bytes)
         mbar_init(&empty[i], 1);   // commit_pair
       }
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < BUFS; ++i) {
         mbar_init(&tmem_full[i], 1);         // commit_pair
         mbar_init(&tmem_empty[i], P8_EPI);   // a half's epilogue warps of both CTAs (leader's barrier)
       }
@@ -225,24 +226,24 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       // ===================== MMA issuer (leader) =====================
       constexpr uint32_t idesc = idesc_f8(256, NH);
       const uint32_t ring = smem_u32(smem);
-      int s = 0, i = 0;
-      uint32_t phase = 0;
+      int s = 0, b = 0;
+      uint32_t phase = 0, phase_b = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        for (int kb = 0; kb < KB && ok; ++kb, ++i) {
+        for (int kb = 0; kb < KB && ok; ++kb) {
           if (!(ok = wait8(&full[s], phase))) break;
           tc_fence_after();
           const uint32_t at = ring + s * 2 * P8_HALF;
           const uint64_t x = make_smem_desc_sw128(at);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int b = (i & 1) * 2 + h;
-            if (!(ok = ok && wait8(&tmem_empty[b], (uint32_t)(i >> 1 & 1) ^ 1))) break;
+            if (!(ok = ok && wait8(&tmem_empty[b], phase_b ^ 1))) break;
             tc_fence_after();
             const uint64_t w = make_smem_desc_sw128(at + P8_HALF + h * (NH / 2) * W8_GROUP);
 #pragma unroll
-            for (int k = 0; k < W8_GROUP / 32; ++k) mma_pair_f8(tmem + b * 128, x + (uint64_t)(k * 2), w + (uint64_t)(k * 2), idesc, k > 0);
+            for (int k = 0; k < W8_GROUP / 32; ++k) mma_pair_f8(tmem + b * NH, x + (uint64_t)(k * 2), w + (uint64_t)(k * 2), idesc, k > 0);
             commit_pair(&tmem_full[b], leader);
+            if (++b == BUFS) b = 0, phase_b ^= 1;
           }
           if (!ok) break;
           commit_pair(&empty[s], leader);
@@ -261,12 +262,12 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     // ===================== epilogue (both CTAs): lane = token, column = weight row =====================
     set_regs<P8_REGS_EPI, true>();
     const int quarter = warp & 3, half = warp >> 2;
-    const uint32_t from = tmem + half * 128 + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t free0 = dsmem_addr(smem_u32(tmem_empty), leader) + half * 8;
+    const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t free0 = dsmem_addr(smem_u32(tmem_empty), leader);
     uint8_t* way = smem + P8_RING + P8_BARS + P8_MOST + warp * P8_OUT;
-    uint64_t* mine = tmem_full + half;
     griddep_wait();   // the scales of the rows; y may still be in use by the previous kernels
-    int i = 0;
+    int b = half;   // this half's next accumulator
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = pair, turn = 0; tile < tiles && ok; tile += pairs, turn ^= 1) {
       const int n_tile = tile / pa.x_tiles, t = tile % pa.x_tiles * 256 + rank * 128 + quarter * 32 + lane;
@@ -292,10 +293,10 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       load(0);
       // One chunk of columns is added while the next one is on its way out of TMEM, across k-blocks too.
       uint32_t r[2][32];
-      ok = __all_sync(0xffffffffu, wait8(&mine[(i & 1) * 2], (uint32_t)(i >> 1 & 1)));
+      ok = __all_sync(0xffffffffu, wait8(&tmem_full[b], phase));
       if (ok) {
         tc_fence_after();
-        tmem_ld<32>(from + (i & 1) * 256, r[0]);
+        tmem_ld<32>(from + b * NH, r[0]);
       }
       for (int at = 0; at < KB && ok; at += P8_AHEAD) {
         float f[P8_AHEAD], f2[P8_AHEAD];
@@ -314,16 +315,17 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
             uint32_t* next = r[(u * CH + c + 1) & 1];
             tmem_ld_wait();
             if (c + 1 < CH) {
-              tmem_ld<32>(from + (i & 1) * 256 + (c + 1) * 32, next);
+              tmem_ld<32>(from + b * NH + (c + 1) * 32, next);
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_tmem(free0 + (i & 1) * 16);
-              ++i;
+              if (lane == 0) mbar_arrive_tmem(free0 + b * 8);
+              b += 2;
+              if (b >= BUFS) b -= BUFS, phase ^= 1;
               if (at + u + 1 < KB) {
-                ok = __all_sync(0xffffffffu, wait8(&mine[(i & 1) * 2], (uint32_t)(i >> 1 & 1)));
+                ok = __all_sync(0xffffffffu, wait8(&tmem_full[b], phase));
                 tc_fence_after();
-                tmem_ld<32>(from + (i & 1) * 256, next);
+                tmem_ld<32>(from + b * NH, next);
               }
             }
 #pragma unroll
@@ -389,12 +391,14 @@ cudaError_t launch_pair8(const CUtensorMap& w, const CUtensorMap& w2, const CUte
                           stream, 2 * S, w, w2, x, a);
 }
 
-// Chunks of a half and pieces of k: those whose waves cost least.  A k-block costs 1 + CH (in units of a quarter of a whole tile's beyond the first), a
-// wave's beginning and end P8_ENDS of the widest, and another P8_MEET where pieces meet.
-constexpr int P8_ENDS = 8, P8_MEET = 6;
+// Chunks of a half and pieces of k: those whose waves take least, in hundredths of a microsecond.  A k-block of 256 x 64 CH takes P8_BLOCK[CH] while it is the
+// epilogue's chain that bounds it, a wave's beginning and end P8_ENDS, P8_MEET more where pieces meet; pieces are for one wave.  Measured (us; taken
+// first): 256 x 4096 x 4096 CH 2, S 2: 12.1; CH 4, S 1: 19.4; CH 2, S 1: 13.8; CH 4, S 2: 14.8.  512 x 6144 x 4096 CH 3: 18.1, CH 4: 20.3, CH 2: 24.7.  301 x 2128 x 11264
+// CH 4, S 2: 25.5, CH 4, S 1: 43.1, CH 2, S 1: 31.4.  1024 x 512 x 8192 CH 4, S 4: 15.6 (CH 2, S 2: 15.6), CH 2, S 1: 23.3.  2048 x 8192 x 8192 CH 4: 130, CH 3: 144, CH 2: 162.
+constexpr int P8_BLOCK[5] = {0, 0, 30, 38, 43}, P8_ENDS = 500, P8_MEET = 200;
 struct Plan { int ch, s; };
 template <class OT>
-cudaError_t plan(int N, int x_tiles, int G, bool gated, int num_sms, Plan* out) {
+cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
   static ClustersAtOnce at_once;
   long long least = -1;
   for (int s = 1; s <= 4 && s <= G; s *= 2) {
@@ -402,11 +406,11 @@ cudaError_t plan(int N, int x_tiles, int G, bool gated, int num_sms, Plan* out) 
     const cudaError_t e = at_once(gemm8_pair_kernel<4, 1, false, OT>, P8_THREADS, P8_SMEM, 2 * s, &n);
     if (e != cudaSuccess) return e;
     for (int c = 4; c >= 2; --c) {
-      if (gated ? c < 4 : (s == 2 && c == 3) || (s == 4 && c < 4)) continue;   // (a thread's share of what pieces leave: 32 columns at least)
+      if (gated ? c < 4 : (s == 2 && c == 3) || (s == 4 && c < 4)) continue;   // (a thread's share of what pieces leave: whole runs of 64 bytes)
       const int rows = gated ? 128 : 64 * c;
       const long long tiles = (long long)((N + rows - 1) / rows) * x_tiles, waves = (tiles + n - 1) / n;
       if (s > 1 && waves > 1) continue;
-      const long long cost = waves * ((1 + c) * ((G + s - 1) / s) + 5 * (P8_ENDS + (s > 1 ? P8_MEET : 0)));
+      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS + (s > 1 ? P8_MEET : 0);
       if (least < 0 || cost < least) *out = Plan{c, s}, least = cost;
     }
   }
@@ -424,7 +428,7 @@ template <class OT>
 cudaError_t product_pair8(const tgis_w8_rows& x, const tgis_w8_matrix& w, const Gemm8Args& g, int num_sms, cudaStream_t stream) {
   Pair8Args a{g, 0, (g.T + 255) / 256};
   Plan p{4, 1};
-  cudaError_t e = plan<OT>(g.N, a.x_tiles, g.G, false, num_sms, &p);
+  cudaError_t e = plan<OT>(g.N, a.x_tiles, g.G, false, &p);
   if (e != cudaSuccess) return e;
   a.n_tiles = (g.N + 64 * p.ch - 1) / (64 * p.ch);
   CUtensorMap wm, xm;
@@ -450,7 +454,7 @@ cudaError_t gemm8_pair_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix&
   if (e == cudaSuccess) e = map8(&xm, x.codes, x.t, x.k, x.ld, 128);
   if (e != cudaSuccess) return e;
   Plan p{4, 1};
-  if ((e = plan<__nv_bfloat16>(g.N, a.x_tiles, g.G, true, num_sms, &p)) != cudaSuccess) return e;
+  if ((e = plan<__nv_bfloat16>(g.N, a.x_tiles, g.G, true, &p)) != cudaSuccess) return e;
   return p.s == 4 ? launch_pair8<4, 4, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream)
        : p.s == 2 ? launch_pair8<4, 2, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream) : launch_pair8<4, 1, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream);
 }

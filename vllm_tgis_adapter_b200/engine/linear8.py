@@ -52,9 +52,10 @@ def _run(function, device: torch.device, *args) -> None:
 
 def _pitch(name: str, x: torch.Tensor, device: torch.device | None = None) -> int:
     """Row pitch of a 2-D bf16 or fp32 CUDA tensor with contiguous rows."""
-    if x.dtype not in TYPES or x.dim() != 2 or not x.is_cuda or (device is not None and x.device != device):
+    shape = x.shape
+    if x.dtype not in TYPES or len(shape) != 2 or not x.is_cuda or (device is not None and x.device != device):
         raise ValueError(f"{name}: a bf16 or fp32 tensor [rows, numbers] on {device or 'a CUDA device'} is wanted")
-    rows, width = x.shape
+    rows, width = shape
     pitch, step = x.stride()
     if step != 1 and width > 1:
         raise ValueError(f"{name}: contiguous rows are wanted")
@@ -158,10 +159,12 @@ class Linear8:
             rows = torch.zeros((n, blocks[1] * GROUP), dtype=torch.uint8, device=codes.device)
             rows[:, :k] = codes.view(torch.uint8)
             codes, pitch = rows.view(torch.float8_e4m3fn)[:, :k], blocks[1] * GROUP
-        self.codes, self.scales, self.device, self.n, self.k = codes, scales, codes.device, n, k
-        self.record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), pitch, n, k)
-        self.at = C.addressof(self.record)
-        self._on, self._product = _of(self.device), _load().product
+        self._keep(codes, scales, codes.device, TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), pitch, n, k))
+
+    def _keep(self, codes: torch.Tensor, scales: torch.Tensor, device: torch.device, record: TgisW8Matrix) -> None:
+        self.codes, self.scales, self.device, self.n, self.k = codes, scales, device, record.n, record.k
+        self.record, self.at = record, C.addressof(record)
+        self._on, self._product = _of(device), _load().product
 
     @classmethod
     def from_weight(cls, w: torch.Tensor) -> "Linear8":
@@ -173,9 +176,10 @@ class Linear8:
         groups = -(-k // GROUP)
         on = _of(w.device)
         codes, scales = on.codes.new_empty((n, groups * GROUP)), on.fp32.new_empty((-(-n // GROUP), groups))
-        record = TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), groups * GROUP, n, k)
-        _run(_load().weight, w.device, w.data_ptr(), TYPES[w.dtype], ld, C.addressof(record))
-        return cls(codes if k == groups * GROUP else codes[:, :k], scales)
+        made = cls.__new__(cls)
+        made._keep(codes if k == groups * GROUP else codes[:, :k], scales, w.device, TgisW8Matrix(codes.data_ptr(), scales.data_ptr(), groups * GROUP, n, k))
+        _run(_load().weight, made.device, w.data_ptr(), TYPES[w.dtype], ld, made.at)
+        return made
 
     def values(self) -> torch.Tensor:
         """What the matrix stands for, fp32 [n, k]."""
