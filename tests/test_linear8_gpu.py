@@ -350,3 +350,126 @@ def test_codes_of_bf16_numbers_by_many_scales(lib):
     codes, scales = checks.groups_of(more, 1)
     rows = lib.quantise(more)
     same_groups(rows.codes, rows.scales, codes, scales.t())
+
+
+def test_matrices_that_lie_otherwise(lib):
+    """Codes by columns, broadcast, out of a larger tensor, a single row at an odd place."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    codes = (torch.randn(300, 260, device="cuda", generator=gen) * 40).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.rand(3, 3, device="cuda", generator=gen)
+    rows = lib.quantise(torch.randn(20, 260, device="cuda", generator=gen))
+    want = lib.Linear8(codes.clone(), scales)(rows)
+    by_columns = codes.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn)
+    assert by_columns.stride(1) != 1 and torch.equal(lib.Linear8(by_columns, scales)(rows), want)
+    for left in (0, 1, 16):
+        wide = torch.zeros(300, 304, dtype=torch.uint8, device="cuda")
+        wide[:, left:left + 260] = codes.view(torch.uint8)
+        assert torch.equal(lib.Linear8(wide.view(torch.float8_e4m3fn)[:, left:left + 260], scales)(rows), want)
+    one = lib.Linear8(codes[7:8], scales[:1])
+    assert torch.equal(one(rows)[:, 0], lib.Linear8(codes[7:8].clone(), scales[:1])(rows)[:, 0])
+    same = lib.Linear8(codes[:1].expand(300, 260), scales)
+    assert torch.equal(same(rows), lib.Linear8(codes[:1].expand(300, 260).contiguous(), scales)(rows))
+
+
+def test_offsets_behind_32_bits(lib):
+    """Codes and results whose places need more than 31 bits."""
+    t, k = 16500, 131072                                    # 2.16e9 codes
+    x = torch.zeros(t, k, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, k, device="cuda").bfloat16()
+    x[5] = 1.0
+    layer = lib.Linear8.from_weight(torch.randn(40, k, device="cuda") * k ** -0.5)
+    rows = lib.quantise(x)
+    del x
+    y = layer(rows, dtype=torch.float32)
+    some = lib.Rows8(4, k, y.device)
+    some.codes.view(torch.uint8)[:] = rows.codes.view(torch.uint8)[[5, t - 3, t - 2, t - 1]]
+    some.scales[:] = rows.scales[:, [5, t - 3, t - 2, t - 1]]
+    want, off = checks.product(some, layer)
+    checks.assert_near(y[[5, t - 3, t - 2, t - 1]], want, off, torch.float32)
+    assert (y[6:t - 3] == 0).all() and (y[:5] == 0).all()
+    del rows, y, some
+    t, n, k = 70000, 33000, 130                             # 2.3e9 results
+    x = torch.randn(t, k, device="cuda")
+    layer = lib.Linear8.from_weight(torch.randn(n, k, device="cuda"))
+    rows = lib.quantise(x)
+    y = layer(rows)
+    for at in (0, 40000, t - 1):
+        some = lib.quantise(x[at:at + 1])
+        want, off = checks.product(some, layer)
+        checks.assert_near(y[at:at + 1], want, off, torch.bfloat16)
+    del y
+    h = lib.FeedForward8(layer, layer, lib.Linear8.from_weight(torch.randn(8, n, device="cuda"))).hidden(rows)   # 2.3e9 codes
+    some = lib.quantise(x[t - 1:])
+    want, off = checks.hidden(some, layer, layer)
+    got = lib.Rows8(1, n, x.device)
+    got.codes.view(torch.uint8)[:] = h.codes.view(torch.uint8)[t - 1:]
+    got.scales[:] = h.scales[:, t - 1:]
+    checks.assert_hidden(got, want, off)
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first quantisation and product are captured."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from vllm_tgis_adapter_b200.engine import linear8 as lib
+x = torch.randn(3, 256, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        lib.Linear8.from_weight(x)
+    raise SystemExit("a layer was made")
+except ValueError as e:
+    assert "before a capture" in str(e), e
+with torch.cuda.graph(graph):
+    first = lib.quantise(x)
+graph.replay()
+assert torch.equal(first.codes.float(), lib.quantise(x).codes.float())
+layers = [lib.Linear8.from_weight(torch.randn(n, 256, device="cuda")) for n in (300, 300, 200)]
+layers[2] = lib.Linear8.from_weight(torch.randn(256, 300, device="cuda"))
+ff, wide = lib.FeedForward8(*layers), torch.randn(400, 256, device="cuda").bfloat16()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = [ff(lib.quantise(z)) for z in (x, wide)]
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, ff(lib.quantise(z))) for a, z in zip(y, (x, wide)))
+ff.check()
+print("ok")
+"""
+    from pathlib import Path
+
+    got = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip().endswith("ok"), got.stderr[-2000:] + got.stdout
+
+
+def test_threads_call_at_once(lib):
+    """Host threads on streams of their own: launches, shared layers, first calls of a size."""
+    import threading
+
+    layer = lib.Linear8.from_weight(torch.randn(512, 640, device="cuda"))
+    xs = [torch.randn(t, 640, device="cuda") for t in (1, 30, 90, 200, 600, 1200)]
+    want = [layer(lib.quantise(x)) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for k in range(30):
+                    j = (i + k) % len(xs)
+                    y = layer(lib.quantise(xs[j]))
+                    torch.cuda.current_stream().synchronize()
+                    if not torch.equal(y, want[j]):
+                        bad.append((i, j))
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad

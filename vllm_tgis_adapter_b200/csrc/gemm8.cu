@@ -1,13 +1,20 @@
 // y[t, n] = sum_g sx[t, g] sw[n / 128, g] sum_{k in g} cx[t, k] cw[n, k]: 8-bit weights (include/tgis_w8.h) times rows in 8 bits, and the gated
 // form h = silu(x gate^T) * (x up^T), which leaves as rows in 8 bits.
 //
-// A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and up to 256 rows of activations (B, a column each): with few tokens
-// such a product is bound by its weight bytes, which are then read once.  The tensor cores (tcgen05 kind::f8f6f4) sum one group of 128 k, that
-// is one k-block, in an accumulator; the epilogue's threads take it over, times both scales, into fp32 registers while the next one is summed
-// in the other half of TMEM.  A tile's weights have one scale a k-block and a column has one, so a warp of its own puts their product where
-// the epilogue reads it.  K is split over the CTAs of a cluster, whose sums meet in distributed shared memory in the order of k.
+// Up to 128 tokens (gemm8_pair.cu has more).  A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and all tokens (B, a column
+// each): such a product is bound by its weight bytes, which are read once.  The tensor cores (tcgen05 kind::f8f6f4) sum one group of 128 k, that is
+// one k-block, in an accumulator; the epilogue's threads take it over, times both scales, into fp32 registers while the next one is summed in the
+// other half of the CTA's TMEM.  A tile's weights have one scale a k-block and a column has one, so a warp of its own puts their product where the
+// epilogue reads it.  K is cut into pieces for the CTAs of a cluster, which push their sums into the shared memory of the CTA that a token belongs to:
+// added there in the order of k, so that a result is the same in every call, without a workspace.
 //
-// Roles: warps 0..7 epilogue, warp 8 TMA producer, warp 9 MMA issuer and TMEM owner, warp 10 scales.  No wait is unbounded.
+// Measured on one B200, us (weight bytes a second), T x N x K, launches one behind the other with cold weights: 1 x 4096 x 4096 6.4 (2.6 TB/s), 1 x 8192 x 8192 13.6
+// (4.9), 32 x 4096 x 14336 14.0 (4.3), 64 x 8192 x 8192 16.7 (4.1), 128 x 4096 x 14336 20 (3.0); gated 1 x 14336 x 4096 22.6 (5.2), 48: 25.1, 128: 40.  What bounds it: of
+// 4096 x 4096 a launch's beginning (0.6 us), the first bytes' way (2.5, of which the bytes themselves are most) and the cluster's end (two
+// barriers and the sums, 2 to 3); large ones the memory, short of a copy's 6.5 TB/s by those 4 us.
+//
+// Roles: warps 0..7 epilogue, warp 8 TMA producer, warp 9 MMA issuer and TMEM owner, warp 10 scales.  Waits on barriers in shared memory end
+// after about two seconds.
 #include <stdarg.h>
 
 #include <algorithm>
@@ -24,7 +31,7 @@ constexpr int G8_EPI = 8, G8_WARPS = 11, G8_THREADS = G8_WARPS * 32;   // epilog
 constexpr int G8_LOAD = 8, G8_MMA = 9, G8_SCALE = 10;
 constexpr int G8_W_BYTES = 128 * W8_GROUP;                   // a k-block of a weight tile
 constexpr int G8_SLOTS = 4;                                  // k-blocks whose scales are there
-constexpr int G8_ENDS = 6;
+constexpr int G8_ENDS = 6;                                    // what a wave's beginning and end take, in k-blocks
 
 // D[tmem] (+)= A[smem] B[smem], e4m3, fp32 sums
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -35,7 +42,9 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Tokens of a tile, and what follows from them.  Two CTAs share an SM while their accumulators (TMEM has 512 columns) and registers allow.
+
+// Tokens of a tile, and what follows from them.  Two CTAs share an SM while their accumulators (TMEM has 512 columns) and registers allow: 64 x 8192 x 8192 in 256
+// CTAs 16.7 us, in the 128 of one an SM 22.
 template <int NT, bool GATED>
 struct Form {
   static constexpr int HALVES = GATED ? 2 : 1;                       // matrices
@@ -107,7 +116,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
-  if (!a.late) griddep_launch();
+  griddep_launch();
 
   if (warp == G8_LOAD) {
     // ===================== TMA producer =====================
@@ -124,12 +133,11 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       if (!a.early) griddep_wait();
       for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
       if (a.early) griddep_wait();
-      if (a.late) griddep_launch_after();
       for (int i = 0; i < pre; ++i) load_x(i, kb0 + i);
       int s = pre % F::STAGES;
       uint32_t phase = pre == F::STAGES ? 1 : 0;
       for (int kb = kb0 + pre; kb < kb1; ++kb) {
-        if (!wait8(&empty[s], phase ^ 1)) {
+        if (!bounded_wait(&empty[s], phase ^ 1)) {
           *gave_up = 1;
           break;
         }
@@ -147,7 +155,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
         const int i = kb - kb0, buf = i & 1;
-        if (!wait8(&tmem_empty[buf], (uint32_t)(i >> 1 & 1) ^ 1) || !wait8(&full[s], phase)) {
+        if (!bounded_wait(&tmem_empty[buf], (uint32_t)(i >> 1 & 1) ^ 1) || !bounded_wait(&full[s], phase)) {
           *gave_up = 1;
           break;
         }
@@ -199,7 +207,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       for (int u = 0; u < AHEAD; ++u) {
         if (at + u >= kb1) break;
         const int i = at + u - kb0, slot = i % G8_SLOTS;
-        if (!__all_sync(0xffffffffu, wait8(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1))) {
+        if (!warp_wait(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1)) {
           if (lane == 0) *gave_up = 1;
           ok = false;
           break;
@@ -220,10 +228,9 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
     float acc[F::NC];
 #pragma unroll
     for (int j = 0; j < F::NC; ++j) acc[j] = 0.f;
-    bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
       const int i = kb - kb0, buf = i & 1, slot = i % G8_SLOTS;
-      ok = wait8(&scale_full[slot], (uint32_t)(i / G8_SLOTS & 1)) && wait8(&tmem_full[buf], (uint32_t)(i >> 1 & 1));
+      const bool ok = bounded_wait(&scale_full[slot], (uint32_t)(i / G8_SLOTS & 1)) && bounded_wait(&tmem_full[buf], (uint32_t)(i >> 1 & 1));
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) *gave_up = 1;
         break;
@@ -383,7 +390,7 @@ cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y
   Gemm8Args a{};
   a.sx = x.scales; a.lds = x.lds; a.sw = w.scales;
   a.T = x.t; a.N = w.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
-  a.y = y; a.ldy = ldy; a.status = call.status; a.stalled = call.stalled; a.early = call.early; a.late = call.late;
+  a.y = y; a.ldy = ldy; a.status = call.status; a.stalled = call.stalled; a.early = call.early;
   if (gemm8_pair_takes(a.T)) return gemm8_pair_launch(x, w, a, f32, num_sms, stream);
   CUtensorMap wm;
   cudaError_t e = map8(&wm, w.codes, w.n, w.k, w.ld, 128);
@@ -398,7 +405,7 @@ cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate
   a.sx = x.scales; a.lds = x.lds; a.sw = gate.scales; a.sw2 = up.scales;
   a.T = x.t; a.N = gate.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
   a.codes = (uint8_t*)out.codes; a.ldc = out.ld; a.sh = out.scales; a.ldh = out.lds;
-  a.status = call.status; a.stalled = call.stalled; a.early = call.early; a.late = call.late;
+  a.status = call.status; a.stalled = call.stalled; a.early = call.early;
   if (gemm8_pair_takes(a.T)) return gemm8_pair_gated_launch(x, gate, up, a, num_sms, stream);
   CUtensorMap wm, wm2;
   cudaError_t e = map8(&wm, gate.codes, gate.n, gate.k, gate.ld, 128);
@@ -517,12 +524,8 @@ int tgis_w8_feed_forward(const tgis_w8_rows* x, const tgis_w8_matrix* gate, cons
   if (check_plain("y", y, type, ldy, down->n) != 0) return -1;
   int sms = 0;
   if (sms_of_device(&sms) != 0) return -1;
-  // The second launch begins once the kernels before the first are complete, so the down projection's weights, which the first does not write, are
-  // asked for while it runs.
-  tgis::Gemm8Call first{status}, second{status};
-  first.late = second.early = true;
-  const int rc = done(tgis::gemm8_gated_launch(*x, *gate, *up, *hidden, first, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
-  return rc != 0 ? rc : done(tgis::gemm8_launch(*hidden, *down, y, type == TGIS_W8_F32, ldy, second, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
+  const int rc = done(tgis::gemm8_gated_launch(*x, *gate, *up, *hidden, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
+  return rc != 0 ? rc : done(tgis::gemm8_launch(*hidden, *down, y, type == TGIS_W8_F32, ldy, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");
 }
 
 }  // extern "C"

@@ -1,12 +1,21 @@
-// The products of gemm8.cu for prompts, on CTA pairs (tcgen05 cta_group::2, kind::f8f6f4).
+// The products of gemm8.cu for more than 128 tokens, on CTA pairs (tcgen05 cta_group::2, kind::f8f6f4).
 //
 // Two neighbouring SMs work on one tile of 256 tokens x up to 256 weight rows.  Here tokens are the MMA's A operand (a CTA has 128 of them, a lane
 // each) and weights its B operand (a CTA holds half of them and the tensor cores read both halves): a thread of the epilogue has one token, whose
 // scale is one number a k-block, and its columns lie in at most two blocks of weights, so scaling costs a group's sums nothing but the multiply-add
-// that adds them up.  A k-block is one group of 128; its sums are taken from one half of TMEM while the tensor cores fill the other.
+// that adds them up.  A k-block is one group of 128.  Each half of the columns is an MMA, an accumulator and a set of four warps of its own, so that one
+// half's sums are taken while the tensor cores make the other's, and accumulators go round through all of TMEM.
+//
+// Measured on one B200, T x N x K: 2048 x 8192 x 8192 130 us (2110 TFLOP/s), 2048 x 4096 x 14336 113 (2140), 512 x 8192 x 8192 35 (1950), 256 x 4096 x 4096 12.2; gated 2048 x 14336 x
+// 4096 215 (2240).  (Back to back for a second, at the power limit's clock: 157 for the first.)  What bounds it: a k-block of 256 x 256 takes some 820 clocks where
+// the tensor cores need 512: the epilogue's chain of barrier, TMEM loads and 64 multiply-adds of pairs a thread (305 clocks of the SM's fp32 lanes).
+// Without the multiply-adds a k-block takes 680 clocks, without the loads as well 600.  What mattered: arrivals that wait for no memory (mbar_arrive_tmem: 311 -> 172 us),
+// 32 columns a load instead of 16 (172 -> 146), a chunk on its way while one is added (-> 141), results through shared memory (-> 130).
+// Against gemm8.cu, us: 128 tokens x 4096 x 14336 24.7 and 20.3, 200: 25.6 and 32.0; x 8192 x 8192 128: 22.9 and 22.2, 200: 23.4 and 35.1.
 //
 // Roles per CTA: warps 0..7 epilogue (two a lane quarter, half of the columns each), warp 8 TMA producer, warp 9 MMA issuer (leader CTA only) and
-// TMEM owner.  The leader's `full` barrier counts both CTAs' bytes; tcgen05.commit releases a ring slot in both.  No wait is unbounded.
+// TMEM owner.  The leader's `full` barrier counts both CTAs' bytes; tcgen05.commit releases a ring slot in both.  Waits on barriers in shared
+// memory end after about two seconds.
 #include <algorithm>
 
 #include "launch.cuh"
@@ -41,7 +50,7 @@ struct Pair8Args {
 };
 
 // A thread's row of 64 bytes (v: four 16-byte words) of rows that lie `pitch` bytes apart: the warp's 32 of them leave in runs of 64 bytes, eight
-// rows an instruction (a row a lane takes 32 lines an instruction: 5600 clocks a tile of 128 x 256 where this takes a third).
+// rows an instruction (a row a lane takes 32 lines an instruction: 5600 clocks a tile of 128 x 256 where this takes 1500).
 __device__ __forceinline__ void leave64(uint8_t* way, int lane, const uint32_t (&v)[16], uint8_t* first_row, int64_t pitch, int rows) {
   __syncwarp();
 #pragma unroll
@@ -170,7 +179,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
   cluster_sync_all();   // the peer's barriers exist
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
-  if (!a.late) griddep_launch();
+  griddep_launch();
 
   // how all warps end (in either branch: what follows the two has the registers of the poorer one)
   auto meet = [&] {
@@ -207,14 +216,13 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       if (!a.early) griddep_wait();
       for (int kb = 0; kb < pre; ++kb) load_w(kb, pair, kb);
       if (a.early) griddep_wait();
-      if (a.late) griddep_launch_after();
       for (int kb = 0; kb < pre; ++kb) load_x(kb, pair, kb);
       int s = pre % P8_STAGES;
       uint32_t phase = pre == P8_STAGES ? 1 : 0;
       bool ok = true;
       for (int tile = pair, first = pre; tile < tiles && ok; tile += pairs, first = 0) {
         for (int kb = first; kb < KB; ++kb) {
-          if (!(ok = wait8(&empty[s], phase ^ 1))) break;
+          if (!(ok = bounded_wait(&empty[s], phase ^ 1))) break;
           load_w(s, tile, kb);
           load_x(s, tile, kb);
           if (++s == P8_STAGES) s = 0, phase ^= 1;
@@ -231,13 +239,13 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
         for (int kb = 0; kb < KB && ok; ++kb) {
-          if (!(ok = wait8(&full[s], phase))) break;
+          if (!(ok = bounded_wait(&full[s], phase))) break;
           tc_fence_after();
           const uint32_t at = ring + s * 2 * P8_HALF;
           const uint64_t x = make_smem_desc_sw128(at);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!(ok = ok && wait8(&tmem_empty[b], phase_b ^ 1))) break;
+            if (!(ok = ok && bounded_wait(&tmem_empty[b], phase_b ^ 1))) break;
             tc_fence_after();
             const uint64_t w = make_smem_desc_sw128(at + P8_HALF + h * (NH / 2) * W8_GROUP);
 #pragma unroll
@@ -293,7 +301,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       load(0);
       // One chunk of columns is added while the next one is on its way out of TMEM, across k-blocks too.
       uint32_t r[2][32];
-      ok = __all_sync(0xffffffffu, wait8(&tmem_full[b], phase));
+      ok = warp_wait(&tmem_full[b], phase);
       if (ok) {
         tc_fence_after();
         tmem_ld<32>(from + b * NH, r[0]);
@@ -323,7 +331,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
               b += 2;
               if (b >= BUFS) b -= BUFS, phase ^= 1;
               if (at + u + 1 < KB) {
-                ok = __all_sync(0xffffffffu, wait8(&tmem_full[b], phase));
+                ok = warp_wait(&tmem_full[b], phase);
                 tc_fence_after();
                 tmem_ld<32>(from + b * NH, next);
               }

@@ -3,6 +3,10 @@
 // One pass each, bound by memory.  A half-warp has a group of 128 neighbours of a row, eight a lane: its maximum is four exchanges away and
 // its codes are eight bytes a lane.  With a norm the factor 1 / rms is the same for a whole row, so the codes are those of r * norm
 // and only the scales wait for the row's sum of squares: nothing is read twice or held.
+//
+// Measured on one B200: 2048 rows x 4096 with residual and norm 14.4 us in bf16 (4.1 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.1 us.  What bounds the
+// former: two rounds of a row's loads a CTA with their latency, and some 200 instructions for eight numbers a lane.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
+// copy's rate), from bf16 158 (4.5 TB/s: a division's worth of arithmetic a number).
 #include "launch.cuh"
 #include "linear8.cuh"
 #include "ptx.cuh"

@@ -22,6 +22,7 @@ from ._lib import TgisW8Matrix, TgisW8Rows
 GROUP, MAX_K, MAX_ROWS = 128, 131072, 1 << 22
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
 _functions = None
+_current_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 class _Functions:
@@ -41,11 +42,11 @@ def _load() -> _Functions:
 
 def _run(function, device: torch.device, *args) -> None:
     index = device.index
-    if torch.cuda.current_device() == index:
-        rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        rc = function(*args, _stream(index))
     else:
         with torch.cuda.device(index):
-            rc = function(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = function(*args, _stream(index))
     if rc != 0:
         raise ValueError((_load().error() or b"").decode(errors="replace"))
 
@@ -63,12 +64,21 @@ def _pitch(name: str, x: torch.Tensor, device: torch.device | None = None) -> in
 
 
 class _Device:
-    """What calls on a device share: the status word, and tensors whose new_empty costs half of torch.empty's time."""
+    """What calls on a device share: empty tensors, whose new_empty costs half of torch.empty's time, and the status word."""
 
     def __init__(self, device: torch.device):
-        self.status = torch.zeros(1, dtype=torch.int32, device=device)
-        self.status_at = self.status.data_ptr()
+        self.device, self.status, self.status_at = device, None, None
         self.fp32, self.bf16, self.codes, self.bytes = (torch.empty(0, dtype=t, device=device) for t in (torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8))
+
+    def with_status(self) -> "_Device":
+        if self.status is None:
+            if torch.cuda.is_current_stream_capturing():   # (the word would be a graph's, and zeroed by its replays)
+                raise ValueError("the first layer on a device is made before a capture begins")
+            with torch.cuda.device(self.device):
+                self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+                torch.cuda.current_stream().synchronize()
+            self.status_at = self.status.data_ptr()
+        return self
 
 
 _devices: dict[int, _Device] = {}
@@ -110,13 +120,14 @@ def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-
     """Rows of x [T, k] (bf16 or fp32) in 8 bits.  `residual` (like x): x + residual, rounded to their type, takes the place of x and is stored in
     `residual_out` (None: residual itself).  `norm` (bf16 [k]): the RMS norm's weight, v = r * norm / sqrt(mean r^2 + eps)."""
     ld = _pitch("x", x)
-    device, (T, k) = x.device, x.shape
+    device, dtype, shape = x.device, x.dtype, x.shape
+    T, k = shape
     if k < 1 or k > MAX_K or T > MAX_ROWS:
         raise ValueError(f"x: at most {MAX_ROWS} rows of 1 to {MAX_K} numbers are wanted, not {T} of {k}")
     norm_at = res_at = to_at = None
     ldr = ldt = 0
     if norm is not None:
-        if norm.dtype != torch.bfloat16 or norm.dim() != 1 or norm.shape[0] != k or norm.device != device or not norm.is_contiguous():
+        if norm.dtype != torch.bfloat16 or norm.shape != (k,) or norm.device != device or not norm.is_contiguous():
             raise ValueError(f"norm: {k} contiguous bf16 numbers on {device} are wanted")
         norm_at = norm.data_ptr()
     if residual is not None:
@@ -125,8 +136,8 @@ def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-
             residual_out, ldt = residual, ldr
         else:
             ldt = _pitch("residual_out", residual_out, device)
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual_out.shape != x.shape or residual_out.dtype != x.dtype:
-            raise ValueError(f"residual, residual_out: {x.dtype} tensors [{T}, {k}] are wanted")
+        if residual.shape != shape or residual.dtype != dtype or residual_out.shape != shape or residual_out.dtype != dtype:
+            raise ValueError(f"residual, residual_out: {dtype} tensors [{T}, {k}] are wanted")
         res_at, to_at = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out: there is no residual")
@@ -135,7 +146,7 @@ def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-
     elif out.shape != (T, k) or out.device != device:
         raise ValueError(f"out: {T} rows of {k} numbers on {device} are wanted")
     if T or norm is not None:
-        _run(_load().rows, device, x.data_ptr(), TYPES[x.dtype], ld, norm_at, eps, res_at, ldr, to_at, ldt, out.at)
+        _run(_load().rows, device, x.data_ptr(), TYPES[dtype], ld, norm_at, eps, res_at, ldr, to_at, ldt, out.at)
     return out
 
 
@@ -164,7 +175,7 @@ class Linear8:
     def _keep(self, codes: torch.Tensor, scales: torch.Tensor, device: torch.device, record: TgisW8Matrix) -> None:
         self.codes, self.scales, self.device, self.n, self.k = codes, scales, device, record.n, record.k
         self.record, self.at = record, C.addressof(record)
-        self._on, self._product = _of(device), _load().product
+        self._on, self._product = _of(device).with_status(), _load().product
 
     @classmethod
     def from_weight(cls, w: torch.Tensor) -> "Linear8":
@@ -229,7 +240,7 @@ class FeedForward8:
         if gate.n > MAX_K:
             raise ValueError(f"gate: at most {MAX_K} rows are wanted")
         self.gate, self.up, self.down, self.device = gate, up, down, gate.device
-        self._on, self._call = _of(gate.device), _load().feed_forward
+        self._on, self._call = gate._on, _load().feed_forward
         self._groups = -(-gate.n // GROUP)
 
     def hidden(self, x: Rows8, out: Rows8 | None = None) -> Rows8:
