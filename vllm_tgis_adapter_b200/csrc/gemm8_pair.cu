@@ -400,10 +400,10 @@ cudaError_t launch_pair8(const CUtensorMap& w, const CUtensorMap& w2, const CUte
 }
 
 // Chunks of a half and pieces of k: those whose waves take least, in hundredths of a microsecond.  A k-block of 256 x 64 CH takes P8_BLOCK[CH] while it is the
-// epilogue's chain that bounds it, a wave's beginning and end P8_ENDS, P8_MEET more where pieces meet; pieces are for one wave.  Measured (us; taken
-// first): 256 x 4096 x 4096 CH 2, S 2: 12.1; CH 4, S 1: 19.4; CH 2, S 1: 13.8; CH 4, S 2: 14.8.  512 x 6144 x 4096 CH 3: 18.1, CH 4: 20.3, CH 2: 24.7.  301 x 2128 x 11264
-// CH 4, S 2: 25.5, CH 4, S 1: 43.1, CH 2, S 1: 31.4.  1024 x 512 x 8192 CH 4, S 4: 15.6 (CH 2, S 2: 15.6), CH 2, S 1: 23.3.  2048 x 8192 x 8192 CH 4: 130, CH 3: 144, CH 2: 162.
-constexpr int P8_BLOCK[5] = {0, 0, 30, 38, 43}, P8_ENDS = 500, P8_MEET = 200;
+// epilogue's chain that bounds it, a launch's beginning and end P8_ENDS[pieces]; pieces are for one wave.  Measured (us; taken first): 256 x 4096 x 4096 CH 2, S 2: 12.1;
+// CH 4, S 1: 19.4; CH 2, S 1: 13.8; CH 4, S 2: 14.8.  512 x 6144 x 4096 CH 3: 18.1, CH 4: 20.3, CH 2: 24.7.  301 x 2128 x 11264 CH 4, S 2: 25.5, CH 4, S 1: 43.1, CH 2, S 1: 31.4.
+// 1024 x 512 x 8192 CH 4, S 4: 15.6 (CH 2, S 2: 15.6), CH 2, S 1: 23.3.  203 x 512 x 1536 CH 2, S 1: 7.1, CH 4, S 4: 9.1.  2048 x 8192 x 8192 CH 4: 130, CH 3: 144, CH 2: 162.
+constexpr int P8_BLOCK[5] = {0, 0, 30, 38, 43}, P8_ENDS[5] = {0, 400, 600, 0, 870};
 struct Plan { int ch, s; };
 template <class OT>
 cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
@@ -418,7 +418,7 @@ cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
       const int rows = gated ? 128 : 64 * c;
       const long long tiles = (long long)((N + rows - 1) / rows) * x_tiles, waves = (tiles + n - 1) / n;
       if (s > 1 && waves > 1) continue;
-      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS + (s > 1 ? P8_MEET : 0);
+      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS[s];
       if (least < 0 || cost < least) *out = Plan{c, s}, least = cost;
     }
   }

@@ -4,9 +4,9 @@
 // its codes are eight bytes a lane.  With a norm the factor 1 / rms is the same for a whole row, so the codes are those of r * norm
 // and only the scales wait for the row's sum of squares: nothing is read twice or held.
 //
-// Measured on one B200: 2048 rows x 4096 with residual and norm 14.4 us in bf16 (4.1 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.1 us.  What bounds the
-// former: two rounds of a row's loads a CTA with their latency, and some 200 instructions for eight numbers a lane.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
-// copy's rate), from bf16 158 (4.5 TB/s: a division's worth of arithmetic a number).
+// Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.1 us.  What bounds the
+// former: two rounds of a row's loads a CTA with their latency, three waves of CTAs.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
+// copy's rate), from bf16 143 (4.9 TB/s: the arithmetic of a number is the same).
 #include "launch.cuh"
 #include "linear8.cuh"
 #include "ptx.cuh"
@@ -90,7 +90,7 @@ __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s) {
 // A CTA: a row, two of its groups a warp at a time; what the next two need is on its way before these are stored (a compiler cannot know that
 // outputs and inputs are apart).  The row's scales wait in shared memory for its sum of squares (NORM).
 template <class X, bool VEC, bool NORM, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) rows8_kernel(const Rows8Args a) {
+__global__ void __launch_bounds__(WARPS * 32, sizeof(X) == 2 && WARPS == 8 ? 5 : 1) rows8_kernel(const Rows8Args a) {
   extern __shared__ float held[];                // NORM: [groups]
   __shared__ float sums[WARPS];
   griddep_launch();
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows8_kernel(const Rows8Args a) {
 
 // A CTA: a block of 128 x 128, eight rows a thread
 template <class X, bool VEC>
-__global__ void __launch_bounds__(R8_THREADS) weight8_kernel(const X* __restrict__ w, int64_t ldw, int N, int K, uint8_t* __restrict__ codes_out, int64_t ldc,
+__global__ void __launch_bounds__(R8_THREADS, sizeof(X) == 2 ? 4 : 2) weight8_kernel(const X* __restrict__ w, int64_t ldw, int N, int K, uint8_t* __restrict__ codes_out, int64_t ldc,
                                                              float* __restrict__ scales) {
   constexpr int EACH = W8_GROUP / (2 * R8_WARPS);
   __shared__ uint32_t most[R8_WARPS];
