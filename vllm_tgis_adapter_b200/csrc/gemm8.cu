@@ -192,8 +192,8 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       }
     };
     load(kb0);
-    bool ok = true;
-    for (int at = kb0; at < kb1 && ok; at += AHEAD) {
+    long long patience = WAIT_LIMIT;
+    for (int at = kb0; at < kb1; at += AHEAD) {
       float f[AHEAD][F::HALVES][EACH];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
@@ -207,11 +207,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       for (int u = 0; u < AHEAD; ++u) {
         if (at + u >= kb1) break;
         const int i = at + u - kb0, slot = i % G8_SLOTS;
-        if (!warp_wait(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1)) {
-          if (lane == 0) *gave_up = 1;
-          ok = false;
-          break;
-        }
+        await(&scale_empty[slot], (uint32_t)(i / G8_SLOTS & 1) ^ 1, patience);
         float* to = scale + slot * F::HALVES * NT;
 #pragma unroll
         for (int h = 0; h < F::HALVES; ++h)
@@ -222,19 +218,18 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         if (lane == 0) mbar_arrive(&scale_full[slot]);
       }
     }
+    if (patience == 0) *gave_up = 1;
   } else {
     // ===================== epilogue: lane = weight row, column = token =====================
     const int quarter = warp & 3, half = warp >> 2, col0 = half * F::NC;   // gated: the other half is the other matrix
     float acc[F::NC];
 #pragma unroll
     for (int j = 0; j < F::NC; ++j) acc[j] = 0.f;
+    long long patience = WAIT_LIMIT;
     for (int kb = kb0; kb < kb1; ++kb) {
       const int i = kb - kb0, buf = i & 1, slot = i % G8_SLOTS;
-      const bool ok = bounded_wait(&scale_full[slot], (uint32_t)(i / G8_SLOTS & 1)) && bounded_wait(&tmem_full[buf], (uint32_t)(i >> 1 & 1));
-      if (!__all_sync(0xffffffffu, ok)) {
-        if (lane == 0) *gave_up = 1;
-        break;
-      }
+      await(&scale_full[slot], (uint32_t)(i / G8_SLOTS & 1), patience);
+      await(&tmem_full[buf], (uint32_t)(i >> 1 & 1), patience);
       tc_fence_after();
       const uint32_t at = tmem + buf * F::COLS + col0 + ((uint32_t)(quarter * 32) << 16);
       const float4* sc = reinterpret_cast<const float4*>(scale + slot * F::HALVES * NT + col0);
@@ -262,16 +257,15 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       __syncwarp();
       if (lane == 0) mbar_arrive(&scale_empty[slot]);
     }
+    if (patience == 0) *gave_up = 1;
     if (S > 1) cluster_sync_all();   // every CTA's ring is done with: the sums take its place
     // Token t is the CTA's of rank t mod S: sums [CTA that they come from][matrix][token / S][weight row].  (Stores that nobody waits for: with sums kept here
     // and read from there, 64 tokens' latency was 1400 to 3900 clocks.)
-    if (!*gave_up) {
-      const uint32_t mine = smem_u32(smem) + (uint32_t)(((rank * F::HALVES + (GATED ? half : 0)) * (NT >> log_s)) * 512 + (quarter * 32 + lane) * 4);
+    const uint32_t mine = smem_u32(smem) + (uint32_t)(((rank * F::HALVES + (GATED ? half : 0)) * (NT >> log_s)) * 512 + (quarter * 32 + lane) * 4);
 #pragma unroll
-      for (int j = 0; j < F::NC; ++j) {
-        const int t = (GATED ? 0 : col0) + j;
-        if (t0 + t < a.T) st_dsmem_f32(dsmem_addr(mine + (uint32_t)(t >> log_s) * 512, t & (S - 1)), acc[j]);
-      }
+    for (int j = 0; j < F::NC; ++j) {
+      const int t = (GATED ? 0 : col0) + j;
+      if (t0 + t < a.T) st_dsmem_f32(dsmem_addr(mine + (uint32_t)(t >> log_s) * 512, t & (S - 1)), acc[j]);
     }
   }
   __syncwarp();

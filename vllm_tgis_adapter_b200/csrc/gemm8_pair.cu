@@ -29,7 +29,7 @@ constexpr int P8_EPI = 8, P8_LOAD = 8, P8_MMA = 9, P8_THREADS = 384;
 constexpr int P8_REGS = 168, P8_REGS_EPI = 232, P8_REGS_REST = 40;
 static_assert(2 * P8_REGS_EPI + P8_REGS_REST <= 3 * P8_REGS, "a split may not be more than the block was launched with");
 constexpr int P8_HALF = 128 * W8_GROUP;          // one CTA's share of a k-block of either operand
-constexpr int P8_STAGES = 6, P8_AHEAD = 2;       // k-blocks in flight; k-blocks whose scales are asked for at once
+constexpr int P8_STAGES = 6;                   // k-blocks in flight
 constexpr int P8_RING = P8_STAGES * 2 * P8_HALF;
 constexpr int P8_BARS = 256, P8_MOST = 2 * 256 * 4, P8_OUT = 2048;   // barriers; maxima of a gated tile [parity][256]; a warp's way out: 32 rows of 64 bytes
 constexpr int P8_SMEM = P8_RING + P8_BARS + P8_MOST + P8_EPI * P8_OUT + 1024;
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(P8_THREADS, 1)
 gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wmap2, const __grid_constant__ CUtensorMap xmap,
                   const __grid_constant__ Pair8Args pa) {
   constexpr int NH = 32 * CH, N_TILE = GATED ? 128 : 2 * NH;   // columns of a half; weight rows (features) of a tile
+  constexpr int AHEAD = GATED ? 2 : 4;   // k-blocks whose scales are asked for at once (registers; 2048 x 8192 x 8192 121.2 us by two, 118.9 by four, gated 2048 x 14336 x 4096 206 and 212)
   constexpr int BUFS = 512 / NH;   // accumulators of a half in TMEM, the halves in turn: 4, 5 or 8
   static_assert(!GATED || CH == 4, "");
   extern __shared__ uint8_t smem_raw[];
@@ -276,8 +277,8 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     griddep_wait();   // the scales of the rows; y may still be in use by the previous kernels
     int b = half;   // this half's next accumulator
     uint32_t phase = 0;
-    bool ok = true;
-    for (int tile = pair, turn = 0; tile < tiles && ok; tile += pairs, turn ^= 1) {
+    long long patience = WAIT_LIMIT;
+    for (int tile = pair, turn = 0; tile < tiles; tile += pairs, turn ^= 1) {
       const int n_tile = tile / pa.x_tiles, t = tile % pa.x_tiles * 256 + rank * 128 + quarter * 32 + lane;
       const int n0 = n_tile * N_TILE + half * (N_TILE / 2);   // first column (gated: feature)
       // columns [0, cut) have the scales sw, those behind them sw2
@@ -288,35 +289,35 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
       float acc[NH];
 #pragma unroll
       for (int j = 0; j < NH; ++j) acc[j] = 0.f;
-      float x[P8_AHEAD], w[P8_AHEAD], w2[P8_AHEAD];
+      float x[AHEAD] = {}, w[AHEAD] = {}, w2[AHEAD] = {};
+      const float *px = sx + (size_t)kb0 * a.lds, *pw = sw + kb0, *pw2 = sw2 + kb0;
       auto load = [&](int kb) {
 #pragma unroll
-        for (int u = 0; u < P8_AHEAD; ++u) {
-          const int k = kb0 + min(kb + u, KB - 1);
-          x[u] = sx[(size_t)k * a.lds];
-          w[u] = sw[k];
-          w2[u] = sw2[k];
-        }
+        for (int u = 0; u < AHEAD; ++u)
+          if (kb + u < KB) {
+            x[u] = *px;
+            w[u] = *pw++;
+            w2[u] = *pw2++;
+            px += a.lds;
+          }
       };
       load(0);
       // One chunk of columns is added while the next one is on its way out of TMEM, across k-blocks too.
       uint32_t r[2][32];
-      ok = warp_wait(&tmem_full[b], phase);
-      if (ok) {
-        tc_fence_after();
-        tmem_ld<32>(from + b * NH, r[0]);
-      }
-      for (int at = 0; at < KB && ok; at += P8_AHEAD) {
-        float f[P8_AHEAD], f2[P8_AHEAD];
+      await(&tmem_full[b], phase, patience);
+      tc_fence_after();
+      tmem_ld<32>(from + b * NH, r[0]);
+      for (int at = 0; at < KB; at += AHEAD) {
+        float f[AHEAD], f2[AHEAD];
 #pragma unroll
-        for (int u = 0; u < P8_AHEAD; ++u) {
+        for (int u = 0; u < AHEAD; ++u) {
           f[u] = x[u] * w[u];
           f2[u] = x[u] * w2[u];
         }
-        if (at + P8_AHEAD < KB) load(at + P8_AHEAD);
+        if (at + AHEAD < KB) load(at + AHEAD);
 #pragma unroll
-        for (int u = 0; u < P8_AHEAD; ++u) {
-          if (at + u >= KB || !ok) break;
+        for (int u = 0; u < AHEAD; ++u) {
+          if (at + u >= KB) break;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             uint32_t* now = r[(u * CH + c) & 1];
@@ -331,7 +332,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
               b += 2;
               if (b >= BUFS) b -= BUFS, phase ^= 1;
               if (at + u + 1 < KB) {
-                ok = warp_wait(&tmem_full[b], phase);
+                await(&tmem_full[b], phase, patience);
                 tc_fence_after();
                 tmem_ld<32>(from + b * NH, next);
               }
@@ -344,11 +345,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
           }
         }
       }
-      static_assert(P8_AHEAD * CH % 2 == 0, "r[0] is the first chunk's in every turn");
-      if (!ok) {
-        if (lane == 0) *gave_up = 1;
-        break;
-      }
+      static_assert(AHEAD * CH % 2 == 0, "r[0] is the first chunk's in every turn");
       if constexpr (S == 1) {
         finish<NH, GATED, OT>(a, acc, t, n0, n_tile, half, quarter * 32 + lane, most + turn * 256, 2, way, lane, 1 + quarter, 64);
       } else {
@@ -359,6 +356,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
         for (int j = 0; j < NH; j += 4) sums[j / 4 * 128] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
       }
     }
+    if (patience == 0) *gave_up = 1;
     meet();
     if constexpr (S > 1) {
       // a warp: 32 of the CTA's 128 / S tokens and a 2 S-th of the columns
