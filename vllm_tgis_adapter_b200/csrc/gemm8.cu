@@ -1,7 +1,7 @@
 // y[t, n] = sum_g sx[t, g] sw[n / 128, g] sum_{k in g} cx[t, k] cw[n, k]: 8-bit weights (include/tgis_w8.h) times rows in 8 bits, and the gated
 // form h = silu(x gate^T) * (x up^T), which leaves as rows in 8 bits.
 //
-// Up to 128 tokens (gemm8_pair.cu has more).  A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and all tokens (B, a column
+// Up to 128 tokens, gated up to 64 (gemm8_pair.cu has more).  A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and all tokens (B, a column
 // each): such a product is bound by its weight bytes, which are read once.  The tensor cores (tcgen05 kind::f8f6f4) sum one group of 128 k, that is
 // one k-block, in an accumulator; the epilogue's threads take it over, times both scales, into fp32 registers while the next one is summed in the
 // other half of the CTA's TMEM.  A tile's weights have one scale a k-block and a column has one, so a warp of its own puts their product where the
@@ -9,7 +9,7 @@
 // added there in the order of k, so that a result is the same in every call, without a workspace.
 //
 // Measured on one B200, us (weight bytes a second), T x N x K, launches one behind the other with cold weights: 1 x 4096 x 4096 6.4 (2.6 TB/s), 1 x 8192 x 8192 13.6
-// (4.9), 32 x 4096 x 14336 14.0 (4.3), 64 x 8192 x 8192 16.7 (4.1), 128 x 4096 x 14336 20 (3.0); gated 1 x 14336 x 4096 22.6 (5.2), 48: 25.1, 128: 40.  What bounds it: of
+// (4.9), 32 x 4096 x 14336 14.0 (4.3), 64 x 8192 x 8192 16.7 (4.1), 128 x 4096 x 14336 20 (3.0); gated 1 x 14336 x 4096 22.6 (5.2), 48: 25.3.  What bounds it: of
 // 4096 x 4096 a launch's beginning (0.6 us), the first bytes' way (2.5, of which the bytes themselves are most) and the cluster's end (two
 // barriers and the sums, 2 to 3); large ones the memory, short of a copy's 6.5 TB/s by those 4 us.
 //
@@ -84,7 +84,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 
   const int warp = threadIdx.x >> 5, lane = (int)lane_id();
   const int rank = (int)cluster_ctarank(), S = (int)gridDim.z, log_s = __ffs(S) - 1;   // cluster: the CTAs of blockIdx.z, one, two, four or eight
-  const int nb = (int)blockIdx.x, t0 = (int)blockIdx.y * NT;
+  const int nb = (int)blockIdx.x;
   const int kb0 = (int)((long long)rank * a.G / S), kb1 = (int)((long long)(rank + 1) * a.G / S);
 
   if (warp == G8_LOAD && elect_one()) {
@@ -128,7 +128,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         tma_load_2d_hint(&wmap, &full[s], smem + s * F::STAGE, kb * W8_GROUP, nb * 128, once);
         if (GATED) tma_load_2d_hint(&wmap2, &full[s], smem + s * F::STAGE + G8_W_BYTES, kb * W8_GROUP, nb * 128, once);
       };
-      auto load_x = [&](int s, int kb) { tma_load_2d(&xmap, &full[s], smem + s * F::STAGE + G8_W_BYTES * F::HALVES, kb * W8_GROUP, t0); };
+      auto load_x = [&](int s, int kb) { tma_load_2d(&xmap, &full[s], smem + s * F::STAGE + G8_W_BYTES * F::HALVES, kb * W8_GROUP, 0); };
       const int pre = min(kb1 - kb0, F::STAGES);
       if (!a.early) griddep_wait();
       for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
@@ -179,7 +179,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
     const float* sw = a.sw + (size_t)nb * a.G;
     const float* sw2 = GATED ? a.sw2 + (size_t)nb * a.G : nullptr;
     // (AHEAD k-blocks at a time, asked for while those before them are handed out: one at a time took the L2's latency for each)
-    constexpr int EACH = (NT + 31) / 32, AHEAD = NT > 128 ? 4 : 8;
+    constexpr int EACH = (NT + 31) / 32, AHEAD = 8;
     float x[AHEAD][EACH], w[AHEAD], w2[AHEAD];
     auto load = [&](int from) {
 #pragma unroll
@@ -188,7 +188,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
         w[u] = sw[kb];
         w2[u] = GATED ? sw2[kb] : 0.f;
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) x[u][j] = j * 32 + lane < NT && t0 + j * 32 + lane < a.T ? a.sx[(size_t)kb * a.lds + t0 + j * 32 + lane] : 0.f;
+        for (int j = 0; j < EACH; ++j) x[u][j] = j * 32 + lane < NT && j * 32 + lane < a.T ? a.sx[(size_t)kb * a.lds + j * 32 + lane] : 0.f;
       }
     };
     load(kb0);
@@ -265,7 +265,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 #pragma unroll
     for (int j = 0; j < F::NC; ++j) {
       const int t = (GATED ? 0 : col0) + j;
-      if (t0 + t < a.T) st_dsmem_f32(dsmem_addr(mine + (uint32_t)(t >> log_s) * 512, t & (S - 1)), acc[j]);
+      if (t < a.T) st_dsmem_f32(dsmem_addr(mine + (uint32_t)(t >> log_s) * 512, t & (S - 1)), acc[j]);
     }
   }
   __syncwarp();
@@ -284,7 +284,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   }
   // ===================== the cluster's sums -> y or h: a warp a token, four weight rows a lane =====================
   griddep_wait();
-  for (int i = warp, t; t = (i << log_s) + rank, t < NT && t0 + t < a.T; i += G8_WARPS) {
+  for (int i = warp, t; t = (i << log_s) + rank, t < NT && t < a.T; i += G8_WARPS) {
     float v[F::HALVES][4] = {};
     for (int r = 0; r < S; ++r)
 #pragma unroll
@@ -303,10 +303,10 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
       }
       const float s = scale_of(__reduce_max_sync(0xffffffffu, m));
       codes_near(h, s, c);
-      *reinterpret_cast<uint32_t*>(a.codes + (size_t)(t0 + t) * a.ldc + n) = c[0];
-      if (lane == 0) a.sh[(size_t)nb * a.ldh + t0 + t] = s;
+      *reinterpret_cast<uint32_t*>(a.codes + (size_t)t * a.ldc + n) = c[0];
+      if (lane == 0) a.sh[(size_t)nb * a.ldh + t] = s;
     } else {
-      OT* y = reinterpret_cast<OT*>(a.y) + (size_t)(t0 + t) * a.ldy + n;
+      OT* y = reinterpret_cast<OT*>(a.y) + (size_t)t * a.ldy + n;
       constexpr int ALIGN = 4 * (int)sizeof(OT);
       if (n + 4 <= a.N && (reinterpret_cast<uintptr_t>(y) & (ALIGN - 1)) == 0) {
         if constexpr (sizeof(OT) == 4) {
@@ -330,8 +330,7 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
   static OncePerDevice once;
   cudaError_t e = once([] { return cudaFuncSetAttribute(gemm8_kernel<NT, GATED, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
   if (e != cudaSuccess) return e;
-  const int tiles = (a.N + 127) / 128, x_tiles = (a.T + NT - 1) / NT;
-  if (x_tiles > 65535) return cudaErrorInvalidValue;
+  const int tiles = (a.N + 127) / 128;
   // The pieces of k whose waves take the fewest k-blocks: a wave's beginning and end take about G8_ENDS of them.  (A tenth of a wave too many costs less than
   // a wave, for the memory is what all wait for: 32 x 4096 x 14336 in 32 clusters of eight where 30 run at once 14.4 us, of four 15.5, of two 20.7)
   static ClustersAtOnce at_once;
@@ -340,12 +339,12 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
   for (int s = 1; s <= 8 && s * 2 <= std::max(a.G, 2); s *= 2) {
     int n = 0;
     if ((e = at_once(gemm8_kernel<NT, GATED, OT>, G8_THREADS, F::SMEM, s, &n)) != cudaSuccess) return e;
-    const float waves = (float)tiles * (float)x_tiles / (float)(n * F::CTAS);   // (the answer is for one CTA an SM)
+    const float waves = (float)tiles / (float)(n * F::CTAS);   // (the answer is for one CTA an SM)
     const float cost = std::max(std::ceil(waves - 0.1f), 1.f) * (float)((a.G + s - 1) / s + G8_ENDS);
     if (least < 0.f || cost < least) S = s, least = cost;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles, (unsigned)x_tiles, (unsigned)S);
+  cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)S);
   cfg.blockDim = dim3(G8_THREADS);
   cfg.dynamicSmemBytes = F::SMEM;
   cfg.stream = stream;
@@ -372,7 +371,9 @@ cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgi
     case 16: return launch8<16, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
     case 32: return launch8<32, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
     case 64: return launch8<64, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
-    default: return launch8<128, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
+    default:
+      if constexpr (GATED) return cudaErrorInvalidValue;   // (gemm8_pair_takes)
+      else return launch8<128, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
   }
 }
 
@@ -385,7 +386,7 @@ cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y
   a.sx = x.scales; a.lds = x.lds; a.sw = w.scales;
   a.T = x.t; a.N = w.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
   a.y = y; a.ldy = ldy; a.status = call.status; a.stalled = call.stalled; a.early = call.early;
-  if (gemm8_pair_takes(a.T)) return gemm8_pair_launch(x, w, a, f32, num_sms, stream);
+  if (gemm8_pair_takes(a.T, a.G, false)) return gemm8_pair_launch(x, w, a, f32, num_sms, stream);
   CUtensorMap wm;
   cudaError_t e = map8(&wm, w.codes, w.n, w.k, w.ld, 128);
   if (e != cudaSuccess) return e;
@@ -400,7 +401,7 @@ cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate
   a.T = x.t; a.N = gate.n; a.K = x.k; a.G = (x.k + W8_GROUP - 1) / W8_GROUP;
   a.codes = (uint8_t*)out.codes; a.ldc = out.ld; a.sh = out.scales; a.ldh = out.lds;
   a.status = call.status; a.stalled = call.stalled; a.early = call.early;
-  if (gemm8_pair_takes(a.T)) return gemm8_pair_gated_launch(x, gate, up, a, num_sms, stream);
+  if (gemm8_pair_takes(a.T, a.G, true)) return gemm8_pair_gated_launch(x, gate, up, a, num_sms, stream);
   CUtensorMap wm, wm2;
   cudaError_t e = map8(&wm, gate.codes, gate.n, gate.k, gate.ld, 128);
   if (e == cudaSuccess) e = map8(&wm2, up.codes, up.n, up.k, up.ld, 128);
@@ -422,7 +423,7 @@ int fail(const char* form, ...) {
 }
 int done(cudaError_t e, const char* what) { return e == cudaSuccess ? 0 : fail("%s: %s", what, cudaGetErrorString(e)); }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-constexpr int MAX_ROWS = 1 << 22;   // (65535 tiles of a gated product's 128)
+constexpr int MAX_ROWS = 1 << 22;
 
 int check_size(const char* name, int64_t rows, int64_t k) {
   if (rows < 0 || rows > MAX_ROWS) return fail("%s: %lld rows are not in 0 .. %d", name, (long long)rows, MAX_ROWS);

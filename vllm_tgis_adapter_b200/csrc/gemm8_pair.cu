@@ -6,12 +6,11 @@
 // that adds them up.  A k-block is one group of 128.  Each half of the columns is an MMA, an accumulator and a set of four warps of its own, so that one
 // half's sums are taken while the tensor cores make the other's, and accumulators go round through all of TMEM.
 //
-// Measured on one B200, T x N x K: 2048 x 8192 x 8192 130 us (2110 TFLOP/s), 2048 x 4096 x 14336 113 (2140), 512 x 8192 x 8192 35 (1950), 256 x 4096 x 4096 12.2; gated 2048 x 14336 x
-// 4096 215 (2240).  (Back to back for a second, at the power limit's clock: 157 for the first.)  What bounds it: a k-block of 256 x 256 takes some 820 clocks where
-// the tensor cores need 512: the epilogue's chain of barrier, TMEM loads and 64 multiply-adds of pairs a thread (305 clocks of the SM's fp32 lanes).
-// Without the multiply-adds a k-block takes 680 clocks, without the loads as well 600.  What mattered: arrivals that wait for no memory (mbar_arrive_tmem: 311 -> 172 us),
-// 32 columns a load instead of 16 (172 -> 146), a chunk on its way while one is added (-> 141), results through shared memory (-> 130).
-// Against gemm8.cu, us: 128 tokens x 4096 x 14336 24.7 and 20.3, 200: 25.6 and 32.0; x 8192 x 8192 128: 22.9 and 22.2, 200: 23.4 and 35.1.
+// Measured on one B200, T x N x K: 2048 x 8192 x 8192 118 us (2330 TFLOP/s), 2048 x 6144 x 4096 47 (2170), 512 x 8192 x 8192 32.5 (2110), 256 x 4096 x 4096 12.5; gated 2048 x 14336 x
+// 4096 208 (2310).  What bounds it: a k-block of 256 x 256 takes some 740 clocks where the tensor cores need 512 and their operands' way through shared memory (A is read for
+// each half) 640: the epilogue's chain of barrier, TMEM loads and 64 multiply-adds of pairs a thread (305 clocks of the SM's fp32 lanes).  Back to back for a second it is the
+// power limit.  What mattered for the first: arrivals that wait for no memory (mbar_arrive_tmem: 311 -> 172 us), 32 columns a load instead of 16 (-> 146), a chunk on
+// its way while one is added (-> 141), results through shared memory (-> 130), waits without a vote (-> 122), scales four k-blocks ahead by pointers that move (-> 118).
 //
 // Roles per CTA: warps 0..7 epilogue (two a lane quarter, half of the columns each), warp 8 TMA producer, warp 9 MMA issuer (leader CTA only) and
 // TMEM owner.  The leader's `full` barrier counts both CTAs' bytes; tcgen05.commit releases a ring slot in both.  Waits on barriers in shared
@@ -398,10 +397,10 @@ cudaError_t launch_pair8(const CUtensorMap& w, const CUtensorMap& w2, const CUte
 }
 
 // Chunks of a half and pieces of k: those whose waves take least, in hundredths of a microsecond.  A k-block of 256 x 64 CH takes P8_BLOCK[CH] while it is the
-// epilogue's chain that bounds it, a launch's beginning and end P8_ENDS[pieces]; pieces are for one wave.  Measured (us; taken first): 256 x 4096 x 4096 CH 2, S 2: 12.1;
-// CH 4, S 1: 19.4; CH 2, S 1: 13.8; CH 4, S 2: 14.8.  512 x 6144 x 4096 CH 3: 18.1, CH 4: 20.3, CH 2: 24.7.  301 x 2128 x 11264 CH 4, S 2: 25.5, CH 4, S 1: 43.1, CH 2, S 1: 31.4.
-// 1024 x 512 x 8192 CH 4, S 4: 15.6 (CH 2, S 2: 15.6), CH 2, S 1: 23.3.  203 x 512 x 1536 CH 2, S 1: 7.1, CH 4, S 4: 9.1.  2048 x 8192 x 8192 CH 4: 130, CH 3: 144, CH 2: 162.
-constexpr int P8_BLOCK[5] = {0, 0, 30, 38, 43}, P8_ENDS[5] = {0, 400, 600, 0, 870};
+// epilogue's chain that bounds it, a launch's beginning and end P8_ENDS[S] and P8_WIDE[S] more for every chunk above two; pieces are for one wave.  Measured (us; taken first):
+// 256 x 4096 x 4096 CH 2, S 2: 12.6; CH 2, S 1: 13.6; CH 4, S 2: 14.6; CH 4, S 1: 16.6.  512 x 6144 x 4096 CH 3: 17.0, CH 4: 18.3, CH 2: 24.4.  301 x 2128 x 11264 CH 4, S 2: 25.5, CH 2, S 1: 30.2,
+// CH 4, S 1: 35.3.  1024 x 512 x 8192 CH 4, S 4: 15.5, CH 2, S 2: 15.2, S 1: 22.2.  203 x 512 x 1536 CH 2, S 1: 6.8, S 2: 7.0, CH 4, S 4: 8.9.  2048 x 8192 x 8192 CH 4: 118, CH 3: 131, CH 2: 154.
+constexpr int P8_BLOCK[5] = {0, 0, 30, 33, 36}, P8_ENDS[5] = {0, 400, 600, 0, 700}, P8_WIDE[5] = {0, 50, 100, 0, 100};
 struct Plan { int ch, s; };
 template <class OT>
 cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
@@ -416,7 +415,7 @@ cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
       const int rows = gated ? 128 : 64 * c;
       const long long tiles = (long long)((N + rows - 1) / rows) * x_tiles, waves = (tiles + n - 1) / n;
       if (s > 1 && waves > 1) continue;
-      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS[s];
+      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS[s] + P8_WIDE[s] * (c - 2);
       if (least < 0 || cost < least) *out = Plan{c, s}, least = cost;
     }
   }
@@ -445,7 +444,9 @@ cudaError_t product_pair8(const tgis_w8_rows& x, const tgis_w8_matrix& w, const 
 
 }  // namespace
 
-bool gemm8_pair_takes(int T) { return T > 128; }
+// More than 128 tokens; from 65 on gated ones (us, gemm8.cu and here: 65 tokens, 4096 / 14336 38.5 and 33.5, 512 / 1536 9.4 and 6.0; 64 tokens 26.5 and 33) and those of few
+// k-blocks, whose end is what counts (65 x 512 x 512 6.4 and 4.1, but 65 x 2128 x 2048 7.8 and 9.2, 128 x 4096 x 14336 20.3 and 24.4; 200: 32.0 and 25.6).
+bool gemm8_pair_takes(int T, int G, bool gated) { return T > 128 || (T > 64 && (gated || G <= 8)); }
 
 cudaError_t gemm8_pair_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, const Gemm8Args& g, bool f32, int num_sms, cudaStream_t stream) {
   return f32 ? product_pair8<float>(x, w, g, num_sms, stream) : product_pair8<__nv_bfloat16>(x, w, g, num_sms, stream);

@@ -158,7 +158,7 @@ cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate
                                const Gemm8Call& call, int num_sms, cudaStream_t stream);
 
 // ---- gemm8_pair.cu: prompts
-bool gemm8_pair_takes(int T);
+bool gemm8_pair_takes(int T, int G, bool gated);
 cudaError_t gemm8_pair_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, const Gemm8Args& g, bool f32, int num_sms, cudaStream_t stream);
 cudaError_t gemm8_pair_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const Gemm8Args& g, int num_sms,
                                     cudaStream_t stream);
