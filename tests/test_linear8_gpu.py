@@ -473,3 +473,46 @@ def test_threads_call_at_once(lib):
     for th in threads:
         th.join()
     assert not bad
+
+
+# 65 to 128 tokens and more than eight k-blocks: the widest form of the kernel that has the weights on its rows
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,n,k", [(65, 1, 1025), (65, 129, 1100), (96, 300, 2048), (100, 77, 1200), (127, 2128, 4096), (128, 128, 1152), (128, 513, 20001), (128, 6144, 4096), (72, 40, 131072)])
+def test_product_of_a_wide_batch(lib, t, n, k, dtype):
+    x, w = checks.case(t, n, k, t + n + k)
+    rows, layer = lib.quantise(x), lib.Linear8.from_weight(w)
+    out = torch.full((t + 2, n + 5), 7.0, device="cuda", dtype=dtype)
+    y = layer(rows, out=out[1 : t + 1, 2 : n + 2])
+    want, off = checks.product(rows, layer)
+    checks.assert_near(y, want, off, dtype)
+    assert torch.equal(bits(layer(rows, dtype=dtype).contiguous()), bits(y.contiguous()))
+    out[1 : t + 1, 2 : n + 2] = 7.0
+    assert (out == 7.0).all()
+
+
+def test_what_is_not_finite_in_a_wide_batch(lib):
+    x, w = checks.case(100, 300, 2000, 5)
+    x[3, 700], x[41, 0], x[99, 1999], w[140, 1500] = float("nan"), float("inf"), float("-inf"), float("nan")
+    y = lib.Linear8.from_weight(w)(lib.quantise(x))
+    gone = torch.zeros(100, 300, dtype=torch.bool, device="cuda")
+    gone[[3, 41, 99]] = True
+    gone[:, 128:256] = True
+    assert torch.equal(y.isnan(), gone) and y[~gone].isfinite().all()
+
+
+def test_rows_of_a_wide_batch_do_not_depend_on_their_neighbours(lib):
+    x, w = checks.case(120, 640, 4096, 9)
+    layer = lib.Linear8.from_weight(w)
+    y = layer(lib.quantise(x))
+    x[:60] = 3.0
+    assert torch.equal(layer(lib.quantise(x))[60:], y[60:])
+
+
+# as many rows as run at once, one more, and those around the sizes where a row's CTA grows
+@pytest.mark.parametrize("t", [147, 149, 295, 297, 591, 593])
+@pytest.mark.parametrize("k", [1024, 1040, 2048, 2056, 4096])
+def test_rows_around_full_waves(lib, t, k):
+    x, _ = checks.case(t, 1, k, t + k)
+    rows = lib.quantise(x)
+    codes, scales = checks.groups_of(x.float(), 1)
+    same_groups(rows.codes, rows.scales, codes, scales.t())
