@@ -4,7 +4,7 @@
 // its codes are eight bytes a lane.  With a norm the factor 1 / rms is the same for a whole row, so the codes are those of r * norm
 // and only the scales wait for the row's sum of squares: nothing is read twice or held.
 //
-// Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.1 us.  What bounds the
+// Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.0 us.  What bounds the
 // former: two rounds of a row's loads a CTA with their latency, three waves of CTAs.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
 // copy's rate), from bf16 143 (4.9 TB/s: the arithmetic of a number is the same).
 #include "launch.cuh"
@@ -212,8 +212,9 @@ bool on16(const void* p, int64_t ld, int size) { return (reinterpret_cast<uintpt
 template <class X, bool VEC, bool NORM>
 cudaError_t rows8_some(const Rows8Args& a, int num_sms, cudaStream_t stream) {
   const int G = (a.K + W8_GROUP - 1) / W8_GROUP;
-  // Two groups a warp: few rows want all of theirs at once, many rows small CTAs
-  const int warps = G <= 8 ? 4 : G <= 16 || a.T > 4 * num_sms ? 8 : 16;
+  // Few rows want all of theirs asked for at once, more rows CTAs of which more run at a time.  Measured with norm and residual, 16 and 8 warps, us: 1 x 4096 2.0 / 2.1,
+  // 148 x 4096 3.0 / 3.3, 200 x 4096 4.9 / 4.8, 592 x 4096 9.8 / 6.0, 2048 x 4096 30.7 / 13.3; 148 x 8192 4.1 / 5.1, 296 x 8192 7.4 / 8.3, 300 x 8192 9.1 / 8.4.
+  const int warps = G <= 8 ? 4 : G <= 16 || a.T > (G <= 32 ? 1 : 2) * num_sms ? 8 : 16;
   auto go = [&](auto kernel) { return launch_k(kernel, dim3((unsigned)a.T), dim3((unsigned)warps * 32), NORM ? (size_t)G * sizeof(float) : 0, stream, a); };
   return warps == 4 ? go(rows8_kernel<X, VEC, NORM, 4>) : warps == 8 ? go(rows8_kernel<X, VEC, NORM, 8>) : go(rows8_kernel<X, VEC, NORM, 16>);
 }
