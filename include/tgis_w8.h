@@ -11,7 +11,8 @@
  * Conventions: every pointer inside the records and every other one is device memory of the current device, the records themselves are
  * host memory and read before the call returns; `stream` is a cudaStream_t.  Calls return after the launch: 0, or < 0 with
  * tgis_w8_last_error() (per thread) and nothing launched.  They may be captured into CUDA graphs and keep no workspace: calls may run at
- * the same time.  Inputs and outputs do not overlap but for the residual, which may be updated in place.
+ * the same time.  Inputs and outputs do not overlap but for residual_out, which may be the residual or x.  A result is the same in every call; its
+ * last bits depend on the call's sizes (which kernel, how many pieces of k), never on the other rows.
  * *status (int32, may be NULL) collects TGIS_W8_* bits.
  */
 #ifndef TGIS_W8_H_
@@ -45,7 +46,7 @@ typedef struct {
 
 /* Rows of x [t, ldx] (TGIS_W8_BF16 or _F32) in 8 bits; t, k are the record's, its ld no less than k rounded up to 128 (the rest of a row's last
  * group is zeroed).  residual (may be NULL; type of x): r = x + residual, rounded to the type and stored at residual_out (may be residual
- * itself), takes x's place.  norm [k] (bf16, may be NULL): the row is v = r * norm / sqrt(mean r^2 + eps): the codes are those of r * norm and
+ * or x itself), takes x's place.  norm [k] (bf16, may be NULL): the row is v = r * norm / sqrt(mean r^2 + eps): the codes are those of r * norm and
  * its groups' scales are multiplied by the root's reciprocal, both in fp32. */
 int tgis_w8_quantise_rows(const void* x, int32_t type, int64_t ldx, const void* norm, float eps, const void* residual, int64_t ldr,
                           void* residual_out, int64_t ldro, const tgis_w8_rows* out, void* stream);

@@ -101,6 +101,14 @@ def test_products_refuse(lib):
     refused(lib, lib.tgis_w8_feed_forward(at(r), at(m), at(m), at(down), at(h), None, 0, 64, None, None), "y:")
 
 
+@pytest.mark.parametrize("change", [dict(), dict(scales=AT + 4096), dict(codes=AT + 4096)])
+def test_rows_do_not_take_the_place_of_those_they_are_made_of(lib, change):
+    at = C.addressof
+    r, m, h, down = rows(), matrix(), rows(k=130, **change), matrix(n=64, k=130)
+    refused(lib, lib.tgis_w8_gated(at(r), at(m), at(m), at(h), None, None), "out: x itself")
+    refused(lib, lib.tgis_w8_feed_forward(at(r), at(m), at(m), at(down), at(h), AT, 0, 64, None, None), "hidden: x itself")
+
+
 def test_nothing_to_do_is_no_error(lib):
     at, r, m = C.addressof, rows(t=0, codes=None), matrix()
     assert lib.tgis_w8_quantise_rows(None, 0, 0, None, 0.0, None, 0, None, 0, at(r), None) == 0

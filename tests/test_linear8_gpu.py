@@ -516,3 +516,26 @@ def test_rows_around_full_waves(lib, t, k):
     rows = lib.quantise(x)
     codes, scales = checks.groups_of(x.float(), 1)
     same_groups(rows.codes, rows.scales, codes, scales.t())
+
+
+def test_hidden_rows_do_not_take_the_place_of_x(lib):
+    ff = block(lib, 5, 256, 256, 1)[1]
+    rows = lib.quantise(checks.case(5, 1, 256, 3)[0])
+    keep = rows.codes.view(torch.uint8).clone()
+    with pytest.raises(ValueError, match="x itself"):
+        ff.hidden(rows, out=rows)
+    assert torch.equal(rows.codes.view(torch.uint8), keep)
+
+
+@pytest.mark.parametrize("t,k,norm", [(1, 4096, True), (300, 1000, False), (600, 77, True), (200, 2304, True)])
+def test_the_sum_takes_the_place_of_x_or_of_both(lib, t, k, norm):
+    w = torch.rand(k, device="cuda").to(torch.bfloat16) + 0.5 if norm else None
+    x, other = checks.case(t, 1, k, 1)[0], checks.case(t, 1, k, 2)[0]
+    r = (x.float() + other.float()).to(x.dtype)
+    want = lib.quantise(r.clone(), norm=w)
+    rows = lib.quantise(x, norm=w, residual=other, residual_out=x)
+    assert torch.equal(x, r) and torch.equal(rows.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(rows.scales, want.scales)
+    twice = (other.float() * 2).to(x.dtype)
+    want = lib.quantise(twice.clone(), norm=w)
+    rows = lib.quantise(other, norm=w, residual=other)
+    assert torch.equal(other, twice) and torch.equal(rows.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(rows.scales, want.scales)

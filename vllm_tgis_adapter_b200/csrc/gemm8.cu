@@ -449,6 +449,10 @@ int check_rows(const char* name, const tgis_w8_rows* x, bool made) {
   if (x->lds < x->t) return fail("%s: scales of %lld rows where %d are", name, (long long)x->lds, x->t);
   return check_codes(name, x->codes, x->scales, x->ld, made ? (x->k + 127ll) / 128 * 128 : x->k);
 }
+// (a CTA's features are written while others still read all of x)
+int check_apart(const char* name, const tgis_w8_rows& x, const tgis_w8_rows& out) {
+  return x.codes == out.codes || x.scales == out.scales ? fail("%s: x itself is not wanted", name) : 0;
+}
 int check_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out) {
   if (check_rows("x", x, false) != 0 || check_matrix("gate", gate, false) != 0 || check_matrix("up", up, false) != 0 || check_rows("out", out, true) != 0) return -1;
   if (x->k != gate->k || x->k != up->k || gate->n != up->n) return fail("x has rows of %d numbers, gate is %d x %d, up %d x %d", x->k, gate->n, gate->k, up->n, up->k);
@@ -506,6 +510,7 @@ int tgis_w8_product(const tgis_w8_rows* x, const tgis_w8_matrix* w, void* y, int
 int tgis_w8_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out, int32_t* status, void* stream) {
   if (check_gated(x, gate, up, out) != 0) return -1;
   if (x->t == 0) return 0;
+  if (check_apart("out", *x, *out) != 0) return -1;
   int sms = 0;
   if (sms_of_device(&sms) != 0) return -1;
   return done(tgis::gemm8_gated_launch(*x, *gate, *up, *out, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_gated");
@@ -516,7 +521,7 @@ int tgis_w8_feed_forward(const tgis_w8_rows* x, const tgis_w8_matrix* gate, cons
   if (check_type(type) != 0 || check_gated(x, gate, up, hidden) != 0 || check_matrix("down", down, false) != 0) return -1;
   if (hidden->k != down->k) return fail("hidden has rows of %d numbers, down of %d", hidden->k, down->k);
   if (x->t == 0) return 0;
-  if (check_plain("y", y, type, ldy, down->n) != 0) return -1;
+  if (check_plain("y", y, type, ldy, down->n) != 0 || check_apart("hidden", *x, *hidden) != 0) return -1;
   int sms = 0;
   if (sms_of_device(&sms) != 0) return -1;
   const int rc = done(tgis::gemm8_gated_launch(*x, *gate, *up, *hidden, tgis::Gemm8Call{status}, sms, (cudaStream_t)stream), "tgis_w8_feed_forward");

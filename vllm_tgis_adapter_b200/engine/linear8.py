@@ -7,8 +7,8 @@
     y = FeedForward8(gate, up, down)(rows)            # silu(gate x) * (up x) in 8-bit rows, then the down projection
 
 `Linear8(codes, scales)` takes a checkpoint's block-scaled matrix as it is.  Calls go to the current stream of their tensors' device and return
-after the launch; they may be captured into CUDA graphs and, having no workspace, run at the same time.  Arguments that the host
-can check raise ValueError.
+after the launch; they may be captured into CUDA graphs and, having no workspace, run at the same time.  Results do not take the place of what they are
+made of, the residual's sum excepted.  Arguments that the host can check raise ValueError.
 """
 from __future__ import annotations
 
@@ -118,7 +118,7 @@ class Rows8:
 def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-5, residual: torch.Tensor | None = None,
              residual_out: torch.Tensor | None = None, out: Rows8 | None = None) -> Rows8:
     """Rows of x [T, k] (bf16 or fp32) in 8 bits.  `residual` (like x): x + residual, rounded to their type, takes the place of x and is stored in
-    `residual_out` (None: residual itself).  `norm` (bf16 [k]): the RMS norm's weight, v = r * norm / sqrt(mean r^2 + eps)."""
+    `residual_out` (None: residual itself; x will do).  `norm` (bf16 [k]): the RMS norm's weight, v = r * norm / sqrt(mean r^2 + eps)."""
     ld = _pitch("x", x)
     device, dtype, shape = x.device, x.dtype, x.shape
     T, k = shape
