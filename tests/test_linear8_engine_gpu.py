@@ -187,3 +187,24 @@ def test_scores_of_prompts_and_sampling_run():
     assert len([r for r in sampled if r.new_token is not None]) == 12
     assert eng.status().errored == 0
     eng.close()
+
+
+def test_profiling_counts_the_products():
+    """Four a layer and the head's, as over 16-bit weights, and of the projections' bytes about half."""
+    from vllm_tgis_adapter_b200.engine.core import make_sampling_params
+
+    cfg = CONFIGS["small"]
+    weights = synthetic_weights(cfg, seed=1)
+    prompt = np.random.RandomState(5).randint(3, cfg.vocab, size=40).tolist()
+    calls, moved = {}, {}
+    for quantization in (None, "fp8"):
+        eng = engine("small", weights, quantization=quantization)
+        eng.set_profiling(1)
+        eng.generate_sync([prompt], make_sampling_params(greedy=True, max_tokens=6, min_tokens=6, eos_token_id=2))
+        eng.set_profiling(False)
+        st = eng.status()
+        calls[quantization], moved[quantization] = st.gemm_calls / st.steps, st.gemm_bytes
+        assert st.errored == 0 and st.gemm_ms > 0
+        eng.close()
+    assert calls["fp8"] == calls[None] == 4 * cfg.n_layers + 1
+    assert moved["fp8"] < moved[None]

@@ -496,8 +496,8 @@ struct tgis_engine {
   std::vector<double> prof_bytes;  // algorithmic bytes of the GEMM between events 2i and 2i+1 (< 0: an exchange)
   double gemm_ms = 0, gemm_bytes = 0, exchange_ms = 0;
   long long gemm_calls = 0, exchange_calls = 0;
-  // event pair around an exchange (profiling only)
-  cudaEvent_t prof_begin_exchange() {
+  // event pair around a GEMM of so many algorithmic bytes (profiling only): the first is recorded, the second the caller's
+  cudaEvent_t prof_begin(double bytes) {
     if (!(profiling && (!prof_decode_only || step_is_decode))) return nullptr;
     while (prof_events.size() < prof_used + 2) {
       cudaEvent_t ev;
@@ -507,9 +507,10 @@ struct tgis_engine {
     cudaEvent_t e1 = prof_events[prof_used + 1];
     CK(cudaEventRecord(prof_events[prof_used], stream));
     prof_used += 2;
-    prof_bytes.push_back(-1.0);
+    prof_bytes.push_back(bytes);
     return e1;
   }
+  cudaEvent_t prof_begin_exchange() { return prof_begin(-1.0); }
   // CUDA graphs of pure-decode steps, keyed by (batch size, number of KV splits)
   std::unordered_map<uint64_t, cudaGraphExec_t> graphs;
   std::unordered_map<uint64_t, long long> graph_nodes;
@@ -3261,20 +3262,8 @@ struct tgis_engine {
             int out_f32 = 0, const CUtensorMap* next_wm = nullptr, int nT = 0, int nN = 0, int nK = 0, int ldy = 0,
             const GemmRope* rope = nullptr, const GemmNorm* norm = nullptr, bool late = false) {
     if (ldy == 0) ldy = N;
-    cudaEvent_t pe0 = nullptr, pe1 = nullptr;
-    if (profiling && (!prof_decode_only || step_is_decode)) {
-      while (prof_events.size() < prof_used + 2) {
-        cudaEvent_t ev;
-        CK(cudaEventCreate(&ev));
-        prof_events.push_back(ev);
-      }
-      pe0 = prof_events[prof_used];
-      pe1 = prof_events[prof_used + 1];
-      prof_used += 2;
-      // algorithmic bytes: weights once + activations in + result out
-      prof_bytes.push_back((double)N * K * 2 + (double)T * K * 2 + (double)T * N * (out_f32 == 1 ? 4 : out_f32 == 2 ? 1 : 2));
-      CK(cudaEventRecord(pe0, stream));
-    }
+    // algorithmic bytes: weights once + activations in + result out
+    const cudaEvent_t pe = prof_begin((double)N * K * 2 + (double)T * K * 2 + (double)T * N * (out_f32 == 1 ? 4 : out_f32 == 2 ? 1 : 2));
     if (cfg.debug_gemm_ref) {
       CK(gemm_bf16_ref_launch(X, K, W, Y, ldy, T, N, K, stream, out_f32));
     } else {
@@ -3283,7 +3272,7 @@ struct tgis_engine {
       CK(gemm_bf16_launch(wm, xmaps[bt_index(T, N, num_sms)], Y, ldy, T, N, K, gemm_ws.p, gemm_counters.p, num_sms, stream, out_f32,
                           nx.kb_prefetch > 0 ? next_wm : nullptr, nx.kb_prefetch > 0 ? &nx : nullptr, rope, norm, X, W, late));
     }
-    if (pe1) CK(cudaEventRecord(pe1, stream));
+    if (pe) CK(cudaEventRecord(pe, stream));
     ++n_launches;
   }
 
@@ -3317,7 +3306,6 @@ struct tgis_engine {
     const int32_t* d_tok = ds<int32_t>(off_tok);
     const AttnSeq* d_seqs = ds<AttnSeq>(off_seqs);
     const int32_t* d_bt = ds<int32_t>(off_bt);
-    const float scale = attn_scale;
 
     if (rank == 0) {
       CK(bitmap_set_launch(seen_bitmap.p, bitmap_words, ds<int32_t>(off_tokslot), d_tok, T, stream));
@@ -3386,7 +3374,10 @@ struct tgis_engine {
         attend(li, T, S, n_dec, n_tiles, max_dec_kv, false);
         w8_product(w8_rows(attn_out.p, q_dim, T, nullptr, false), l.o8, tmp.p, H);
         const tgis_w8_rows h{h8_codes.p, h8_scales.p, l.d8.ld, T, T, F};
-        CK(gemm8_gated_launch(w8_rows(tmp.p, H, T, l.ln2, true), l.gate8, l.up8, h, w8_call(), num_sms, stream));
+        const tgis_w8_rows x2 = w8_rows(tmp.p, H, T, l.ln2, true);
+        const cudaEvent_t pe = prof_begin(2. * F * H + (double)T * H + (double)T * F);
+        CK(gemm8_gated_launch(x2, l.gate8, l.up8, h, w8_call(), num_sms, stream));
+        if (pe) CK(cudaEventRecord(pe, stream));
         ++n_launches;
         w8_product(h, l.d8, tmp.p, H);
         continue;
@@ -3547,7 +3538,9 @@ struct tgis_engine {
     return call;
   }
   void w8_product(const tgis_w8_rows& x, const tgis_w8_matrix& w, bf16* y, int ldy) {
+    const cudaEvent_t pe = prof_begin((double)w.n * w.k + (double)x.t * x.k + (double)x.t * w.n * 2);   // (scales: a hundredth)
     CK(gemm8_launch(x, w, y, false, ldy, w8_call(), num_sms, stream));
+    if (pe) CK(cudaEventRecord(pe, stream));
     ++n_launches;
   }
 

@@ -325,7 +325,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
 }
 
 template <int NT, bool GATED, class OT>
-cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorMap& x, const Gemm8Args& a, int box, int num_sms, cudaStream_t stream) {
+cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorMap& x, const Gemm8Args& a, int box, cudaStream_t stream) {
   using F = Form<NT, GATED>;
   static OncePerDevice once;
   cudaError_t e = once([] { return cudaFuncSetAttribute(gemm8_kernel<NT, GATED, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
@@ -361,19 +361,19 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
 }
 
 template <bool GATED, class OT>
-cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgis_w8_rows& x, const Gemm8Args& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgis_w8_rows& x, const Gemm8Args& a, cudaStream_t stream) {
   const int nt = a.T <= 16 ? 16 : a.T <= 32 ? 32 : a.T <= 64 ? 64 : 128;
   const int box = std::min(nt, a.T);
   CUtensorMap xm;
   cudaError_t e = map8(&xm, x.codes, x.t, x.k, x.ld, box);
   if (e != cudaSuccess) return e;
   switch (nt) {
-    case 16: return launch8<16, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
-    case 32: return launch8<32, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
-    case 64: return launch8<64, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
+    case 16: return launch8<16, GATED, OT>(w, w2, xm, a, box, stream);
+    case 32: return launch8<32, GATED, OT>(w, w2, xm, a, box, stream);
+    case 64: return launch8<64, GATED, OT>(w, w2, xm, a, box, stream);
     default:
       if constexpr (GATED) return cudaErrorInvalidValue;   // (gemm8_pair_takes)
-      else return launch8<128, GATED, OT>(w, w2, xm, a, box, num_sms, stream);
+      else return launch8<128, GATED, OT>(w, w2, xm, a, box, stream);
   }
 }
 
@@ -390,7 +390,7 @@ cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y
   CUtensorMap wm;
   cudaError_t e = map8(&wm, w.codes, w.n, w.k, w.ld, 128);
   if (e != cudaSuccess) return e;
-  return f32 ? launch_tokens<false, float>(wm, wm, x, a, num_sms, stream) : launch_tokens<false, __nv_bfloat16>(wm, wm, x, a, num_sms, stream);
+  return f32 ? launch_tokens<false, float>(wm, wm, x, a, stream) : launch_tokens<false, __nv_bfloat16>(wm, wm, x, a, stream);
 }
 
 cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate, const tgis_w8_matrix& up, const tgis_w8_rows& out,
@@ -406,7 +406,7 @@ cudaError_t gemm8_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix& gate
   cudaError_t e = map8(&wm, gate.codes, gate.n, gate.k, gate.ld, 128);
   if (e == cudaSuccess) e = map8(&wm2, up.codes, up.n, up.k, up.ld, 128);
   if (e != cudaSuccess) return e;
-  return launch_tokens<true, __nv_bfloat16>(wm, wm2, x, a, num_sms, stream);
+  return launch_tokens<true, __nv_bfloat16>(wm, wm2, x, a, stream);
 }
 
 }  // namespace tgis
