@@ -77,7 +77,7 @@ def test_quantise_weight_refuses(lib, change, says):
 
 
 def test_products_refuse(lib):
-    at = C.addressof
+    at = C.byref
     for change, says in BAD_ROWS:
         r, m = rows(**change), matrix()
         refused(lib, lib.tgis_w8_product(at(r), at(m), AT, 0, 130, None, None), says)
@@ -103,14 +103,14 @@ def test_products_refuse(lib):
 
 @pytest.mark.parametrize("change", [dict(), dict(scales=AT + 4096), dict(codes=AT + 4096)])
 def test_rows_do_not_take_the_place_of_those_they_are_made_of(lib, change):
-    at = C.addressof
+    at = C.byref
     r, m, h, down = rows(), matrix(), rows(k=130, **change), matrix(n=64, k=130)
     refused(lib, lib.tgis_w8_gated(at(r), at(m), at(m), at(h), None, None), "out: x itself")
     refused(lib, lib.tgis_w8_feed_forward(at(r), at(m), at(m), at(down), at(h), AT, 0, 64, None, None), "hidden: x itself")
 
 
 def test_nothing_to_do_is_no_error(lib):
-    at, r, m = C.addressof, rows(t=0, codes=None), matrix()
+    at, r, m = C.byref, rows(t=0, codes=None), matrix()
     assert lib.tgis_w8_quantise_rows(None, 0, 0, None, 0.0, None, 0, None, 0, at(r), None) == 0
     assert lib.tgis_w8_product(at(r), at(m), None, 0, 0, None, None) == 0
     h = rows(t=0, k=130)
