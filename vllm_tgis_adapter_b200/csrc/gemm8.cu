@@ -1,7 +1,7 @@
 // y[t, n] = sum_g sx[t, g] sw[n / 128, g] sum_{k in g} cx[t, k] cw[n, k]: 8-bit weights (include/tgis_w8.h) times rows in 8 bits, and the gated
 // form h = silu(x gate^T) * (x up^T), which leaves as rows in 8 bits.
 //
-// Up to 128 tokens, gated up to 64 (gemm8_pair.cu has more).  A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and all tokens (B, a column
+// Up to 128 tokens, gated up to 64 (gemm8_pair.cu has more, and those above 64 of few k-blocks).  A CTA has a block of 128 weight rows (the MMA's A operand, a lane a row) and all tokens (B, a column
 // each): such a product is bound by its weight bytes, which are read once.  The tensor cores (tcgen05 kind::f8f6f4) sum one group of 128 k, that is
 // one k-block, in an accumulator; the epilogue's threads take it over, times both scales, into fp32 registers while the next one is summed in the
 // other half of the CTA's TMEM.  A tile's weights have one scale a k-block and a column has one, so a warp of its own puts their product where the

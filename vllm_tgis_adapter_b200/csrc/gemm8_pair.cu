@@ -1,4 +1,4 @@
-// The products of gemm8.cu for more than 128 tokens, on CTA pairs (tcgen05 cta_group::2, kind::f8f6f4).
+// The products of gemm8.cu for more tokens (gemm8_pair_takes), on CTA pairs (tcgen05 cta_group::2, kind::f8f6f4).
 //
 // Two neighbouring SMs work on one tile of 256 tokens x up to 256 weight rows.  Here tokens are the MMA's A operand (a CTA has 128 of them, a lane
 // each) and weights its B operand (a CTA holds half of them and the tensor cores read both halves): a thread of the epilogue has one token, whose

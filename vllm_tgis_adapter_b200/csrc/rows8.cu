@@ -4,7 +4,7 @@
 // its codes are eight bytes a lane.  With a norm the factor 1 / rms is the same for a whole row, so the codes are those of r * norm
 // and only the scales wait for the row's sum of squares: nothing is read twice or held.
 //
-// Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18.5 in fp32 (5.9 TB/s); one row 2.0 us.  What bounds the
+// Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18 to 22 in fp32 (4.9 to 5.9 TB/s); one row 2.0 us.  What bounds the
 // former: two rounds of a row's loads a CTA with their latency, three waves of CTAs.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
 // copy's rate), from bf16 143 (4.9 TB/s: the arithmetic of a number is the same).
 #include "launch.cuh"
