@@ -146,6 +146,28 @@ struct DevBuf {
   }
 };
 
+// Copies and launches of a call on an engine's device, whichever one its thread has; that one is current again afterwards.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    int now = -1;
+    cudaError_t e = cudaGetDevice(&now);
+    if (e == cudaSuccess && now != device && (e = cudaSetDevice(device)) == cudaSuccess) before_ = now;
+    if (e != cudaSuccess) {
+      cudaGetLastError();   // (or a later launch would be blamed for it)
+      throw CudaError("device " + std::to_string(device) + ": " + cudaGetErrorString(e));
+    }
+  }
+  ~OnDevice() {
+    if (before_ >= 0) cudaSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+
+ private:
+  int before_ = -1;
+};
+
 struct LayerW {
   bf16 *wqkv, *wo, *wgu, *wd, *ln1, *ln2;
   tgis_w8_matrix qkv8{}, o8{}, gate8{}, up8{}, d8{};   // in place of the first four: TGIS_WEIGHTS_E4M3
@@ -4685,7 +4707,12 @@ int tgis_engine_create_spec(const tgis_config* cfg, const tgis_model_spec* spec,
 int tgis_engine_load_weight(tgis_engine* e, const char* name, const void* ptr, int64_t rows, int64_t cols, int32_t dtype) {
   if (!e || !name || !ptr) return fail("null argument");
   if (e->started) return fail("engine already started");
-  return e->load_weight(name, ptr, rows, cols, dtype);
+  try {
+    const OnDevice here(e->cfg.device);   // (some tensors are widened or quantised by kernels)
+    return e->load_weight(name, ptr, rows, cols, dtype);
+  } catch (const std::exception& ex) {
+    return fail(ex.what());
+  }
 }
 
 int tgis_engine_start(tgis_engine* e) {
