@@ -121,6 +121,9 @@ int tgis_k_tp_wait(const uint64_t* counters, const int32_t* failed, const int32_
 /* The attention kernels' bounded wait by one warp: lanes whose bit of `arrived` is set wait for a barrier that has been arrived at, the others for one
  * that never is, for `limit` clocks.  *told: a bit a lane, whether it was told to go on (all are or none is).  Returns when the kernel has ended. */
 int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told);
+/* A kernel on `stream` that lets the one behind it begin at once and itself goes on for `clocks` of its SM (no more than 6e9, and no longer than six
+ * seconds): what a kernel launched next waits for from inside. */
+int tgis_k_hold(int64_t clocks, void* stream);
 /* debug builds only (-DTGIS_GEMM_TIMELINE): %globaltimer stamps of CTA 0 and CTA grid/2, [4][16] u64; else -2 */
 int tgis_k_gemm_timeline(uint64_t* out64);
 /* debug builds only (-DTGIS_STEP_TIMELINE; else -2): CTA 0 of every kernel launch records {kernel id, %globaltimer at

@@ -149,6 +149,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   } else if (warp == G8_MMA) {
     // ===================== MMA issuer =====================
     if (elect_one()) {
+      griddep_wait();   // (rows and scales come after the grids before this one, which may take longer than a wait has patience)
       constexpr uint32_t idesc = idesc_f8(128, NT);
       const uint32_t ring = smem_u32(smem);
       int s = 0;
@@ -221,6 +222,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
     if (patience == 0) *gave_up = 1;
   } else {
     // ===================== epilogue: lane = weight row, column = token =====================
+    griddep_wait();   // (as the issuer)
     const int quarter = warp & 3, half = warp >> 2, col0 = half * F::NC;   // gated: the other half is the other matrix
     float acc[F::NC];
 #pragma unroll
@@ -283,7 +285,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
     tmem_dealloc<F::TMEM>(tmem);
   }
   // ===================== the cluster's sums -> y or h: a warp a token, four weight rows a lane =====================
-  griddep_wait();
+  griddep_wait();   // (the issuer's and the producer's other lanes; y may still be in use by the kernels before)
   for (int i = warp, t; t = (i << log_s) + rank, t < NT && t < a.T; i += G8_WARPS) {
     float v[F::HALVES][4] = {};
     for (int r = 0; r < S; ++r)

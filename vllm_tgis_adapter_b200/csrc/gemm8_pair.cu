@@ -232,6 +232,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     }
     if (warp == P8_MMA && rank == 0 && elect_one()) {
       // ===================== MMA issuer (leader) =====================
+      griddep_wait();   // (rows and scales come after the grids before this one, which may take longer than a wait has patience)
       constexpr uint32_t idesc = idesc_f8(256, NH);
       const uint32_t ring = smem_u32(smem);
       int s = 0, b = 0;

@@ -58,6 +58,17 @@ __global__ void warp_wait_kernel(uint32_t arrived, long long limit, uint32_t* to
   if (lane == 0) *told = all;
 }
 
+__global__ void hold_kernel(long long clocks) {
+  griddep_launch();
+  auto now = [] {
+    unsigned long long ns;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(ns));
+    return ns;
+  };
+  const unsigned long long begun = now();
+  for (const long long t0 = clock64(); clock64() - t0 < clocks && now() - begun < 6000000000ull;) __nanosleep(1000);
+}
+
 int test_num_sms() {
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -89,6 +100,13 @@ int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told) {
   warp_wait_kernel<<<1, 32>>>(arrived, limit, d.p);
   KCK(cudaGetLastError());
   KCK(cudaMemcpy(told, d.p, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  return 0;
+}
+
+int tgis_k_hold(int64_t clocks, void* stream) {
+  if (clocks < 0 || clocks > 6000000000ll) return kfail("0 to 6e9 clocks are wanted");
+  hold_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(clocks);
+  KCK(cudaGetLastError());
   return 0;
 }
 
