@@ -85,3 +85,62 @@ def test_another_thread_loads_for_an_engine_on_another_device():
         eng.close()
     torch.cuda.set_device(0)
     assert np.array_equal(*got)
+
+
+def test_tensors_that_come_in_pieces():
+    """Matrices of more numbers than are on their way at a time: rows of 2 048 and of 11 264 numbers."""
+    cfg = dataclasses.replace(CONFIGS["small"], hidden=2048, n_q_heads=16, n_kv_heads=4, ffn=11264, n_layers=1)
+    assert cfg.hidden * cfg.ffn > 2 * (8 << 20)
+    CONFIGS["pieces"] = cfg
+    try:
+        weights = synthetic_weights(cfg, seed=2)
+        eng = engine("pieces", weights)
+    finally:
+        del CONFIGS["pieces"]
+    tokens = np.random.RandomState(1).randint(3, cfg.vocab, size=40).tolist()
+    got = eng.trace_step([("a", tokens, [10, 39])], end=["a"])
+    eng.close()
+    ora = OracleW8(cfg, weights)
+    want = ora.step([(ora.new_seq(), tokens)], want_all_logits=True)[[10, 39]].numpy()
+    spread = max(float(np.abs(want).std()), 1)
+    assert np.abs(got - want).mean() < 2e-3 * WIDER * spread and np.abs(got - want).max() < 2e-2 * WIDER * spread
+
+
+def test_nothing_is_held_that_only_loading_needs():
+    """What an engine takes, when it is made and once it runs, beside the same one with 16-bit weights."""
+    from vllm_tgis_adapter_b200.engine.core import ModelConfig, NativeEngine, make_sampling_params
+
+    cfg = dataclasses.replace(CONFIGS["llama3-8b"], n_layers=2, vocab=1024)
+    names = {f.name for f in dataclasses.fields(ModelConfig)}
+    mc = ModelConfig(**{f.name: getattr(cfg, f.name) for f in dataclasses.fields(cfg) if f.name in names})
+    H, F, kv, T = cfg.hidden, cfg.ffn, cfg.n_kv_heads * cfg.head_dim, 256
+    shapes = {"self_attn.q_proj": (H, H), "self_attn.k_proj": (kv, H), "self_attn.v_proj": (kv, H), "self_attn.o_proj": (H, H), "mlp.gate_proj": (F, H), "mlp.up_proj": (F, H),
+              "mlp.down_proj": (H, F)}
+    zeros = torch.zeros(H * F, dtype=torch.bfloat16)
+
+    def free():
+        torch.cuda.synchronize()
+        return torch.cuda.mem_get_info()[0]
+
+    made, running = {}, {}
+    for quantization in (None, "fp8", None, "fp8"):   # (the first two load the kernels)
+        before = free()
+        eng = NativeEngine(mc, max_num_seqs=4, max_batched_tokens=T, kv_cache_bytes=256 << 20, quantization=quantization, use_cuda_graphs=False)
+        made[quantization] = before - free()
+        for layer in range(cfg.n_layers):
+            for name, (n, k) in shapes.items():
+                eng.load_weight(f"model.layers.{layer}.{name}.weight", zeros[: n * k].view(n, k))
+            for name in ("input_layernorm", "post_attention_layernorm"):
+                eng.load_weight(f"model.layers.{layer}.{name}.weight", torch.ones(H))
+        eng.load_weight("model.embed_tokens.weight", zeros[: cfg.vocab * H].view(cfg.vocab, H))
+        eng.load_weight("model.norm.weight", torch.ones(H))
+        eng.load_weight("tgis.rope_cos_sin", rope_table(cfg))
+        eng.generate_sync([[5, 6, 7]], make_sampling_params(greedy=True, max_tokens=3, min_tokens=3))
+        running[quantization] = before - free()
+        eng.close()
+    numbers = cfg.n_layers * sum(n * k for n, k in shapes.values())
+    rows = T * (H + F) * (1 + 4 / 128)
+    saved = numbers * (2 - 1 - 4 / 128 ** 2) - rows
+    room = 24 << 20   # (allocations are rounded up; a tensor on its way would be 117 MB)
+    assert abs(made[None] - made["fp8"] - saved) < room, (made, saved)
+    assert abs(running[None] - running["fp8"] - saved) < room, (running, saved)

@@ -141,9 +141,12 @@ struct DevBuf {
     CK(cudaMalloc(&p, std::max<size_t>(count, 1) * sizeof(T)));
   }
   void zero() { CK(cudaMemset(p, 0, n * sizeof(T))); }
-  ~DevBuf() {
+  void free() {
     if (p) cudaFree(p);
+    p = nullptr;
+    n = 0;
   }
+  ~DevBuf() { free(); }
 };
 
 // Copies and launches of a call on an engine's device, whichever one its thread has; that one is current again afterwards.
@@ -415,7 +418,7 @@ struct tgis_engine {
   bool w8 = false;                                   // TGIS_WEIGHTS_E4M3: the layers' projections on linear8.cuh
   DevBuf<uint8_t> w8_codes, x8_codes, h8_codes;      // all layers' weights; a step's rows, before the projections and inside the feed-forward block
   DevBuf<float> w8_scales, x8_scales, h8_scales;
-  DevBuf<bf16> w8_load;                              // a tensor on its way into 8 bits (until start)
+  DevBuf<bf16> w8_load;                              // rows of a tensor on their way into 8 bits: from the first one (the cache's size is known then) until finalize_weights
   size_t kv8_layer_bytes = 0;
   size_t kv_layer_elems = 0;
   int num_blocks = 0;
@@ -1154,7 +1157,6 @@ struct tgis_engine {
     w8_codes.alloc(codes);
     w8_scales.alloc(scales);
     each([&](tgis_w8_matrix& m, size_t n, size_t k) { m = {w8_codes.p + codes, w8_scales.p + scales, (int64_t)up(k), (int32_t)n, (int32_t)k}; });
-    w8_load.alloc(std::max({H * F, H * (size_t)q_dim}));
     const size_t x = up(std::max(H, (size_t)q_dim));
     x8_codes.alloc(T * x);
     x8_scales.alloc(T * (x / W8_GROUP));
@@ -1163,7 +1165,6 @@ struct tgis_engine {
   }
   int w8_load_weight(LayerW& l, const std::string& sub, const std::string& name, const void* ptr, int64_t rows, int64_t cols) {
     const int64_t H = cfg.hidden, F = cfg.ffn, kvd = (int64_t)nkv * HEAD_DIM;
-    if (w8_load.p == nullptr) return fail("weights are loaded before the engine starts: " + name);
     const tgis_w8_matrix* m = nullptr;
     int64_t first = 0, n = 0;   // rows of m
     if (sub == "self_attn.q_proj.weight") m = &l.qkv8, n = q_dim;
@@ -1176,10 +1177,15 @@ struct tgis_engine {
     else return fail("unknown layer weight " + name);
     if (rows * cols != n * m->k) return fail("shape mismatch for " + name + ": got " + std::to_string(rows) + "x" + std::to_string(cols) + " expected " +
                                              std::to_string(n) + "x" + std::to_string(m->k));
-    cudaError_t e = cudaMemcpy(w8_load.p, ptr, (size_t)(n * m->k) * sizeof(bf16), cudaMemcpyDefault);
-    if (e == cudaSuccess)   // (heads are 128 rows: q, k and v begin at blocks)
-      e = weight8_launch(w8_load.p, false, m->k, (int)n, m->k, (uint8_t*)m->codes + (size_t)first * m->ld, m->ld,
-                         m->scales + first / W8_GROUP * ((m->k + W8_GROUP - 1) / W8_GROUP), cudaStreamLegacy);
+    // so many blocks of rows at a time as 16 MB hold (the pieces' copies and kernels follow one another on the legacy stream)
+    const int64_t k = m->k, groups = (k + W8_GROUP - 1) / W8_GROUP, piece = std::max<int64_t>((8 << 20) / k / W8_GROUP, 1) * W8_GROUP;
+    if (w8_load.p == nullptr) w8_load.alloc(std::max<size_t>(8 << 20, (size_t)W8_GROUP * std::max({H, F, (int64_t)q_dim})));
+    cudaError_t e = cudaSuccess;
+    for (int64_t r = 0; r < n && e == cudaSuccess; r += piece) {
+      const int64_t rows_now = std::min(piece, n - r), at = first + r;   // (heads are 128 rows: q, k and v begin at blocks)
+      e = cudaMemcpy(w8_load.p, static_cast<const bf16*>(ptr) + r * k, (size_t)(rows_now * k) * sizeof(bf16), cudaMemcpyDefault);
+      if (e == cudaSuccess) e = weight8_launch(w8_load.p, false, k, (int)rows_now, (int)k, (uint8_t*)m->codes + at * m->ld, m->ld, m->scales + at / W8_GROUP * groups, cudaStreamLegacy);
+    }
     if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (e != cudaSuccess) return fail(std::string("weight in 8 bits failed: ") + cudaGetErrorString(e));
     return 0;
@@ -1325,6 +1331,7 @@ struct tgis_engine {
   }
 
   void finalize_weights() {
+    w8_load.free();
     if (pnx_on) {  // a checkpoint with a tensor missing must not come up on zeros
       if (pnx_loaded.size() != pnx_expected_tensors)
         throw CudaError("checkpoint incomplete: " + std::to_string(pnx_loaded.size()) + " of " +
