@@ -124,6 +124,10 @@ int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told);
 /* A kernel on `stream` that lets the one behind it begin at once and itself goes on for `clocks` of its SM (no more than 6e9, and no longer than six
  * seconds): what a kernel launched next waits for from inside. */
 int tgis_k_hold(int64_t clocks, void* stream);
+/* Products with 8-bit weights, host only: how the launchers cut one where at_once[i] clusters of 2^i CTAs run at the same time (0: none).  pieces: of k, for `tiles`
+ * tiles of 128 weight rows, `groups` groups of 128 numbers and `ctas` CTAs an SM; pair_plan: 16 * chunks of 32 columns of half a tile + pieces of k.  -1: not at all. */
+int tgis_k_w8_pieces(int32_t tiles, int32_t groups, int32_t ctas, const int32_t* at_once);
+int tgis_k_w8_pair_plan(int32_t n, int32_t x_tiles, int32_t groups, int32_t gated, const int32_t* at_once);
 /* debug builds only (-DTGIS_GEMM_TIMELINE): %globaltimer stamps of CTA 0 and CTA grid/2, [4][16] u64; else -2 */
 int tgis_k_gemm_timeline(uint64_t* out64);
 /* debug builds only (-DTGIS_STEP_TIMELINE; else -2): CTA 0 of every kernel launch records {kernel id, %globaltimer at

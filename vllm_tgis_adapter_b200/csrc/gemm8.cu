@@ -333,18 +333,11 @@ cudaError_t launch8(const CUtensorMap& w, const CUtensorMap& w2, const CUtensorM
   cudaError_t e = once([] { return cudaFuncSetAttribute(gemm8_kernel<NT, GATED, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
   if (e != cudaSuccess) return e;
   const int tiles = (a.N + 127) / 128;
-  // The pieces of k whose waves take the fewest k-blocks: a wave's beginning and end take about G8_ENDS of them.  (A tenth of a wave too many costs less than
-  // a wave, for the memory is what all wait for: 32 x 4096 x 14336 in 32 clusters of eight where 30 run at once 14.4 us, of four 15.5, of two 20.7)
   static ClustersAtOnce at_once;
-  int S = 1;
-  float least = -1.f;
-  for (int s = 1; s <= 8 && s * 2 <= std::max(a.G, 2); s *= 2) {
-    int n = 0;
-    if ((e = at_once(gemm8_kernel<NT, GATED, OT>, G8_THREADS, F::SMEM, s, &n)) != cudaSuccess) return e;
-    const float waves = (float)tiles / (float)(n * F::CTAS);   // (the answer is for one CTA an SM)
-    const float cost = std::max(std::ceil(waves - 0.1f), 1.f) * (float)((a.G + s - 1) / s + G8_ENDS);
-    if (least < 0.f || cost < least) S = s, least = cost;
-  }
+  int n[4] = {}, S = 1;
+  for (int i = 0; i < 4 && (i == 0 || a.G >= 2 << i); ++i)
+    if ((e = at_once(gemm8_kernel<NT, GATED, OT>, G8_THREADS, F::SMEM, 1 << i, &n[i])) != cudaSuccess) return e;
+  if ((e = gemm8_plan(tiles, a.G, F::CTAS, n, &S)) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)tiles, 1, (unsigned)S);
   cfg.blockDim = dim3(G8_THREADS);
@@ -380,6 +373,19 @@ cudaError_t launch_tokens(const CUtensorMap& w, const CUtensorMap& w2, const tgi
 }
 
 }  // namespace
+
+// The pieces of k whose waves take the fewest k-blocks: a wave's beginning and end take about G8_ENDS of them.  (A tenth of a wave too many costs less than
+// a wave, for the memory is what all wait for: 32 x 4096 x 14336 in 32 clusters of eight where 30 run at once 14.4 us, of four 15.5, of two 20.7)
+cudaError_t gemm8_plan(int tiles, int G, int ctas, const int (&at_once)[4], int* pieces) {
+  float least = -1.f;
+  for (int i = 0; i < 4 && (i == 0 || G >= 2 << i); ++i) {
+    if (at_once[i] < 1) continue;
+    const float waves = (float)tiles / (float)(at_once[i] * ctas);   // (the answer is for one CTA an SM)
+    const float cost = std::max(std::ceil(waves - 0.1f), 1.f) * (float)((G + (1 << i) - 1) / (1 << i) + G8_ENDS);
+    if (least < 0.f || cost < least) *pieces = 1 << i, least = cost;
+  }
+  return least < 0.f ? cudaErrorLaunchOutOfResources : cudaSuccess;
+}
 
 cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, const Gemm8Call& call, int num_sms,
                          cudaStream_t stream) {

@@ -397,34 +397,19 @@ cudaError_t launch_pair8(const CUtensorMap& w, const CUtensorMap& w2, const CUte
                           stream, 2 * S, w, w2, x, a);
 }
 
-// Chunks of a half and pieces of k: those whose waves take least, in hundredths of a microsecond.  A k-block of 256 x 64 CH takes P8_BLOCK[CH] while it is the
-// epilogue's chain that bounds it, a launch's beginning and end P8_ENDS[S] and P8_WIDE[S] more for every chunk above two; pieces are for one wave.  Measured (us; taken first):
-// 256 x 4096 x 4096 CH 2, S 2: 12.6; CH 2, S 1: 13.6; CH 4, S 2: 14.6; CH 4, S 1: 16.6.  512 x 6144 x 4096 CH 3: 17.0, CH 4: 18.3, CH 2: 24.4.  301 x 2128 x 11264 CH 4, S 2: 25.5, CH 2, S 1: 30.2,
-// CH 4, S 1: 35.3.  1024 x 512 x 8192 CH 4, S 4: 15.5, CH 2, S 2: 15.2, S 1: 22.2.  203 x 512 x 1536 CH 2, S 1: 6.8, S 2: 7.0, CH 4, S 4: 8.9.  2048 x 8192 x 8192 CH 4: 118, CH 3: 131, CH 2: 154.
-constexpr int P8_BLOCK[5] = {0, 0, 30, 33, 36}, P8_ENDS[5] = {0, 400, 600, 0, 700}, P8_WIDE[5] = {0, 50, 100, 0, 100};
-struct Plan { int ch, s; };
 template <class OT>
-cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan* out) {
+cudaError_t plan(int N, int x_tiles, int G, bool gated, Plan8* out) {
   static ClustersAtOnce at_once;
-  long long least = -1;
-  for (int s = 1; s <= 4 && s <= G; s *= 2) {
-    int n = 0;
-    const cudaError_t e = at_once(gemm8_pair_kernel<4, 1, false, OT>, P8_THREADS, P8_SMEM, 2 * s, &n);
+  int n[4] = {};
+  for (int i = 1; i < 4 && G >= 1 << (i - 1); ++i) {
+    const cudaError_t e = at_once(gemm8_pair_kernel<4, 1, false, OT>, P8_THREADS, P8_SMEM, 1 << i, &n[i]);
     if (e != cudaSuccess) return e;
-    for (int c = 4; c >= 2; --c) {
-      if (gated ? c < 4 : (s == 2 && c == 3) || (s == 4 && c < 4)) continue;   // (a thread's share of what pieces leave: whole runs of 64 bytes)
-      const int rows = gated ? 128 : 64 * c;
-      const long long tiles = (long long)((N + rows - 1) / rows) * x_tiles, waves = (tiles + n - 1) / n;
-      if (s > 1 && waves > 1) continue;
-      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS[s] + P8_WIDE[s] * (c - 2);
-      if (least < 0 || cost < least) *out = Plan{c, s}, least = cost;
-    }
   }
-  return cudaSuccess;
+  return gemm8_pair_plan(N, x_tiles, G, gated, n, out);
 }
 
 template <class OT>
-cudaError_t launch_plain(const Plan& p, const CUtensorMap& w, const CUtensorMap& x, const Pair8Args& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_plain(const Plan8& p, const CUtensorMap& w, const CUtensorMap& x, const Pair8Args& a, int num_sms, cudaStream_t stream) {
   if (p.s == 4) return launch_pair8<4, 4, false, OT>(w, w, x, a, num_sms, stream);
   if (p.s == 2) return p.ch == 4 ? launch_pair8<4, 2, false, OT>(w, w, x, a, num_sms, stream) : launch_pair8<2, 2, false, OT>(w, w, x, a, num_sms, stream);
   return p.ch == 4 ? launch_pair8<4, 1, false, OT>(w, w, x, a, num_sms, stream) : p.ch == 3 ? launch_pair8<3, 1, false, OT>(w, w, x, a, num_sms, stream)
@@ -433,7 +418,7 @@ cudaError_t launch_plain(const Plan& p, const CUtensorMap& w, const CUtensorMap&
 template <class OT>
 cudaError_t product_pair8(const tgis_w8_rows& x, const tgis_w8_matrix& w, const Gemm8Args& g, int num_sms, cudaStream_t stream) {
   Pair8Args a{g, 0, (g.T + 255) / 256};
-  Plan p{4, 1};
+  Plan8 p{4, 1};
   cudaError_t e = plan<OT>(g.N, a.x_tiles, g.G, false, &p);
   if (e != cudaSuccess) return e;
   a.n_tiles = (g.N + 64 * p.ch - 1) / (64 * p.ch);
@@ -444,6 +429,28 @@ cudaError_t product_pair8(const tgis_w8_rows& x, const tgis_w8_matrix& w, const 
 }
 
 }  // namespace
+
+// Chunks of a half and pieces of k: those whose waves take least, in hundredths of a microsecond.  A k-block of 256 x 64 CH takes P8_BLOCK[CH] while it is the
+// epilogue's chain that bounds it, a launch's beginning and end P8_ENDS[S] and P8_WIDE[S] more for every chunk above two; pieces are for one wave.  Measured (us; taken first):
+// 256 x 4096 x 4096 CH 2, S 2: 12.6; CH 2, S 1: 13.6; CH 4, S 2: 14.6; CH 4, S 1: 16.6.  512 x 6144 x 4096 CH 3: 17.0, CH 4: 18.3, CH 2: 24.4.  301 x 2128 x 11264 CH 4, S 2: 25.5, CH 2, S 1: 30.2,
+// CH 4, S 1: 35.3.  1024 x 512 x 8192 CH 4, S 4: 15.5, CH 2, S 2: 15.2, S 1: 22.2.  203 x 512 x 1536 CH 2, S 1: 6.8, S 2: 7.0, CH 4, S 4: 8.9.  2048 x 8192 x 8192 CH 4: 118, CH 3: 131, CH 2: 154.
+constexpr int P8_BLOCK[5] = {0, 0, 30, 33, 36}, P8_ENDS[5] = {0, 400, 600, 0, 700}, P8_WIDE[5] = {0, 50, 100, 0, 100};
+cudaError_t gemm8_pair_plan(int N, int x_tiles, int G, bool gated, const int (&at_once)[4], Plan8* out) {
+  long long least = -1;
+  for (int i = 1, s = 1; i < 4 && s <= G; ++i, s *= 2) {
+    const int n = at_once[i];
+    if (n < 1) continue;
+    for (int c = 4; c >= 2; --c) {
+      if (gated ? c < 4 : (s == 2 && c == 3) || (s == 4 && c < 4)) continue;   // (a thread's share of what pieces leave: whole runs of 64 bytes)
+      const int rows = gated ? 128 : 64 * c;
+      const long long tiles = (long long)((N + rows - 1) / rows) * x_tiles, waves = (tiles + n - 1) / n;
+      if (s > 1 && waves > 1) continue;
+      const long long cost = waves * ((long long)P8_BLOCK[c] * ((G + s - 1) / s)) + P8_ENDS[s] + P8_WIDE[s] * (c - 2);
+      if (least < 0 || cost < least) *out = Plan8{c, s}, least = cost;
+    }
+  }
+  return least < 0 ? cudaErrorLaunchOutOfResources : cudaSuccess;
+}
 
 // More than 128 tokens; from 65 on gated ones (us, gemm8.cu and here: 65 tokens, 4096 / 14336 38.5 and 33.5, 512 / 1536 9.4 and 6.0; 64 tokens 26.5 and 33) and those of few
 // k-blocks, whose end is what counts (65 x 512 x 512 6.4 and 4.1, but 65 x 2128 x 2048 7.8 and 9.2, 128 x 4096 x 14336 20.3 and 24.4; 200: 32.0 and 25.6).
@@ -461,7 +468,7 @@ cudaError_t gemm8_pair_gated_launch(const tgis_w8_rows& x, const tgis_w8_matrix&
   if (e == cudaSuccess) e = map8(&wm2, up.codes, up.n, up.k, up.ld, 128);
   if (e == cudaSuccess) e = map8(&xm, x.codes, x.t, x.k, x.ld, 128);
   if (e != cudaSuccess) return e;
-  Plan p{4, 1};
+  Plan8 p{4, 1};
   if ((e = plan<__nv_bfloat16>(g.N, a.x_tiles, g.G, true, &p)) != cudaSuccess) return e;
   return p.s == 4 ? launch_pair8<4, 4, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream)
        : p.s == 2 ? launch_pair8<4, 2, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream) : launch_pair8<4, 1, true, __nv_bfloat16>(wm, wm2, xm, a, num_sms, stream);

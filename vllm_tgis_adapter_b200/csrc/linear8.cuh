@@ -123,16 +123,18 @@ inline cudaError_t map8(CUtensorMap* out, const void* codes, int64_t rows, int64
   return make_tmap_u8_2d(out, codes, (uint64_t)rows, (uint64_t)cols, (uint64_t)ld, (uint32_t)box, W8_GROUP) == 0 ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// Clusters of a kernel that run at once, asked once a device and size: an SM's share of a GPC is not always a whole number of clusters
+// Clusters of a kernel that run at once, asked once a device and size: an SM's share of a GPC is not always a whole number of clusters.  0: not one does (a GPC
+// may have fewer SMs, a partition of a device fewer still)
 struct ClustersAtOnce {
-  std::atomic<int> known[OncePerDevice::MAX][4] = {};
+  std::atomic<int> known[OncePerDevice::MAX][4] = {};   // (one more than the answer)
   template <class K>
   cudaError_t operator()(K kernel, int threads, int smem, int cluster, int* out) {   // cluster: 1, 2, 4 or 8
+    const int at = __builtin_ctz((unsigned)cluster);
+    if (cluster != 1 << at || at > 3) return cudaErrorInvalidValue;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const int at = cluster == 8 ? 3 : cluster / 2;
-    if (dev < OncePerDevice::MAX && (*out = known[dev][at].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    if (dev < OncePerDevice::MAX && (*out = known[dev][at].load(std::memory_order_relaxed) - 1) >= 0) return cudaSuccess;
     if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(cluster * 1024));
@@ -145,11 +147,21 @@ struct ClustersAtOnce {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     e = cudaOccupancyMaxActiveClusters(out, kernel, &cfg);
-    if (e == cudaSuccess && *out < 1) e = cudaErrorLaunchOutOfResources;
-    if (e == cudaSuccess && dev < OncePerDevice::MAX) known[dev][at].store(*out, std::memory_order_relaxed);
+    if (e == cudaErrorInvalidClusterSize || e == cudaErrorLaunchOutOfResources) {
+      cudaGetLastError();
+      *out = 0;
+      e = cudaSuccess;
+    }
+    if (e == cudaSuccess && dev < OncePerDevice::MAX) known[dev][at].store(*out + 1, std::memory_order_relaxed);
     return e;
   }
 };
+
+// How the launchers cut a product, where at_once[i] clusters of 2^i CTAs run at the same time (0: none, so such pieces are not taken; cudaErrorLaunchOutOfResources where
+// nothing is left).  gemm8.cu: pieces of k of `tiles` tiles, `ctas` to an SM; gemm8_pair.cu: chunks of a half of a tile and pieces of k.
+struct Plan8 { int ch, s; };
+cudaError_t gemm8_plan(int tiles, int G, int ctas, const int (&at_once)[4], int* pieces);
+cudaError_t gemm8_pair_plan(int N, int x_tiles, int G, bool gated, const int (&at_once)[4], Plan8* out);
 
 // y = x w^T (y bf16, or fp32: f32), and h of both matrices
 cudaError_t gemm8_launch(const tgis_w8_rows& x, const tgis_w8_matrix& w, void* y, bool f32, int64_t ldy, const Gemm8Call& call, int num_sms,

@@ -7,6 +7,7 @@
 
 #include "../../include/tgis_kernels.h"
 #include "kernels.h"
+#include "linear8.cuh"
 #include "ptx.cuh"
 #include "tc_attention.cuh"
 
@@ -108,6 +109,17 @@ int tgis_k_hold(int64_t clocks, void* stream) {
   hold_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(clocks);
   KCK(cudaGetLastError());
   return 0;
+}
+
+int tgis_k_w8_pieces(int32_t tiles, int32_t groups, int32_t ctas, const int32_t* at_once) {
+  const int n[4] = {at_once[0], at_once[1], at_once[2], at_once[3]};
+  int s = 0;
+  return gemm8_plan(tiles, groups, ctas, n, &s) == cudaSuccess ? s : kfail("no cluster fits");
+}
+int tgis_k_w8_pair_plan(int32_t n, int32_t x_tiles, int32_t groups, int32_t gated, const int32_t* at_once) {
+  const int fit[4] = {at_once[0], at_once[1], at_once[2], at_once[3]};
+  Plan8 p{};
+  return gemm8_pair_plan(n, x_tiles, groups, gated != 0, fit, &p) == cudaSuccess ? 16 * p.ch + p.s : kfail("no cluster fits");
 }
 
 int tgis_k_pair_fault(int32_t nth) { return gemm_pair_fault(nth); }
