@@ -13,6 +13,7 @@ made of, the residual's sum excepted.  Arguments that the host can check raise V
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -22,6 +23,7 @@ from ._lib import TgisW8Matrix, TgisW8Rows
 GROUP, MAX_K, MAX_ROWS = 128, 131072, 1 << 22
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
 _functions = None
+_lock = threading.Lock()   # of what is made once a device, and of the status words' counts
 _current_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -67,18 +69,32 @@ class _Device:
     """What calls on a device share: empty tensors, whose new_empty costs half of torch.empty's time, and the status word."""
 
     def __init__(self, device: torch.device):
-        self.device, self.status, self.status_at = device, None, None
+        self.device, self.status, self.status_at, self.stalls = device, None, None, 0
         self.fp32, self.bf16, self.codes, self.bytes = (torch.empty(0, dtype=t, device=device) for t in (torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8))
 
     def with_status(self) -> "_Device":
-        if self.status is None:
-            if torch.cuda.is_current_stream_capturing():   # (the word would be a graph's, and zeroed by its replays)
-                raise ValueError("the first layer on a device is made before a capture begins")
-            with torch.cuda.device(self.device):
-                self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
-                torch.cuda.current_stream().synchronize()
-            self.status_at = self.status.data_ptr()
+        if self.status_at is None:
+            with _lock:
+                if self.status_at is None:
+                    if torch.cuda.is_current_stream_capturing():   # (the word would be a graph's, and zeroed by its replays)
+                        raise ValueError("the first layer on a device is made before a capture begins")
+                    with torch.cuda.device(self.device):
+                        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+                        torch.cuda.current_stream().synchronize()
+                    self.status_at = self.status.data_ptr()
         return self
+
+    def stalls_so_far(self) -> int:
+        """How often a check has found the word raised, with this one, which waits for the device.  The word is taken back here and the count is what a layer
+        compares with what it saw last, so that no check takes another layer's report."""
+        with torch.cuda.device(self.device):
+            torch.cuda.synchronize()
+            with _lock:
+                if int(self.status.item()):
+                    self.status.zero_()
+                    torch.cuda.current_stream().synchronize()
+                    self.stalls += 1
+                return self.stalls
 
 
 _devices: dict[int, _Device] = {}
@@ -87,8 +103,24 @@ _devices: dict[int, _Device] = {}
 def _of(device: torch.device) -> _Device:
     got = _devices.get(device.index)
     if got is None:
-        got = _devices[device.index] = _Device(device)
+        made = _Device(device)
+        with _lock:
+            got = _devices.setdefault(device.index, made)
     return got
+
+
+class _Checked:
+    """A layer's check; `_watch` when it is made."""
+
+    def _watch(self, on: _Device) -> None:
+        self._on, self._seen = on, on.stalls
+
+    def check(self) -> None:
+        """Waits for the device and raises if a call on it, whichever layer's, has given up since this layer's last check."""
+        stalls = self._on.stalls_so_far()
+        seen, self._seen = self._seen, stalls
+        if stalls != seen:
+            raise RuntimeError("a wait inside a kernel ran out")
 
 
 class Rows8:
@@ -150,7 +182,7 @@ def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-
     return out
 
 
-class Linear8:
+class Linear8(_Checked):
     """A weight matrix in 8 bits: `codes` e4m3 [n, k], `scales` fp32 [blocks of 128 rows, groups of 128].  Codes whose rows do not start on
     16 bytes are copied once."""
 
@@ -175,7 +207,8 @@ class Linear8:
     def _keep(self, codes: torch.Tensor, scales: torch.Tensor, device: torch.device, record: TgisW8Matrix) -> None:
         self.codes, self.scales, self.device, self.n, self.k = codes, scales, device, record.n, record.k
         self.record, self.at = record, C.addressof(record)
-        self._on, self._product = _of(device).with_status(), _load().product
+        self._watch(_of(device).with_status())
+        self._product = _load().product
 
     @classmethod
     def from_weight(cls, w: torch.Tensor) -> "Linear8":
@@ -207,10 +240,6 @@ class Linear8:
             _run(self._product, self.device, x.at, self.at, out.data_ptr(), TYPES[out.dtype], ld, self._on.status_at)
         return out
 
-    def check(self) -> None:
-        """Waits for the device and raises if a call on it has given up since the last check."""
-        _check(self._on.status)
-
 
 def _result(out: torch.Tensor | None, dtype: torch.dtype, T: int, n: int, on: _Device, device: torch.device) -> tuple[torch.Tensor, int]:
     if out is None:
@@ -223,15 +252,7 @@ def _result(out: torch.Tensor | None, dtype: torch.dtype, T: int, n: int, on: _D
     return out, ld
 
 
-def _check(status: torch.Tensor) -> None:
-    with torch.cuda.device(status.device):
-        torch.cuda.synchronize()
-    if int(status.item()):
-        status.zero_()
-        raise RuntimeError("a wait inside a kernel ran out")
-
-
-class FeedForward8:
+class FeedForward8(_Checked):
     """y = down h, h = silu(gate x) * (up x) held in 8-bit rows between the two launches."""
 
     def __init__(self, gate: Linear8, up: Linear8, down: Linear8):
@@ -240,7 +261,8 @@ class FeedForward8:
         if gate.n > MAX_K:
             raise ValueError(f"gate: at most {MAX_K} rows are wanted")
         self.gate, self.up, self.down, self.device = gate, up, down, gate.device
-        self._on, self._call = gate._on, _load().feed_forward
+        self._watch(gate._on)
+        self._call = _load().feed_forward
         self._groups = -(-gate.n // GROUP)
 
     def hidden(self, x: Rows8, out: Rows8 | None = None) -> Rows8:
@@ -271,7 +293,3 @@ class FeedForward8:
             h = TgisW8Rows(at, at + T * width, width, T, T, self.gate.n)
             _run(self._call, self.device, x.at, self.gate.at, self.up.at, self.down.at, C.addressof(h), out.data_ptr(), TYPES[out.dtype], ld, self._on.status_at)
         return out
-
-    def check(self) -> None:
-        """Waits for the device and raises if a call on it has given up since the last check."""
-        _check(self._on.status)
