@@ -22,6 +22,7 @@ from ._lib import TgisW8Matrix, TgisW8Rows
 
 GROUP, MAX_K, MAX_ROWS = 128, 131072, 1 << 22
 TYPES = {torch.bfloat16: 0, torch.float32: 1}
+NOT_ROWS = "x: rows in 8 bits are wanted (Rows8, of quantise)"
 _functions = None
 _lock = threading.Lock()   # of what is made once a device, and of the status words' counts
 _current_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -175,7 +176,7 @@ def quantise(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-
         raise ValueError("residual_out: there is no residual")
     if out is None:
         out = Rows8(T, k, device)
-    elif out.shape != (T, k) or out.device != device:
+    elif not isinstance(out, Rows8) or out.shape != (T, k) or out.device != device:
         raise ValueError(f"out: {T} rows of {k} numbers on {device} are wanted")
     if T or norm is not None:
         _run(_load().rows, device, x.data_ptr(), TYPES[dtype], ld, norm_at, eps, res_at, ldr, to_at, ldt, out.at)
@@ -232,6 +233,8 @@ class Linear8(_Checked):
 
     def __call__(self, x: Rows8, out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """x w^T [T, n], in `dtype` (bf16 or fp32) or into `out`."""
+        if not isinstance(x, Rows8):
+            raise ValueError(NOT_ROWS)
         T, k = x.record.t, x.record.k
         if k != self.k or x.device != self.device:
             raise ValueError(f"x: rows of {self.k} numbers on {self.device} are wanted, not of {k} on {x.device}")
@@ -256,6 +259,8 @@ class FeedForward8(_Checked):
     """y = down h, h = silu(gate x) * (up x) held in 8-bit rows between the two launches."""
 
     def __init__(self, gate: Linear8, up: Linear8, down: Linear8):
+        if not all(isinstance(m, Linear8) for m in (gate, up, down)):
+            raise ValueError("gate, up, down: 8-bit matrices are wanted (Linear8)")
         if up.n != gate.n or up.k != gate.k or down.k != gate.n or up.device != gate.device or down.device != gate.device:
             raise ValueError(f"gate [{gate.n}, {gate.k}], up [{up.n}, {up.k}], down [{down.n}, {down.k}] on one device do not make a feed-forward block")
         if gate.n > MAX_K:
@@ -271,13 +276,15 @@ class FeedForward8(_Checked):
         T = x.record.t
         if out is None:
             out = Rows8(T, self.gate.n, self.device)
-        elif out.shape != (T, self.gate.n) or out.device != self.device:
+        elif not isinstance(out, Rows8) or out.shape != (T, self.gate.n) or out.device != self.device:
             raise ValueError(f"out: {T} rows of {self.gate.n} numbers on {self.device} are wanted")
         if T:
             _run(_load().gated, self.device, x.at, self.gate.at, self.up.at, out.at, self._on.status_at)
         return out
 
     def _fits(self, x: Rows8) -> None:
+        if not isinstance(x, Rows8):
+            raise ValueError(NOT_ROWS)
         if x.record.k != self.gate.k or x.device != self.device:
             raise ValueError(f"x: rows of {self.gate.k} numbers on {self.device} are wanted, not of {x.record.k} on {x.device}")
 
