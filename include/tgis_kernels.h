@@ -121,6 +121,10 @@ int tgis_k_tp_wait(const uint64_t* counters, const int32_t* failed, const int32_
 /* The attention kernels' bounded wait by one warp: lanes whose bit of `arrived` is set wait for a barrier that has been arrived at, the others for one
  * that never is, for `limit` clocks.  *told: a bit a lane, whether it was told to go on (all are or none is).  Returns when the kernel has ended. */
 int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told);
+/* The wait of the products with 8-bit weights, by one warp: lanes as above, then all of them for the barrier that is never arrived at, each with what patience it has left of
+ * `limit` clocks, then the CTA's report.  *told: a bit a lane, whether the first wait left it patience; *status: what the call's status word holds (0 before), *stalled: the
+ * engine's word; `words`: 1 the former is given to the kernel, 2 the latter, 3 both.  Returns when the kernel has ended. */
+int tgis_k_await8(uint32_t arrived, int64_t limit, int32_t words, uint32_t* told, int32_t* status, int32_t* stalled);
 /* A kernel on `stream` that lets the one behind it begin at once and itself goes on for `clocks` of its SM (no more than 6e9, and no longer than six
  * seconds): what a kernel launched next waits for from inside. */
 int tgis_k_hold(int64_t clocks, void* stream);

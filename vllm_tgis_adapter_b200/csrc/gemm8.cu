@@ -275,11 +275,7 @@ gemm8_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ C
   tc_fence_before();
   if (S > 1) cluster_sync_all();
   else __syncthreads();
-  if (*gave_up) {   // copies and MMAs in flight, all issued by now, are done long before this millisecond is over
-    for (const long long t1 = clock64(); clock64() - t1 < 2000000ll;) {}
-    if (threadIdx.x == 0) say_stalled8(a);
-    __syncthreads();
-  }
+  if (say_if_stalled8(a, gave_up)) __syncthreads();
   if (warp == G8_MMA) {
     tc_fence_after();
     tmem_dealloc<F::TMEM>(tmem);

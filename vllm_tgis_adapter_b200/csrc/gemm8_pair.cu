@@ -186,10 +186,7 @@ gemm8_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constan
     __syncwarp();
     tc_fence_before();
     asm volatile("bar.sync 0;\n" ::: "memory");
-    if (*gave_up) {   // copies and MMAs in flight, all issued by now, are done long before this millisecond is over
-      for (const long long t1 = clock64(); clock64() - t1 < 2000000ll;) {}
-      if (threadIdx.x == 0) say_stalled8(a);
-    }
+    say_if_stalled8(a, gave_up);
     cluster_sync_all();   // nobody leaves while the peer may still read its shared memory or signal its barriers
   };
   if (warp >= P8_EPI) {

@@ -97,6 +97,13 @@ __device__ __forceinline__ void await(uint64_t* bar, uint32_t parity, long long&
   }
   __syncwarp();
 }
+// ... and a CTA at its end, all of it (true: one of its roles has given up)
+__device__ __forceinline__ bool say_if_stalled8(const Gemm8Args& a, const volatile int* gave_up) {
+  if (!*gave_up) return false;
+  for (const long long t1 = clock64(); clock64() - t1 < 2000000ll;) {}   // copies and MMAs in flight, all issued by now, are done long before this millisecond is over
+  if (threadIdx.x == 0) say_stalled8(a);
+  return true;
+}
 
 // silu(g) u: exp and quotient are the approximate ones, within some steps of 2^-23 of what is rounded to 2^-4 next
 __device__ __forceinline__ float swiglu(float g, float u) {

@@ -59,6 +59,29 @@ __global__ void warp_wait_kernel(uint32_t arrived, long long limit, uint32_t* to
   if (lane == 0) *told = all;
 }
 
+__global__ void await8_kernel(uint32_t arrived, long long limit, const __grid_constant__ Gemm8Args a, uint32_t* told) {
+  __shared__ uint64_t bar[2];
+  __shared__ int word;
+  volatile int* gave_up = &word;
+  const int lane = threadIdx.x;
+  if (lane == 0) {
+    mbar_init(&bar[0], 1);
+    mbar_init(&bar[1], 1);
+    fence_barrier_init();
+    mbar_arrive(&bar[0]);
+    *gave_up = 0;
+  }
+  __syncwarp();
+  long long patience = limit;
+  await(&bar[arrived >> lane & 1 ? 0 : 1], 0, patience);
+  const uint32_t left = __ballot_sync(0xffffffffu, patience != 0);
+  if (left != 0xffffffffu) await(&bar[1], 0, patience);   // (the next wait of a role that has given up)
+  if (patience == 0) *gave_up = 1;
+  __syncthreads();
+  say_if_stalled8(a, gave_up);
+  if (lane == 0) *told = left;
+}
+
 __global__ void hold_kernel(long long clocks) {
   griddep_launch();
   auto now = [] {
@@ -101,6 +124,30 @@ int tgis_k_warp_wait(uint32_t arrived, int64_t limit, uint32_t* told) {
   warp_wait_kernel<<<1, 32>>>(arrived, limit, d.p);
   KCK(cudaGetLastError());
   KCK(cudaMemcpy(told, d.p, sizeof(uint32_t), cudaMemcpyDeviceToHost));
+  return 0;
+}
+
+int tgis_k_await8(uint32_t arrived, int64_t limit, int32_t words, uint32_t* told, int32_t* status, int32_t* stalled) {
+  if (told == nullptr || status == nullptr || stalled == nullptr) return kfail("places for what the kernel says are wanted");
+  if (limit < 1 || limit > WAIT_LIMIT || words < 0 || words > 3) return kfail("the limit is that of the kernels at most, words 0 to 3");
+  Tmp<uint32_t> d;
+  const int32_t none = 0;
+  Tmp<int32_t> s;
+  KCK(d.alloc(1));
+  KCK(s.upload(&none, 1));
+  int* host = nullptr;
+  KCK(cudaHostAlloc(&host, sizeof(int), cudaHostAllocMapped));
+  *host = 0;
+  Gemm8Args a{};
+  a.status = words & 1 ? s.p : nullptr;
+  a.stalled = words & 2 ? host : nullptr;
+  await8_kernel<<<1, 32>>>(arrived, limit, a, d.p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpy(told, d.p, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess) e = cudaMemcpy(status, s.p, sizeof(int32_t), cudaMemcpyDeviceToHost);
+  *stalled = *reinterpret_cast<volatile int*>(host);
+  cudaFreeHost(host);
+  KCK(e);
   return 0;
 }
 
