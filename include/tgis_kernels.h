@@ -112,7 +112,7 @@ int tgis_k_lora_swiglu(const void* x_dev, int32_t ldx, const int32_t* tok_slot_d
 /* ... and where no token has one: act[t, j] = bf16(silu(gate_up[t, 2j])) * gate_up[t, 2j + 1] */
 int tgis_k_silu_mul_interleaved(const void* gate_up_dev, void* act_dev, int32_t T, int32_t ffn);
 const char* tgis_k_last_error(void);
-/* Products on CTA pairs (csrc/gemm_pair.cu): the host raises the launches' error word at the nth launch from now on, as that launch
+/* Products on CTA pairs (csrc/gemm_pair.cu) and an engine's over 8-bit weights: the host raises the launches' error word at the nth launch from now on, as that launch
  * would if one of its waits ran out (0: at none); a raised word is taken back.  Returns the launches since the last call. */
 int tgis_k_pair_fault(int32_t nth);
 /* Tensor parallelism, host only (csrc/engine.cu wait_workers): rank 0's wait until the counter of every worker 1 .. tp - 1 stands at

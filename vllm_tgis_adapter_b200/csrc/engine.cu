@@ -3562,7 +3562,7 @@ struct tgis_engine {
   }
   Gemm8Call w8_call() {
     Gemm8Call call;
-    CK(gemm_pair_word(&call.stalled));
+    CK(gemm_pair_claim(&call.stalled));
     call.early = true;   // (weights are static)
     return call;
   }

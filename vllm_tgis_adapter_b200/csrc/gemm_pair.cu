@@ -634,22 +634,12 @@ cudaError_t make_pair_word() {
 
 std::atomic<int> pair_launches{0}, pair_fault_in{0};   // gemm_pair_fault
 
-// the error word for one launch (and the host's stand-in for a wait of it that runs out, gemm_pair_fault)
-cudaError_t claim_pair_word(int*& err) {
-  const cudaError_t word = gemm_pair_prepare();
-  if (word != cudaSuccess) return word;
-  err = pair_word.load(std::memory_order_acquire);
-  pair_launches.fetch_add(1, std::memory_order_relaxed);
-  if (pair_fault_in.load(std::memory_order_relaxed) > 0 && pair_fault_in.fetch_sub(1) == 1) *reinterpret_cast<volatile int*>(err) = 1;
-  return cudaSuccess;
-}
-
 template <bool GROUPED>
 cudaError_t launch_pair(const CUtensorMap& wmap, const CUtensorMap& xmap, PairArgs a, int grid, cudaStream_t stream) {
   static const cudaError_t attr =
       cudaFuncSetAttribute(gemm_pair_kernel<GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(GROUPED));
   if (attr != cudaSuccess) return attr;
-  const cudaError_t word = claim_pair_word(a.err);
+  const cudaError_t word = gemm_pair_claim(&a.err);
   if (word != cudaSuccess) return word;
   return launch_k_cluster(gemm_pair_kernel<GROUPED>, dim3(grid), dim3(PAIR_THREADS), pair_smem(GROUPED), stream, 2, wmap, xmap, a);
 }
@@ -657,6 +647,14 @@ cudaError_t launch_pair(const CUtensorMap& wmap, const CUtensorMap& xmap, PairAr
 }  // namespace
 
 cudaError_t gemm_pair_prepare() { return pair_word.load(std::memory_order_acquire) != nullptr ? cudaSuccess : make_pair_word(); }
+
+cudaError_t gemm_pair_claim(int** word) {
+  const cudaError_t e = gemm_pair_word(word);
+  if (e != cudaSuccess) return e;
+  pair_launches.fetch_add(1, std::memory_order_relaxed);
+  if (pair_fault_in.load(std::memory_order_relaxed) > 0 && pair_fault_in.fetch_sub(1) == 1) *reinterpret_cast<volatile int*>(*word) = 1;
+  return cudaSuccess;
+}
 
 cudaError_t gemm_pair_word(int** word) {
   const cudaError_t e = gemm_pair_prepare();
@@ -784,7 +782,7 @@ cudaError_t gemm_rows_launch(const void* X, const void* W, void* Y, int ldy, int
     return cudaErrorInvalidValue;
   static const cudaError_t attr = cudaFuncSetAttribute(gemm_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ROWS_SMEM);
   if (attr != cudaSuccess) return attr;
-  const cudaError_t word = claim_pair_word(a.err);
+  const cudaError_t word = gemm_pair_claim(&a.err);
   if (word != cudaSuccess) return word;
   return launch_k_cluster(gemm_rows_kernel, dim3(2 * std::min(ra.tiles, pairs)), dim3(PAIR_THREADS), ROWS_SMEM, stream, 2, wm, xm, ra);
 }

@@ -139,6 +139,7 @@ int gemm_pair_plan(int T, int N, int pairs);   // token tiles of the dense launc
 cudaError_t gemm_pair_prepare();               // host memory of the launches: to be called before any of them is captured
 bool gemm_pair_failed();                       // a wait inside a launch of this process ran out
 cudaError_t gemm_pair_word(int** word);        // the word that such a wait raises (for kernels that share it)
+cudaError_t gemm_pair_claim(int** word);       // ... for one launch that the tests' stand-in counts
 // Tests: the host raises the error word at the nth launch from now on (0: at none), as that launch would if a wait of it ran out;
 // a raised word is taken back.  Returns the launches since the last call.
 int gemm_pair_fault(int nth);
