@@ -47,19 +47,20 @@ typedef struct {
 /* Rows of x [t, ldx] (TGIS_W8_BF16 or _F32) in 8 bits; t, k are the record's, its ld no less than k rounded up to 128 (the rest of a row's last
  * group is zeroed).  residual (may be NULL; type of x): r = x + residual, rounded to the type and stored at residual_out (may be residual
  * or x itself), takes x's place.  norm [k] (bf16, may be NULL): the row is v = r * norm / sqrt(mean r^2 + eps): the codes are those of r * norm and
- * its groups' scales are multiplied by the root's reciprocal, both in fp32. */
+ * its groups' scales are multiplied by the root's reciprocal, both in fp32 (a row whose sum of squares passes 2^128 has scales of 0). */
 int tgis_w8_quantise_rows(const void* x, int32_t type, int64_t ldx, const void* norm, float eps, const void* residual, int64_t ldr,
                           void* residual_out, int64_t ldro, const tgis_w8_rows* out, void* stream);
 
 /* A weight matrix w [n, ldw] (TGIS_W8_BF16 or _F32) in 8 bits; its record's ld no less than k rounded up to 128 (zeroed there). */
 int tgis_w8_quantise_weight(const void* w, int32_t type, int64_t ldw, const tgis_w8_matrix* out, void* stream);
 
-/* y[t, n] (TGIS_W8_BF16 or _F32, rows of ldy numbers) = x w^T: every group's sum of code products in fp32, times both scales, groups added in
- * fp32 */
+/* y[t, n] (TGIS_W8_BF16 or _F32, rows of ldy numbers) = x w^T: every group's sum of code products in fp32, times the product of both scales, groups added in
+ * fp32.  That product of scales is one number of fp32: below 2^-126 it keeps fewer bits, above 2^128 it is an infinity (and NaN where the sum is 0). */
 int tgis_w8_product(const tgis_w8_rows* x, const tgis_w8_matrix* w, void* y, int32_t type, int64_t ldy, int32_t* status, void* stream);
 
-/* h = g / (1 + exp(-g)) * u, g = x gate^T, u = x up^T, in 8 bits (out: t = x's, k = the matrices' n, ld as for tgis_w8_quantise_rows); nothing is
- * rounded before that */
+/* h = g / (1 + exp(-g)) * u, g = x gate^T, u = x up^T, in 8 bits (out: t = x's, k = the matrices' n, ld as for tgis_w8_quantise_rows); g, u and h are
+ * fp32 before that.  exp and the quotient are within (4 + 1.2 |g|) * 2^-22 of what they stand for (below -87 the quotient may be 0), and codes are e4m3(h * fl(1 / s)) where other rows'
+ * are of the rounded quotient: that product is off by 3 * 2^-24 at most, so a code is the quotient's neighbour where that lies so near to the middle of two, one in a million. */
 int tgis_w8_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out, int32_t* status,
                   void* stream);
 

@@ -105,7 +105,7 @@ __device__ __forceinline__ bool say_if_stalled8(const Gemm8Args& a, const volati
   return true;
 }
 
-// silu(g) u: exp and quotient are the approximate ones, within some steps of 2^-23 of what is rounded to 2^-4 next
+// silu(g) u: exp and quotient are the approximate ones, within some steps of 2^-23 of what is rounded to 2^-4 next (told in tgis_w8.h, as codes_near is)
 __device__ __forceinline__ float swiglu(float g, float u) {
   float e, q;
   e = ex2(g * -1.4426950408889634f);
