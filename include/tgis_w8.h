@@ -60,7 +60,7 @@ int tgis_w8_product(const tgis_w8_rows* x, const tgis_w8_matrix* w, void* y, int
 
 /* h = g / (1 + exp(-g)) * u, g = x gate^T, u = x up^T, in 8 bits (out: t = x's, k = the matrices' n, ld as for tgis_w8_quantise_rows); g, u and h are
  * fp32 before that.  exp and the quotient are within (4 + 1.2 |g|) * 2^-22 of what they stand for (below -87 the quotient may be 0), and codes are e4m3(h * fl(1 / s)) where other rows'
- * are of the rounded quotient: that product is off by 3 * 2^-24 at most, so a code is the quotient's neighbour where that lies so near to the middle of two, one in a million. */
+ * are of the rounded quotient: that product is off by 3 * 2^-24 at most, so a code is the quotient's neighbour where that lies so near to the middle of two, a few in a million. */
 int tgis_w8_gated(const tgis_w8_rows* x, const tgis_w8_matrix* gate, const tgis_w8_matrix* up, const tgis_w8_rows* out, int32_t* status,
                   void* stream);
 

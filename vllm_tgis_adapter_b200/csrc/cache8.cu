@@ -74,8 +74,8 @@ struct Batches {
 };
 
 // CTAs [0, qk_ctas), warps: every parts-th quad of query and key heads of one token, eight lanes a head (a lane has dims 8 c .. 8 c + 7 and
-// their partners 64 further).  The others: a window of tokens of one value head; SINGLE: a row a warp.  2614 tokens of 32 + 8 heads on a B200: 16.2 us, 3.7 TB/s
-// (memory bound it would be 9; the rest goes to some 250 instructions for every four heads of a token).
+// their partners 64 further).  The others: a window of tokens of one value head; SINGLE: a row a warp.  2614 tokens of 32 + 8 heads in six prompts on a B200: 14.6 us, 4.1 TB/s
+// (memory bound it would be 9; the rest goes to some 190 instructions for every four heads of a token, issue slots 33 % used by a third of the warps that fit).
 template <bool SINGLE>
 __global__ void __launch_bounds__(W8_THREADS)
 kv8_write_kernel(uint8_t* __restrict__ pages, int n_pages, int n_kv, const __nv_bfloat16* qkv, int64_t ld, int T, int n_q,
@@ -311,7 +311,7 @@ cudaError_t kv8_write_launch(uint8_t* pages, int n_pages, int n_kv, const __nv_b
   if (T <= 0) return cudaSuccess;
   const int first = q_out != nullptr ? 0 : n_q, quads = (n_q + n_kv - first + 3) / 4;
   // a warp a quad while there are few of them; two warps a token (whose cos and sin they then have for several heads) otherwise
-  // (ten quads a token: 256 tokens 4.9 us and 5.9, 512: 8.1 and 7.7, 1024: 10.2 and 8.5, 4000: 32.7 and 24.8)
+  // (ten quads a token: 96 single tokens 3.0 us and 4.0; of one prompt 256 tokens 4.9 and 5.3, 384: 6.5 and 6.8, 512: 7.7 and 8.2, 768: 6.4 and 6.2, 1024: 7.8 and 6.7, 4000: 26.6 and 20.5)
   const int parts = (long long)T * quads <= W8_ALL_AT_ONCE ? quads : std::min(quads, 2);
   const bool single = (long long)T * n_kv <= W8_SINGLE;
   const long long qk = ((long long)T * parts + W8_WARPS - 1) / W8_WARPS, ctas = qk + v_ctas(T, n_kv, single);

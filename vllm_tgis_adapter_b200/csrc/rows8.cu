@@ -5,8 +5,10 @@
 // and only the scales wait for the row's sum of squares: nothing is read twice or held.
 //
 // Measured on one B200: 2048 rows x 4096 with residual and norm 13.3 us in bf16 (4.4 TB/s; memory bound it would be 9.0), 18 to 22 in fp32 (4.9 to 5.9 TB/s); one row 2.0 us.  What bounds the
-// former: two rounds of a row's loads a CTA with their latency, three waves of CTAs.  Weights 28672 x 8192 from fp32 176 us (6.7 TB/s, a
-// copy's rate), from bf16 143 (4.9 TB/s: the arithmetic of a number is the same).
+// former: two rounds of a row's loads a CTA with their latency, three waves of CTAs.  Weights 28672 x 8192 from fp32 174 us (6.7 TB/s, a
+// copy's rate), from bf16 143 (4.9 TB/s).  What bounds the latter: 64 registers, so that four CTAs run on an SM, do not hold a thread's eight rows (132 bytes of them go to local memory and 264 come back: for
+// 117 MB of bf16 as many bytes pass the L2 as for 235 MB of fp32), and a CTA asks for all it reads before its barrier and works after it: issue slots 55 % used, the busiest pipe (alu) 43 %, memory 45 %.  Three CTAs of 80
+// registers (68 bytes to local memory) took 137.
 #include "launch.cuh"
 #include "linear8.cuh"
 #include "ptx.cuh"
