@@ -46,3 +46,10 @@ def test_pairs(lib, n, x_tiles, groups, gated, want):
         assert fit[s.bit_length()] > 0 and (chunks, s) in [(4, 4), (4, 2), (2, 2), (4, 1), (3, 1), (2, 1)] and (not gated or chunks == 4)
     assert pair_plan(lib, n, x_tiles, groups, gated, (0, 0, 0, 0)) == -1
 
+
+
+def test_hooks_refuse(lib):
+    fit = (C.c_int32 * 4)(*B200)
+    assert lib.tgis_k_w8_pieces(1, 1, 1, None) == -1 and lib.tgis_k_w8_pair_plan(1, 1, 1, 0, None) == -1
+    assert [lib.tgis_k_w8_pieces(*a, fit) for a in ((0, 1, 1), (1, 0, 1), (1, 1, 0))] == [-1] * 3
+    assert [lib.tgis_k_w8_pair_plan(*a, 0, fit) for a in ((0, 1, 1), (1, 0, 1), (1, 1, 0))] == [-1] * 3

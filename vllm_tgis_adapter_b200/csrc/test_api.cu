@@ -159,11 +159,13 @@ int tgis_k_hold(int64_t clocks, void* stream) {
 }
 
 int tgis_k_w8_pieces(int32_t tiles, int32_t groups, int32_t ctas, const int32_t* at_once) {
+  if (at_once == nullptr || tiles < 1 || groups < 1 || ctas < 1) return kfail("tiles, groups, CTAs and four numbers of clusters are wanted");
   const int n[4] = {at_once[0], at_once[1], at_once[2], at_once[3]};
   int s = 0;
   return gemm8_plan(tiles, groups, ctas, n, &s) == cudaSuccess ? s : kfail("no cluster fits");
 }
 int tgis_k_w8_pair_plan(int32_t n, int32_t x_tiles, int32_t groups, int32_t gated, const int32_t* at_once) {
+  if (at_once == nullptr || n < 1 || x_tiles < 1 || groups < 1) return kfail("rows, tiles, groups and four numbers of clusters are wanted");
   const int fit[4] = {at_once[0], at_once[1], at_once[2], at_once[3]};
   Plan8 p{};
   return gemm8_pair_plan(n, x_tiles, groups, gated != 0, fit, &p) == cudaSuccess ? 16 * p.ch + p.s : kfail("no cluster fits");
